@@ -37,6 +37,7 @@
 #include "ops_attn.h"
 #include "ops_decode.h"
 #include "ops_stream.h"
+#include "ops_serve.h"
 #include "validate.h"
 #include "static_plan.h"
 
@@ -624,6 +625,9 @@ __device__ void dispatch(int op, const Ctx& c) {
     case 303: op_splitk_reduce(c); break;
     case 304: op_matmul_mma_bf16_256(c); break;
     case 305: op_adamw_bf16(c); break;
+    case 312: op_kv_append_q8(c); break;
+    case 313: op_attn_decode_q8(c); break;
+    case 314: op_logits_adjust(c); break;
     default: if (threadIdx.x == 0) c.fail(KVM_ERR_BAD_OP, op, 0);
   }
 }

@@ -3,6 +3,7 @@
 // an operator read or write outside its buffers, apart from data-dependent indices (token ids, KV lengths), which the
 // operators check on the device. Extent rules follow the reference's (runtime/ref_gpt.py, ref_extra.py `extents`).
 #pragma once
+#include <cmath>
 #include <cstring>
 #include <string>
 #include <vector>
@@ -41,7 +42,7 @@ static const OpSig* find_op(int id) { for (const OpSig& o : kRegistry) if (o.id 
 static bool implemented(int id) {
   static const int ids[] = {0, 1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 32, 33, 34, 35, 36, 37, 38, 39, 40, 41, 42, 43, 44, 45, 46, 47, 48, 49, 50,
                             51, 52, 53, 54, 55, 56, 57, 58, 59, 60, 61, 62, 63, 96, 97, 98, 99, 100, 101, 102, 103, 104, 113, 114, 115,
-                            116, 117, 118, 120, 121, 122, 123, 126, 127, 134, 135, 136, 300, 301, 302, 303, 304, 305, 306, 308, 309, 310, 311};
+                            116, 117, 118, 120, 121, 122, 123, 126, 127, 134, 135, 136, 300, 301, 302, 303, 304, 305, 306, 308, 309, 310, 311, 312, 313, 314};
   for (int i : ids) if (i == id) return true;
   return false;
 }
@@ -112,11 +113,32 @@ static char arg_class(int op, const std::string& n) {
     case 311: return in({"gamma"}) ? 'f' : 'a';
     case 302: return in({"bias"}) ? 'f' : 'a';
     case 303: return in({"out"}) ? 'a' : 'f';
+    case 312: return in({"kq", "vq", "lens"}) ? 'i' : in({"ks", "vs", "kgamma"}) ? 'f' : 'a';
+    case 313: return in({"kq", "vq", "lens", "cnt"}) ? 'i' : in({"ks", "vs", "qgamma", "part"}) ? 'f' : 'a';
+    case 314: return in({"logits", "out"}) ? 'a' : in({"par", "bval"}) ? 'f' : 'i';
     default: return 'f';
   }
 }
 
 static bool attn_hd(int hd) { return hd == 16 || hd == 32 || hd == 64 || hd == 128; }
+
+// The 8-bit cache of ops 312 and 313 (layout: mvm_ops_kvm.def) for sequences [0, B).
+static void cache_q8(Check& k, long long B, int Hkv, int hd, const char* gamma) {
+  const int blk = k.I("blk");
+  k.need(blk == 16 || blk == 32 || blk == 64 || blk == 128, "blk must be 16, 32, 64 or 128");
+  k.need(hd > 0 && hd <= 128 && hd % 4 == 0, "hd must be a multiple of 4 up to 128");
+  const MvmBuf *kq = k.B("kq"), *vq = k.B("vq"), *ks = k.B("ks"), *vs = k.B("vs");
+  if (!kq || !vq || !ks || !vs || hd <= 0) return;
+  k.need(kq->cols == hd / 4 && vq->cols == hd / 4, "kq and vq must have hd / 4 columns");
+  k.need(ks->cols == vs->cols && (long long)ks->cols * blk <= 0x7fffffffll, "ks and vs must have the same columns, one per block");
+  const char* names[] = {"kq", "vq", "ks", "vs", "kt", "vt"};
+  for (int i = 0; i < 6; ++i) for (int j = 0; j < i; ++j) k.need(k.a[k.idx(names[i])] != k.a[k.idx(names[j])], "kq, vq, ks, vs, kt and vt must be buffers of their own");
+  const long long pairs = B * Hkv, Tmax = (long long)ks->cols * blk;
+  k.ext("kq", pairs * Tmax, 0); k.ext("vq", pairs * Tmax, 0); k.ext("ks", pairs, 0); k.ext("vs", pairs, 0);
+  k.ext("kt", pairs * blk, hd); k.ext("vt", pairs * blk, hd); k.extn("lens", B); k.extn(gamma, hd);
+  const float theta = k.F("theta"), eps = k.F("eps");
+  k.need(std::isfinite(theta) && theta >= 0.f && std::isfinite(eps) && eps >= 0.f, "theta and eps must be finite and not negative");
+}
 
 // Operand extents of one task; mirrors the reference's extent functions for the ops implemented here.
 static void extents(int op, Check& k) {
@@ -298,6 +320,29 @@ static void extents(int op, Check& k) {
       k.ext("part", (long long)(S - 1) * M + r1, N); k.ext("out", r1, N); break; }
     case 300: { int r1 = k.I("r1"), H = k.I("H"), hd = k.I("hd"); k.range(k.I("r0"), r1); k.need(H > 0 && hd > 0, "bad H/hd");
       k.ext("x", r1, (long long)H * hd); k.ext("out", r1, (long long)H * hd); k.extn("gamma", hd); break; }
+    case 312: { const int b0 = k.I("b0"), b1 = k.I("b1"), h0 = k.I("h0"), h1 = k.I("h1"), p = k.I("p"), P = k.I("P"), nn = k.I("n_new"), Hkv = k.I("Hkv"), hd = k.I("hd");
+      k.range(b0, b1); k.need(0 <= h0 && h0 <= h1 && h1 <= Hkv && Hkv > 0 && 0 <= p && p < P && nn > 0, "bad h0/h1/Hkv/p/P/n_new");
+      cache_q8(k, b1, Hkv, hd, "kgamma");
+      k.ext("knew", (long long)b1 * nn, (long long)Hkv * hd); k.ext("vnew", (long long)b1 * nn, (long long)Hkv * hd); break; }
+    case 313: { const int b = k.I("b"), kvh = k.I("kvh"), s = k.I("s"), S = k.I("S"), nn = k.I("n_new"), H = k.I("H"), Hkv = k.I("Hkv"), hd = k.I("hd");
+      k.need(b >= 0 && Hkv > 0 && H > 0 && H % Hkv == 0 && 0 <= kvh && kvh < Hkv && 0 <= s && s < S, "bad b/kvh/s/S/H/Hkv");
+      k.need(nn > 0 && (Hkv <= 0 || (long long)nn * (H / Hkv) <= 32), "n_new * H / Hkv must be 1 .. 32");
+      const long long n = (long long)b + 1;
+      cache_q8(k, n, Hkv, hd, "qgamma");
+      k.ext("q", n * nn, (long long)H * hd); k.ext("o", n * nn, (long long)H * hd); k.extn("cnt", n * Hkv);
+      k.ext("part", n * S * H * nn, (long long)hd + 2);
+      k.need(k.a[k.idx("o")] != k.a[k.idx("q")], "o must not be q");
+      k.need(std::isfinite(k.F("scale")), "scale must be finite"); break; }
+    case 314: { const int r0 = k.I("r0"), r1 = k.I("r1"), v0 = k.I("v0"), v1 = k.I("v1"), V = k.I("V"); k.range(r0, r1);
+      k.need(V > 0 && 0 <= v0 && v0 <= v1 && v1 <= V, "bad v0/v1/V");
+      k.ext("logits", r1, V); k.ext("out", r1, V); k.ext("par", r1, 3);
+      const MvmBuf* h = k.B("hist"); const MvmBuf* bi = k.B("bidx"); const MvmBuf* bv = k.B("bval");
+      k.need(!h == !k.B("plen") && !h == !k.B("hlen") && (h || !k.B("last")), "hist, plen and hlen go together, last needs them");
+      k.need(!bi == !bv && (!bi || (bi->cols <= 2047 && bv->cols >= bi->cols)), "bidx and bval go together, at most 2047 entries a row");
+      k.need(k.B("mask") || !k.B("mrow"), "mrow needs mask");
+      k.need(!h || h->cols < (1 << 20), "hist holds less than 2^20 tokens a row");
+      k.ext("hist", r1, 0); k.extn("plen", r1); k.extn("hlen", r1); k.extn("last", r1); k.ext("bidx", r1, 0); k.ext("bval", r1, 0);
+      k.ext("mask", k.B("mrow") ? 1 : r1, ((long long)V + 31) / 32); k.extn("mrow", r1); break; }
     default: k.need(false, "no extent rule");
   }
 }

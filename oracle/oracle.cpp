@@ -791,6 +791,121 @@ void op_gemv_swiglu(const Ctx& c) {
   }
 }
 
+// This executor's ops 312-314 (semantics: include/mvm_ops_kvm.def), from the definition in double: the cache's scale is an f32
+// product as it is stored, a byte is the exact quotient rounded to nearest even.
+static void q8_turned(std::vector<double>& x, const V& g, float eps, float theta, long long t) {
+  const int hd = (int)x.size(), half = hd / 2;
+  if (g.ok()) {
+    double ss = 0; for (double v : x) ss += v * v;
+    const double rs = 1.0 / std::sqrt(ss / hd + eps);
+    for (int k = 0; k < hd; ++k) x[k] *= rs * g.f[k];
+  }
+  if (theta > 0.f)
+    for (int i = 0; i < half; ++i) {
+      const double a = (double)t * std::exp(-2.0 * i / hd * std::log((double)theta)), x1 = x[i], x2 = x[i + half];
+      x[i] = x1 * std::cos(a) - x2 * std::sin(a); x[i + half] = x1 * std::sin(a) + x2 * std::cos(a);
+    }
+}
+void op_kv_append_q8(const Ctx& c) {
+  V kn = c.buf(0), vn = c.buf(1), kq = c.buf(2), ks = c.buf(3), vq = c.buf(4), vs = c.buf(5), kt = c.buf(6), vt = c.buf(7), lens = c.buf(8), kg = c.buf(9, true);
+  const int b0 = c.i(10), b1 = c.i(11), h0 = c.i(12), h1 = c.i(13), p = c.i(14), P = c.i(15), n = c.i(16), Hkv = c.i(17), hd = c.i(18), blk = c.i(19);
+  const float theta = c.fl(20), eps = c.fl(21);
+  for (int b = b0; b < b1; ++b) if (lens.i[b] < -1 || (long long)lens.i[b] + n > (long long)blk * ks.cols) fail("kv_append_q8: length");
+  for (int b = b0; b < b1; ++b) {
+    const long long L = lens.i[b];
+    if (L < 0) continue;
+    const long long j0 = L / blk, jE = (L + n) / blk, mid = std::max(0ll, jE - j0 - 1), m0 = j0 + 1 + mid * p / P, m1 = j0 + 1 + mid * (p + 1) / P;
+    for (int h = h0; h < h1; ++h) for (int w = 0; w < 2; ++w) {
+      const V &src = w ? vn : kn, &tail = w ? vt : kt, &Q = w ? vq : kq, &S = w ? vs : ks;
+      const long long pair = (long long)b * Hkv + h;
+      for (long long j = j0; j <= jE; ++j) {
+        if (j == j0 || j == jE ? p != 0 : j < m0 || j >= m1) continue;
+        std::vector<float> x((size_t)blk * hd);
+        double amax = 0; bool finite = true;
+        for (int r = 0; r < blk; ++r) {
+          const long long t = j * blk + r;
+          if (t >= L + n || (j == jE && t < L)) continue;
+          std::vector<double> row(hd);
+          for (int k = 0; k < hd; ++k) row[k] = t < L ? tail.at(pair * blk + r, k) : src.at((long long)b * n + t - L, (long long)h * hd + k);
+          if (t >= L && !w) q8_turned(row, kg, eps, theta, t);
+          for (int k = 0; k < hd; ++k) {
+            const float v = tail.dtype == 2 ? bf16r(f32(row[k])) : f32(row[k]);
+            x[(size_t)r * hd + k] = v;
+            if (std::isfinite(v)) amax = std::max(amax, (double)std::fabs(v)); else finite = false;
+            if (j == jE) tail.stf((pair * blk + r) * tail.cols + k, v);
+          }
+        }
+        if (j == jE) continue;
+        float s = f32(f32(amax) * (double)f32(1.0 / 127.0));
+        if (s < 1.17549435e-38f) s = 0.f;
+        S.f[pair * S.cols + j] = finite ? s : NAN;
+        for (int r = 0; r < blk; ++r) for (int k = 0; k < hd; ++k) {
+          const double q = finite && s > 0.f ? std::nearbyint((double)x[(size_t)r * hd + k] / (double)s) : 0.0;
+          ((signed char*)Q.i)[(pair * S.cols + j) * blk * hd + (w ? k * blk + r : r * hd + k)] = (signed char)std::max(-127.0, std::min(127.0, q));
+        }
+      }
+    }
+  }
+}
+void op_attn_decode_q8(const Ctx& c) {   // the whole context in the task of split 0: the splits are the device's matter
+  V q = c.buf(0), kq = c.buf(1), ks = c.buf(2), vq = c.buf(3), vs = c.buf(4), kt = c.buf(5), vt = c.buf(6), lens = c.buf(7), o = c.buf(9), qg = c.buf(11, true);
+  const int b = c.i(12), kvh = c.i(13), s = c.i(14), n = c.i(16), H = c.i(17), Hkv = c.i(18), hd = c.i(19), blk = c.i(20), G = H / Hkv;
+  const double scale = c.fl(21); const float theta = c.fl(22), eps = c.fl(23);
+  const long long L = lens.i[b], pair = (long long)b * Hkv + kvh;
+  if (L < -1 || L + n > (long long)blk * ks.cols) fail("attn_decode_q8: length");
+  if (s) return;
+  const long long whole = (L + n) / blk * blk;
+  auto at = [&](const V& Q, const V& S, const V& T, bool vals, long long t, int d) -> double {
+    if (t >= whole) return T.at(pair * blk + t - whole, d);
+    const long long j = t / blk, r = t % blk;
+    return (double)((const signed char*)Q.i)[(pair * S.cols + j) * blk * hd + (vals ? d * blk + r : r * hd + d)] * S.f[pair * S.cols + j];
+  };
+  for (int i = 0; i < n; ++i) for (int g = 0; g < G; ++g) {
+    const long long row = (long long)b * n + i, col = (long long)(kvh * G + g) * hd;
+    if (L < 0) { for (int d = 0; d < hd; ++d) o.st(row * o.cols + col + d, 0.0); continue; }
+    std::vector<double> x(hd), p(L + i + 1);
+    for (int d = 0; d < hd; ++d) x[d] = q.at(row, col + d);
+    q8_turned(x, qg, eps, theta, L + i);
+    double m = -INFINITY, l = 0;
+    for (long long t = 0; t <= L + i; ++t) {
+      double a = 0; for (int d = 0; d < hd; ++d) a += x[d] * at(kq, ks, kt, false, t, d);
+      p[t] = a * scale; m = std::max(m, p[t]);
+    }
+    for (double& v : p) { v = std::exp(v - m); l += v; }
+    for (int d = 0; d < hd; ++d) {
+      double a = 0; for (long long t = 0; t <= L + i; ++t) a += p[t] * at(vq, vs, vt, true, t, d);
+      o.st(row * o.cols + col + d, a / l);
+    }
+  }
+}
+void op_logits_adjust(const Ctx& c) {
+  V x = c.buf(0), out = c.buf(1), par = c.buf(2), hist = c.buf(3, true), plen = c.buf(4, true), hlen = c.buf(5, true), last = c.buf(6, true);
+  V bidx = c.buf(7, true), bval = c.buf(8, true), mask = c.buf(9, true), mrow = c.buf(10, true);
+  const int r0 = c.i(11), r1 = c.i(12), v0 = c.i(13), v1 = c.i(14), V_ = c.i(15);
+  for (int r = r0; r < r1; ++r) {
+    const int n = hist.ok() ? hlen.i[r] : 0, pl = hist.ok() ? plen.i[r] : 0, mr = mask.ok() ? (mrow.ok() ? mrow.i[r] : r) : -1;
+    if (n < 0 || pl < 0 || pl > n || (hist.ok() && n + (last.ok() ? 1 : 0) > hist.cols)) fail("logits_adjust: history length");
+    if (mrow.ok() && (mr < -1 || mr >= mask.rows)) fail("logits_adjust: mask row");
+    std::vector<int> times(V_, 0); std::vector<char> seen(V_, 0); std::vector<double> bias(V_, 0.0);
+    auto put = [&](int v, bool gen) { if (v >= 0 && v < V_) { seen[v] = 1; times[v] += gen; } };
+    for (int k = 0; k < n; ++k) put(hist.i[(long long)r * hist.cols + k], k >= pl);
+    if (last.ok()) put(last.i[r], true);
+    if (bidx.ok()) for (int k = 0; k < bidx.cols; ++k) {
+      const int v = bidx.i[(long long)r * bidx.cols + k]; if (v >= 0 && v < V_) bias[v] += bval.at(r, k);
+    }
+    const double rep = par.at(r, 0), freq = par.at(r, 1), pres = par.at(r, 2);
+    for (int v = v0; v < v1; ++v) {
+      double y = x.at(r, v);
+      if (seen[v]) y = y > 0 ? y / rep : y * rep;
+      if (times[v]) y = y - freq * times[v] - pres;
+      y += bias[v];
+      if (mr >= 0 && !((mask.i[(long long)mr * mask.cols + v / 32] >> (v % 32)) & 1)) y = -INFINITY;
+      out.st((long long)r * out.cols + v, y);
+    }
+    if (last.ok() && v0 == 0) hist.i[(long long)r * hist.cols + n] = last.i[r];
+  }
+}
+
 typedef void (*OpFn)(const Ctx&);
 struct OpEnt { int id; OpFn fn; };
 const OpEnt kOps[] = {
@@ -808,6 +923,7 @@ const OpEnt kOps[] = {
   {113, op_round_bf16}, {114, op_matmul_tile_bf16}, {122, op_matmul_mma_bf16}, {134, op_gemv_bf16},
   {135, op_attn_decode_part}, {136, op_attn_decode_merge}, {115, op_adamw_lr}, {116, op_lr_schedule}, {117, op_scale_flat},
   {118, op_add_rowtile}, {120, op_matmul_tile_silu_mul}, {121, op_matmul_tile_silu_mul_bwd}, {300, op_head_rmsnorm}, {301, op_gemv_bf16_rows}, {311, op_gemv_swiglu}, {302, op_matmul_mma_bf16_kr}, {303, op_splitk_reduce}, {304, op_matmul_mma_bf16_256}, {305, op_adamw_bf16}, {306, op_attn_decode_part_qkn}, {310, op_attn_decode_part_merge}, {308, op_matmul_mma_bf16_delta},
+  {312, op_kv_append_q8}, {313, op_attn_decode_q8}, {314, op_logits_adjust},
 };
 OpFn find_op(int id) { for (const OpEnt& e : kOps) if (e.id == id) return e.fn; return nullptr; }
 
