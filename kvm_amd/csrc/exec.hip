@@ -625,8 +625,8 @@ __device__ void dispatch(int op, const Ctx& c) {
     case 303: op_splitk_reduce(c); break;
     case 304: op_matmul_mma_bf16_256(c); break;
     case 305: op_adamw_bf16(c); break;
-    case 312: op_kv_append_q8(c); break;
-    case 313: op_attn_decode_q8(c); break;
+    case 312: if (!op_kv_append_q8_fast(c)) op_kv_append_q8(c); break;
+    case 313: if (!op_attn_decode_q8_fast(c)) op_attn_decode_q8(c); break;
     case 314: op_logits_adjust(c); break;
     default: if (threadIdx.x == 0) c.fail(KVM_ERR_BAD_OP, op, 0);
   }

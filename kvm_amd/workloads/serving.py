@@ -48,11 +48,9 @@ def kv_append_q8(b: Builder, c: CacheQ8, knew: str, vnew: str, lens: str, n_new:
     pairs = c.batch * c.kv_heads
     P = max(1, min(tasks // pairs, n_new // c.blk))
     kw = dict(knew=knew, vnew=vnew, lens=lens, kgamma=kgamma, theta=theta, eps=eps, n_new=n_new, P=P, **c.args())
-    out = []
-    for b0, b1 in split(c.batch, max(1, tasks // (c.kv_heads * P))):
-        for h0, h1 in split(c.kv_heads, max(1, tasks // (c.batch * P))):
-            out += [b.task('kv_append_q8', after=after, b0=b0, b1=b1, h0=h0, h1=h1, p=p, **kw) for p in range(P)]
-    return out
+    seqs = split(c.batch, tasks // P)
+    heads = split(c.kv_heads, tasks // (len(seqs) * P))
+    return [b.task('kv_append_q8', after=after, b0=b0, b1=b1, h0=h0, h1=h1, p=p, **kw) for b0, b1 in seqs for h0, h1 in heads for p in range(P)]
 
 
 def attn_decode_q8(b: Builder, c: CacheQ8, q: str, o: str, lens: str, heads: int, n_new: int = 1, scale: float | None = None, after=(),
