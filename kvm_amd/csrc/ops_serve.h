@@ -10,11 +10,18 @@ namespace kvm {
 
 // ---------------------------------------------------------------------------------------------- 8-bit KV cache
 // Rotation of position t by frequency i: theta^(-2 i / hd) and the angle in double (at positions of 10^5 an f32 angle is off
-// by up to 4e-3), reduced to one turn there; sine and cosine in f32.
+// by up to 4e-3), there reduced to a quarter turn around 0; sine and cosine by their Taylor series in f32, whose next terms are
+// below 2e-9 at pi / 4. (The library's sincosf, with its path for large arguments, is ten times the code.)
 __device__ __forceinline__ double q8_freq(int i, int hd, double ln_theta) { return exp(-2.0 * i / hd * ln_theta); }
 __device__ __forceinline__ void q8_turn(long long t, double freq, float& sn, float& co) {
-  const double turns = (double)t * freq * 0.15915494309189533577;      // 1 / (2 pi)
-  sincosf((float)((turns - rint(turns)) * 6.28318530717958647693), &sn, &co);
+  const double turns = (double)t * freq * 0.15915494309189533577, quarter = rint(4.0 * turns);      // 1 / (2 pi)
+  const float x = (float)((turns - 0.25 * quarter) * 6.28318530717958647693), y = x * x;
+  const float s = x + x * y * (-1.f / 6 + y * (1.f / 120 + y * (-1.f / 5040 + y * (1.f / 362880))));
+  const float c = 1.f + y * (-1.f / 2 + y * (1.f / 24 + y * (-1.f / 720 + y * (1.f / 40320 + y * (-1.f / 3628800)))));
+  const int k = (int)((long long)quarter & 3);
+  sn = k & 1 ? c : s; co = k & 1 ? s : c;
+  if (k & 2) sn = -sn;
+  if (k == 1 || k == 2) co = -co;
 }
 // The 8-bit number of x in a block of scale s: x / s rounded to the nearest whole number, ties to even, with no
 // error from the reciprocal: one fused multiply-add gives the sign of (k + 1/2) s - |x| exactly. `inv` is 1 / s, 0 where s is 0.
@@ -38,37 +45,62 @@ typedef u32x4_t u32x4a4 __attribute__((aligned(4)));                   // 16 and
 typedef u32x2_t u32x2a4 __attribute__((aligned(4)));
 // Whether rows of X can be read and written in vectors of 8 elements at columns that are multiples of 8.
 __device__ __forceinline__ bool rows8_ok(const View& X) { return ((uintptr_t)X.p & 15) == 0 && (X.cols & 7) == 0; }
-__device__ __forceinline__ void row8(const View& X, long long o, float (&v)[8]) {
-  if (X.dtype == 2) {
-    const u16x8_t h = *(const GLOBAL u16x8_t*)(X.h() + o);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = bf2f(h[i]);
-  } else {
-    const f32x4n a = *(const GLOBAL f32x4n*)(X.f() + o), b = *(const GLOBAL f32x4n*)(X.f() + o + 4);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) { v[i] = a[i]; v[4 + i] = b[i]; }
+// Eight values as they lie in memory (bf16: the first half), so that a batch of loads is requested before any is converted.
+struct Raw8 {
+  u32x4_t lo, hi;
+  __device__ __forceinline__ void load(const View& X, long long o) {
+    if (X.dtype == 2) lo = *(const GLOBAL u32x4_t*)(X.h() + o);
+    else { lo = *(const GLOBAL u32x4_t*)(X.f() + o); hi = *(const GLOBAL u32x4_t*)(X.f() + o + 4); }
   }
+  __device__ __forceinline__ void get(bool half, float (&v)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[i] = __uint_as_float(!half ? lo[i] : i & 1 ? lo[i / 2] & 0xffff0000u : lo[i / 2] << 16);
+      v[4 + i] = __uint_as_float(!half ? hi[i] : i & 1 ? lo[2 + i / 2] & 0xffff0000u : lo[2 + i / 2] << 16);
+    }
+  }
+};
+template <int CTRL> __device__ __forceinline__ float dpp(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
 }
-// A head of HD values spread over HD / 8 neighbouring lanes, 8 each: RMS norm (g: this lane's gains, or none) and rotation of
+// Reduction over N = 8 or 16 neighbouring lanes, in registers: neighbours, pairs, then the mirrored half row and row.
+template <int N, class F> __device__ __forceinline__ float lanes_all(float v, F f) {
+  v = f(v, dpp<0xB1>(v));
+  v = f(v, dpp<0x4E>(v));
+  v = f(v, dpp<0x141>(v));
+  return N == 16 ? f(v, dpp<0x140>(v)) : v;
+}
+template <int N> __device__ __forceinline__ float lanes_sum(float v) { return lanes_all<N>(v, [](float a, float b) { return a + b; }); }
+template <int N> __device__ __forceinline__ float lanes_max(float v) { return lanes_all<N>(v, [](float a, float b) { return fmaxf(a, b); }); }
+// Over the four rows of 16 lanes of a wave: lane n of each gets f over lanes n, n + 16, n + 32, n + 48.
+template <class F> __device__ __forceinline__ float rows_all(float v, F f) {
+  auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = f(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return f(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float rows_sum(float v) { return rows_all(v, [](float a, float b) { return a + b; }); }
+__device__ __forceinline__ float rows_max(float v) { return rows_all(v, [](float a, float b) { return fmaxf(a, b); }); }
+// A head of HD values spread over HD / 8 neighbouring lanes, 8 each: RMS norm (gamma: the gains, or none) and rotation of
 // position t (freq: the HD / 2 frequencies in LDS, or none), in f32. The other half of a pair is HD / 16 lanes away; the lanes
-// share out the row's angles through `ang`, 2 HD floats of LDS for each row in flight (HD / 8 lanes of one wave).
+// share out the row's angles through `ang`, HD floats of LDS for each row in flight (HD / 8 lanes of one wave).
 template <int HD> __device__ __forceinline__ void head8_turn(float (&v)[8], const GLOBAL float* gamma, float eps, const LDS double* freq, long long t, LDS float* ang) {
   constexpr int LPR = HD / 8;
   const int ln = lane() % LPR;
-  if (gamma) {
-    float ss = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) ss += v[i] * v[i];
-#pragma unroll
-    for (int o = LPR / 2; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
-    const float rs = 1.f / sqrtf(ss / HD + eps);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = v[i] * rs * gamma[8 * ln + i];
-  }
   if (freq) {
 #pragma unroll 1
     for (int i = ln; i < HD / 2; i += LPR) { float sn, co; q8_turn(t, freq[i], sn, co); ang[i] = sn; ang[HD / 2 + i] = co; }
     __builtin_amdgcn_wave_barrier();                                   // one wave's LDS operations stay in order
+  }
+  if (gamma) {
+    float ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ss += v[i] * v[i];
+    const float rs = 1.f / sqrtf(lanes_sum<LPR>(ss) / HD + eps);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = v[i] * rs * gamma[8 * ln + i];
+  }
+  if (freq) {
     const float sign = ln >= LPR / 2 ? 1.f : -1.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -96,6 +128,12 @@ struct AppendQ8 {
       if (L < -1 || (long long)L + n > (long long)blk * nblk) { bad = true; c.fail(KVM_ERR_OP_KVLEN, b, L); }
     }
     return !__syncthreads_or(bad);
+  }
+  // Whether a block becomes full in this task's share.
+  __device__ bool finishes() const {
+    bool any = false;
+    for (int b = b0 + tid(); b < b1; b += KVM_THREADS) { const int L = lens.i()[b]; any = any || (L >= 0 && (L + n) / blk > L / blk); }
+    return __syncthreads_or(any);
   }
 };
 
@@ -181,82 +219,81 @@ __device__ __noinline__ void op_kv_append_q8(const Ctx& c) {
 }
 
 // KV append in 8 bits at head sizes 64 and 128, rows in whole vectors. Bound: a few dependent loads (length, row) and the launch
-// for single tokens, bytes for prompts. A row is HD / 8 lanes of 8 values, so a pass of the workgroup takes 16 or 32 rows: a
-// finished block is in registers as a whole (K and V together, one load round, one reduction of both maxima). Keys to be
-// normalised or rotated go through LDS first, row by row. Keys are stored as they lie, 8 bytes a lane; values turn through LDS.
-// Tail rows of all pairs of the task go in one range, a row to HD / 8 lanes.
-template <int HD> __device__ __noinline__ void append_q8_t(const Ctx& c) {
-  constexpr int LPR = HD / 8, RPP = KVM_THREADS / LPR, NP = 128 / RPP;    // lanes a row, rows a pass, passes of the largest block
+// for single tokens, bytes for prompts. A row is HD / 8 lanes of 8 values, so a pass of the workgroup takes 16 or 32 rows.
+// The tail rows of all pairs of the task go in one range, a row to HD / 8 lanes; blocks that become full (of single tokens one call in
+// blk) are a function of their own, whose registers the tail rows' callers need not save.
+// A full block is in registers as a whole, all its loads requested before any is used, K and V with one reduction of both maxima.
+// Keys to be normalised or rotated
+// go through LDS first, row by row. Keys are stored as they lie, 8 bytes a lane; values turn through LDS.
+template <int HD> struct AppendLds {
+  LDS double* freq; LDS float* red; LDS float* keys; LDS float* angs; LDS unsigned char* turn;
+  __device__ explicit AppendLds(LDS char* p)
+      : freq((LDS double*)p), red((LDS float*)(freq + HD / 2)), keys(red + 16), angs(keys + 128 * HD), turn((LDS unsigned char*)(angs + KVM_THREADS * 8)) {}
+};
+template <int HD, int NP> __device__ __noinline__ void append_q8_blocks(const Ctx& c) {
+  constexpr int LPR = HD / 8, RPP = KVM_THREADS / LPR;                 // lanes a row, rows a pass; NP passes hold a block
   const AppendQ8 A(c);
-  if (!A.lengths_ok(c)) return;
-  LDS double* freq = (LDS double*)c.smem;                              // [HD / 2]
-  LDS float* red = (LDS float*)(freq + HD / 2);                        // [8]
-  LDS float* keys = red + 16;                                          // [blk][HD]
-  LDS float* angs = keys + 128 * HD;                                   // [RPP][2 HD / 2]
-  LDS unsigned char* turn = (LDS unsigned char*)(angs + RPP * HD);     // [HD][blk + 4]
+  const AppendLds<HD> M(c.smem);                                       // keys [blk][HD], turn [HD][blk + 4]
   const int ln = tid() % LPR, rw = tid() / LPR, blk = A.blk;
   const GLOBAL float* gamma = A.kg.ok() ? A.kg.f() : nullptr;
-  const LDS double* rot = A.theta > 0.f ? freq : nullptr;
-  if (rot && tid() < HD / 2) freq[tid()] = q8_freq(tid(), HD, log((double)A.theta));
-  __syncthreads();
+  const LDS double* rot = A.theta > 0.f ? M.freq : nullptr;
+  const bool turned = gamma || rot, nkh = A.kn.dtype == 2, nvh = A.vn.dtype == 2, tkh = A.kt.dtype == 2, tvh = A.vt.dtype == 2;
   const int nh = A.h1 - A.h0;
   for (int u = 0; u < (A.b1 - A.b0) * nh; ++u) {
-    const int b = A.b0 + u / nh, h = A.h0 + u % nh, L = A.lens.i()[b];
+    const int b = A.b0 + u / nh, h = A.h0 + u % nh, L = rfl(A.lens.i()[b]);
     if (L < 0) continue;
     const long long pair = (long long)b * A.Hkv + h;
     const int j0 = L / blk, jE = (L + A.n) / blk, mid = max(0, jE - j0 - 1);
     const int m0 = (int)((long long)mid * A.p / A.P), m1 = (int)((long long)mid * (A.p + 1) / A.P);
     for (int it = A.p == 0 && jE > j0 ? m0 - 1 : m0; it < m1; ++it) {  // (p = 0: m0 = 0, and -1 is the first block)
-      const int j = j0 + 1 + it;
-      const long long t0 = (long long)j * blk;
-      auto new_row = [&](const View& X, long long t) { return ((long long)b * A.n + (t - L)) * X.cols + h * HD + 8 * ln; };
-      if (gamma || rot) {
+      const int j = j0 + 1 + it, old = max(0, L - j * blk);            // rows below `old` are in the tail
+      const long long new0 = (long long)b * A.n + ((long long)j * blk - L), tail0 = pair * blk;
+      if (turned) {
         __syncthreads();
 #pragma unroll 1
         for (int r = rw; r < blk; r += RPP) {
           float x[8];
-          if (t0 + r >= L) {
-            row8(A.kn, new_row(A.kn, t0 + r), x);
-            head8_turn<HD>(x, gamma, A.eps, rot, t0 + r, angs + rw * HD);
-          } else row8(A.kt, (pair * blk + r) * A.kt.cols + 8 * ln, x);
+          Raw8 w;
+          if (r >= old) {
+            w.load(A.kn, (new0 + r) * A.kn.cols + h * HD + 8 * ln); w.get(nkh, x);
+            head8_turn<HD>(x, gamma, A.eps, rot, (long long)j * blk + r, M.angs + rw * HD);
+          } else { w.load(A.kt, (tail0 + r) * A.kt.cols + 8 * ln); w.get(tkh, x); }
 #pragma unroll
-          for (int e = 0; e < 8; ++e) keys[r * HD + 8 * ln + e] = x[e];
+          for (int e = 0; e < 8; ++e) M.keys[r * HD + 8 * ln + e] = x[e];
         }
       }
-      float k[NP][8], v[NP][8];
+      Raw8 rk[NP], rv[NP];
 #pragma unroll
       for (int i = 0; i < NP; ++i) {
         const int r = i * RPP + rw;
         if (r >= blk) break;
-        if (gamma || rot) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) k[i][e] = keys[r * HD + 8 * ln + e];      // this thread's own
-        }
-        if (t0 + r < L) {
-          if (!(gamma || rot)) row8(A.kt, (pair * blk + r) * A.kt.cols + 8 * ln, k[i]);
-          row8(A.vt, (pair * blk + r) * A.vt.cols + 8 * ln, v[i]);
-        } else {
-          if (!(gamma || rot)) row8(A.kn, new_row(A.kn, t0 + r), k[i]);
-          row8(A.vn, new_row(A.vn, t0 + r), v[i]);
-        }
+        const bool in_tail = r < old;
+        if (!turned) rk[i].load(in_tail ? A.kt : A.kn, in_tail ? (tail0 + r) * A.kt.cols + 8 * ln : (new0 + r) * A.kn.cols + h * HD + 8 * ln);
+        rv[i].load(in_tail ? A.vt : A.vn, in_tail ? (tail0 + r) * A.vt.cols + 8 * ln : (new0 + r) * A.vn.cols + h * HD + 8 * ln);
       }
-      float ka = 0.f, va = 0.f;
+      float k[NP][8], v[NP][8], ka = 0.f, va = 0.f;
 #pragma unroll
       for (int i = 0; i < NP; ++i) {
-        if (i * RPP + rw >= blk) break;
+        const int r = i * RPP + rw;
+        if (r >= blk) break;
+        if (turned) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) k[i][e] = M.keys[r * HD + 8 * ln + e];    // this thread's own
+        } else rk[i].get(r < old ? tkh : nkh, k[i]);
+        rv[i].get(r < old ? tvh : nvh, v[i]);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          if (A.kt.dtype == 2) k[i][e] = round_bf(k[i][e]);
-          if (A.vt.dtype == 2) v[i][e] = round_bf(v[i][e]);
+          if (tkh) k[i][e] = round_bf(k[i][e]);
+          if (tvh) v[i][e] = round_bf(v[i][e]);
           ka = q8_amax(ka, k[i][e]); va = q8_amax(va, v[i][e]);
         }
       }
-      ka = wave_max(ka); va = wave_max(va);
+      ka = rows_max(lanes_max<16>(ka)); va = rows_max(lanes_max<16>(va));
       __syncthreads();                                                 // the block before is out of `turn` and `red`
-      if (lane() == 0) { red[wave()] = ka; red[4 + wave()] = va; }
+      if (lane() == 0) { M.red[wave()] = ka; M.red[4 + wave()] = va; }
       __syncthreads();
-      const float sk = q8_scale(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]))), ik = sk > 0.f ? 1.f / sk : 0.f;
-      const float sv = q8_scale(fmaxf(fmaxf(red[4], red[5]), fmaxf(red[6], red[7]))), iv = sv > 0.f ? 1.f / sv : 0.f;
+      const float sk = q8_scale(fmaxf(fmaxf(M.red[0], M.red[1]), fmaxf(M.red[2], M.red[3]))), ik = sk > 0.f ? 1.f / sk : 0.f;
+      const float sv = q8_scale(fmaxf(fmaxf(M.red[4], M.red[5]), fmaxf(M.red[6], M.red[7]))), iv = sv > 0.f ? 1.f / sv : 0.f;
       if (tid() == 0) { stwt32(A.ks.f() + (pair * A.ks.cols + j), sk); stwt32(A.vs.f() + (pair * A.vs.cols + j), sv); }
       const long long byte0 = (pair * A.nblk + j) * blk * HD;
       const __amdgpu_buffer_rsrc_t ok = wt_rsrc((const char*)A.kq.p + byte0, blk * HD), ov = wt_rsrc((const char*)A.vq.p + byte0, blk * HD);
@@ -268,16 +305,30 @@ template <int HD> __device__ __noinline__ void append_q8_t(const Ctx& c) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           w[e / 4] |= (uint32_t)(q8_of(k[i][e], sk, ik) & 255) << (8 * (e % 4));
-          turn[(8 * ln + e) * (blk + 4) + r] = (unsigned char)q8_of(v[i][e], sv, iv);
+          M.turn[(8 * ln + e) * (blk + 4) + r] = (unsigned char)q8_of(v[i][e], sv, iv);
         }
         __builtin_amdgcn_raw_buffer_store_b64(u32x2_t{w[0], w[1]}, ok, r * HD + 8 * ln, 0, 16 /* SC1 */);
       }
       __syncthreads();
       for (int e = tid(); e < HD * blk / 16; e += KVM_THREADS) {
-        const LDS uint32_t* x = (const LDS uint32_t*)(turn + (16 * e / blk) * (blk + 4) + 16 * e % blk);
+        const LDS uint32_t* x = (const LDS uint32_t*)(M.turn + (16 * e / blk) * (blk + 4) + 16 * e % blk);
         stwt_buf(ov, 16 * e, __builtin_bit_cast(f32x4n, u32x4_t{x[0], x[1], x[2], x[3]}));
       }
     }
+  }
+}
+template <int HD> __device__ __forceinline__ void append_q8_t(const Ctx& c) {
+  constexpr int LPR = HD / 8, RPP = KVM_THREADS / LPR;
+  const AppendQ8 A(c);
+  if (!A.lengths_ok(c)) return;
+  const AppendLds<HD> M(c.smem);
+  const int ln = tid() % LPR, rw = tid() / LPR, blk = A.blk, nh = A.h1 - A.h0;
+  const GLOBAL float* gamma = A.kg.ok() ? A.kg.f() : nullptr;
+  const LDS double* rot = A.theta > 0.f ? M.freq : nullptr;
+  if (rot && tid() < HD / 2) M.freq[tid()] = q8_freq(tid(), HD, log((double)A.theta));
+  if (A.finishes()) {                                                  // (a barrier on both ways)
+    if (blk <= 4 * RPP) append_q8_blocks<HD, 4>(c);
+    else append_q8_blocks<HD, 128 / RPP>(c);
   }
   if (A.p != 0) return;
   __syncthreads();                                                     // old rows of the tail have been read
@@ -288,10 +339,12 @@ template <int HD> __device__ __noinline__ void append_q8_t(const Ctx& c) {
     const long long t = max((long long)L, (long long)((L + A.n) / blk) * blk) + u % most;
     if (t >= (long long)L + A.n) continue;
     const long long row = (long long)b * A.n + (t - L), at = ((long long)b * A.Hkv + h) * blk + t % blk;
+    Raw8 rk, rv;
+    rk.load(A.kn, row * A.kn.cols + h * HD + 8 * ln);
+    rv.load(A.vn, row * A.vn.cols + h * HD + 8 * ln);
     float k[8], v[8];
-    row8(A.kn, row * A.kn.cols + h * HD + 8 * ln, k);
-    row8(A.vn, row * A.vn.cols + h * HD + 8 * ln, v);
-    if (gamma || rot) head8_turn<HD>(k, gamma, A.eps, rot, t, angs + rw * HD);
+    rk.get(A.kn.dtype == 2, k); rv.get(A.vn.dtype == 2, v);
+    if (gamma || rot) head8_turn<HD>(k, gamma, A.eps, rot, t, M.angs + rw * HD);
     st8(A.kt, at * A.kt.cols + 8 * ln, k);
     st8(A.vt, at * A.vt.cols + 8 * ln, v);
   }
@@ -325,7 +378,9 @@ struct DecodeQ8 {
     return false;
   }
 };
-// The split that counts itself last merges the `live` splits' partials; maxima are in units of log2.
+// The split that counts itself last merges the `live` splits' partials; maxima are in units of log2. A wave takes a row at a time:
+// lane i has the maximum and sum of split i, the weights go from there to all lanes, which add up to two head dims each, the loads
+// of 16 splits in flight.
 __device__ __forceinline__ void q8_arrive(const Ctx& c, const DecodeQ8& D, int live, LDS int* flag) {
   wait_stores();
   __syncthreads();
@@ -336,28 +391,35 @@ __device__ __forceinline__ void q8_arrive(const Ctx& c, const DecodeQ8& D, int l
   if (old < 0 || old >= live) { if (tid() == 0) c.fail(KVM_ERR_OP_RANGE, D.b * D.Hkv + D.kvh, old); return; }
   if (old != live - 1) return;
   fence_acquire();                                                     // the other splits' partials, stored before their counts
-  constexpr int SB = 16;                                               // splits in flight: their loads wait for memory together
-  for (int e = tid(); e < D.R * D.hd; e += KVM_THREADS) {
-    const int r = e / D.hd, d = e % D.hd;
-    float M = -INFINITY, a = 0.f, l = 0.f;
-    for (int s0 = 0; s0 < live; s0 += SB) {
-      float x[SB], m[SB], z[SB], top = M;
+  constexpr int SB = 16;
+  const int l = lane(), hd = D.hd, d0 = min(l, hd - 1), d1 = min(l + 64, hd - 1);
+  const long long step = D.part_at(1, 0) - D.part_at(0, 0);
+  for (int r = wave(); r < D.R; r += KVM_WAVES) {
+    const GLOBAL float* base = D.part.f() + D.part_at(0, r);
+    float M = -INFINITY, a0 = 0.f, a1 = 0.f, z = 0.f;
+    for (int s0 = 0; s0 < live; s0 += 64) {
+      const bool mine = s0 + l < live;
+      const GLOBAL float* y = base + (long long)min(s0 + l, live - 1) * step;
+      const float m = mine ? y[hd] : -INFINITY, x = mine ? y[hd + 1] : 0.f;
+      const float top = fmaxf(M, wave_max(m)), f = M == -INFINITY ? 0.f : exp2f(M - top), e = m == -INFINITY ? 0.f : exp2f(m - top);
+      z = z * f + e * x; a0 *= f; a1 *= f; M = top;
+      for (int s1 = 0; s1 < 64 && s0 + s1 < live; s1 += SB) {
+        float x0[SB], x1[SB];
 #pragma unroll
-      for (int i = 0; i < SB; ++i) {
-        const GLOBAL float* y = D.part.f() + D.part_at(min(s0 + i, live - 1), r);
-        x[i] = y[d]; m[i] = y[D.hd]; z[i] = y[D.hd + 1];
-      }
+        for (int i = 0; i < SB; ++i) {
+          const GLOBAL float* w = base + (long long)min(s0 + s1 + i, live - 1) * step;
+          x0[i] = w[d0]; x1[i] = w[d1];
+        }
 #pragma unroll
-      for (int i = 0; i < SB; ++i) top = fmaxf(top, m[i]);
-      const float f = M == -INFINITY ? 0.f : exp2f(M - top);
-      a *= f; l *= f; M = top;
-#pragma unroll
-      for (int i = 0; i < SB; ++i) {
-        const float w = m[i] == -INFINITY ? 0.f : exp2f(m[i] - M);
-        if (s0 + i < live) { a += w * x[i]; l += w * z[i]; }
+        for (int i = 0; i < SB; ++i) {
+          const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(e), s1 + i));
+          if (s0 + s1 + i < live) { a0 += w * x0[i]; a1 += w * x1[i]; }
+        }
       }
     }
-    D.o.st(D.o_at(r) + d, a / l);
+    z = wave_sum(z);
+    if (l < hd) D.o.st(D.o_at(r) + l, a0 / z);
+    if (l + 64 < hd) D.o.st(D.o_at(r) + l + 64, a1 / z);
   }
   if (tid() == 0) st_relaxed((int*)cnt, 0);
 }
@@ -515,68 +577,93 @@ template <int HD, int NT> __device__ __noinline__ void attn_q8_t(const Ctx& c) {
     for (int d = 0; d < VT; ++d) U.v[d] = *(const GLOBAL u32x4a4*)(vb + (16 * d + nn) * blk);
     U.ks = KS[(t0 >> lb) + j]; U.vs = VS[(t0 >> lb) + j];
   };
+  // everything that a short context needs is requested at once: query rows, the unfinished block, the first unit
+  constexpr int QP = (16 * NT + RPP - 1) / RPP, TP = 4;
+  Raw8 rq[QP], rk[TP], rv[TP];
+#pragma unroll
+  for (int i = 0; i < QP; ++i) if (i * RPP + rw < D.R) rq[i].load(D.q, D.q_at(i * RPP + rw) + 8 * ln);
+  auto load_tail = [&](int t0) {
+#pragma unroll
+    for (int i = 0; i < TP; ++i) {
+      const long long t = pair * blk + min(t0 + i * RPP + rw, nt - 1);
+      if (t0 + i * RPP < nt) { rk[i].load(D.kt, t * D.kt.cols + 8 * ln); rv[i].load(D.vt, t * D.vt.cols + 8 * ln); }
+    }
+  };
+  if (tail) load_tail(0);
   UnitQ8<HD> U;
-  if (D.theta > 0.f && tid() < HD / 2) freq[tid()] = q8_freq(tid(), HD, log((double)D.theta));
   if (u0 + w < u1) load(U, u0 + w);
+  if (D.theta > 0.f && tid() < HD / 2) freq[tid()] = q8_freq(tid(), HD, log((double)D.theta));
   __syncthreads();
   // query rows: norm, rotation, then scaled so that the largest magnitude of a row lies in [2^10, 2^11)
-  for (int r = rw; r < 16 * NT; r += RPP) {
+#pragma unroll
+  for (int i = 0; i < QP; ++i) {
+    const int r = i * RPP + rw;
+    if (r >= 16 * NT) break;
     float x[8] = {};
     if (r < D.R) {
-      row8(D.q, D.q_at(r) + 8 * ln, x);
+      rq[i].get(D.q.dtype == 2, x);
       head8_turn<HD>(x, D.qg.ok() ? D.qg.f() : nullptr, D.eps, D.theta > 0.f ? freq : nullptr, D.L + r / D.G, ts + rw * HD);
     }
     float big = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) big = fmaxf(big, fabsf(x[i]));
-#pragma unroll
-    for (int o = LPR / 2; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor(big, o, 64));
+    for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(x[e]));
+    big = lanes_max<LPR>(big);
     const int ex = max(20, (int)(__float_as_uint(big) >> 23));
     const float up = __uint_as_float((uint32_t)(264 - ex) << 23), down = __uint_as_float((uint32_t)(ex - 10) << 23);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) qs[r * QS + 8 * ln + i] = x[i] * up;
+    for (int e = 0; e < 8; ++e) qs[r * QS + 8 * ln + e] = x[e] * up;
     if (ln == 0) cr[r] = down * D.scale * LOG2E;
   }
   __syncthreads();
   if (tail) {                                                          // scores of the unfinished block, then its own softmax and P V
-    for (int t0 = 0; t0 < nt; t0 += 4 * RPP) {
-      float x[4][8], y[4][8];
+    for (int t0 = 0; t0 < nt; t0 += TP * RPP) {
+      if (t0) load_tail(t0);
+      float x[TP][8];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int t = min(t0 + i * RPP + rw, nt - 1);
-        row8(D.kt, (pair * blk + t) * D.kt.cols + 8 * ln, x[i]);
-        row8(D.vt, (pair * blk + t) * D.vt.cols + 8 * ln, y[i]);
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < TP; ++i) {
         const int t = t0 + i * RPP + rw;
         if (t >= nt) break;
+        float y[8];
+        rk[i].get(D.kt.dtype == 2, x[i]);
+        rv[i].get(D.vt.dtype == 2, y);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) tv[t * HD + 8 * ln + e] = y[i][e];
-        for (int r = 0; r < D.R; ++r) {
+        for (int e = 0; e < 8; ++e) tv[t * HD + 8 * ln + e] = y[e];
+      }
+      for (int r = 0; r < D.R; ++r) {
+        float q[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) q[e] = qs[r * QS + 8 * ln + e];
+        const int seen = min(nt, D.L + r / D.G + 1 - whole);
+#pragma unroll
+        for (int i = 0; i < TP; ++i) {
+          const int t = t0 + i * RPP + rw;
           float a = 0.f;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) a += qs[r * QS + 8 * ln + e] * x[i][e];
-#pragma unroll
-          for (int o = LPR / 2; o > 0; o >>= 1) a += __shfl_xor(a, o, 64);
-          if (ln == 0) ts[r * 128 + t] = whole + t <= D.L + r / D.G ? a * cr[r] : -INFINITY;
+          for (int e = 0; e < 8; ++e) a += q[e] * x[i][e];
+          a = lanes_sum<LPR>(a);
+          if (ln == 0 && t < nt) ts[r * 128 + t] = t < seen ? a * cr[r] : -INFINITY;
         }
       }
     }
     __syncthreads();
     for (int r = w; r < D.R; r += KVM_WAVES) {
       const float a = l < nt ? ts[r * 128 + l] : -INFINITY, b = 64 + l < nt ? ts[r * 128 + 64 + l] : -INFINITY;
-      const float m = wave_max(fmaxf(a, b)), pa = a == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(a - m), pb = b == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(b - m);
-      const float z = wave_sum(pa + pb);
+      const float m = rows_max(lanes_max<16>(fmaxf(a, b)));
+      const float pa = a == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(a - m), pb = b == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(b - m);
+      const float z = rows_sum(lanes_sum<16>(pa + pb));
       ts[r * 128 + l] = pa; ts[r * 128 + 64 + l] = pb;
       if (l == 0) { st[256 + r] = m; st[288 + r] = z; }
     }
     __syncthreads();
     for (int r = tid() / HD; r < D.R; r += KVM_THREADS / HD) {
       const int d = tid() % HD, seen = min(nt, D.L + r / D.G + 1 - whole);   // a value that the row may not see does not count, NaN neither
-      float a = 0.f;
-      for (int t = 0; t < seen; ++t) a += ts[r * 128 + t] * tv[t * HD + d];
-      to[r * HD + d] = a;
+      float a[4] = {0.f, 0.f, 0.f, 0.f};
+      int t = 0;
+      for (; t + 8 <= seen; t += 8)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) a[e % 4] += ts[r * 128 + t + e] * tv[(t + e) * HD + d];
+      for (; t < seen; ++t) a[0] += ts[r * 128 + t] * tv[t * HD + d];
+      to[r * HD + d] = (a[0] + a[1]) + (a[2] + a[3]);
     }
   }
   // the queries as B operands: row nn of tile g, dims 16 (qq + 4 h) + 8 p ..
@@ -606,7 +693,7 @@ template <int HD, int NT> __device__ __noinline__ void attn_q8_t(const Ctx& c) {
   for (int u = u0 + w; u < u1; u += KVM_WAVES) {
     UnitQ8<HD> N;
     if (u + KVM_WAVES < u1) load(N, u + KVM_WAVES);
-    const float vm0 = U.vs == U.vs ? U.vs : 0.f, vm1 = fmaxf(vm0, __shfl_xor(vm0, 16, 64)), vm = fmaxf(vm1, __shfl_xor(vm1, 32, 64));
+    const float vm0 = U.vs == U.vs ? U.vs : 0.f, vm = rows_max(vm0);
     float fv = 1.f;
     if (vm > vref) {                                                   // uniform: the four lane groups hold the unit's scales
       const float nv = __uint_as_float((__float_as_uint(vm) & 0x7f800000u) + 0x00800000u);
@@ -644,8 +731,7 @@ template <int HD, int NT> __device__ __noinline__ void attn_q8_t(const Ctx& c) {
       float m = mrun[g];
 #pragma unroll
       for (int i = 0; i < 16; ++i) if (i < seen) m = fmaxf(m, sc[g][i]);
-      m = fmaxf(m, __shfl_xor(m, 16, 64));
-      m = fmaxf(m, __shfl_xor(m, 32, 64));
+      m = rows_max(m);
       const float base = m == -INFINITY ? 0.f : m;                     // nothing seen yet (or NaN, which stays)
       const float f = __builtin_amdgcn_exp2f(mrun[g] - base);
       float z = 0.f;
@@ -682,8 +768,7 @@ template <int HD, int NT> __device__ __noinline__ void attn_q8_t(const Ctx& c) {
 #pragma unroll
   for (int g = 0; g < NT; ++g) {
     const int r = 16 * g + nn;
-    float z = lrun[g] + __shfl_xor(lrun[g], 16, 64);
-    z += __shfl_xor(z, 32, 64);
+    const float z = rows_sum(lrun[g]);
     if (r < D.R) {
 #pragma unroll
       for (int d = 0; d < VT; ++d)
@@ -725,25 +810,28 @@ __device__ __noinline__ bool op_attn_decode_q8_fast(const Ctx& c) {
 }
 
 // ---------------------------------------------------------------------------------------------- logits
-// Adjusted logits (op 314): the token counts of the sequence in LDS, one word per logit of a chunk (generated: bits 0..19,
-// bias slot + 1: bits 20..30, prompt: bit 31), then the logits against them. Bound: the bytes of the logits, and per task the
-// history, which every task of a row reads as a whole (a few KB, from the L2), and the clearing of the words. Logits go
-// in vectors of 4 from any element (a bf16 row from its first aligned one), eight loads in flight per thread; most have the
-// word 0 and only meet the mask. Entries of one token in the bias list share the slot of the first, with their sum in list order.
-constexpr int ADJ_CHUNK = 26624, ADJ_BIAS = 2047;
+// Adjusted logits (op 314): the token counts of the sequence in LDS, one word per logit of a chunk (generated: bits 0..19, bias
+// slot: bits 20..30, prompt: bit 31), then the logits against them. Bound: the bytes of the logits, and per task the history, which
+// every task of a row reads as a whole (a few KB, from the L2), and the clearing of the words. Logits go in vectors of 4
+// from any element (a bf16 row from its first aligned one), eight per thread requested before the ones before are used;
+// most have the word 0 and only meet the mask. A token's entries in the bias list meet by an atomic maximum of (2047 - entry),
+// which leaves the slot of the first; the others are added to it in list order, one after another (they are few).
+constexpr int ADJ_CHUNK = 26624, ADJ_BIAS = 2047, ADJ_NB = 8;
 struct AdjustArgs {
   View x, out, par, hist, plen, hlen, last, bidx, bval, mask, mrow;
   int r0, r1, v0, v1, V;
   __device__ explicit AdjustArgs(const Ctx& c)
       : x(c.buf(0)), out(c.buf(1)), par(c.buf(2)), hist(c.buf(3)), plen(c.buf(4)), hlen(c.buf(5)), last(c.buf(6)), bidx(c.buf(7)), bval(c.buf(8)),
         mask(c.buf(9)), mrow(c.buf(10)), r0(c.i(11)), r1(c.i(12)), v0(c.i(13)), v1(c.i(14)), V(c.i(15)) {}
+  // All rows of the task are checked before anything is written.
   __device__ bool rows_ok(const Ctx& c) const {
-    for (int r = r0; r < r1; ++r) {
+    bool bad = false;
+    for (int r = r0 + tid(); r < r1; r += KVM_THREADS) {
       const int n = hist.ok() ? hlen.i()[r] : 0, pl = hist.ok() ? plen.i()[r] : 0, m = mrow.ok() ? mrow.i()[r] : 0;
-      if (n < 0 || pl < 0 || pl > n || (hist.ok() && n + (last.ok() ? 1 : 0) > hist.cols)) { if (tid() == 0) c.fail(KVM_ERR_OP_RANGE, r, n); return false; }
-      if (mrow.ok() && (m < -1 || m >= mask.rows)) { if (tid() == 0) c.fail(KVM_ERR_OP_RANGE, r, m); return false; }
+      if (n < 0 || pl < 0 || pl > n || (hist.ok() && n + (last.ok() ? 1 : 0) > hist.cols)) { bad = true; c.fail(KVM_ERR_OP_RANGE, r, n); }
+      if (mrow.ok() && (m < -1 || m >= mask.rows)) { bad = true; c.fail(KVM_ERR_OP_RANGE, r, m); }
     }
-    return true;
+    return !__syncthreads_or(bad);
   }
 };
 __device__ __forceinline__ float adjusted(float x, uint32_t w, float rep, float freq, float pres, const LDS float* bsum) {
@@ -751,49 +839,28 @@ __device__ __forceinline__ float adjusted(float x, uint32_t w, float rep, float 
     const uint32_t times = w & 0xfffffu, slot = (w >> 20) & 2047u;
     if (times || (w >> 31)) x = x > 0.f ? x / rep : x * rep;
     if (times) { x -= freq * (float)times; x -= pres; }
-    if (slot) x += bsum[slot - 1];
+    if (slot) x += bsum[ADJ_BIAS - slot];
   }
   return x;
 }
+__device__ __forceinline__ void lds_or(LDS uint32_t* p, uint32_t v) { __hip_atomic_fetch_or(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP); }
 __device__ __noinline__ void op_logits_adjust(const Ctx& c) {
   const AdjustArgs A(c);
   if (!A.rows_ok(c)) return;
   LDS uint32_t* cnt = (LDS uint32_t*)c.smem;                           // [ADJ_CHUNK + 8]
-  LDS float* bsum = (LDS float*)(cnt + ADJ_CHUNK + 8);                 // [ADJ_BIAS + 1]
-  LDS int* bidx = (LDS int*)(bsum + ADJ_BIAS + 1);                     // [ADJ_BIAS + 1]; -1 for an entry that is not its token's first
+  LDS float* bsum = (LDS float*)(cnt + ADJ_CHUNK + 8);                 // [ADJ_BIAS + 1] an entry's value, the first one's the sum
+  LDS int* later = (LDS int*)(bsum + ADJ_BIAS + 1);                    // [ADJ_BIAS + 1] first entry of the same token, or -1
   static_assert((ADJ_CHUNK + 8 + 2 * (ADJ_BIAS + 1)) * 4 <= KVM_LDS_BYTES, "logits LDS map");
-  constexpr int NB = 8;
+  constexpr int NB = ADJ_NB;
   const int nb = A.bidx.ok() ? A.bidx.cols : 0;
   const bool xh = A.x.dtype == 2, oh = A.out.dtype == 2;
   for (int r = A.r0; r < A.r1; ++r) {
     const float rep = A.par.at(r, 0), freq = A.par.at(r, 1), pres = A.par.at(r, 2);
     const int n = A.hist.ok() ? A.hlen.i()[r] : 0, pl = A.hist.ok() ? A.plen.i()[r] : 0, last = A.last.ok() ? A.last.i()[r] : -1;
     const GLOBAL int* hist = A.hist.ok() ? A.hist.i() + (long long)r * A.hist.cols : nullptr;
+    const GLOBAL int* bidx = nb ? A.bidx.i() + (long long)r * A.bidx.cols : nullptr;
     const int mr = A.mask.ok() ? (A.mrow.ok() ? A.mrow.i()[r] : r) : -1;
     const GLOBAL int* mask = mr >= 0 ? A.mask.i() + (long long)mr * A.mask.cols : nullptr;
-    if (nb) {
-      __syncthreads();
-      for (int j = tid(); j < nb; j += KVM_THREADS) bidx[j] = A.bidx.i()[(long long)r * A.bidx.cols + j];
-      __syncthreads();
-      int mine[(ADJ_BIAS + KVM_THREADS) / KVM_THREADS];
-#pragma unroll
-      for (int i = 0; i < (ADJ_BIAS + KVM_THREADS) / KVM_THREADS; ++i) {
-        const int j = tid() + i * KVM_THREADS;
-        mine[i] = -1;
-        if (j >= nb) continue;
-        const int v = bidx[j];
-        if (v < A.v0 || v >= A.v1) continue;
-        float s = 0.f;
-        bool first = true;
-        for (int k = 0; k < nb; ++k)
-          if (bidx[k] == v) { first = first && k >= j; s += A.bval.f()[(long long)r * A.bval.cols + k]; }
-        bsum[j] = s;
-        if (first) mine[i] = v;
-      }
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < (ADJ_BIAS + KVM_THREADS) / KVM_THREADS; ++i) if (tid() + i * KVM_THREADS < nb) bidx[tid() + i * KVM_THREADS] = mine[i];
-    }
     for (int c0 = A.v0; c0 < A.v1; c0 += ADJ_CHUNK) {
       const int len = min(A.v1 - c0, ADJ_CHUNK);
       const GLOBAL char* xp = (const GLOBAL char*)A.x.p + ((long long)r * A.x.cols + c0) * (xh ? 2 : 4);
@@ -801,27 +868,59 @@ __device__ __noinline__ void op_logits_adjust(const Ctx& c) {
       // vectors start where bf16 storage is 4-byte aligned, on both sides; rows that never are go one by one
       const int px = xh ? (int)((uintptr_t)xp >> 1) & 1 : 0, po = oh ? (int)((uintptr_t)op >> 1) & 1 : 0;
       const int peel = min(len, max(px, po)), nv = xh && oh && px != po ? 0 : (len - peel) / 4;
+      const bool whole = ((c0 + peel) & 3) == 0;                       // no vector's mask bits lie in two words
       LDS uint32_t* w = cnt + (4 - peel) % 4;                          // word of logit c0 + i: w[i], a vector's at 16 bytes
       const __amdgpu_buffer_rsrc_t ro = wt_rsrc((const char*)op, (long long)len * (oh ? 2 : 4));
+      u32x4_t x[NB];
+      uint32_t m0[NB], m1[NB];
+      auto request = [&](int q0) {
+#pragma unroll
+        for (int u = 0; u < NB; ++u) {
+          const int i = peel + 4 * min(q0 + u * KVM_THREADS, nv - 1), v = c0 + i;
+          if (xh) { const u32x2_t t = *(const GLOBAL u32x2a4*)(xp + 2 * i); x[u].x = t.x; x[u].y = t.y; }
+          else x[u] = *(const GLOBAL u32x4a4*)(xp + 4 * i);
+          m0[u] = m1[u] = ~0u;
+          if (mask) { m0[u] = mask[v >> 5]; if (!whole) m1[u] = mask[(v + 3) >> 5]; }
+        }
+      };
+      if (tid() < nv) request(tid());
       __syncthreads();
       for (int i = tid(); i < (len + 11) / 4; i += KVM_THREADS) ((LDS u32x4_t*)cnt)[i] = u32x4_t{0, 0, 0, 0};
       __syncthreads();
-      for (int j = tid(); j < nb; j += KVM_THREADS) {
-        const int v = bidx[j] - c0;
-        if (v >= 0 && v < len) __hip_atomic_fetch_or(&w[v], (uint32_t)(j + 1) << 20, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+      if (nb) {
+        for (int j = tid(); j < nb; j += KVM_THREADS) {
+          const int v = bidx[j] - c0;
+          if (v >= 0 && v < len) __hip_atomic_fetch_max(&w[v], (uint32_t)(ADJ_BIAS - j) << 20, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+        }
+        __syncthreads();
+        bool many = false;
+        for (int j = tid(); j < nb; j += KVM_THREADS) {
+          const int v = bidx[j] - c0, first = v >= 0 && v < len ? ADJ_BIAS - (int)(w[v] >> 20) : j;
+          bsum[j] = A.bval.f()[(long long)r * A.bval.cols + j];
+          later[j] = first == j ? -1 : first;
+          many = many || first != j;
+        }
+        if (__syncthreads_or(many) && wave() == 0)                     // entries of one token, in list order
+          for (int j0 = 0; j0 < nb; j0 += 64) {
+            const int mine = j0 + lane() < nb ? later[j0 + lane()] : -1;
+            for (uint64_t left = __ballot(mine >= 0); left; left &= left - 1) {
+              const int j = __ffsll((long long)left) - 1, to = __builtin_amdgcn_readlane(mine, j);
+              if (lane() == 0) bsum[to] += bsum[j0 + j];
+            }
+          }
       }
       auto said = [&](int k, int token) {
         const int v = token - c0;
         if (v < 0 || v >= len) return;
-        if (k < pl) __hip_atomic_fetch_or(&w[v], 0x80000000u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+        if (k < pl) lds_or(&w[v], 0x80000000u);
         else __hip_atomic_fetch_add(&w[v], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
       };
-      for (int k0 = 4 * tid(); k0 < n / 4 * 4; k0 += 4 * NB * KVM_THREADS) {
-        u32x4_t h[NB];
+      for (int k0 = 4 * tid(); k0 < n / 4 * 4; k0 += 16 * KVM_THREADS) {
+        u32x4_t h[4];
 #pragma unroll
-        for (int u = 0; u < NB; ++u) h[u] = *(const GLOBAL u32x4a4*)(hist + min(k0 + 4 * u * KVM_THREADS, n / 4 * 4 - 4));
+        for (int u = 0; u < 4; ++u) h[u] = *(const GLOBAL u32x4a4*)(hist + min(k0 + 4 * u * KVM_THREADS, n / 4 * 4 - 4));
 #pragma unroll
-        for (int u = 0; u < NB; ++u) {
+        for (int u = 0; u < 4; ++u) {
           const int k = k0 + 4 * u * KVM_THREADS;
           if (k >= n / 4 * 4) break;
 #pragma unroll
@@ -832,31 +931,29 @@ __device__ __noinline__ void op_logits_adjust(const Ctx& c) {
       if (tid() == 4) said(n, last);
       __syncthreads();
       for (int q0 = tid(); q0 < nv; q0 += NB * KVM_THREADS) {
-        u32x4_t x[NB];
-        uint64_t bits[NB];
+        f32x4n y[NB];
+        uint32_t bits[NB];
 #pragma unroll
         for (int u = 0; u < NB; ++u) {
-          const int i = peel + 4 * min(q0 + u * KVM_THREADS, nv - 1);
-          if (xh) { const u32x2_t t = *(const GLOBAL u32x2a4*)(xp + 2 * i); x[u] = u32x4_t{t.x << 16, t.x & 0xffff0000u, t.y << 16, t.y & 0xffff0000u}; }
-          else x[u] = *(const GLOBAL u32x4a4*)(xp + 4 * i);
-          const int v = c0 + i;
-          bits[u] = ~0ull;
-          if (mask) bits[u] = (((uint64_t)(uint32_t)mask[(v + 3) >> 5] << 32) | (uint32_t)mask[v >> 5]) >> (v & 31);
+          const int sh = (c0 + peel + 4 * (q0 + u * KVM_THREADS)) & 31;
+          if (xh) y[u] = __builtin_bit_cast(f32x4n, u32x4_t{x[u].x << 16, x[u].x & 0xffff0000u, x[u].y << 16, x[u].y & 0xffff0000u});
+          else y[u] = __builtin_bit_cast(f32x4n, x[u]);
+          bits[u] = (uint32_t)((((uint64_t)m1[u] << 32) | m0[u]) >> sh);
         }
+        if (q0 + NB * KVM_THREADS < nv) request(q0 + NB * KVM_THREADS);
 #pragma unroll
         for (int u = 0; u < NB; ++u) {
           const int q = q0 + u * KVM_THREADS, i = peel + 4 * q;
           if (q >= nv) break;
-          f32x4n y = __builtin_bit_cast(f32x4n, x[u]);
           const u32x4_t t = *(const LDS u32x4_t*)(w + i);
           if (t.x | t.y | t.z | t.w) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) y[e] = adjusted(y[e], t[e], rep, freq, pres, bsum);
+            for (int e = 0; e < 4; ++e) y[u][e] = adjusted(y[u][e], t[e], rep, freq, pres, bsum);
           }
 #pragma unroll
-          for (int e = 0; e < 4; ++e) if (!((bits[u] >> e) & 1)) y[e] = -INFINITY;
-          if (oh) stwt_bf4_buf(ro, 2 * i, y);
-          else stwt_buf(ro, 4 * i, y);
+          for (int e = 0; e < 4; ++e) if (!((bits[u] >> e) & 1)) y[u][e] = -INFINITY;
+          if (oh) stwt_bf4_buf(ro, 2 * i, y[u]);
+          else stwt_buf(ro, 4 * i, y[u]);
         }
       }
       for (int k = tid(); k < len - 4 * nv; k += KVM_THREADS) {         // before the first vector and behind the last
