@@ -357,89 +357,37 @@ __device__ __noinline__ bool op_kv_append_q8_fast(const Ctx& c) {
   return true;
 }
 
-// Arguments of op 313; R = n * G query rows of a task, row r = i * G + g is token i of head kvh * G + g.
+// Arguments of op 313. A pair is a sequence and a kv head; its R = n * G query rows: row r = i * G + g is token i of head kvh * G + g.
 struct DecodeQ8 {
   View q, kq, ks, vq, vs, kt, vt, lens, part, o, cnt, qg;
-  int b, kvh, s, S, n, H, Hkv, hd, blk, G, R, L;
+  int b0, b1, s, S, n, H, Hkv, hd, blk, G, R;
   float scale, theta, eps;
   __device__ explicit DecodeQ8(const Ctx& c)
       : q(c.buf(0)), kq(c.buf(1)), ks(c.buf(2)), vq(c.buf(3)), vs(c.buf(4)), kt(c.buf(5)), vt(c.buf(6)), lens(c.buf(7)), part(c.buf(8)), o(c.buf(9)),
-        cnt(c.buf(10)), qg(c.buf(11)), b(c.i(12)), kvh(c.i(13)), s(c.i(14)), S(c.i(15)), n(c.i(16)), H(c.i(17)), Hkv(c.i(18)), hd(c.i(19)), blk(c.i(20)),
-        scale(c.f(21)), theta(c.f(22)), eps(c.f(23)) { G = H / Hkv; R = n * G; L = lens.i()[b]; }
-  __device__ long long q_at(int r) const { return ((long long)b * n + r / G) * q.cols + (kvh * G + r % G) * hd; }
-  __device__ long long o_at(int r) const { return ((long long)b * n + r / G) * o.cols + (kvh * G + r % G) * hd; }
-  // This split's partial of row r: unnormalised P V, then the maximum and the sum.
-  __device__ long long part_at(int split, int r) const { return ((((long long)b * S + split) * H + kvh * G) * n + r) * part.cols; }
-  // false: nothing to do (a length out of range is reported; a slot that serves no sequence gives zeros).
-  __device__ bool begin(const Ctx& c) const {
-    if (L < -1 || (long long)L + n > (long long)blk * ks.cols) { if (tid() == 0) c.fail(KVM_ERR_OP_KVLEN, b, L); return false; }
-    if (L >= 0) return true;
-    if (s == 0) for (int e = tid(); e < R * hd; e += KVM_THREADS) o.st(o_at(e / hd) + e % hd, 0.f);
+        cnt(c.buf(10)), qg(c.buf(11)), b0(c.i(12)), b1(c.i(13)), s(c.i(14)), S(c.i(15)), n(c.i(16)), H(c.i(17)), Hkv(c.i(18)), hd(c.i(19)), blk(c.i(20)),
+        scale(c.f(21)), theta(c.f(22)), eps(c.f(23)) { G = H / Hkv; R = n * G; }
+  __device__ long long at(const View& X, int b, int h, int r) const { return ((long long)b * n + r / G) * X.cols + (h * G + r % G) * hd; }
+  __device__ bool length_ok(const Ctx& c, int b, int L) const {
+    if (L >= -1 && (long long)L + n <= (long long)blk * ks.cols) return true;
+    c.fail(KVM_ERR_OP_KVLEN, b, L);
     return false;
   }
+  __device__ void zeros(int b, int h) const { for (int e = tid(); e < R * hd; e += KVM_THREADS) o.st(at(o, b, h, e / hd) + e % hd, 0.f); }
 };
-// The split that counts itself last merges the `live` splits' partials; maxima are in units of log2. A wave takes a row at a time:
-// lane i has the maximum and sum of split i, the weights go from there to all lanes, which add up to two head dims each, the loads
-// of 16 splits in flight.
-__device__ __forceinline__ void q8_arrive(const Ctx& c, const DecodeQ8& D, int live, LDS int* flag) {
-  wait_stores();
-  __syncthreads();
-  GLOBAL int* cnt = D.cnt.i() + ((long long)D.b * D.Hkv + D.kvh);
-  if (tid() == 0) *flag = add_relaxed((int*)cnt, 1);
-  __syncthreads();
-  const int old = *flag;
-  if (old < 0 || old >= live) { if (tid() == 0) c.fail(KVM_ERR_OP_RANGE, D.b * D.Hkv + D.kvh, old); return; }
-  if (old != live - 1) return;
-  fence_acquire();                                                     // the other splits' partials, stored before their counts
-  constexpr int SB = 16;
-  const int l = lane(), hd = D.hd, d0 = min(l, hd - 1), d1 = min(l + 64, hd - 1);
-  const long long step = D.part_at(1, 0) - D.part_at(0, 0);
-  for (int r = wave(); r < D.R; r += KVM_WAVES) {
-    const GLOBAL float* base = D.part.f() + D.part_at(0, r);
-    float M = -INFINITY, a0 = 0.f, a1 = 0.f, z = 0.f;
-    for (int s0 = 0; s0 < live; s0 += 64) {
-      const bool mine = s0 + l < live;
-      const GLOBAL float* y = base + (long long)min(s0 + l, live - 1) * step;
-      const float m = mine ? y[hd] : -INFINITY, x = mine ? y[hd + 1] : 0.f;
-      const float top = fmaxf(M, wave_max(m)), f = M == -INFINITY ? 0.f : exp2f(M - top), e = m == -INFINITY ? 0.f : exp2f(m - top);
-      z = z * f + e * x; a0 *= f; a1 *= f; M = top;
-      for (int s1 = 0; s1 < 64 && s0 + s1 < live; s1 += SB) {
-        float x0[SB], x1[SB];
-#pragma unroll
-        for (int i = 0; i < SB; ++i) {
-          const GLOBAL float* w = base + (long long)min(s0 + s1 + i, live - 1) * step;
-          x0[i] = w[d0]; x1[i] = w[d1];
-        }
-#pragma unroll
-        for (int i = 0; i < SB; ++i) {
-          const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(e), s1 + i));
-          if (s0 + s1 + i < live) { a0 += w * x0[i]; a1 += w * x1[i]; }
-        }
-      }
-    }
-    z = wave_sum(z);
-    if (l < hd) D.o.st(D.o_at(r) + l, a0 / z);
-    if (l + 64 < hd) D.o.st(D.o_at(r) + l + 64, a1 / z);
-  }
-  if (tid() == 0) st_relaxed((int*)cnt, 0);
-}
 
-// Decode attention over the 8-bit cache, any alignment and head size: 256 tokens at a time, a thread to a token for the scores
-// and to an output element for P V, each row with its running maximum and sum.
-__device__ __noinline__ void op_attn_decode_q8(const Ctx& c) {
-  const DecodeQ8 D(c);
-  if (!D.begin(c)) return;
+// Decode attention over the 8-bit cache, any alignment and head size: whole pairs, every S-th one; 256 tokens at a time, a thread
+// to a token for the scores and to an output element for P V, each row with its running maximum and sum.
+__device__ __forceinline__ void attn_q8_pair(const Ctx& c, const DecodeQ8& D, int b, int kvh, int L) {
   constexpr float LOG2E = 1.44269504088896340736f;
-  const int n = D.L + D.n, whole = n / D.blk * D.blk, live = min(D.S, (n + 255) / 256);
-  if (D.s >= live) return;
-  const int per = ((n + live - 1) / live + 255) / 256 * 256, j0 = min(n, D.s * per), j1 = min(n, j0 + per);
+  const int n = L + D.n, whole = n / D.blk * D.blk;
+  __syncthreads();
   LDS float* q = (LDS float*)c.smem;                                   // [32][128]
   LDS float* p = q + 32 * 128;                                         // [32][256]
   LDS float* st = p + 32 * 256;                                        // [32] factors of the last step, then flags and sums
   LDS float* red = st + 32;
   const int hd = D.hd, half = hd / 2;
   for (int r = 0; r < D.R; ++r) {
-    for (int k = tid(); k < hd; k += KVM_THREADS) q[r * hd + k] = D.q.ld(D.q_at(r) + k);
+    for (int k = tid(); k < hd; k += KVM_THREADS) q[r * hd + k] = D.q.ld(D.at(D.q, b, kvh, r) + k);
     __syncthreads();
     if (D.qg.ok()) {
       float ss = 0.f;
@@ -450,13 +398,13 @@ __device__ __noinline__ void op_attn_decode_q8(const Ctx& c) {
     }
     if (D.theta > 0.f)
       for (int i = tid(); i < half; i += KVM_THREADS) {
-        float sn, co; q8_turn(D.L + r / D.G, q8_freq(i, hd, log((double)D.theta)), sn, co);
+        float sn, co; q8_turn(L + r / D.G, q8_freq(i, hd, log((double)D.theta)), sn, co);
         const float x1 = q[r * hd + i], x2 = q[r * hd + i + half];
         q[r * hd + i] = x1 * co - x2 * sn; q[r * hd + i + half] = x1 * sn + x2 * co;
       }
   }
   __syncthreads();
-  const long long pair = (long long)D.b * D.Hkv + D.kvh, bytes0 = pair * D.ks.cols * D.blk * hd;
+  const long long pair = (long long)b * D.Hkv + kvh, bytes0 = pair * D.ks.cols * D.blk * hd;
   const GLOBAL signed char* K = (const GLOBAL signed char*)D.kq.p + bytes0;
   const GLOBAL signed char* V = (const GLOBAL signed char*)D.vq.p + bytes0;
   float acc[16];                                                       // of rows tid / hd, + 256 / hd, .. (hd < 16: some of them)
@@ -464,12 +412,12 @@ __device__ __noinline__ void op_attn_decode_q8(const Ctx& c) {
   LDS float* m_run = red + 16; LDS float* l_run = m_run + 32;
   for (int r = tid(); r < D.R; r += KVM_THREADS) { m_run[r] = -INFINITY; l_run[r] = 0.f; }
   for (int i = 0; i < 16; ++i) acc[i] = 0.f;
-  for (int t0 = j0; t0 < j1; t0 += KVM_THREADS) {
-    const int t = t0 + tid(), cnt = min(j1 - t0, KVM_THREADS);
+  for (int t0 = 0; t0 < n; t0 += KVM_THREADS) {
+    const int t = t0 + tid(), cnt = min(n - t0, KVM_THREADS);
     __syncthreads();
     for (int r = 0; r < D.R; ++r) {
       float a = -INFINITY;
-      if (t < j1 && t <= D.L + r / D.G) {
+      if (t < n && t <= L + r / D.G) {
         a = 0.f;
         if (t < whole) {
           for (int k = 0; k < hd; ++k) a += q[r * hd + k] * (float)K[(long long)t * hd + k];
@@ -491,7 +439,7 @@ __device__ __noinline__ void op_attn_decode_q8(const Ctx& c) {
         float a = acc[i] * st[r];
         for (int u = 0; u < cnt; ++u) {
           const int tt = t0 + u;
-          if (tt > D.L + r / D.G) break;
+          if (tt > L + r / D.G) break;
           const float v = tt < whole ? (float)V[(long long)(tt / D.blk) * D.blk * hd + d * D.blk + tt % D.blk] * D.vs.f()[pair * D.vs.cols + tt / D.blk]
                                      : D.vt.at(pair * D.blk + tt - whole, d);
           a += p[r * KVM_THREADS + u] * v;
@@ -504,12 +452,131 @@ __device__ __noinline__ void op_attn_decode_q8(const Ctx& c) {
     for (int i = 0; i < 16; ++i) {
       const int r = ra + i * rows;
       if (r >= D.R) break;
-      if (live == 1) { D.o.st(D.o_at(r) + d, acc[i] / l_run[r]); continue; }
-      GLOBAL float* x = D.part.f() + D.part_at(D.s, r);
-      stwt32(x + d, acc[i]);
-      if (d == 0) { stwt32(x + hd, m_run[r]); stwt32(x + hd + 1, l_run[r]); }
+      D.o.st(D.at(D.o, b, kvh, r) + d, acc[i] / l_run[r]);
     }
-  if (live > 1) q8_arrive(c, D, live, (LDS int*)st);
+}
+__device__ __noinline__ void op_attn_decode_q8(const Ctx& c) {
+  const DecodeQ8 D(c);
+  for (int p = D.s; p < (D.b1 - D.b0) * D.Hkv; p += D.S) {
+    const int b = D.b0 + p / D.Hkv, h = p % D.Hkv, L = D.lens.i()[b];
+    if (L == -1) D.zeros(b, h);
+    else if (L >= -1 && (long long)L + D.n <= (long long)D.blk * D.ks.cols) attn_q8_pair(c, D, b, h, L);
+    else { if (tid() == 0) D.length_ok(c, b, L); return; }
+  }
+}
+
+// ---- The work of a call over its tasks: every pair costs Q8_PAIR (query rows, the unfinished block, the end) and one per unit of 64
+// tokens of its whole blocks; the pairs in order, by sequence and head, are cut into equal shares, in the tasks alike from the
+// lengths. A cut within Q8_SNAP of a pair's end moves there: a small piece costs more than it balances. A pair that is cut has one piece in
+// each of consecutive tasks; the first has the unfinished block.
+constexpr int Q8_PAIR = 8, Q8_SNAP = 12, Q8_SHARE = 24, Q8_SEQS = 1024;
+// (32 bits are enough: a unit is 4 KB and more of cache, whose buffers hold less than 2^33 bytes.)
+struct WorkQ8 {
+  const LDS int* pre;          // [seqs + 1] cost of the sequences before, for one head
+  int seqs, Hkv, share, total;
+  // The pair at x: its sequence and head, where it starts, its cost.
+  struct At { int b, h, start, cost; };
+  __device__ __forceinline__ At find(int x) const {
+    int b = 0;
+    for (int j0 = 0; j0 < seqs; j0 += 64) b += __popcll(__ballot(j0 + lane() < seqs && pre[j0 + lane()] * Hkv <= x));
+    b = rfl(b) - 1;
+    const int p0 = rfl(pre[b]), cost = rfl(pre[b + 1]) - p0, h = (int)((unsigned)(x - p0 * Hkv) / (unsigned)cost);
+    return At{b, h, p0 * Hkv + h * cost, cost};
+  }
+  // Where task i starts.
+  __device__ __forceinline__ int cut(int i) const {
+    const int x = (int)min((long long)i * share, (long long)total);
+    if (x == total) return total;
+    const At a = find(x);
+    const int off = x - a.start;
+    return off < Q8_SNAP ? a.start : a.cost - off < Q8_SNAP ? a.start + a.cost : x;
+  }
+  // The first task that starts inside the pair, and how many do.
+  __device__ __forceinline__ int first_inside(const At& a) const { return (int)((unsigned)(a.start + Q8_SNAP + share - 1) / (unsigned)share); }
+  __device__ __forceinline__ int inside(const At& a) const {
+    if (a.cost < 2 * Q8_SNAP) return 0;
+    return max(0, (int)((unsigned)(a.start + a.cost - Q8_SNAP + share) / (unsigned)share) - first_inside(a));
+  }
+};
+// Lengths and cost sums of the call's sequences into LDS; false if a length is out of range (reported).
+__device__ __forceinline__ bool q8_work(const Ctx& c, const DecodeQ8& D, LDS int* pre, LDS int* len, LDS int* tot, WorkQ8& W) {
+  constexpr int PER = Q8_SEQS / KVM_THREADS;
+  const int seqs = D.b1 - D.b0;
+  int cost[PER], sum = 0;
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int k = tid() * PER + i;
+    cost[i] = 0;
+    if (k < seqs) {
+      const int L = D.lens.i()[D.b0 + k];
+      bad = bad || !D.length_ok(c, D.b0 + k, L);
+      len[k] = L;
+      cost[i] = L < 0 ? 1 : Q8_PAIR + (int)(((((unsigned)L + D.n) & -(unsigned)D.blk) + 63) >> 6);
+      sum += cost[i];
+    }
+  }
+  int upto = sum;
+  for (int o = 1; o < 64; o <<= 1) { const int y = __shfl_up(upto, o, 64); if (lane() >= o) upto += y; }
+  if (lane() == 63) tot[wave()] = upto;
+  if (__syncthreads_or(bad)) return false;
+  int at = upto - sum;
+  for (int w = 0; w < KVM_WAVES; ++w) at += w < wave() ? tot[w] : 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int k = tid() * PER + i;
+    if (k < seqs) { pre[k] = at; at += cost[i]; if (k == seqs - 1) pre[seqs] = at; }
+  }
+  __syncthreads();
+  W.pre = pre; W.seqs = seqs; W.Hkv = D.Hkv;
+  W.total = rfl(pre[seqs]) * D.Hkv;
+  // equal shares, but none below Q8_SHARE unless there are tasks enough for a pair each
+  W.share = max((int)((unsigned)(W.total + D.S - 1) / (unsigned)D.S), min(Q8_SHARE, (int)((unsigned)(W.total + seqs * D.Hkv - 1) / (unsigned)(seqs * D.Hkv))));
+  return true;
+}
+// The piece of a pair that counts itself last merges them; maxima are in units of log2. Piece k lies in the partials of task i0 + k - 1,
+// the first one in their second half. A wave takes a row at a time: lane i has the maximum and sum of piece i, the weights go from
+// there to all lanes, which add up to two head dims each, the loads of 16 pieces in flight.
+__device__ __forceinline__ void q8_arrive(const Ctx& c, const DecodeQ8& D, int b, int h, int i0, int live, LDS int* flag) {
+  wait_stores();
+  __syncthreads();
+  GLOBAL int* cnt = D.cnt.i() + ((long long)b * D.Hkv + h);
+  if (tid() == 0) *flag = add_relaxed((int*)cnt, 1);
+  __syncthreads();
+  const int old = *flag;
+  if (old < 0 || old >= live) { if (tid() == 0) c.fail(KVM_ERR_OP_RANGE, b * D.Hkv + h, old); return; }
+  if (old != live - 1) return;
+  fence_acquire();                                                     // the other pieces' partials, stored before their counts
+  constexpr int SB = 16;
+  const int l = lane(), hd = D.hd, d0 = min(l, hd - 1), d1 = min(l + 64, hd - 1);
+  for (int r = wave(); r < D.R; r += KVM_WAVES) {
+    auto piece = [&](int k) { return D.part.f() + ((long long)(2 * i0 - 2 + (k ? 2 * k : 1)) * D.R + r) * D.part.cols; };
+    float M = -INFINITY, a0 = 0.f, a1 = 0.f, z = 0.f;
+    for (int s0 = 0; s0 < live; s0 += 64) {
+      const bool mine = s0 + l < live;
+      const GLOBAL float* y = piece(min(s0 + l, live - 1));
+      const float m = mine ? y[hd] : -INFINITY, x = mine ? y[hd + 1] : 0.f;
+      const float top = fmaxf(M, rows_max(lanes_max<16>(m))), f = M == -INFINITY ? 0.f : exp2f(M - top), e = m == -INFINITY ? 0.f : exp2f(m - top);
+      z = z * f + e * x; a0 *= f; a1 *= f; M = top;
+      for (int s1 = 0; s1 < 64 && s0 + s1 < live; s1 += SB) {
+        float x0[SB], x1[SB];
+#pragma unroll
+        for (int i = 0; i < SB; ++i) {
+          const GLOBAL float* w = piece(min(s0 + s1 + i, live - 1));
+          x0[i] = w[d0]; x1[i] = w[d1];
+        }
+#pragma unroll
+        for (int i = 0; i < SB; ++i) {
+          const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(e), s1 + i));
+          if (s0 + s1 + i < live) { a0 += w * x0[i]; a1 += w * x1[i]; }
+        }
+      }
+    }
+    z = rows_sum(lanes_sum<16>(z));
+    if (l < hd) D.o.st(D.at(D.o, b, h, r) + l, a0 / z);
+    if (l + 64 < hd) D.o.st(D.at(D.o, b, h, r) + l + 64, a1 / z);
+  }
+  if (tid() == 0) st_relaxed((int*)cnt, 0);
 }
 
 // Decode attention over the 8-bit cache at head sizes 64 and 128, on the matrix units. Bound: streaming the cache's bytes.
@@ -524,7 +591,7 @@ __device__ __noinline__ void op_attn_decode_q8(const Ctx& c) {
 // to 2^12, so that no remainder that matters falls below f16's numbers), two products each, summed in f32. A block's key
 // scale multiplies its scores; its value scale the probabilities, relative to the largest so far (vref, a power of two).
 // Each unit's P V is summed on its own and added to the running one in f32 (the units' chained sums round towards -inf).
-// The unfinished block is f32 work of all lanes in the last split: at most blk - 1 tokens.
+// The unfinished block is f32 work of all lanes: at most blk - 1 tokens.
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 // Eight signed bytes (two words) as f16.
@@ -539,27 +606,32 @@ __device__ __forceinline__ f16x8 q8_half(uint32_t w0, uint32_t w1) {
   return r;
 }
 template <int HD> struct UnitQ8 { u32x4_t k[4][HD / 64], v[HD / 16]; float ks, vs; };
-template <int HD, int NT> __device__ __noinline__ void attn_q8_t(const Ctx& c) {
+// LDS of a task. The work and the frequencies stay through its pieces; the tail's scores and values give way to the waves' P V.
+template <int HD> struct DecodeLds {
+  LDS int* pre; LDS int* len; LDS double* freq; LDS float* qs; LDS float* to; LDS float* st; LDS float* cr; LDS float* ts; LDS float* tv;
+  __device__ explicit DecodeLds(LDS char* p)
+      : pre((LDS int*)p),                                              // [Q8_SEQS + 1]
+        len(pre + Q8_SEQS + 4),                                        // [Q8_SEQS]
+        freq((LDS double*)(len + Q8_SEQS)),                            // [HD / 2]
+        qs((LDS float*)(freq + HD / 2)),                               // [32][HD + 4] queries
+        to(qs + 32 * (HD + 4)),                                        // [32][HD] the tail's P V
+        st(to + 32 * HD),                                              // [5][2][32] maxima and sums of the waves and the tail
+        cr(st + 320),                                                  // [32] factors from a product to a score
+        ts(cr + 32),                                                   // [32][128] the tail's scores
+        tv(ts + 32 * 128) {}                                           // [128][HD] its values
+  static_assert((2 * Q8_SEQS + 4 + HD + 32 * (HD + 4) + 32 * HD + 352 + 32 * 128 + 128 * HD) * 4 <= KVM_LDS_BYTES, "decode attention LDS map");
+};
+// One piece of a pair: units [u0, u1), with `first` also the unfinished block; `live` pieces in all, piece 1 in task i0's partials.
+template <int HD, int NT> __device__ __noinline__ void attn_q8_piece(const Ctx& c, int b, int kvh, int L, int u0, int u1, bool first, int i0, int live) {
   constexpr float LOG2E = 1.44269504088896340736f, PS = 4096.f;
   constexpr int KH = HD / 64, VT = HD / 16, LPR = HD / 8, RPP = KVM_THREADS / LPR, QS = HD + 4;
+  const DecodeLds<HD> M(c.smem);
+  LDS float *const qs = M.qs, *const to = M.to, *const st = M.st, *const cr = M.cr, *const ts = M.ts, *const tv = M.tv;
   const DecodeQ8 D(c);
-  if (!D.begin(c)) return;
-  const int n = D.L + D.n, blk = rfl(D.blk), lb = 31 - __clz(blk), whole = rfl(n & -blk), nt = n - whole;
-  const int units = (whole + 63) >> 6, live = min(D.S, max(1, units));
-  if (D.s >= live) return;
-  const int u0 = (int)(((long long)D.s * units + live - 1) / live), u1 = (int)(((long long)(D.s + 1) * units + live - 1) / live);
-  const bool tail = D.s == live - 1 && nt > 0;
+  const int blk = rfl(D.blk), lb = 31 - __clz(blk), n = L + D.n, whole = n & -blk, nt = first ? n - whole : 0;
+  const bool tail = nt > 0;
   const int l = lane(), w = wave(), nn = l & 15, qq = l >> 4, ln = tid() % LPR, rw = tid() / LPR;
-  // LDS: queries, the tail's P V and its stats stay; the tail's scores and values give way to the waves' P V at the end
-  LDS float* qs = (LDS float*)c.smem;                                  // [32][HD + 4]
-  LDS float* to = qs + 32 * QS;                                        // [32][HD]
-  LDS float* st = to + 32 * HD;                                        // [5][2][32] maxima and sums of the waves and the tail
-  LDS float* cr = st + 320;                                            // [32] factors from a product to a score
-  LDS double* freq = (LDS double*)(cr + 32);                           // [HD / 2]
-  LDS float* ts = (LDS float*)(freq + HD / 2);                         // [32][128]
-  LDS float* tv = ts + 32 * 128;                                       // [128][HD]
-  static_assert((32 * (HD + 4) + 32 * HD + 352 + HD + 32 * 128 + 128 * HD) * 4 <= KVM_LDS_BYTES, "decode attention LDS map");
-  const long long pair = (long long)D.b * D.Hkv + D.kvh, byte0 = pair * D.ks.cols * blk * HD;
+  const long long pair = (long long)b * D.Hkv + kvh, byte0 = pair * D.ks.cols * blk * HD;
   const GLOBAL char* K = (const GLOBAL char*)D.kq.p + byte0;
   const GLOBAL char* V = (const GLOBAL char*)D.vq.p + byte0;
   const GLOBAL float* KS = D.ks.f() + pair * D.ks.cols;
@@ -581,7 +653,7 @@ template <int HD, int NT> __device__ __noinline__ void attn_q8_t(const Ctx& c) {
   constexpr int QP = (16 * NT + RPP - 1) / RPP, TP = 4;
   Raw8 rq[QP], rk[TP], rv[TP];
 #pragma unroll
-  for (int i = 0; i < QP; ++i) if (i * RPP + rw < D.R) rq[i].load(D.q, D.q_at(i * RPP + rw) + 8 * ln);
+  for (int i = 0; i < QP; ++i) if (i * RPP + rw < D.R) rq[i].load(D.q, D.at(D.q, b, kvh, i * RPP + rw) + 8 * ln);
   auto load_tail = [&](int t0) {
 #pragma unroll
     for (int i = 0; i < TP; ++i) {
@@ -592,8 +664,6 @@ template <int HD, int NT> __device__ __noinline__ void attn_q8_t(const Ctx& c) {
   if (tail) load_tail(0);
   UnitQ8<HD> U;
   if (u0 + w < u1) load(U, u0 + w);
-  if (D.theta > 0.f && tid() < HD / 2) freq[tid()] = q8_freq(tid(), HD, log((double)D.theta));
-  __syncthreads();
   // query rows: norm, rotation, then scaled so that the largest magnitude of a row lies in [2^10, 2^11)
 #pragma unroll
   for (int i = 0; i < QP; ++i) {
@@ -602,7 +672,7 @@ template <int HD, int NT> __device__ __noinline__ void attn_q8_t(const Ctx& c) {
     float x[8] = {};
     if (r < D.R) {
       rq[i].get(D.q.dtype == 2, x);
-      head8_turn<HD>(x, D.qg.ok() ? D.qg.f() : nullptr, D.eps, D.theta > 0.f ? freq : nullptr, D.L + r / D.G, ts + rw * HD);
+      head8_turn<HD>(x, D.qg.ok() ? D.qg.f() : nullptr, D.eps, D.theta > 0.f ? M.freq : nullptr, L + r / D.G, ts + rw * HD);
     }
     float big = 0.f;
 #pragma unroll
@@ -633,7 +703,7 @@ template <int HD, int NT> __device__ __noinline__ void attn_q8_t(const Ctx& c) {
         float q[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) q[e] = qs[r * QS + 8 * ln + e];
-        const int seen = min(nt, D.L + r / D.G + 1 - whole);
+        const int seen = min(nt, L + r / D.G + 1 - whole);
 #pragma unroll
         for (int i = 0; i < TP; ++i) {
           const int t = t0 + i * RPP + rw;
@@ -655,15 +725,19 @@ template <int HD, int NT> __device__ __noinline__ void attn_q8_t(const Ctx& c) {
       if (l == 0) { st[256 + r] = m; st[288 + r] = z; }
     }
     __syncthreads();
-    for (int r = tid() / HD; r < D.R; r += KVM_THREADS / HD) {
-      const int d = tid() % HD, seen = min(nt, D.L + r / D.G + 1 - whole);   // a value that the row may not see does not count, NaN neither
-      float a[4] = {0.f, 0.f, 0.f, 0.f};
-      int t = 0;
-      for (; t + 8 <= seen; t += 8)
+    constexpr int RB = 2 * KVM_THREADS / HD;                           // two rows a thread, RB in all
+    for (int r0 = tid() / HD; r0 < D.R; r0 += RB) {
+      const int d = tid() % HD, r1 = min(r0 + RB / 2, D.R - 1);
+      const int s0 = min(nt, L + r0 / D.G + 1 - whole), s1 = min(nt, L + r1 / D.G + 1 - whole);   // values not to be seen do not count, NaN neither
+      float a[2][4] = {};
+      for (int t = 0; t < s1; t += 8)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) a[e % 4] += ts[r * 128 + t + e] * tv[(t + e) * HD + d];
-      for (; t < seen; ++t) a[0] += ts[r * 128 + t] * tv[t * HD + d];
-      to[r * HD + d] = (a[0] + a[1]) + (a[2] + a[3]);
+        for (int e = 0; e < 8; ++e) {
+          const float x = tv[(t + e) * HD + d], y0 = ts[r0 * 128 + t + e] * x, y1 = ts[r1 * 128 + t + e] * x;
+          a[0][e % 4] += t + e < s0 ? y0 : 0.f; a[1][e % 4] += t + e < s1 ? y1 : 0.f;
+        }
+      to[r0 * HD + d] = (a[0][0] + a[0][1]) + (a[0][2] + a[0][3]);
+      to[r1 * HD + d] = (a[1][0] + a[1][1]) + (a[1][2] + a[1][3]);
     }
   }
   // the queries as B operands: row nn of tile g, dims 16 (qq + 4 h) + 8 p ..
@@ -685,7 +759,7 @@ template <int HD, int NT> __device__ __noinline__ void attn_q8_t(const Ctx& c) {
           qh[g][h][p][e] = hi; ql[g][h][p][e] = (_Float16)(x - (float)hi);
         }
     crow[g] = cr[r]; mrun[g] = -INFINITY; lrun[g] = 0.f;
-    lim[g] = r < D.R ? min(whole, D.L + r / D.G + 1) : 0;
+    lim[g] = r < D.R ? min(whole, L + r / D.G + 1) : 0;
 #pragma unroll
     for (int d = 0; d < VT; ++d) o[g][d] = f32x4n{0.f, 0.f, 0.f, 0.f};
   }
@@ -792,19 +866,36 @@ template <int HD, int NT> __device__ __noinline__ void attn_q8_t(const Ctx& c) {
       const float m = st[256 + r], f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - M);
       a += f * to[r * HD + d]; z += f * st[288 + r];
     }
-    if (live == 1) { D.o.st(D.o_at(r) + d, a / z); continue; }
-    GLOBAL float* x = D.part.f() + D.part_at(D.s, r);
+    if (live == 1) { D.o.st(D.at(D.o, b, kvh, r) + d, a / z); continue; }
+    GLOBAL float* x = D.part.f() + ((long long)(2 * D.s + first) * D.R + r) * D.part.cols;
     stwt32(x + d, a);
     if (d == 0) { stwt32(x + HD, M); stwt32(x + HD + 1, z); }
   }
-  if (live > 1) q8_arrive(c, D, live, (LDS int*)qs);
+  if (live > 1) q8_arrive(c, D, b, kvh, i0, live, (LDS int*)qs);
+}
+template <int HD> __device__ __forceinline__ void attn_q8_t(const Ctx& c) {
+  const DecodeLds<HD> M(c.smem);
+  const DecodeQ8 D(c);
+  WorkQ8 W;
+  if (!q8_work(c, D, M.pre, M.len, (LDS int*)M.ts, W)) return;
+  if (D.theta > 0.f && tid() < HD / 2) M.freq[tid()] = q8_freq(tid(), HD, log((double)D.theta));
+  const int stop = W.cut(D.s + 1);
+  for (int at = W.cut(D.s); at < stop;) {
+    const WorkQ8::At P = W.find(at);
+    const int off = at - P.start, end = min(P.cost, stop - P.start), L = rfl(M.len[P.b]), b = D.b0 + P.b;
+    at = P.start + end;
+    if (L < 0) { D.zeros(b, P.h); continue; }
+    const bool cut = off > 0 || end < P.cost;
+    const int u0 = max(0, off - Q8_PAIR), u1 = max(0, end - Q8_PAIR), i0 = cut ? W.first_inside(P) : 0, live = cut ? W.inside(P) + 1 : 1;
+    __syncthreads();                                                   // frequencies; the piece before is out of LDS
+    if (D.R > 16) attn_q8_piece<HD, 2>(c, b, P.h, L, u0, u1, off == 0, i0, live);
+    else attn_q8_piece<HD, 1>(c, b, P.h, L, u0, u1, off == 0, i0, live);
+  }
 }
 __device__ __noinline__ bool op_attn_decode_q8_fast(const Ctx& c) {
   if (!rows8_ok(c.buf(0)) || !rows8_ok(c.buf(5)) || !rows8_ok(c.buf(6))) return false;
-  const int hd = c.i(19);
-  const bool two = c.i(16) * (c.i(17) / c.i(18)) > 16;
-  if (hd == 128) { if (two) attn_q8_t<128, 2>(c); else attn_q8_t<128, 1>(c); }
-  else if (hd == 64) { if (two) attn_q8_t<64, 2>(c); else attn_q8_t<64, 1>(c); }
+  if (c.i(19) == 128) attn_q8_t<128>(c);
+  else if (c.i(19) == 64) attn_q8_t<64>(c);
   else return false;
   return true;
 }

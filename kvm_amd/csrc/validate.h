@@ -324,13 +324,13 @@ static void extents(int op, Check& k) {
       k.range(b0, b1); k.need(0 <= h0 && h0 <= h1 && h1 <= Hkv && Hkv > 0 && 0 <= p && p < P && nn > 0, "bad h0/h1/Hkv/p/P/n_new");
       cache_q8(k, b1, Hkv, hd, "kgamma");
       k.ext("knew", (long long)b1 * nn, (long long)Hkv * hd); k.ext("vnew", (long long)b1 * nn, (long long)Hkv * hd); break; }
-    case 313: { const int b = k.I("b"), kvh = k.I("kvh"), s = k.I("s"), S = k.I("S"), nn = k.I("n_new"), H = k.I("H"), Hkv = k.I("Hkv"), hd = k.I("hd");
-      k.need(b >= 0 && Hkv > 0 && H > 0 && H % Hkv == 0 && 0 <= kvh && kvh < Hkv && 0 <= s && s < S, "bad b/kvh/s/S/H/Hkv");
+    case 313: { const int b0 = k.I("b0"), b1 = k.I("b1"), s = k.I("s"), S = k.I("S"), nn = k.I("n_new"), H = k.I("H"), Hkv = k.I("Hkv"), hd = k.I("hd");
+      k.range(b0, b1); k.need((long long)b1 - b0 <= 1024, "at most 1024 sequences a call");
+      k.need(Hkv > 0 && H > 0 && H % Hkv == 0 && 0 <= s && s < S && S <= (1 << 20), "bad s/S/H/Hkv");
       k.need(nn > 0 && (Hkv <= 0 || (long long)nn * (H / Hkv) <= 32), "n_new * H / Hkv must be 1 .. 32");
-      const long long n = (long long)b + 1;
-      cache_q8(k, n, Hkv, hd, "qgamma");
-      k.ext("q", n * nn, (long long)H * hd); k.ext("o", n * nn, (long long)H * hd); k.extn("cnt", n * Hkv);
-      k.ext("part", n * S * H * nn, (long long)hd + 2);
+      cache_q8(k, b1, Hkv, hd, "qgamma");
+      k.ext("q", (long long)b1 * nn, (long long)H * hd); k.ext("o", (long long)b1 * nn, (long long)H * hd); k.extn("cnt", (long long)b1 * Hkv);
+      if (Hkv > 0) k.ext("part", 2ll * S * nn * (H / Hkv), (long long)hd + 2);
       k.need(k.a[k.idx("o")] != k.a[k.idx("q")], "o must not be q");
       k.need(std::isfinite(k.F("scale")), "scale must be finite"); break; }
     case 314: { const int r0 = k.I("r0"), r1 = k.I("r1"), v0 = k.I("v0"), v1 = k.I("v1"), V = k.I("V"); k.range(r0, r1);

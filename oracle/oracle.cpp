@@ -847,13 +847,14 @@ void op_kv_append_q8(const Ctx& c) {
     }
   }
 }
-void op_attn_decode_q8(const Ctx& c) {   // the whole context in the task of split 0: the splits are the device's matter
+void op_attn_decode_q8(const Ctx& c) { // whole pairs, every S-th one: how the device cuts them is its matter
   V q = c.buf(0), kq = c.buf(1), ks = c.buf(2), vq = c.buf(3), vs = c.buf(4), kt = c.buf(5), vt = c.buf(6), lens = c.buf(7), o = c.buf(9), qg = c.buf(11, true);
-  const int b = c.i(12), kvh = c.i(13), s = c.i(14), n = c.i(16), H = c.i(17), Hkv = c.i(18), hd = c.i(19), blk = c.i(20), G = H / Hkv;
+  const int b0 = c.i(12), b1 = c.i(13), s = c.i(14), S = c.i(15), n = c.i(16), H = c.i(17), Hkv = c.i(18), hd = c.i(19), blk = c.i(20), G = H / Hkv;
   const double scale = c.fl(21); const float theta = c.fl(22), eps = c.fl(23);
+  for (int b = b0; b < b1; ++b) if (lens.i[b] < -1 || (long long)lens.i[b] + n > (long long)blk * ks.cols) fail("attn_decode_q8: length");
+  for (int u = s; u < (b1 - b0) * Hkv; u += S) {
+  const int b = b0 + u / Hkv, kvh = u % Hkv;
   const long long L = lens.i[b], pair = (long long)b * Hkv + kvh;
-  if (L < -1 || L + n > (long long)blk * ks.cols) fail("attn_decode_q8: length");
-  if (s) return;
   const long long whole = (L + n) / blk * blk;
   auto at = [&](const V& Q, const V& S, const V& T, bool vals, long long t, int d) -> double {
     if (t >= whole) return T.at(pair * blk + t - whole, d);
@@ -876,6 +877,7 @@ void op_attn_decode_q8(const Ctx& c) {   // the whole context in the task of spl
       double a = 0; for (long long t = 0; t <= L + i; ++t) a += p[t] * at(vq, vs, vt, true, t, d);
       o.st(row * o.cols + col + d, a / l);
     }
+  }
   }
 }
 void op_logits_adjust(const Ctx& c) {

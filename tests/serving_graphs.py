@@ -62,7 +62,7 @@ def append_graph(c, knew, vnew, lens, hkv, n_new, tail='bf16', new='bf16', tasks
     return compiled(b, data)
 
 
-def attend_graph(c, q, lens, hkv, heads, n_new, scale, tail='bf16', qdt='bf16', odt=None, splits=0, gamma=None, theta=0.0, eps=0.0, extra=0):
+def attend_graph(c, q, lens, hkv, heads, n_new, scale, tail='bf16', qdt='bf16', odt=None, tasks=256, gamma=None, theta=0.0, eps=0.0, extra=0):
     b, data = Builder(0), {}
     cache = add_cache(b, data, c, hkv, tail)
     add(b, data, 'q', np.pad(q, ((0, 0), (0, extra))), qdt)
@@ -70,7 +70,7 @@ def attend_graph(c, q, lens, hkv, heads, n_new, scale, tail='bf16', qdt='bf16', 
     add(b, data, 'lens', np.asarray(lens, np.int32)[:, None])
     if gamma is not None:
         add(b, data, 'qgamma', gamma[None])
-    serving.attn_decode_q8(b, cache, 'q', 'o', 'lens', heads, n_new, scale, qgamma=None if gamma is None else 'qgamma', theta=theta, eps=eps, splits=splits)
+    serving.attn_decode_q8(b, cache, 'q', 'o', 'lens', heads, n_new, scale, qgamma=None if gamma is None else 'qgamma', theta=theta, eps=eps, tasks=tasks)
     return compiled(b, data)
 
 
@@ -127,6 +127,10 @@ ATTENDS = [
     (32, 32, 2, 4, 'f32', 2, [0, 62, 300]),
     (16, 100, 1, 3, 'f32', 1, [15, 16, 77]),
     (16, 4, 1, 2, 'f32', 1, [40]),
+    (64, 128, 2, 8, 'f32', 1, [5000, 3, -1, 1800, 9000]),            # pairs that are shared out over tasks, among short ones
+    (16, 64, 1, 8, 'f32', 4, [3000, 100]),
+    (128, 128, 1, 16, 'bf16', 2, [8190, 70]),
+    (16, 64, 1, 1, 'f32', 1, [(37 * i) % 190 - 1 for i in range(300)]),   # sequences of several rounds of the search
 ]
 
 

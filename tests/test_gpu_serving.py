@@ -118,16 +118,16 @@ def test_append_token_by_token():
 
 
 @pytest.mark.parametrize('rope', [False, True])
-@pytest.mark.parametrize('splits', [1, 3, 8])
-@pytest.mark.parametrize('case', sg.ATTENDS, ids=str)
-def test_attend(case, splits, rope):
-    print(f'attend {case} splits {splits} rope {rope}', flush=True)
+@pytest.mark.parametrize('tasks', [1, 7, 256])
+@pytest.mark.parametrize('case', sg.ATTENDS, ids=lambda c: str(c)[:60])
+def test_attend(case, tasks, rope):
+    print(f'attend {case} tasks {tasks} rope {rope}', flush=True)
     blk, hd, hkv, heads, dt, n_new, lens = case
     c, q = sg.attend_case(case)
     g = np.random.default_rng(1).random(hd).astype(np.float32) + 0.5
     kw = dict(gamma=g, theta=1e6, eps=1e-6) if rope else {}
-    lb, init = sg.attend_graph(c, q, lens, hkv, heads, n_new, 0.1, dt, dt, splits=splits, extra=3 if splits == 3 else 0, **kw)
-    got = _run(lb, init, PATH_STATIC if splits == 8 else PATH_DYNAMIC, times=2)
+    lb, init = sg.attend_graph(c, q, lens, hkv, heads, n_new, 0.1, dt, dt, tasks=tasks, extra=3 if tasks == 7 else 0, **kw)
+    got = _run(lb, init, PATH_STATIC if tasks == 256 else PATH_DYNAMIC, times=2)
     want, bound = f64.attend(c, q, lens, hkv, heads, n_new, np.float32(0.1), *((g, np.float32(1e-6), 1e6) if rope else ()))
     o = got['o'].reshape(len(q), -1)
     sg.near(o[:, :heads * hd], want, bound, dt)
@@ -141,8 +141,8 @@ def test_attend_long_f32_error():
     print('attend long', flush=True)
     case = (64, 128, 1, 4, 'f32', 1, [30000])
     c, q = sg.attend_case(case)
-    for splits in (1, 16):
-        lb, init = sg.attend_graph(c, q, case[6], 1, 4, 1, 1 / np.sqrt(128), 'f32', 'f32', splits=splits)
+    for tasks in (1, 16):
+        lb, init = sg.attend_graph(c, q, case[6], 1, 4, 1, 1 / np.sqrt(128), 'f32', 'f32', tasks=tasks)
         want, _ = f64.attend(c, q, case[6], 1, 4, 1, np.float32(1 / np.sqrt(128)))
         got = _run(lb, init)['o'].astype(np.float64)
         assert np.linalg.norm(got - want.ravel()) <= (np.sqrt(30000) + 64) * 2.0 ** -24 * np.linalg.norm(want)
@@ -162,7 +162,7 @@ def test_attend_values_of_any_size():
         c['ks'][1, 1], c['vs'][1, 1] = np.nan, np.nan               # tokens 16 .. 31 of the second sequence
         many = rng.standard_normal((40, hd)).astype(np.float32)       # tokens 12 .. 31: the first four may not see the NaN block
         for heads, n_new, lens, x in ((3, 1, [127, -1], q.reshape(2, -1)), (1, 3, [124, 13], q), (1, 20, [100, 12], many)):
-            lb, init = sg.attend_graph(c, x, lens, 1, heads, n_new, 0.3, 'f32', 'f32', splits=2)
+            lb, init = sg.attend_graph(c, x, lens, 1, heads, n_new, 0.3, 'f32', 'f32')
             got = _run(lb, init)['o']
             want, bound = f64.attend(c, x, lens, 1, heads, n_new, np.float32(0.3))
             sg.near(got, want, bound, 'f32')
@@ -257,7 +257,7 @@ def test_buffers_at_any_element(skip):
     for case in (sg.ATTENDS[2], sg.ATTENDS[5]):
         blk, hd, hkv, heads, dt, n_new, lens = case
         c, q = sg.attend_case(case)
-        lb, init = sg.attend_graph(c, q, lens, hkv, heads, n_new, 0.1, dt, dt, splits=2)
+        lb, init = sg.attend_graph(c, q, lens, hkv, heads, n_new, 0.1, dt, dt)
         want, bound = f64.attend(c, q, lens, hkv, heads, n_new, np.float32(0.1))
         sg.near(_shifted(lb, init, skip)['o'], want, bound, dt)
     for case in sg.ADJUSTS[3:5]:

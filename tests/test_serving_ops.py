@@ -29,7 +29,7 @@ def test_append_oracle(case, tasks):
         np.testing.assert_array_equal(got[n], want[n], err_msg=n)
 
 
-@pytest.mark.parametrize('case', sg.ATTENDS, ids=str)
+@pytest.mark.parametrize('case', sg.ATTENDS, ids=lambda c: str(c)[:60])
 def test_attend_oracle(case):
     blk, hd, hkv, heads, dt, n_new, lens = case
     c, q = sg.attend_case(case)
@@ -114,7 +114,7 @@ def _append():
 def _attend():
     case = sg.ATTENDS[2]
     c, q = sg.attend_case(case)
-    return sg.attend_graph(c, q, case[6], case[2], case[3], case[5], 0.1, 'f32', 'f32', splits=2, gamma=np.ones(case[1], np.float32))
+    return sg.attend_graph(c, q, case[6], case[2], case[3], case[5], 0.1, 'f32', 'f32', tasks=2, gamma=np.ones(case[1], np.float32))
 
 
 def _adjust():
@@ -133,8 +133,8 @@ def test_append_refusals(change, what):
 
 
 @pytest.mark.parametrize('change,what', [
-    ({'n_new': 17}, '1 .. 32'), ({'n_new': 0}, '1 .. 32'), ({'H': 5}, 'H/Hkv'), ({'Hkv': 0}, 'b/kvh'), ({'kvh': 2}, 'b/kvh'), ({'s': 2}, 'b/kvh'),
-    ({'b': 5}, 'too small'), ({'S': 4}, 'too small'), ({'o': 'q'}, 'o must not be q'), ({'scale': float('inf')}, 'scale'), ({'theta': -2.0}, 'theta'),
+    ({'n_new': 17}, '1 .. 32'), ({'n_new': 0}, '1 .. 32'), ({'H': 5}, 'H/Hkv'), ({'Hkv': 0}, 's/S'), ({'s': 2}, 's/S'), ({'s': -1}, 's/S'),
+    ({'b1': 6}, 'too small'), ({'b0': -1}, 'range'), ({'b1': 1030}, '1024'), ({'S': 4}, 'too small'), ({'o': 'q'}, 'o must not be q'), ({'scale': float('inf')}, 'scale'), ({'theta': -2.0}, 'theta'),
     ({'cnt': 'q'}, 'i32'), ({'q': 'lens'}, 'f32 or bf16'), ({'qgamma': 'lens'}, 'f32'), ({'o.part.cols': 129}, 'too small'), ({'blk': 0}, 'blk')], ids=str)
 def test_attend_refusals(change, what):
     _refused(_attend, 'attn_decode_q8', change, what)
