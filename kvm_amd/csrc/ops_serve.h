@@ -32,6 +32,26 @@ __device__ __forceinline__ int q8_of(float x, float s, float inv) {
   q = s > 0.f ? min(q, 127) : 0;                                       // a NaN scale stands for itself: its bytes are 0
   return x < 0.f ? -q : q;
 }
+// Eight values of a block of scale s as two words of bytes, the lowest first. x / s is rounded by adding 1.5 * 2^23, exactly so where
+// x * inv is not within 2^-12 of the middle between two whole numbers (it is off by 127 * 2^-22 at most), by q8_of in the others.
+// A NaN scale (or 0) comes with inv = 0.
+__device__ __forceinline__ void q8_pack(const float (&x)[8], float s, float inv, uint32_t& w0, uint32_t& w1) {
+  constexpr float MAGIC = 12582912.f;
+  uint32_t y[8];
+  float far = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float z = fmaf(x[e], inv, MAGIC);
+    far = fmaxf(far, fabsf(fmaf(x[e], inv, -(z - MAGIC))));
+    y[e] = __float_as_uint(z);
+  }
+  if (far > 0.5f - 0x1p-12f)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = (uint32_t)q8_of(x[e], s, inv);
+  w0 = __builtin_amdgcn_perm(__builtin_amdgcn_perm(y[3], y[2], 0x0c0c0400u), __builtin_amdgcn_perm(y[1], y[0], 0x0c0c0400u), 0x05040100u);
+  w1 = __builtin_amdgcn_perm(__builtin_amdgcn_perm(y[7], y[6], 0x0c0c0400u), __builtin_amdgcn_perm(y[5], y[4], 0x0c0c0400u), 0x05040100u);
+  if (!(s > 0.f)) w0 = w1 = 0;
+}
 // The scale of a block from its largest magnitude (infinity for a block with a value that is not finite), times 1 / 127 as f32 has it:
 // NaN for such a block, 0 where it falls below the normal numbers.
 __device__ __forceinline__ float q8_scale(float amax) {
@@ -117,23 +137,28 @@ struct AppendQ8 {
   int b0, b1, h0, h1, p, P, n, Hkv, hd, blk, nblk;
   float theta, eps;
   __device__ explicit AppendQ8(const Ctx& c)
-      : kn(c.buf(0)), vn(c.buf(1)), kq(c.buf(2)), ks(c.buf(3)), vq(c.buf(4)), vs(c.buf(5)), kt(c.buf(6)), vt(c.buf(7)), lens(c.buf(8)), kg(c.buf(9)),
-        b0(c.i(10)), b1(c.i(11)), h0(c.i(12)), h1(c.i(13)), p(c.i(14)), P(c.i(15)), n(c.i(16)), Hkv(c.i(17)), hd(c.i(18)), blk(c.i(19)),
+      : kn(uview(c, 0)), vn(uview(c, 1)), kq(uview(c, 2)), ks(uview(c, 3)), vq(uview(c, 4)), vs(uview(c, 5)), kt(uview(c, 6)), vt(uview(c, 7)), lens(uview(c, 8)), kg(uview(c, 9)),
+        b0(rfl(c.i(10))), b1(rfl(c.i(11))), h0(rfl(c.i(12))), h1(rfl(c.i(13))), p(rfl(c.i(14))), P(rfl(c.i(15))), n(rfl(c.i(16))), Hkv(rfl(c.i(17))), hd(rfl(c.i(18))), blk(rfl(c.i(19))),
         nblk(ks.cols), theta(c.f(20)), eps(c.f(21)) {}
-  // The lengths of the task's sequences are all checked before anything is written.
-  __device__ bool lengths_ok(const Ctx& c) const {
-    bool bad = false;
+  // The lengths of the task's sequences are all checked before anything is written (-1: one is out of range, reported); otherwise
+  // whether a block becomes full.
+  __device__ int lengths(const Ctx& c, LDS int* word) const {
+    bool bad = false, full = false;
     for (int b = b0 + tid(); b < b1; b += KVM_THREADS) {
       const int L = lens.i()[b];
       if (L < -1 || (long long)L + n > (long long)blk * nblk) { bad = true; c.fail(KVM_ERR_OP_KVLEN, b, L); }
+      else full = full || (L >= 0 && (L + n) / blk > L / blk);
     }
-    return !__syncthreads_or(bad);
+    const int mine = (__ballot(bad) ? 1 : 0) | (__ballot(full) ? 2 : 0);
+    if (lane() == 0) word[wave()] = mine;
+    __syncthreads();
+    const int all = word[0] | word[1] | word[2] | word[3];
+    return all & 1 ? -1 : all >> 1;
   }
-  // Whether a block becomes full in this task's share.
-  __device__ bool finishes() const {
-    bool any = false;
-    for (int b = b0 + tid(); b < b1; b += KVM_THREADS) { const int L = lens.i()[b]; any = any || (L >= 0 && (L + n) / blk > L / blk); }
-    return __syncthreads_or(any);
+  // Task p's share [m0, m1) of `full` blocks that become full; p = 0 has the first one in any case.
+  __device__ void share(int full, int& m0, int& m1) const {
+    const int per = (int)((unsigned)(full + P - 1) / (unsigned)P);
+    m0 = (int)min((long long)p * per, (long long)full); m1 = min(m0 + per, full);
   }
 };
 
@@ -163,7 +188,7 @@ __device__ __forceinline__ void q8_new_key(const AppendQ8& A, LDS float* x, long
 // when it is full and stored to the tail otherwise.
 __device__ __noinline__ void op_kv_append_q8(const Ctx& c) {
   const AppendQ8 A(c);
-  if (!A.lengths_ok(c)) return;
+  if (A.lengths(c, (LDS int*)c.smem) < 0) return;
   LDS float* x = (LDS float*)c.smem;                                   // [blk][hd], one of K and V at a time
   LDS float* red = x + 128 * 128;
   LDS float* row = red + 16;
@@ -171,19 +196,18 @@ __device__ __noinline__ void op_kv_append_q8(const Ctx& c) {
     const int L = A.lens.i()[b];
     if (L < 0) continue;
     const int j0 = L / A.blk, jE = (L + A.n) / A.blk;                  // touched blocks j0 .. jE, the last one unfinished
-    const int mid = max(0, jE - j0 - 1), m0 = (int)((long long)mid * A.p / A.P), m1 = (int)((long long)mid * (A.p + 1) / A.P);
+    int m0, m1;
+    A.share(jE - j0, m0, m1);
     for (int h = A.h0; h < A.h1; ++h) {
       const long long pair = (long long)b * A.Hkv + h;
       for (int which = 0; which < 2; ++which) {
         const View& src = which ? A.vn : A.kn; const View& tail = which ? A.vt : A.kt;
         const View& Q = which ? A.vq : A.kq; const View& SC = which ? A.vs : A.ks;
-        // part 0: the first block (it may hold older tokens), then the unfinished one (its rows in the tail are read before
-        // they are overwritten); the blocks between are shared out
-        for (int u = A.p == 0 ? -1 : 0; u <= m1 - m0; ++u) {
-          if (u == m1 - m0 && A.p != 0) break;
-          const int j = u < 0 ? j0 : u < m1 - m0 ? j0 + 1 + m0 + u : jE;
+        // task 0: the first block (it may hold older tokens) among its share, then the unfinished one (its rows in the tail are read
+        // before they are overwritten)
+        for (int u = m0; u < m1 + (A.p == 0); ++u) {
+          const int j = u < m1 ? j0 + u : jE;
           const bool full = j < jE;
-          if (u < 0 && !full) continue;                                // nothing finishes: the unfinished block only
           const long long t0 = (long long)j * A.blk;
           const int r0 = full ? 0 : (int)(max((long long)L, t0) - t0), r1 = full ? A.blk : (int)(L + A.n - t0);
           float amax = 0.f;
@@ -237,16 +261,17 @@ template <int HD, int NP> __device__ __noinline__ void append_q8_blocks(const Ct
   const int ln = tid() % LPR, rw = tid() / LPR, blk = A.blk;
   const GLOBAL float* gamma = A.kg.ok() ? A.kg.f() : nullptr;
   const LDS double* rot = A.theta > 0.f ? M.freq : nullptr;
-  const bool turned = gamma || rot, nkh = A.kn.dtype == 2, nvh = A.vn.dtype == 2, tkh = A.kt.dtype == 2, tvh = A.vt.dtype == 2;
+  const bool turned = gamma || rot, kround = A.kt.dtype == 2 && (turned || A.kn.dtype != 2), vround = A.vt.dtype == 2 && A.vn.dtype != 2, nkh = A.kn.dtype == 2, nvh = A.vn.dtype == 2, tkh = A.kt.dtype == 2, tvh = A.vt.dtype == 2;
   const int nh = A.h1 - A.h0;
   for (int u = 0; u < (A.b1 - A.b0) * nh; ++u) {
     const int b = A.b0 + u / nh, h = A.h0 + u % nh, L = rfl(A.lens.i()[b]);
     if (L < 0) continue;
     const long long pair = (long long)b * A.Hkv + h;
-    const int j0 = L / blk, jE = (L + A.n) / blk, mid = max(0, jE - j0 - 1);
-    const int m0 = (int)((long long)mid * A.p / A.P), m1 = (int)((long long)mid * (A.p + 1) / A.P);
-    for (int it = A.p == 0 && jE > j0 ? m0 - 1 : m0; it < m1; ++it) {  // (p = 0: m0 = 0, and -1 is the first block)
-      const int j = j0 + 1 + it, old = max(0, L - j * blk);            // rows below `old` are in the tail
+    const int lb = 31 - __clz(blk), j0 = L >> lb, jE = (L + A.n) >> lb;
+    int m0, m1;
+    A.share(jE - j0, m0, m1);
+    for (int j = j0 + m0; j < j0 + m1; ++j) {
+      const int old = max(0, L - j * blk);            // rows below `old` are in the tail
       const long long new0 = (long long)b * A.n + ((long long)j * blk - L), tail0 = pair * blk;
       if (turned) {
         __syncthreads();
@@ -271,7 +296,8 @@ template <int HD, int NP> __device__ __noinline__ void append_q8_blocks(const Ct
         if (!turned) rk[i].load(in_tail ? A.kt : A.kn, in_tail ? (tail0 + r) * A.kt.cols + 8 * ln : (new0 + r) * A.kn.cols + h * HD + 8 * ln);
         rv[i].load(in_tail ? A.vt : A.vn, in_tail ? (tail0 + r) * A.vt.cols + 8 * ln : (new0 + r) * A.vn.cols + h * HD + 8 * ln);
       }
-      float k[NP][8], v[NP][8], ka = 0.f, va = 0.f;
+      float k[NP][8], v[NP][8];
+      uint32_t ka = 0, va = 0;                                        // largest magnitudes by their bits: what is not finite is largest
 #pragma unroll
       for (int i = 0; i < NP; ++i) {
         const int r = i * RPP + rw;
@@ -283,14 +309,14 @@ template <int HD, int NP> __device__ __noinline__ void append_q8_blocks(const Ct
         rv[i].get(r < old ? tvh : nvh, v[i]);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          if (tkh) k[i][e] = round_bf(k[i][e]);
-          if (tvh) v[i][e] = round_bf(v[i][e]);
-          ka = q8_amax(ka, k[i][e]); va = q8_amax(va, v[i][e]);
+          if (kround) k[i][e] = round_bf(k[i][e]);
+          if (vround) v[i][e] = round_bf(v[i][e]);
+          ka = max(ka, __float_as_uint(k[i][e]) & 0x7fffffffu); va = max(va, __float_as_uint(v[i][e]) & 0x7fffffffu);
         }
       }
-      ka = rows_max(lanes_max<16>(ka)); va = rows_max(lanes_max<16>(va));
+      const float km = rows_max(lanes_max<16>(__uint_as_float(min(ka, 0x7f800000u)))), vm = rows_max(lanes_max<16>(__uint_as_float(min(va, 0x7f800000u))));
       __syncthreads();                                                 // the block before is out of `turn` and `red`
-      if (lane() == 0) { M.red[wave()] = ka; M.red[4 + wave()] = va; }
+      if (lane() == 0) { M.red[wave()] = km; M.red[4 + wave()] = vm; }
       __syncthreads();
       const float sk = q8_scale(fmaxf(fmaxf(M.red[0], M.red[1]), fmaxf(M.red[2], M.red[3]))), ik = sk > 0.f ? 1.f / sk : 0.f;
       const float sv = q8_scale(fmaxf(fmaxf(M.red[4], M.red[5]), fmaxf(M.red[6], M.red[7]))), iv = sv > 0.f ? 1.f / sv : 0.f;
@@ -301,17 +327,20 @@ template <int HD, int NP> __device__ __noinline__ void append_q8_blocks(const Ct
       for (int i = 0; i < NP; ++i) {
         const int r = i * RPP + rw;
         if (r >= blk) break;
-        uint32_t w[2] = {0, 0};
+        uint32_t w0, w1, x0, x1;
+        q8_pack(k[i], sk, ik, w0, w1);
+        q8_pack(v[i], sv, iv, x0, x1);
+        __builtin_amdgcn_raw_buffer_store_b64(u32x2_t{w0, w1}, ok, r * HD + 8 * ln, 0, 16 /* SC1 */);
+        LDS unsigned char* col = M.turn + 8 * ln * (blk + 4) + r;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          w[e / 4] |= (uint32_t)(q8_of(k[i][e], sk, ik) & 255) << (8 * (e % 4));
-          M.turn[(8 * ln + e) * (blk + 4) + r] = (unsigned char)q8_of(v[i][e], sv, iv);
+        for (int e = 0; e < 4; ++e) {
+          col[e * (blk + 4)] = (unsigned char)(x0 >> (8 * e));
+          col[(4 + e) * (blk + 4)] = (unsigned char)(x1 >> (8 * e));
         }
-        __builtin_amdgcn_raw_buffer_store_b64(u32x2_t{w[0], w[1]}, ok, r * HD + 8 * ln, 0, 16 /* SC1 */);
       }
       __syncthreads();
       for (int e = tid(); e < HD * blk / 16; e += KVM_THREADS) {
-        const LDS uint32_t* x = (const LDS uint32_t*)(M.turn + (16 * e / blk) * (blk + 4) + 16 * e % blk);
+        const LDS uint32_t* x = (const LDS uint32_t*)(M.turn + (16 * e >> lb) * (blk + 4) + (16 * e & (blk - 1)));
         stwt_buf(ov, 16 * e, __builtin_bit_cast(f32x4n, u32x4_t{x[0], x[1], x[2], x[3]}));
       }
     }
@@ -320,33 +349,45 @@ template <int HD, int NP> __device__ __noinline__ void append_q8_blocks(const Ct
 template <int HD> __device__ __forceinline__ void append_q8_t(const Ctx& c) {
   constexpr int LPR = HD / 8, RPP = KVM_THREADS / LPR;
   const AppendQ8 A(c);
-  if (!A.lengths_ok(c)) return;
   const AppendLds<HD> M(c.smem);
+  const int full = A.lengths(c, (LDS int*)M.red);
+  if (full < 0) return;
   const int ln = tid() % LPR, rw = tid() / LPR, blk = A.blk, nh = A.h1 - A.h0;
   const GLOBAL float* gamma = A.kg.ok() ? A.kg.f() : nullptr;
   const LDS double* rot = A.theta > 0.f ? M.freq : nullptr;
   if (rot && tid() < HD / 2) M.freq[tid()] = q8_freq(tid(), HD, log((double)A.theta));
-  if (A.finishes()) {                                                  // (a barrier on both ways)
+  __syncthreads();
+  if (full) {
     if (blk <= 4 * RPP) append_q8_blocks<HD, 4>(c);
     else append_q8_blocks<HD, 128 / RPP>(c);
   }
   if (A.p != 0) return;
   __syncthreads();                                                     // old rows of the tail have been read
   const int most = min(A.n, blk - 1), rows = (A.b1 - A.b0) * nh * most;   // rows of an unfinished block: no more than that
-  for (int u = rw; u < rows; u += RPP) {
-    const int b = A.b0 + u / (nh * most), h = A.h0 + u / most % nh, L = A.lens.i()[b];
-    if (L < 0) continue;
-    const long long t = max((long long)L, (long long)((L + A.n) / blk) * blk) + u % most;
-    if (t >= (long long)L + A.n) continue;
-    const long long row = (long long)b * A.n + (t - L), at = ((long long)b * A.Hkv + h) * blk + t % blk;
-    Raw8 rk, rv;
-    rk.load(A.kn, row * A.kn.cols + h * HD + 8 * ln);
-    rv.load(A.vn, row * A.vn.cols + h * HD + 8 * ln);
-    float k[8], v[8];
-    rk.get(A.kn.dtype == 2, k); rv.get(A.vn.dtype == 2, v);
-    if (gamma || rot) head8_turn<HD>(k, gamma, A.eps, rot, t, M.angs + rw * HD);
-    st8(A.kt, at * A.kt.cols + 8 * ln, k);
-    st8(A.vt, at * A.vt.cols + 8 * ln, v);
+  constexpr int NR = 4;                                                // rows in flight
+  for (int u0 = rw; u0 < rows; u0 += NR * RPP) {
+    Raw8 rk[NR], rv[NR];
+    long long t[NR] = {-1, -1, -1, -1}, at[NR];
+#pragma unroll
+    for (int i = 0; i < NR; ++i) {
+      const int u = u0 + i * RPP;
+      if (u >= rows) break;
+      const int b = A.b0 + u / (nh * most), h = A.h0 + u / most % nh, L = A.lens.i()[b];
+      const long long x = max((long long)L, (long long)((L + A.n) & -blk)) + u % most, row = (long long)b * A.n + (x - L);
+      if (L < 0 || x >= (long long)L + A.n) continue;
+      t[i] = x; at[i] = ((long long)b * A.Hkv + h) * blk + (x & (blk - 1));
+      rk[i].load(A.kn, row * A.kn.cols + h * HD + 8 * ln);
+      rv[i].load(A.vn, row * A.vn.cols + h * HD + 8 * ln);
+    }
+#pragma unroll
+    for (int i = 0; i < NR; ++i) {
+      if (t[i] < 0) continue;
+      float k[8], v[8];
+      rk[i].get(A.kn.dtype == 2, k); rv[i].get(A.vn.dtype == 2, v);
+      if (gamma || rot) head8_turn<HD>(k, gamma, A.eps, rot, t[i], M.angs + rw * HD);
+      st8(A.kt, at[i] * A.kt.cols + 8 * ln, k);
+      st8(A.vt, at[i] * A.vt.cols + 8 * ln, v);
+    }
   }
 }
 __device__ __noinline__ bool op_kv_append_q8_fast(const Ctx& c) {
@@ -363,8 +404,8 @@ struct DecodeQ8 {
   int b0, b1, s, S, n, H, Hkv, hd, blk, G, R;
   float scale, theta, eps;
   __device__ explicit DecodeQ8(const Ctx& c)
-      : q(c.buf(0)), kq(c.buf(1)), ks(c.buf(2)), vq(c.buf(3)), vs(c.buf(4)), kt(c.buf(5)), vt(c.buf(6)), lens(c.buf(7)), part(c.buf(8)), o(c.buf(9)),
-        cnt(c.buf(10)), qg(c.buf(11)), b0(c.i(12)), b1(c.i(13)), s(c.i(14)), S(c.i(15)), n(c.i(16)), H(c.i(17)), Hkv(c.i(18)), hd(c.i(19)), blk(c.i(20)),
+      : q(uview(c, 0)), kq(uview(c, 1)), ks(uview(c, 2)), vq(uview(c, 3)), vs(uview(c, 4)), kt(uview(c, 5)), vt(uview(c, 6)), lens(uview(c, 7)), part(uview(c, 8)), o(uview(c, 9)),
+        cnt(uview(c, 10)), qg(uview(c, 11)), b0(rfl(c.i(12))), b1(rfl(c.i(13))), s(rfl(c.i(14))), S(rfl(c.i(15))), n(rfl(c.i(16))), H(rfl(c.i(17))), Hkv(rfl(c.i(18))), hd(rfl(c.i(19))), blk(rfl(c.i(20))),
         scale(c.f(21)), theta(c.f(22)), eps(c.f(23)) { G = H / Hkv; R = n * G; }
   __device__ long long at(const View& X, int b, int h, int r) const { return ((long long)b * n + r / G) * X.cols + (h * G + r % G) * hd; }
   __device__ bool length_ok(const Ctx& c, int b, int L) const {
@@ -498,36 +539,56 @@ struct WorkQ8 {
     return max(0, (int)((unsigned)(a.start + a.cost - Q8_SNAP + share) / (unsigned)share) - first_inside(a));
   }
 };
-// Lengths and cost sums of the call's sequences into LDS; false if a length is out of range (reported).
+// Inclusive sum over the lanes of a wave: within rows of 16, then the rows' last sums.
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+  return v;
+}
+// Lengths and cost sums of the call's sequences into LDS; false if a length is out of range (reported). Up to 64 sequences by every wave
+// for itself (the same words from all four, no barrier), more by the workgroup.
 __device__ __forceinline__ bool q8_work(const Ctx& c, const DecodeQ8& D, LDS int* pre, LDS int* len, LDS int* tot, WorkQ8& W) {
   constexpr int PER = Q8_SEQS / KVM_THREADS;
   const int seqs = D.b1 - D.b0;
-  int cost[PER], sum = 0;
-  bool bad = false;
+  auto cost_of = [&](int L) { return L < 0 ? 1 : Q8_PAIR + (int)(((((unsigned)L + D.n) & -(unsigned)D.blk) + 63) >> 6); };
+  if (seqs <= 64) {
+    const int L = lane() < seqs ? D.lens.i()[D.b0 + lane()] : -1;
+    if (__ballot(lane() < seqs && !D.length_ok(c, D.b0 + lane(), L))) return false;
+    const int cost = lane() < seqs ? cost_of(L) : 0, upto = wave_scan(cost);
+    if (lane() < seqs) { len[lane()] = L; pre[lane()] = upto - cost; }
+    if (lane() == seqs - 1) pre[seqs] = upto;
+    __builtin_amdgcn_wave_barrier();                                   // one wave's LDS operations stay in order
+  } else {
+    int cost[PER], sum = 0;
+    bool bad = false;
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int k = tid() * PER + i;
-    cost[i] = 0;
-    if (k < seqs) {
-      const int L = D.lens.i()[D.b0 + k];
-      bad = bad || !D.length_ok(c, D.b0 + k, L);
-      len[k] = L;
-      cost[i] = L < 0 ? 1 : Q8_PAIR + (int)(((((unsigned)L + D.n) & -(unsigned)D.blk) + 63) >> 6);
-      sum += cost[i];
+    for (int i = 0; i < PER; ++i) {
+      const int k = tid() * PER + i;
+      cost[i] = 0;
+      if (k < seqs) {
+        const int L = D.lens.i()[D.b0 + k];
+        bad = bad || !D.length_ok(c, D.b0 + k, L);
+        len[k] = L;
+        cost[i] = cost_of(L);
+        sum += cost[i];
+      }
     }
-  }
-  int upto = sum;
-  for (int o = 1; o < 64; o <<= 1) { const int y = __shfl_up(upto, o, 64); if (lane() >= o) upto += y; }
-  if (lane() == 63) tot[wave()] = upto;
-  if (__syncthreads_or(bad)) return false;
-  int at = upto - sum;
-  for (int w = 0; w < KVM_WAVES; ++w) at += w < wave() ? tot[w] : 0;
+    const int upto = wave_scan(sum);
+    if (lane() == 63) tot[wave()] = upto;
+    if (__syncthreads_or(bad)) return false;
+    int at = upto - sum;
+    for (int w = 0; w < KVM_WAVES; ++w) at += w < wave() ? tot[w] : 0;
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int k = tid() * PER + i;
-    if (k < seqs) { pre[k] = at; at += cost[i]; if (k == seqs - 1) pre[seqs] = at; }
+    for (int i = 0; i < PER; ++i) {
+      const int k = tid() * PER + i;
+      if (k < seqs) { pre[k] = at; at += cost[i]; if (k == seqs - 1) pre[seqs] = at; }
+    }
+    __syncthreads();
   }
-  __syncthreads();
   W.pre = pre; W.seqs = seqs; W.Hkv = D.Hkv;
   W.total = rfl(pre[seqs]) * D.Hkv;
   // equal shares, but none below Q8_SHARE unless there are tasks enough for a pair each
@@ -579,19 +640,21 @@ __device__ __forceinline__ void q8_arrive(const Ctx& c, const DecodeQ8& D, int b
   if (tid() == 0) st_relaxed((int*)cnt, 0);
 }
 
-// Decode attention over the 8-bit cache at head sizes 64 and 128, on the matrix units. Bound: streaming the cache's bytes.
-// Each wave takes units of 64 tokens in turn, K and V straight from memory into registers in the layout of the operands:
-//   scores  v_mfma_f32_16x16x32_f16, A = 16 keys, B = up to 16 query rows (NT such tiles). A lane's 16-byte load of a key
-//           feeds two products, so the head dims run in the order of those loads, for the queries alike.
-//   P V     the same instruction with A = V transposed (16 head dims x 32 tokens: the cache keeps a block's values as
-//           [hd][blk], so this too is a 16-byte load), B = P. Tokens go to the rows of the score tiles (row m of tile a: token
-//           16 (m / 4) + 4 a + m % 4) such that the scores' output registers are the B operand, in the loads' order.
-// A byte becomes an f16 by two instructions for two of them (0x6400 | (q + 128) is 1024 + q + 128), exactly. Queries and
-// probabilities are f16 pairs, the value and its remainder (22 bits: queries scaled by a power of two per row, probabilities
-// to 2^12, so that no remainder that matters falls below f16's numbers), two products each, summed in f32. A block's key
-// scale multiplies its scores; its value scale the probabilities, relative to the largest so far (vref, a power of two).
-// Each unit's P V is summed on its own and added to the running one in f32 (the units' chained sums round towards -inf).
-// The unfinished block is f32 work of all lanes: at most blk - 1 tokens.
+// Decode attention over the 8-bit cache at head sizes 64 and 128, on the matrix units. Bound: streaming the cache's bytes, and
+// where few workers stream at once the ~550 vector instructions of a unit.
+// Each wave takes units of 64 tokens in turn, K and V straight from memory into registers in the layout of the operands, a unit ahead:
+//   scores  v_mfma_i32_16x16x64_i8, A = 16 keys as they lie, B = up to 16 query rows (NT such tiles) as three signed bytes of a
+//           fixed-point number per value (22 bits below a power of two above the row's largest): whole numbers, summed exactly.
+//           A lane's 16-byte load of a key is its part of the operand.
+//   P V     v_mfma_f32_16x16x32_f16, A = V transposed (16 head dims x 32 tokens: the cache keeps a block's values as [hd][blk], so
+//           this too is a 16-byte load), B = P. Tokens go to the rows of the score tiles (row m of tile a: token 16 (m / 4) + 4 a +
+//           m % 4) such that the scores' output registers are the B operand, in the loads' order.
+// A byte of V becomes an f16 by two instructions for two of them (0x6400 | (v + 128) is 1024 + v + 128), exactly. Probabilities are
+// f16 pairs, the value and its remainder (22 bits; scaled to 2^12, so that no remainder that matters falls below f16's
+// numbers), two products each, summed in f32. A block's key scale multiplies its scores; its value scale the probabilities, relative
+// to the largest so far (vref, a power of two). Each unit's P V is summed on its own and added to the running one in f32 (the
+// units' chained sums round towards -inf). The unfinished block, at most blk - 1 tokens, is f32 work
+// of all lanes (a wave to a row, the tail in its registers and no barrier, was slower: 24 ragged sequences 52 -> 67 us).
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 // Eight signed bytes (two words) as f16.
@@ -617,20 +680,22 @@ template <int HD> struct DecodeLds {
         to(qs + 32 * (HD + 4)),                                        // [32][HD] the tail's P V
         st(to + 32 * HD),                                              // [5][2][32] maxima and sums of the waves and the tail
         cr(st + 320),                                                  // [32] factors from a product to a score
-        ts(cr + 32),                                                   // [32][128] the tail's scores
+        ts(cr + 32),                                                   // [32][128] the tail's scores; before, the rows' angles
         tv(ts + 32 * 128) {}                                           // [128][HD] its values
   static_assert((2 * Q8_SEQS + 4 + HD + 32 * (HD + 4) + 32 * HD + 352 + 32 * 128 + 128 * HD) * 4 <= KVM_LDS_BYTES, "decode attention LDS map");
 };
 // One piece of a pair: units [u0, u1), with `first` also the unfinished block; `live` pieces in all, piece 1 in task i0's partials.
-template <int HD, int NT> __device__ __noinline__ void attn_q8_piece(const Ctx& c, int b, int kvh, int L, int u0, int u1, bool first, int i0, int live) {
+template <int HD, int NT> __device__ __noinline__ void attn_q8_piece(const Ctx& c, int b_, int kvh_, int L_, int u0_, int u1_, bool first_, int i0_, int live_) {
+  const int b = rfl(b_), kvh = rfl(kvh_), L = rfl(L_), u0 = rfl(u0_), u1 = rfl(u1_), i0 = rfl(i0_), live = rfl(live_);
+  const bool first = rfl(first_) != 0;
   constexpr float LOG2E = 1.44269504088896340736f, PS = 4096.f;
   constexpr int KH = HD / 64, VT = HD / 16, LPR = HD / 8, RPP = KVM_THREADS / LPR, QS = HD + 4;
   const DecodeLds<HD> M(c.smem);
   LDS float *const qs = M.qs, *const to = M.to, *const st = M.st, *const cr = M.cr, *const ts = M.ts, *const tv = M.tv;
   const DecodeQ8 D(c);
-  const int blk = rfl(D.blk), lb = 31 - __clz(blk), n = L + D.n, whole = n & -blk, nt = first ? n - whole : 0;
+  const int blk = D.blk, lb = 31 - __clz(blk), n = L + D.n, whole = n & -blk, nt = first ? n - whole : 0;
   const bool tail = nt > 0;
-  const int l = lane(), w = wave(), nn = l & 15, qq = l >> 4, ln = tid() % LPR, rw = tid() / LPR;
+  const int l = lane(), w = rfl(wave()), nn = l & 15, qq = l >> 4, ln = tid() % LPR, rw = tid() / LPR;
   const long long pair = (long long)b * D.Hkv + kvh, byte0 = pair * D.ks.cols * blk * HD;
   const GLOBAL char* K = (const GLOBAL char*)D.kq.p + byte0;
   const GLOBAL char* V = (const GLOBAL char*)D.vq.p + byte0;
@@ -664,7 +729,7 @@ template <int HD, int NT> __device__ __noinline__ void attn_q8_piece(const Ctx& 
   if (tail) load_tail(0);
   UnitQ8<HD> U;
   if (u0 + w < u1) load(U, u0 + w);
-  // query rows: norm, rotation, then scaled so that the largest magnitude of a row lies in [2^10, 2^11)
+  // query rows: norm, rotation, then scaled by a power of two to magnitudes below 2^22
 #pragma unroll
   for (int i = 0; i < QP; ++i) {
     const int r = i * RPP + rw;
@@ -674,15 +739,15 @@ template <int HD, int NT> __device__ __noinline__ void attn_q8_piece(const Ctx& 
       rq[i].get(D.q.dtype == 2, x);
       head8_turn<HD>(x, D.qg.ok() ? D.qg.f() : nullptr, D.eps, D.theta > 0.f ? M.freq : nullptr, L + r / D.G, ts + rw * HD);
     }
-    float big = 0.f;
+    uint32_t big = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(x[e]));
-    big = lanes_max<LPR>(big);
-    const int ex = max(20, (int)(__float_as_uint(big) >> 23));
-    const float up = __uint_as_float((uint32_t)(264 - ex) << 23), down = __uint_as_float((uint32_t)(ex - 10) << 23);
+    for (int e = 0; e < 8; ++e) big = max(big, __float_as_uint(x[e]) & 0x7fffffffu);
+    const float top = lanes_max<LPR>(__uint_as_float(min(big, 0x7f800000u)));
+    const int ex = max(24, (int)(__float_as_uint(top) >> 23));
+    const float up = __uint_as_float((uint32_t)(275 - ex) << 23), down = __uint_as_float((uint32_t)(ex - 21) << 23);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) qs[r * QS + 8 * ln + e] = x[e] * up;
-    if (ln == 0) cr[r] = down * D.scale * LOG2E;
+    for (int e = 0; e < 8; ++e) qs[r * QS + 8 * ln + e] = top < INFINITY ? x[e] * up : 0.f;
+    if (ln == 0) cr[r] = top < INFINITY ? down * D.scale * LOG2E : __uint_as_float(0x7fc00000u);   // a row that is not finite is NaN
   }
   __syncthreads();
   if (tail) {                                                          // scores of the unfinished block, then its own softmax and P V
@@ -699,19 +764,33 @@ template <int HD, int NT> __device__ __noinline__ void attn_q8_piece(const Ctx& 
 #pragma unroll
         for (int e = 0; e < 8; ++e) tv[t * HD + 8 * ln + e] = y[e];
       }
-      for (int r = 0; r < D.R; ++r) {
-        float q[8];
+      for (int r0 = 0; r0 < D.R; r0 += 4) {
+        float a[4][TP];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) q[e] = qs[r * QS + 8 * ln + e];
-        const int seen = min(nt, L + r / D.G + 1 - whole);
+        for (int k = 0; k < 4; ++k) {
+          float q[8];
 #pragma unroll
-        for (int i = 0; i < TP; ++i) {
-          const int t = t0 + i * RPP + rw;
-          float a = 0.f;
+          for (int e = 0; e < 8; ++e) q[e] = qs[min(r0 + k, D.R - 1) * QS + 8 * ln + e];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) a += q[e] * x[i][e];
-          a = lanes_sum<LPR>(a);
-          if (ln == 0 && t < nt) ts[r * 128 + t] = t < seen ? a * cr[r] : -INFINITY;
+          for (int i = 0; i < TP; ++i) {
+            a[k][i] = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) a[k][i] += q[e] * x[i][e];
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int i = 0; i < TP; ++i) a[k][i] = lanes_sum<LPR>(a[k][i]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int r = r0 + k, seen = min(nt, L + r / D.G + 1 - whole);
+          const float f = cr[min(r, D.R - 1)];
+#pragma unroll
+          for (int i = 0; i < TP; ++i) {
+            const int t = t0 + i * RPP + rw;
+            if (ln == 0 && t < nt && r < D.R) ts[r * 128 + t] = t < seen ? a[k][i] * f : -INFINITY;
+          }
         }
       }
     }
@@ -740,8 +819,8 @@ template <int HD, int NT> __device__ __noinline__ void attn_q8_piece(const Ctx& 
       to[r1 * HD + d] = (a[1][0] + a[1][1]) + (a[1][2] + a[1][3]);
     }
   }
-  // the queries as B operands: row nn of tile g, dims 16 (qq + 4 h) + 8 p ..
-  f16x8 qh[NT][KH][2], ql[NT][KH][2];
+  // the queries as B operands: row nn of tile g, dims 64 h + 16 qq .., byte p of the fixed-point numbers
+  i32x4_t qb[NT][KH][3];
   float mrun[NT], lrun[NT], crow[NT];
   int lim[NT];
   f32x4n o[NT][VT];
@@ -751,23 +830,25 @@ template <int HD, int NT> __device__ __noinline__ void attn_q8_piece(const Ctx& 
 #pragma unroll
     for (int h = 0; h < KH; ++h)
 #pragma unroll
-      for (int p = 0; p < 2; ++p)
+      for (int v = 0; v < 4; ++v) {
+        uint32_t y[4];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float x = qs[r * QS + 16 * (qq + 4 * h) + 8 * p + e];
-          const _Float16 hi = (_Float16)x;
-          qh[g][h][p][e] = hi; ql[g][h][p][e] = (_Float16)(x - (float)hi);
-        }
+        for (int e = 0; e < 4; ++e) y[e] = ((uint32_t)(int)rintf(qs[r * QS + 64 * h + 16 * qq + 4 * v + e]) + 0x808080u) ^ 0x808080u;
+        const uint32_t a01 = __builtin_amdgcn_perm(y[1], y[0], 0x05010400u), a23 = __builtin_amdgcn_perm(y[3], y[2], 0x05010400u);
+        qb[g][h][0][v] = (int)__builtin_amdgcn_perm(a23, a01, 0x05040100u);
+        qb[g][h][1][v] = (int)__builtin_amdgcn_perm(a23, a01, 0x07060302u);
+        qb[g][h][2][v] = (int)__builtin_amdgcn_perm(__builtin_amdgcn_perm(y[3], y[2], 0x0c0c0602u), __builtin_amdgcn_perm(y[1], y[0], 0x0c0c0602u), 0x05040100u);
+      }
     crow[g] = cr[r]; mrun[g] = -INFINITY; lrun[g] = 0.f;
     lim[g] = r < D.R ? min(whole, L + r / D.G + 1) : 0;
 #pragma unroll
     for (int d = 0; d < VT; ++d) o[g][d] = f32x4n{0.f, 0.f, 0.f, 0.f};
   }
   float vref = 1.17549435e-38f;
-  for (int u = u0 + w; u < u1; u += KVM_WAVES) {
-    UnitQ8<HD> N;
-    if (u + KVM_WAVES < u1) load(N, u + KVM_WAVES);
-    const float vm0 = U.vs == U.vs ? U.vs : 0.f, vm = rows_max(vm0);
+  // one unit; ALL: every row sees every token of it
+  auto unit = [&](int u, auto all) {
+    constexpr bool ALL = decltype(all)::value;
+    const float vm = rows_max(U.vs == U.vs ? U.vs : 0.f);
     float fv = 1.f;
     if (vm > vref) {                                                   // uniform: the four lane groups hold the unit's scales
       const float nv = __uint_as_float((__float_as_uint(vm) & 0x7f800000u) + 0x00800000u);
@@ -778,30 +859,27 @@ template <int HD, int NT> __device__ __noinline__ void attn_q8_piece(const Ctx& 
     float sc[NT][16];
 #pragma unroll
     for (int a = 0; a < 4; ++a) {
-      f32x4n hi[NT], lo[NT];
-#pragma unroll
-      for (int g = 0; g < NT; ++g) hi[g] = lo[g] = f32x4n{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int h = 0; h < KH; ++h)
-#pragma unroll
-        for (int p = 0; p < 2; ++p) {
-          const f16x8 k = q8_half(U.k[a][h][2 * p], U.k[a][h][2 * p + 1]);
-#pragma unroll
-          for (int g = 0; g < NT; ++g) {
-            hi[g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh[g][h][p], hi[g], 0, 0, 0);
-            lo[g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql[g][h][p], lo[g], 0, 0, 0);
-          }
-        }
+      i32x4_t s[NT][3];
 #pragma unroll
       for (int g = 0; g < NT; ++g)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sc[g][4 * a + i] = (hi[g][i] + lo[g][i]) * (crow[g] * U.ks);
+        for (int p = 0; p < 3; ++p) s[g][p] = i32x4_t{0, 0, 0, 0};
+#pragma unroll
+      for (int h = 0; h < KH; ++h)
+#pragma unroll
+        for (int g = 0; g < NT; ++g)
+#pragma unroll
+          for (int p = 0; p < 3; ++p) s[g][p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4_t, U.k[a][h]), qb[g][h][p], s[g][p], 0, 0, 0);
+#pragma unroll
+      for (int g = 0; g < NT; ++g)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sc[g][4 * a + i] = fmaf((float)((s[g][2][i] << 8) + s[g][1][i]), 256.f, (float)s[g][0][i]) * (crow[g] * U.ks);
     }
     f16x8 ph[NT][2], pl[NT][2];
     float fo[NT];
 #pragma unroll
     for (int g = 0; g < NT; ++g) {
-      const int seen = lim[g] - 64 * u - 16 * qq;                      // of this lane's 16 tokens
+      const int seen = ALL ? 16 : lim[g] - 64 * u - 16 * qq;           // of this lane's 16 tokens
       float m = mrun[g];
 #pragma unroll
       for (int i = 0; i < 16; ++i) if (i < seen) m = fmaxf(m, sc[g][i]);
@@ -834,6 +912,12 @@ template <int HD, int NT> __device__ __noinline__ void attn_q8_piece(const Ctx& 
         for (int i = 0; i < 4; ++i) o[g][d][i] = fmaf(o[g][d][i], fo[g], x[i]);
       }
     }
+  };
+  for (int u = u0 + w; u < u1; u += KVM_WAVES) {
+    UnitQ8<HD> N;
+    if (u + KVM_WAVES < u1) load(N, u + KVM_WAVES);
+    if (64 * (u + 1) <= min(whole, L + 1)) unit(u, std::true_type{});
+    else unit(u, std::false_type{});
     U = N;
   }
   // the waves' and the tail's states, then their sum over all of them
@@ -877,7 +961,7 @@ template <int HD> __device__ __forceinline__ void attn_q8_t(const Ctx& c) {
   const DecodeLds<HD> M(c.smem);
   const DecodeQ8 D(c);
   WorkQ8 W;
-  if (!q8_work(c, D, M.pre, M.len, (LDS int*)M.ts, W)) return;
+  if (D.b0 == D.b1 || !q8_work(c, D, M.pre, M.len, (LDS int*)M.st, W)) return;
   if (D.theta > 0.f && tid() < HD / 2) M.freq[tid()] = q8_freq(tid(), HD, log((double)D.theta));
   const int stop = W.cut(D.s + 1);
   for (int at = W.cut(D.s); at < stop;) {
@@ -901,27 +985,33 @@ __device__ __noinline__ bool op_attn_decode_q8_fast(const Ctx& c) {
 }
 
 // ---------------------------------------------------------------------------------------------- logits
-// Adjusted logits (op 314): the token counts of the sequence in LDS, one word per logit of a chunk (generated: bits 0..19, bias
-// slot: bits 20..30, prompt: bit 31), then the logits against them. Bound: the bytes of the logits, and per task the history, which
-// every task of a row reads as a whole (a few KB, from the L2), and the clearing of the words. Logits go in vectors of 4
-// from any element (a bf16 row from its first aligned one), eight per thread requested before the ones before are used;
-// most have the word 0 and only meet the mask. A token's entries in the bias list meet by an atomic maximum of (2047 - entry),
-// which leaves the slot of the first; the others are added to it in list order, one after another (they are few).
-constexpr int ADJ_CHUNK = 26624, ADJ_BIAS = 2047, ADJ_NB = 8;
+// Adjusted logits (op 314). Bound: the bytes of the logits, and per task the history, which every task of a row reads as a whole (a few
+// KB, from the L2). The task's logits go through as a stream that knows only the mask, in vectors of 4 from any element (a bf16
+// row from its first aligned one), 32 KB requested before the ones before are used (vectors of 8 bf16 logits have stores of 16 bytes 32
+// apart: 33 -> 40 us a task of 50257); rows in place without a mask
+// have no stream. The few tokens that the history or the biases name meet in LDS, one word of counts per logit of a chunk
+// (generated: bits 0..19, bias slot: bits 20..30, prompt: bit 31), before the first vectors of the stream have come; behind the stream
+// whoever takes a word out of there (an exchange against 0) writes that logit again. A token's entries in the bias list meet by an
+// atomic maximum of (2047 - entry), which leaves the slot of the first; the others are added to it in list order, one after another
+// (they are few). Adjusting in the stream itself ran its divisions for every wave that met one named token: 256 rows of 50257
+// logits 47 us a task.
+constexpr int ADJ_CHUNK = 26624, ADJ_BIAS = 2047;
 struct AdjustArgs {
   View x, out, par, hist, plen, hlen, last, bidx, bval, mask, mrow;
   int r0, r1, v0, v1, V;
   __device__ explicit AdjustArgs(const Ctx& c)
-      : x(c.buf(0)), out(c.buf(1)), par(c.buf(2)), hist(c.buf(3)), plen(c.buf(4)), hlen(c.buf(5)), last(c.buf(6)), bidx(c.buf(7)), bval(c.buf(8)),
-        mask(c.buf(9)), mrow(c.buf(10)), r0(c.i(11)), r1(c.i(12)), v0(c.i(13)), v1(c.i(14)), V(c.i(15)) {}
-  // All rows of the task are checked before anything is written.
+      : x(uview(c, 0)), out(uview(c, 1)), par(uview(c, 2)), hist(uview(c, 3)), plen(uview(c, 4)), hlen(uview(c, 5)), last(uview(c, 6)), bidx(uview(c, 7)), bval(uview(c, 8)),
+        mask(uview(c, 9)), mrow(uview(c, 10)), r0(rfl(c.i(11))), r1(rfl(c.i(12))), v0(rfl(c.i(13))), v1(rfl(c.i(14))), V(rfl(c.i(15))) {}
+  __device__ bool row_ok(const Ctx& c, int r, int n, int pl, int m) const {
+    if (n < 0 || pl < 0 || pl > n || (hist.ok() && n + (last.ok() ? 1 : 0) > hist.cols)) { c.fail(KVM_ERR_OP_RANGE, r, n); return false; }
+    if (mrow.ok() && (m < -1 || m >= mask.rows)) { c.fail(KVM_ERR_OP_RANGE, r, m); return false; }
+    return true;
+  }
+  // All rows of a task are checked before anything is written (a single one when it is read).
   __device__ bool rows_ok(const Ctx& c) const {
     bool bad = false;
-    for (int r = r0 + tid(); r < r1; r += KVM_THREADS) {
-      const int n = hist.ok() ? hlen.i()[r] : 0, pl = hist.ok() ? plen.i()[r] : 0, m = mrow.ok() ? mrow.i()[r] : 0;
-      if (n < 0 || pl < 0 || pl > n || (hist.ok() && n + (last.ok() ? 1 : 0) > hist.cols)) { bad = true; c.fail(KVM_ERR_OP_RANGE, r, n); }
-      if (mrow.ok() && (m < -1 || m >= mask.rows)) { bad = true; c.fail(KVM_ERR_OP_RANGE, r, m); }
-    }
+    for (int r = r0 + tid(); r < r1; r += KVM_THREADS)
+      bad = bad || !row_ok(c, r, hist.ok() ? hlen.i()[r] : 0, hist.ok() ? plen.i()[r] : 0, mrow.ok() ? mrow.i()[r] : 0);
     return !__syncthreads_or(bad);
   }
 };
@@ -935,61 +1025,112 @@ __device__ __forceinline__ float adjusted(float x, uint32_t w, float rep, float 
   return x;
 }
 __device__ __forceinline__ void lds_or(LDS uint32_t* p, uint32_t v) { __hip_atomic_fetch_or(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP); }
+// Logits [v0, v0 + len) of a row as a stream from xp to op, -inf where the mask row (or none) forbids. VL logits a vector; `first` runs
+// once the first vectors are requested. Rows whose bf16 storage is never 4-byte aligned on both sides go one by one.
+template <bool XH, bool OH, class F>
+__device__ __forceinline__ void adjust_stream(const GLOBAL char* xp, const GLOBAL char* op, const GLOBAL int* mask, int v0, int len, F first) {
+  constexpr int NB = XH ? 16 : 8, VL = 4;                              // 32 KB in flight
+  const int px = XH ? (int)((uintptr_t)xp >> 1) & 1 : 0, po = OH ? (int)((uintptr_t)op >> 1) & 1 : 0;
+  const int peel = min(len, max(px, po)), nv = XH && OH && px != po ? 0 : (len - peel) / VL;
+  u32x4_t x[NB];                                                       // (bf16: the first half)
+  uint32_t m0[NB], m1[NB];
+  auto request = [&](int base) {
+#pragma unroll
+    for (int u = 0; u < NB; ++u) {
+      const int i = peel + VL * min(base + tid() + u * KVM_THREADS, nv - 1), v = v0 + i;
+      if (XH) { const u32x2_t t = *(const GLOBAL u32x2a4*)(xp + 2ll * i); x[u].x = t.x; x[u].y = t.y; }
+      else x[u] = *(const GLOBAL u32x4a4*)(xp + 4ll * i);
+      m0[u] = m1[u] = ~0u;
+      if (mask) { m0[u] = mask[v >> 5]; m1[u] = mask[(v + VL - 1) >> 5]; }      // a vector's bits may lie in two words
+    }
+  };
+  if (nv) request(0);
+  first();
+  for (int base = 0; base < nv; base += NB * KVM_THREADS) {
+    float y[NB][VL];
+    uint32_t bits[NB];
+#pragma unroll
+    for (int u = 0; u < NB; ++u) {
+      const int sh = (v0 + peel + VL * (base + tid() + u * KVM_THREADS)) & 31;
+#pragma unroll
+      for (int e = 0; e < VL; ++e) y[u][e] = __uint_as_float(!XH ? x[u][e % 4] : e & 1 ? x[u][e / 2] & 0xffff0000u : x[u][e / 2] << 16);
+      bits[u] = (uint32_t)((((uint64_t)m1[u] << 32) | m0[u]) >> sh);
+    }
+    if (base + NB * KVM_THREADS < nv) request(base + NB * KVM_THREADS);
+    // a descriptor for the round's vectors: what lies past the last one is out of its range and not stored
+    const __amdgpu_buffer_rsrc_t ro = wt_rsrc((const char*)op + (peel + (long long)VL * base) * (OH ? 2 : 4), (long long)min(VL * NB * KVM_THREADS, VL * (nv - base)) * (OH ? 2 : 4));
+#pragma unroll
+    for (int u = 0; u < NB; ++u) {
+      const int i = VL * (tid() + u * KVM_THREADS);
+#pragma unroll
+      for (int e = 0; e < VL; ++e) if (!((bits[u] >> e) & 1)) y[u][e] = -INFINITY;
+      const f32x4n f = {y[u][0], y[u][1], y[u][2], y[u][3]};
+      if (OH) stwt_bf4_buf(ro, 2 * i, f); else stwt_buf(ro, 4 * i, f);
+    }
+  }
+  for (int k = tid(); k < len - VL * nv; k += KVM_THREADS) {            // before the first vector and behind the last
+    const int i = k < peel ? k : k + VL * nv, v = v0 + i;
+    float y = XH ? bf2f(((const GLOBAL uint16_t*)xp)[i]) : ((const GLOBAL float*)xp)[i];
+    if (mask && !((mask[v >> 5] >> (v & 31)) & 1)) y = -INFINITY;
+    if (OH) stwt16((GLOBAL uint16_t*)op + i, f2bf(y)); else stwt32((GLOBAL float*)op + i, y);
+  }
+}
 __device__ __noinline__ void op_logits_adjust(const Ctx& c) {
   const AdjustArgs A(c);
-  if (!A.rows_ok(c)) return;
-  LDS uint32_t* cnt = (LDS uint32_t*)c.smem;                           // [ADJ_CHUNK + 8]
-  LDS float* bsum = (LDS float*)(cnt + ADJ_CHUNK + 8);                 // [ADJ_BIAS + 1] an entry's value, the first one's the sum
+  LDS uint32_t* cnt = (LDS uint32_t*)c.smem;                           // [ADJ_CHUNK]
+  LDS float* bsum = (LDS float*)(cnt + ADJ_CHUNK);                     // [ADJ_BIAS + 1] an entry's value, the first one's the sum
   LDS int* later = (LDS int*)(bsum + ADJ_BIAS + 1);                    // [ADJ_BIAS + 1] first entry of the same token, or -1
-  static_assert((ADJ_CHUNK + 8 + 2 * (ADJ_BIAS + 1)) * 4 <= KVM_LDS_BYTES, "logits LDS map");
-  constexpr int NB = ADJ_NB;
-  const int nb = A.bidx.ok() ? A.bidx.cols : 0;
+  static_assert((ADJ_CHUNK + 2 * (ADJ_BIAS + 1)) * 4 <= KVM_LDS_BYTES, "logits LDS map");
+  constexpr int NH = 4;                                                // vectors of tokens in flight
+  const int nb = A.bidx.ok() ? A.bidx.cols : 0, len = A.v1 - A.v0;
   const bool xh = A.x.dtype == 2, oh = A.out.dtype == 2;
-  for (int r = A.r0; r < A.r1; ++r) {
+  if (A.r1 - A.r0 > 1 && !A.rows_ok(c)) return;
+  for (int r = A.r0; r < A.r1 && len > 0; ++r) {
     const float rep = A.par.at(r, 0), freq = A.par.at(r, 1), pres = A.par.at(r, 2);
-    const int n = A.hist.ok() ? A.hlen.i()[r] : 0, pl = A.hist.ok() ? A.plen.i()[r] : 0, last = A.last.ok() ? A.last.i()[r] : -1;
+    const int n = A.hist.ok() ? rfl(A.hlen.i()[r]) : 0, pl = A.hist.ok() ? rfl(A.plen.i()[r]) : 0, last = A.last.ok() ? rfl(A.last.i()[r]) : -1;
+    const int mr = A.mask.ok() ? (A.mrow.ok() ? rfl(A.mrow.i()[r]) : r) : -1;
+    if (!A.row_ok(c, r, n, pl, mr)) return;
     const GLOBAL int* hist = A.hist.ok() ? A.hist.i() + (long long)r * A.hist.cols : nullptr;
     const GLOBAL int* bidx = nb ? A.bidx.i() + (long long)r * A.bidx.cols : nullptr;
-    const int mr = A.mask.ok() ? (A.mrow.ok() ? A.mrow.i()[r] : r) : -1;
+    const GLOBAL float* bval = nb ? A.bval.f() + (long long)r * A.bval.cols : nullptr;
     const GLOBAL int* mask = mr >= 0 ? A.mask.i() + (long long)mr * A.mask.cols : nullptr;
-    for (int c0 = A.v0; c0 < A.v1; c0 += ADJ_CHUNK) {
-      const int len = min(A.v1 - c0, ADJ_CHUNK);
-      const GLOBAL char* xp = (const GLOBAL char*)A.x.p + ((long long)r * A.x.cols + c0) * (xh ? 2 : 4);
-      const GLOBAL char* op = (const GLOBAL char*)A.out.p + ((long long)r * A.out.cols + c0) * (oh ? 2 : 4);
-      // vectors start where bf16 storage is 4-byte aligned, on both sides; rows that never are go one by one
-      const int px = xh ? (int)((uintptr_t)xp >> 1) & 1 : 0, po = oh ? (int)((uintptr_t)op >> 1) & 1 : 0;
-      const int peel = min(len, max(px, po)), nv = xh && oh && px != po ? 0 : (len - peel) / 4;
-      const bool whole = ((c0 + peel) & 3) == 0;                       // no vector's mask bits lie in two words
-      LDS uint32_t* w = cnt + (4 - peel) % 4;                          // word of logit c0 + i: w[i], a vector's at 16 bytes
-      const __amdgpu_buffer_rsrc_t ro = wt_rsrc((const char*)op, (long long)len * (oh ? 2 : 4));
-      u32x4_t x[NB];
-      uint32_t m0[NB], m1[NB];
-      auto request = [&](int q0) {
+    const bool named = n || nb || last >= 0;
+    // the tokens of this thread, four at a time: of the history, and (fewer than four, and the token chosen last) behind it
+    u32x4_t h[NH];
+    auto tokens = [&](int k0) {
 #pragma unroll
-        for (int u = 0; u < NB; ++u) {
-          const int i = peel + 4 * min(q0 + u * KVM_THREADS, nv - 1), v = c0 + i;
-          if (xh) { const u32x2_t t = *(const GLOBAL u32x2a4*)(xp + 2 * i); x[u].x = t.x; x[u].y = t.y; }
-          else x[u] = *(const GLOBAL u32x4a4*)(xp + 4 * i);
-          m0[u] = m1[u] = ~0u;
-          if (mask) { m0[u] = mask[v >> 5]; if (!whole) m1[u] = mask[(v + 3) >> 5]; }
+      for (int u = 0; u < NH; ++u) if (k0 + 4 * u * KVM_THREADS < n / 4 * 4) h[u] = *(const GLOBAL u32x4a4*)(hist + k0 + 4 * u * KVM_THREADS);
+    };
+    auto visit = [&](auto f) {
+      for (int k0 = 4 * tid(); k0 < n / 4 * 4; k0 += 4 * NH * KVM_THREADS) {
+        if (n >= 4 * NH * KVM_THREADS) tokens(k0);                     // else they are there
+#pragma unroll
+        for (int u = 0; u < NH; ++u) {
+          const int k = k0 + 4 * u * KVM_THREADS;
+          const int t[4] = {(int)h[u].x, (int)h[u].y, (int)h[u].z, (int)h[u].w};
+          if (k < n / 4 * 4) f(k, t);
         }
-      };
-      if (tid() < nv) request(tid());
+      }
+      const int rest = n / 4 * 4 + tid();
+      const int t[4] = {rest < n ? hist[rest] : rest == n ? last : -1, -1, -1, -1};
+      if (rest <= n) f(rest, t);
+    };
+    auto count = [&](int c0, int most) {
       __syncthreads();
-      for (int i = tid(); i < (len + 11) / 4; i += KVM_THREADS) ((LDS u32x4_t*)cnt)[i] = u32x4_t{0, 0, 0, 0};
+      for (int i = tid(); i < (most + 3) / 4; i += KVM_THREADS) ((LDS u32x4_t*)cnt)[i] = u32x4_t{0, 0, 0, 0};
       __syncthreads();
       if (nb) {
         for (int j = tid(); j < nb; j += KVM_THREADS) {
           const int v = bidx[j] - c0;
-          if (v >= 0 && v < len) __hip_atomic_fetch_max(&w[v], (uint32_t)(ADJ_BIAS - j) << 20, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+          bsum[j] = bval[j];
+          if (v >= 0 && v < most) __hip_atomic_fetch_max(&cnt[v], (uint32_t)(ADJ_BIAS - j) << 20, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
         }
         __syncthreads();
         bool many = false;
         for (int j = tid(); j < nb; j += KVM_THREADS) {
-          const int v = bidx[j] - c0, first = v >= 0 && v < len ? ADJ_BIAS - (int)(w[v] >> 20) : j;
-          bsum[j] = A.bval.f()[(long long)r * A.bval.cols + j];
-          later[j] = first == j ? -1 : first;
-          many = many || first != j;
+          const int v = bidx[j] - c0, one = v >= 0 && v < most ? ADJ_BIAS - (int)(cnt[v] >> 20) : j;
+          later[j] = one == j ? -1 : one;
+          many = many || one != j;
         }
         if (__syncthreads_or(many) && wave() == 0)                     // entries of one token, in list order
           for (int j0 = 0; j0 < nb; j0 += 64) {
@@ -1000,59 +1141,46 @@ __device__ __noinline__ void op_logits_adjust(const Ctx& c) {
             }
           }
       }
-      auto said = [&](int k, int token) {
-        const int v = token - c0;
-        if (v < 0 || v >= len) return;
-        if (k < pl) lds_or(&w[v], 0x80000000u);
-        else __hip_atomic_fetch_add(&w[v], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-      };
-      for (int k0 = 4 * tid(); k0 < n / 4 * 4; k0 += 16 * KVM_THREADS) {
-        u32x4_t h[4];
+      visit([&](int k, const int (&t)[4]) {
 #pragma unroll
-        for (int u = 0; u < 4; ++u) h[u] = *(const GLOBAL u32x4a4*)(hist + min(k0 + 4 * u * KVM_THREADS, n / 4 * 4 - 4));
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int k = k0 + 4 * u * KVM_THREADS;
-          if (k >= n / 4 * 4) break;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) said(k + e, (int)h[u][e]);
+        for (int e = 0; e < 4; ++e) {
+          const int v = t[e] - c0;
+          if (t[e] < 0 || v < 0 || v >= most) continue;
+          if (k + e < pl) lds_or(&cnt[v], 0x80000000u);
+          else __hip_atomic_fetch_add(&cnt[v], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
         }
-      }
-      if (tid() < n % 4) said(n / 4 * 4 + tid(), hist[n / 4 * 4 + tid()]);
-      if (tid() == 4) said(n, last);
+      });
+    };
+    auto first = [&] {
+      if (n && n < 4 * NH * KVM_THREADS) tokens(4 * tid());
+      if (named) count(A.v0, min(len, ADJ_CHUNK));
+    };
+    const GLOBAL char* xp = (const GLOBAL char*)A.x.p + ((long long)r * A.x.cols + A.v0) * (xh ? 2 : 4);
+    const GLOBAL char* op = (const GLOBAL char*)A.out.p + ((long long)r * A.out.cols + A.v0) * (oh ? 2 : 4);
+    if (!mask && A.out.p == A.x.p) first();
+    else if (xh) { if (oh) adjust_stream<true, true>(xp, op, mask, A.v0, len, first); else adjust_stream<true, false>(xp, op, mask, A.v0, len, first); }
+    else { if (oh) adjust_stream<false, true>(xp, op, mask, A.v0, len, first); else adjust_stream<false, false>(xp, op, mask, A.v0, len, first); }
+    for (int c0 = A.v0; c0 < A.v1 && named; c0 += ADJ_CHUNK) {         // the named tokens again
+      const int most = min(A.v1 - c0, ADJ_CHUNK);
+      if (c0 > A.v0) count(c0, most);
+      wait_stores();                                                   // the stream's values of these logits are out
       __syncthreads();
-      for (int q0 = tid(); q0 < nv; q0 += NB * KVM_THREADS) {
-        f32x4n y[NB];
-        uint32_t bits[NB];
+      auto again = [&](const int (&t)[4]) {
+        uint32_t w[4];
+        float x[4];
+        bool ok[4];
 #pragma unroll
-        for (int u = 0; u < NB; ++u) {
-          const int sh = (c0 + peel + 4 * (q0 + u * KVM_THREADS)) & 31;
-          if (xh) y[u] = __builtin_bit_cast(f32x4n, u32x4_t{x[u].x << 16, x[u].x & 0xffff0000u, x[u].y << 16, x[u].y & 0xffff0000u});
-          else y[u] = __builtin_bit_cast(f32x4n, x[u]);
-          bits[u] = (uint32_t)((((uint64_t)m1[u] << 32) | m0[u]) >> sh);
+        for (int e = 0; e < 4; ++e) {
+          const int v = t[e] - c0;
+          w[e] = t[e] >= 0 && v >= 0 && v < most ? __hip_atomic_exchange(&cnt[v], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP) : 0u;
+          if (w[e]) { x[e] = A.x.at(r, t[e]); ok[e] = !mask || ((mask[t[e] >> 5] >> (t[e] & 31)) & 1); }
         }
-        if (q0 + NB * KVM_THREADS < nv) request(q0 + NB * KVM_THREADS);
 #pragma unroll
-        for (int u = 0; u < NB; ++u) {
-          const int q = q0 + u * KVM_THREADS, i = peel + 4 * q;
-          if (q >= nv) break;
-          const u32x4_t t = *(const LDS u32x4_t*)(w + i);
-          if (t.x | t.y | t.z | t.w) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) y[u][e] = adjusted(y[u][e], t[e], rep, freq, pres, bsum);
-          }
-#pragma unroll
-          for (int e = 0; e < 4; ++e) if (!((bits[u] >> e) & 1)) y[u][e] = -INFINITY;
-          if (oh) stwt_bf4_buf(ro, 2 * i, y[u]);
-          else stwt_buf(ro, 4 * i, y[u]);
-        }
-      }
-      for (int k = tid(); k < len - 4 * nv; k += KVM_THREADS) {         // before the first vector and behind the last
-        const int i = k < peel ? k : k + 4 * nv, v = c0 + i;
-        float y = adjusted(A.x.at(r, v), w[i], rep, freq, pres, bsum);
-        if (mask && !((mask[v >> 5] >> (v & 31)) & 1)) y = -INFINITY;
-        A.out.st((long long)r * A.out.cols + v, y);
-      }
+        for (int e = 0; e < 4; ++e)
+          if (w[e]) A.out.st((long long)r * A.out.cols + t[e], ok[e] ? adjusted(x[e], w[e], rep, freq, pres, bsum) : -INFINITY);
+      };
+      visit([&](int, const int (&t)[4]) { again(t); });
+      for (int j = tid(); j < nb; j += KVM_THREADS) { const int t[4] = {bidx[j], -1, -1, -1}; again(t); }
     }
     if (A.last.ok() && A.v0 == 0 && tid() == 0) stwt32i(A.hist.i() + ((long long)r * A.hist.cols + n), last);
   }

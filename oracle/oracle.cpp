@@ -814,12 +814,12 @@ void op_kv_append_q8(const Ctx& c) {
   for (int b = b0; b < b1; ++b) {
     const long long L = lens.i[b];
     if (L < 0) continue;
-    const long long j0 = L / blk, jE = (L + n) / blk, mid = std::max(0ll, jE - j0 - 1), m0 = j0 + 1 + mid * p / P, m1 = j0 + 1 + mid * (p + 1) / P;
+    const long long j0 = L / blk, jE = (L + n) / blk, per = (jE - j0 + P - 1) / P, m0 = std::min(jE, j0 + p * per), m1 = std::min(jE, m0 + per);
     for (int h = h0; h < h1; ++h) for (int w = 0; w < 2; ++w) {
       const V &src = w ? vn : kn, &tail = w ? vt : kt, &Q = w ? vq : kq, &S = w ? vs : ks;
       const long long pair = (long long)b * Hkv + h;
       for (long long j = j0; j <= jE; ++j) {
-        if (j == j0 || j == jE ? p != 0 : j < m0 || j >= m1) continue;
+        if (j == jE ? p != 0 : j < m0 || j >= m1) continue;
         std::vector<float> x((size_t)blk * hd);
         double amax = 0; bool finite = true;
         for (int r = 0; r < blk; ++r) {
