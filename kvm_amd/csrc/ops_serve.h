@@ -246,7 +246,8 @@ __device__ __noinline__ void op_kv_append_q8(const Ctx& c) {
 // for single tokens, bytes for prompts. A row is HD / 8 lanes of 8 values, so a pass of the workgroup takes 16 or 32 rows.
 // The tail rows of all pairs of the task go in one range, a row to HD / 8 lanes; blocks that become full (of single tokens one call in
 // blk) are a function of their own, whose registers the tail rows' callers need not save.
-// A full block is in registers as a whole, all its loads requested before any is used, K and V with one reduction of both maxima.
+// A full block is in registers as a whole, all its loads requested before any is used, K and V together with one reduction of both
+// maxima (of the largest blocks one after the other: their registers would be most of a worker's scratch).
 // Keys to be normalised or rotated
 // go through LDS first, row by row. Keys are stored as they lie, 8 bytes a lane; values turn through LDS.
 template <int HD> struct AppendLds {
@@ -256,6 +257,7 @@ template <int HD> struct AppendLds {
 };
 template <int HD, int NP> __device__ __noinline__ void append_q8_blocks(const Ctx& c) {
   constexpr int LPR = HD / 8, RPP = KVM_THREADS / LPR;                 // lanes a row, rows a pass; NP passes hold a block
+  constexpr int NX = NP > 4 ? 1 : 2;                                   // K and V at once, blocks of more than four passes one after the other
   const AppendQ8 A(c);
   const AppendLds<HD> M(c.smem);                                       // keys [blk][HD], turn [HD][blk + 4]
   const int ln = tid() % LPR, rw = tid() / LPR, blk = A.blk;
@@ -287,61 +289,82 @@ template <int HD, int NP> __device__ __noinline__ void append_q8_blocks(const Ct
           for (int e = 0; e < 8; ++e) M.keys[r * HD + 8 * ln + e] = x[e];
         }
       }
-      Raw8 rk[NP], rv[NP];
+#pragma unroll 1
+      for (int x0 = 0; x0 < 2; x0 += NX) {
+        Raw8 raw[NX][NP];
+        float v[NX][NP][8], scale[NX], inv[NX];
+        auto of = [&](int x, const View& k, const View& w) { return NX == 2 ? (x ? w : k) : (x0 ? w : k); };   // of K or of V
 #pragma unroll
-      for (int i = 0; i < NP; ++i) {
-        const int r = i * RPP + rw;
-        if (r >= blk) break;
-        const bool in_tail = r < old;
-        if (!turned) rk[i].load(in_tail ? A.kt : A.kn, in_tail ? (tail0 + r) * A.kt.cols + 8 * ln : (new0 + r) * A.kn.cols + h * HD + 8 * ln);
-        rv[i].load(in_tail ? A.vt : A.vn, in_tail ? (tail0 + r) * A.vt.cols + 8 * ln : (new0 + r) * A.vn.cols + h * HD + 8 * ln);
-      }
-      float k[NP][8], v[NP][8];
-      uint32_t ka = 0, va = 0;                                        // largest magnitudes by their bits: what is not finite is largest
+        for (int x = 0; x < NX; ++x) {
+          const View tl = of(x, A.kt, A.vt), nw = of(x, A.kn, A.vn);
+          if ((NX == 2 ? x : x0) == 0 && turned) continue;
 #pragma unroll
-      for (int i = 0; i < NP; ++i) {
-        const int r = i * RPP + rw;
-        if (r >= blk) break;
-        if (turned) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) k[i][e] = M.keys[r * HD + 8 * ln + e];    // this thread's own
-        } else rk[i].get(r < old ? tkh : nkh, k[i]);
-        rv[i].get(r < old ? tvh : nvh, v[i]);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          if (kround) k[i][e] = round_bf(k[i][e]);
-          if (vround) v[i][e] = round_bf(v[i][e]);
-          ka = max(ka, __float_as_uint(k[i][e]) & 0x7fffffffu); va = max(va, __float_as_uint(v[i][e]) & 0x7fffffffu);
+          for (int i = 0; i < NP; ++i) {
+            const int r = i * RPP + rw;
+            if (r >= blk) break;
+            raw[x][i].load(r < old ? tl : nw, r < old ? (tail0 + r) * tl.cols + 8 * ln : (new0 + r) * nw.cols + h * HD + 8 * ln);
+          }
         }
-      }
-      const float km = rows_max(lanes_max<16>(__uint_as_float(min(ka, 0x7f800000u)))), vm = rows_max(lanes_max<16>(__uint_as_float(min(va, 0x7f800000u))));
-      __syncthreads();                                                 // the block before is out of `turn` and `red`
-      if (lane() == 0) { M.red[wave()] = km; M.red[4 + wave()] = vm; }
-      __syncthreads();
-      const float sk = q8_scale(fmaxf(fmaxf(M.red[0], M.red[1]), fmaxf(M.red[2], M.red[3]))), ik = sk > 0.f ? 1.f / sk : 0.f;
-      const float sv = q8_scale(fmaxf(fmaxf(M.red[4], M.red[5]), fmaxf(M.red[6], M.red[7]))), iv = sv > 0.f ? 1.f / sv : 0.f;
-      if (tid() == 0) { stwt32(A.ks.f() + (pair * A.ks.cols + j), sk); stwt32(A.vs.f() + (pair * A.vs.cols + j), sv); }
-      const long long byte0 = (pair * A.nblk + j) * blk * HD;
-      const __amdgpu_buffer_rsrc_t ok = wt_rsrc((const char*)A.kq.p + byte0, blk * HD), ov = wt_rsrc((const char*)A.vq.p + byte0, blk * HD);
 #pragma unroll
-      for (int i = 0; i < NP; ++i) {
-        const int r = i * RPP + rw;
-        if (r >= blk) break;
-        uint32_t w0, w1, x0, x1;
-        q8_pack(k[i], sk, ik, w0, w1);
-        q8_pack(v[i], sv, iv, x0, x1);
-        __builtin_amdgcn_raw_buffer_store_b64(u32x2_t{w0, w1}, ok, r * HD + 8 * ln, 0, 16 /* SC1 */);
-        LDS unsigned char* col = M.turn + 8 * ln * (blk + 4) + r;
+        for (int x = 0; x < NX; ++x) {
+          const bool key = (NX == 2 ? x : x0) == 0, round = key ? kround : vround, th = key ? tkh : tvh, nh_ = key ? nkh : nvh;
+          uint32_t big = 0;                                            // largest magnitude by its bits: what is not finite is largest
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          col[e * (blk + 4)] = (unsigned char)(x0 >> (8 * e));
-          col[(4 + e) * (blk + 4)] = (unsigned char)(x1 >> (8 * e));
+          for (int i = 0; i < NP; ++i) {
+            const int r = i * RPP + rw;
+            if (r >= blk) break;
+            if (key && turned) {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) v[x][i][e] = M.keys[r * HD + 8 * ln + e];     // this thread's own
+            } else raw[x][i].get(r < old ? th : nh_, v[x][i]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              if (round) v[x][i][e] = round_bf(v[x][i][e]);
+              big = max(big, __float_as_uint(v[x][i][e]) & 0x7fffffffu);
+            }
+          }
+          scale[x] = rows_max(lanes_max<16>(__uint_as_float(min(big, 0x7f800000u))));
         }
-      }
-      __syncthreads();
-      for (int e = tid(); e < HD * blk / 16; e += KVM_THREADS) {
-        const LDS uint32_t* x = (const LDS uint32_t*)(M.turn + (16 * e >> lb) * (blk + 4) + (16 * e & (blk - 1)));
-        stwt_buf(ov, 16 * e, __builtin_bit_cast(f32x4n, u32x4_t{x[0], x[1], x[2], x[3]}));
+        __syncthreads();                                               // the block before is out of `turn` and `red`
+#pragma unroll
+        for (int x = 0; x < NX; ++x) if (lane() == 0) M.red[4 * x + wave()] = scale[x];
+        __syncthreads();
+#pragma unroll
+        for (int x = 0; x < NX; ++x) {
+          const LDS float* m = M.red + 4 * x;
+          scale[x] = q8_scale(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])));
+          inv[x] = scale[x] > 0.f ? 1.f / scale[x] : 0.f;
+          const View sc = of(x, A.ks, A.vs);
+          if (tid() == 0) stwt32(sc.f() + (pair * sc.cols + j), scale[x]);
+        }
+        const long long byte0 = (pair * A.nblk + j) * blk * HD;
+        const __amdgpu_buffer_rsrc_t ok = wt_rsrc((const char*)A.kq.p + byte0, blk * HD), ov = wt_rsrc((const char*)A.vq.p + byte0, blk * HD);
+#pragma unroll
+        for (int x = 0; x < NX; ++x) {
+          const bool key = (NX == 2 ? x : x0) == 0;
+#pragma unroll
+          for (int i = 0; i < NP; ++i) {
+            const int r = i * RPP + rw;
+            if (r >= blk) break;
+            uint32_t w0, w1;
+            q8_pack(v[x][i], scale[x], inv[x], w0, w1);
+            if (key) __builtin_amdgcn_raw_buffer_store_b64(u32x2_t{w0, w1}, ok, r * HD + 8 * ln, 0, 16 /* SC1 */);
+            else {
+              LDS unsigned char* col = M.turn + 8 * ln * (blk + 4) + r;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                col[e * (blk + 4)] = (unsigned char)(w0 >> (8 * e));
+                col[(4 + e) * (blk + 4)] = (unsigned char)(w1 >> (8 * e));
+              }
+            }
+          }
+        }
+        if (NX == 1 && x0 == 0) continue;
+        __syncthreads();
+        for (int e = tid(); e < HD * blk / 16; e += KVM_THREADS) {
+          const LDS uint32_t* w = (const LDS uint32_t*)(M.turn + (16 * e >> lb) * (blk + 4) + (16 * e & (blk - 1)));
+          stwt_buf(ov, 16 * e, __builtin_bit_cast(f32x4n, u32x4_t{w[0], w[1], w[2], w[3]}));
+        }
       }
     }
   }
@@ -642,7 +665,8 @@ __device__ __forceinline__ void q8_arrive(const Ctx& c, const DecodeQ8& D, int b
 
 // Decode attention over the 8-bit cache at head sizes 64 and 128, on the matrix units. Bound: streaming the cache's bytes, and
 // where few workers stream at once the ~550 vector instructions of a unit.
-// Each wave takes units of 64 tokens in turn, K and V straight from memory into registers in the layout of the operands, a unit ahead:
+// Each wave takes units of 64 tokens in turn, K and V straight from memory into registers in the layout of the operands, one to two
+// units ahead:
 //   scores  v_mfma_i32_16x16x64_i8, A = 16 keys as they lie, B = up to 16 query rows (NT such tiles) as three signed bytes of a
 //           fixed-point number per value (22 bits below a power of two above the row's largest): whole numbers, summed exactly.
 //           A lane's 16-byte load of a key is its part of the operand.
@@ -668,7 +692,8 @@ __device__ __forceinline__ f16x8 q8_half(uint32_t w0, uint32_t w1) {
   for (int i = 0; i < 4; ++i) { x[i] += off; r[2 * i] = x[i].x; r[2 * i + 1] = x[i].y; }
   return r;
 }
-template <int HD> struct UnitQ8 { u32x4_t k[4][HD / 64], v[HD / 16]; float ks, vs; };
+template <int HD> struct KeysQ8 { u32x4_t k[4][HD / 64]; float s; };
+template <int HD> struct ValuesQ8 { u32x4_t v[HD / 16]; float s; };
 // LDS of a task. The work and the frequencies stay through its pieces; the tail's scores and values give way to the waves' P V.
 template <int HD> struct DecodeLds {
   LDS int* pre; LDS int* len; LDS double* freq; LDS float* qs; LDS float* to; LDS float* st; LDS float* cr; LDS float* ts; LDS float* tv;
@@ -701,18 +726,23 @@ template <int HD, int NT> __device__ __noinline__ void attn_q8_piece(const Ctx& 
   const GLOBAL char* V = (const GLOBAL char*)D.vq.p + byte0;
   const GLOBAL float* KS = D.ks.f() + pair * D.ks.cols;
   const GLOBAL float* VS = D.vs.f() + pair * D.vs.cols;
-  auto load = [&](UnitQ8<HD>& U, int u) {                              // tokens past the last whole block: the last ones again, masked below
+  // (tokens past the last whole block: the last ones again, masked later)
+  auto load_keys = [&](KeysQ8<HD>& U, int u) {
     const int t0 = u << 6, rest = whole - t0;
     const GLOBAL char* kb = K + (long long)t0 * HD;
 #pragma unroll
     for (int a = 0; a < 4; ++a)
 #pragma unroll
-      for (int h = 0; h < KH; ++h) U.k[a][h] = *(const GLOBAL u32x4a4*)(kb + min(16 * (nn >> 2) + 4 * a + (nn & 3), rest - 1) * HD + 16 * (qq + 4 * h));
-    const int tt = (t0 & (blk - 1)) + min(16 * qq, rest - 16), j = tt >> lb;   // from the start of the block of t0
-    const GLOBAL char* vb = V + ((long long)(t0 >> lb) << lb) * HD + j * blk * HD + (tt & (blk - 1));
+      for (int h = 0; h < KH; ++h) U.k[a][h] = *(const GLOBAL u32x4a4*)(kb + (min(16 * (nn >> 2) + 4 * a + (nn & 3), rest - 1) * HD + 16 * (qq + 4 * h)));
+    U.s = KS[(t0 + min(16 * qq, rest - 16)) >> lb];
+  };
+  auto load_values = [&](ValuesQ8<HD>& U, int u) {
+    const int t0 = u << 6, tt = (t0 & (blk - 1)) + min(16 * qq, whole - t0 - 16), j = tt >> lb;   // from the start of the block of t0
+    const GLOBAL char* vb = V + ((long long)(t0 >> lb) << lb) * HD;
+    const int at = j * blk * HD + (tt & (blk - 1)) + nn * blk;
 #pragma unroll
-    for (int d = 0; d < VT; ++d) U.v[d] = *(const GLOBAL u32x4a4*)(vb + (16 * d + nn) * blk);
-    U.ks = KS[(t0 >> lb) + j]; U.vs = VS[(t0 >> lb) + j];
+    for (int d = 0; d < VT; ++d) U.v[d] = *(const GLOBAL u32x4a4*)(vb + (at + 16 * d * blk));
+    U.s = VS[(t0 >> lb) + j];
   };
   // everything that a short context needs is requested at once: query rows, the unfinished block, the first unit
   constexpr int QP = (16 * NT + RPP - 1) / RPP, TP = 4;
@@ -727,8 +757,11 @@ template <int HD, int NT> __device__ __noinline__ void attn_q8_piece(const Ctx& 
     }
   };
   if (tail) load_tail(0);
-  UnitQ8<HD> U;
-  if (u0 + w < u1) load(U, u0 + w);
+  constexpr int NK = NT * HD > 128 ? 1 : 2;                            // units of keys under way; two tiles of 128 have registers for one
+  KeysQ8<HD> keys[NK];
+  ValuesQ8<HD> U;
+  if (u0 + w < u1) { load_keys(keys[0], u0 + w); load_values(U, u0 + w); }
+  if (NK > 1 && u0 + w + KVM_WAVES < u1) load_keys(keys[NK - 1], u0 + w + KVM_WAVES);
   // query rows: norm, rotation, then scaled by a power of two to magnitudes below 2^22
 #pragma unroll
   for (int i = 0; i < QP; ++i) {
@@ -820,7 +853,11 @@ template <int HD, int NT> __device__ __noinline__ void attn_q8_piece(const Ctx& 
     }
   }
   // the queries as B operands: row nn of tile g, dims 64 h + 16 qq .., byte p of the fixed-point numbers
-  i32x4_t qb[NT][KH][3];
+  // (two tiles keep them in LDS, over the tail's scores: the same from every wave)
+  i32x4_t qb[NT == 1 ? KH : 1][3];
+  LDS i32x4_t* ql = (LDS i32x4_t*)ts + l;                              // [NT][KH][3][64]
+  auto query = [&](int g, int h, int p) { return NT == 1 ? qb[NT == 1 ? h : 0][p] : ql[((g * KH + h) * 3 + p) * 64]; };
+  if (NT > 1 && tail) __syncthreads();                                 // the scores have been read
   float mrun[NT], lrun[NT], crow[NT];
   int lim[NT];
   f32x4n o[NT][VT];
@@ -828,34 +865,30 @@ template <int HD, int NT> __device__ __noinline__ void attn_q8_piece(const Ctx& 
   for (int g = 0; g < NT; ++g) {
     const int r = 16 * g + nn;
 #pragma unroll
-    for (int h = 0; h < KH; ++h)
+    for (int h = 0; h < KH; ++h) {
+      i32x4_t q[3];
 #pragma unroll
       for (int v = 0; v < 4; ++v) {
         uint32_t y[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) y[e] = ((uint32_t)(int)rintf(qs[r * QS + 64 * h + 16 * qq + 4 * v + e]) + 0x808080u) ^ 0x808080u;
         const uint32_t a01 = __builtin_amdgcn_perm(y[1], y[0], 0x05010400u), a23 = __builtin_amdgcn_perm(y[3], y[2], 0x05010400u);
-        qb[g][h][0][v] = (int)__builtin_amdgcn_perm(a23, a01, 0x05040100u);
-        qb[g][h][1][v] = (int)__builtin_amdgcn_perm(a23, a01, 0x07060302u);
-        qb[g][h][2][v] = (int)__builtin_amdgcn_perm(__builtin_amdgcn_perm(y[3], y[2], 0x0c0c0602u), __builtin_amdgcn_perm(y[1], y[0], 0x0c0c0602u), 0x05040100u);
+        q[0][v] = (int)__builtin_amdgcn_perm(a23, a01, 0x05040100u);
+        q[1][v] = (int)__builtin_amdgcn_perm(a23, a01, 0x07060302u);
+        q[2][v] = (int)__builtin_amdgcn_perm(__builtin_amdgcn_perm(y[3], y[2], 0x0c0c0602u), __builtin_amdgcn_perm(y[1], y[0], 0x0c0c0602u), 0x05040100u);
       }
+#pragma unroll
+      for (int p = 0; p < 3; ++p) { if (NT == 1) qb[h][p] = q[p]; else ql[((g * KH + h) * 3 + p) * 64] = q[p]; }
+    }
     crow[g] = cr[r]; mrun[g] = -INFINITY; lrun[g] = 0.f;
     lim[g] = r < D.R ? min(whole, L + r / D.G + 1) : 0;
 #pragma unroll
     for (int d = 0; d < VT; ++d) o[g][d] = f32x4n{0.f, 0.f, 0.f, 0.f};
   }
   float vref = 1.17549435e-38f;
-  // one unit; ALL: every row sees every token of it
-  auto unit = [&](int u, auto all) {
-    constexpr bool ALL = decltype(all)::value;
-    const float vm = rows_max(U.vs == U.vs ? U.vs : 0.f);
-    float fv = 1.f;
-    if (vm > vref) {                                                   // uniform: the four lane groups hold the unit's scales
-      const float nv = __uint_as_float((__float_as_uint(vm) & 0x7f800000u) + 0x00800000u);
-      fv = vref * __uint_as_float(0x7f000000u - __float_as_uint(nv));
-      vref = nv;
-    }
-    const float pv = U.vs * __uint_as_float(0x7f000000u - __float_as_uint(vref)) * PS;
+  // one unit, its keys in C: the keys of this wave's unit after the next (of its next) are requested into C once the scores are there,
+  // the next unit's values once the P V is
+  auto unit = [&](int u, KeysQ8<HD>& C) {
     float sc[NT][16];
 #pragma unroll
     for (int a = 0; a < 4; ++a) {
@@ -869,27 +902,43 @@ template <int HD, int NT> __device__ __noinline__ void attn_q8_piece(const Ctx& 
 #pragma unroll
         for (int g = 0; g < NT; ++g)
 #pragma unroll
-          for (int p = 0; p < 3; ++p) s[g][p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4_t, U.k[a][h]), qb[g][h][p], s[g][p], 0, 0, 0);
+          for (int p = 0; p < 3; ++p) s[g][p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4_t, C.k[a][h]), query(g, h, p), s[g][p], 0, 0, 0);
 #pragma unroll
       for (int g = 0; g < NT; ++g)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sc[g][4 * a + i] = fmaf((float)((s[g][2][i] << 8) + s[g][1][i]), 256.f, (float)s[g][0][i]) * (crow[g] * U.ks);
+        for (int i = 0; i < 4; ++i) sc[g][4 * a + i] = fmaf((float)((s[g][2][i] << 8) + s[g][1][i]), 256.f, (float)s[g][0][i]) * (crow[g] * C.s);
     }
+    if (u + NK * KVM_WAVES < u1) load_keys(C, u + NK * KVM_WAVES);
+    const float vm = rows_max(U.s == U.s ? U.s : 0.f);
+    float fv = 1.f;
+    if (vm > vref) {                                                   // uniform: the four lane groups hold the unit's scales
+      const float nv = __uint_as_float((__float_as_uint(vm) & 0x7f800000u) + 0x00800000u);
+      fv = vref * __uint_as_float(0x7f000000u - __float_as_uint(nv));
+      vref = nv;
+    }
+    const float pv = U.s * __uint_as_float(0x7f000000u - __float_as_uint(vref)) * PS;
+    const bool all = 64 * (u + 1) <= min(whole, L + 1);                // every row sees every token
     f16x8 ph[NT][2], pl[NT][2];
     float fo[NT];
 #pragma unroll
     for (int g = 0; g < NT; ++g) {
-      const int seen = ALL ? 16 : lim[g] - 64 * u - 16 * qq;           // of this lane's 16 tokens
+      float pg = pv;
+      if (!all) {
+        const int seen = lim[g] - 64 * u - 16 * qq;                    // of this lane's 16 tokens, which lie in one block
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sc[g][i] = i < seen ? sc[g][i] : -INFINITY;
+        pg = seen > 0 ? pv : 0.f;                                      // the scale of a block that is not seen does not count, NaN neither
+      }
       float m = mrun[g];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) if (i < seen) m = fmaxf(m, sc[g][i]);
+      for (int i = 0; i < 16; ++i) m = fmaxf(m, sc[g][i]);
       m = rows_max(m);
       const float base = m == -INFINITY ? 0.f : m;                     // nothing seen yet (or NaN, which stays)
       const float f = __builtin_amdgcn_exp2f(mrun[g] - base);
       float z = 0.f;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const float e = i < seen ? __builtin_amdgcn_exp2f(sc[g][i] - base) : 0.f, x = i < seen ? e * pv : 0.f;
+        const float e = __builtin_amdgcn_exp2f(sc[g][i] - base), x = e * pg;
         z += e;
         const _Float16 hi = (_Float16)x;
         ph[g][i / 8][i % 8] = hi; pl[g][i / 8][i % 8] = (_Float16)(x - (float)hi);
@@ -912,13 +961,11 @@ template <int HD, int NT> __device__ __noinline__ void attn_q8_piece(const Ctx& 
         for (int i = 0; i < 4; ++i) o[g][d][i] = fmaf(o[g][d][i], fo[g], x[i]);
       }
     }
+    if (u + KVM_WAVES < u1) load_values(U, u + KVM_WAVES);
   };
-  for (int u = u0 + w; u < u1; u += KVM_WAVES) {
-    UnitQ8<HD> N;
-    if (u + KVM_WAVES < u1) load(N, u + KVM_WAVES);
-    if (64 * (u + 1) <= min(whole, L + 1)) unit(u, std::true_type{});
-    else unit(u, std::false_type{});
-    U = N;
+  for (int u = u0 + w; u < u1; u += NK * KVM_WAVES) {
+    unit(u, keys[0]);
+    if (NK > 1 && u + KVM_WAVES < u1) unit(u + KVM_WAVES, keys[NK - 1]);
   }
   // the waves' and the tail's states, then their sum over all of them
   __syncthreads();
@@ -991,11 +1038,11 @@ __device__ __noinline__ bool op_attn_decode_q8_fast(const Ctx& c) {
 // apart: 33 -> 40 us a task of 50257); rows in place without a mask
 // have no stream. The few tokens that the history or the biases name meet in LDS, one word of counts per logit of a chunk
 // (generated: bits 0..19, bias slot: bits 20..30, prompt: bit 31), before the first vectors of the stream have come; behind the stream
-// whoever takes a word out of there (an exchange against 0) writes that logit again. A token's entries in the bias list meet by an
+// the words are taken out of there (by an exchange against 0, each once) into a list, whose logits are written again. A token's entries in the bias list meet by an
 // atomic maximum of (2047 - entry), which leaves the slot of the first; the others are added to it in list order, one after another
 // (they are few). Adjusting in the stream itself ran its divisions for every wave that met one named token: 256 rows of 50257
 // logits 47 us a task.
-constexpr int ADJ_CHUNK = 26624, ADJ_BIAS = 2047;
+constexpr int ADJ_CHUNK = 22528, ADJ_BIAS = 2047, ADJ_LIST = 2048;
 struct AdjustArgs {
   View x, out, par, hist, plen, hlen, last, bidx, bval, mask, mrow;
   int r0, r1, v0, v1, V;
@@ -1025,63 +1072,15 @@ __device__ __forceinline__ float adjusted(float x, uint32_t w, float rep, float 
   return x;
 }
 __device__ __forceinline__ void lds_or(LDS uint32_t* p, uint32_t v) { __hip_atomic_fetch_or(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP); }
-// Logits [v0, v0 + len) of a row as a stream from xp to op, -inf where the mask row (or none) forbids. VL logits a vector; `first` runs
-// once the first vectors are requested. Rows whose bf16 storage is never 4-byte aligned on both sides go one by one.
-template <bool XH, bool OH, class F>
-__device__ __forceinline__ void adjust_stream(const GLOBAL char* xp, const GLOBAL char* op, const GLOBAL int* mask, int v0, int len, F first) {
-  constexpr int NB = XH ? 16 : 8, VL = 4;                              // 32 KB in flight
-  const int px = XH ? (int)((uintptr_t)xp >> 1) & 1 : 0, po = OH ? (int)((uintptr_t)op >> 1) & 1 : 0;
-  const int peel = min(len, max(px, po)), nv = XH && OH && px != po ? 0 : (len - peel) / VL;
-  u32x4_t x[NB];                                                       // (bf16: the first half)
-  uint32_t m0[NB], m1[NB];
-  auto request = [&](int base) {
-#pragma unroll
-    for (int u = 0; u < NB; ++u) {
-      const int i = peel + VL * min(base + tid() + u * KVM_THREADS, nv - 1), v = v0 + i;
-      if (XH) { const u32x2_t t = *(const GLOBAL u32x2a4*)(xp + 2ll * i); x[u].x = t.x; x[u].y = t.y; }
-      else x[u] = *(const GLOBAL u32x4a4*)(xp + 4ll * i);
-      m0[u] = m1[u] = ~0u;
-      if (mask) { m0[u] = mask[v >> 5]; m1[u] = mask[(v + VL - 1) >> 5]; }      // a vector's bits may lie in two words
-    }
-  };
-  if (nv) request(0);
-  first();
-  for (int base = 0; base < nv; base += NB * KVM_THREADS) {
-    float y[NB][VL];
-    uint32_t bits[NB];
-#pragma unroll
-    for (int u = 0; u < NB; ++u) {
-      const int sh = (v0 + peel + VL * (base + tid() + u * KVM_THREADS)) & 31;
-#pragma unroll
-      for (int e = 0; e < VL; ++e) y[u][e] = __uint_as_float(!XH ? x[u][e % 4] : e & 1 ? x[u][e / 2] & 0xffff0000u : x[u][e / 2] << 16);
-      bits[u] = (uint32_t)((((uint64_t)m1[u] << 32) | m0[u]) >> sh);
-    }
-    if (base + NB * KVM_THREADS < nv) request(base + NB * KVM_THREADS);
-    // a descriptor for the round's vectors: what lies past the last one is out of its range and not stored
-    const __amdgpu_buffer_rsrc_t ro = wt_rsrc((const char*)op + (peel + (long long)VL * base) * (OH ? 2 : 4), (long long)min(VL * NB * KVM_THREADS, VL * (nv - base)) * (OH ? 2 : 4));
-#pragma unroll
-    for (int u = 0; u < NB; ++u) {
-      const int i = VL * (tid() + u * KVM_THREADS);
-#pragma unroll
-      for (int e = 0; e < VL; ++e) if (!((bits[u] >> e) & 1)) y[u][e] = -INFINITY;
-      const f32x4n f = {y[u][0], y[u][1], y[u][2], y[u][3]};
-      if (OH) stwt_bf4_buf(ro, 2 * i, f); else stwt_buf(ro, 4 * i, f);
-    }
-  }
-  for (int k = tid(); k < len - VL * nv; k += KVM_THREADS) {            // before the first vector and behind the last
-    const int i = k < peel ? k : k + VL * nv, v = v0 + i;
-    float y = XH ? bf2f(((const GLOBAL uint16_t*)xp)[i]) : ((const GLOBAL float*)xp)[i];
-    if (mask && !((mask[v >> 5] >> (v & 31)) & 1)) y = -INFINITY;
-    if (OH) stwt16((GLOBAL uint16_t*)op + i, f2bf(y)); else stwt32((GLOBAL float*)op + i, y);
-  }
-}
 __device__ __noinline__ void op_logits_adjust(const Ctx& c) {
   const AdjustArgs A(c);
   LDS uint32_t* cnt = (LDS uint32_t*)c.smem;                           // [ADJ_CHUNK]
   LDS float* bsum = (LDS float*)(cnt + ADJ_CHUNK);                     // [ADJ_BIAS + 1] an entry's value, the first one's the sum
   LDS int* later = (LDS int*)(bsum + ADJ_BIAS + 1);                    // [ADJ_BIAS + 1] first entry of the same token, or -1
-  static_assert((ADJ_CHUNK + 2 * (ADJ_BIAS + 1)) * 4 <= KVM_LDS_BYTES, "logits LDS map");
-  constexpr int NH = 4;                                                // vectors of tokens in flight
+  LDS uint32_t* list = (LDS uint32_t*)(later + ADJ_BIAS + 1);          // [ADJ_LIST][2] tokens and words taken out of cnt, then how many
+  LDS int* listed = (LDS int*)(list + 2 * ADJ_LIST);
+  static_assert((ADJ_CHUNK + 2 * (ADJ_BIAS + 1) + 2 * ADJ_LIST + 1) * 4 <= KVM_LDS_BYTES, "logits LDS map");
+  constexpr int NH = 4, NB = 16;                                       // vectors of tokens, and of logits, in flight
   const int nb = A.bidx.ok() ? A.bidx.cols : 0, len = A.v1 - A.v0;
   const bool xh = A.x.dtype == 2, oh = A.out.dtype == 2;
   if (A.r1 - A.r0 > 1 && !A.rows_ok(c)) return;
@@ -1095,92 +1094,134 @@ __device__ __noinline__ void op_logits_adjust(const Ctx& c) {
     const GLOBAL float* bval = nb ? A.bval.f() + (long long)r * A.bval.cols : nullptr;
     const GLOBAL int* mask = mr >= 0 ? A.mask.i() + (long long)mr * A.mask.cols : nullptr;
     const bool named = n || nb || last >= 0;
-    // the tokens of this thread, four at a time: of the history, and (fewer than four, and the token chosen last) behind it
+    // The stream: vectors start where bf16 storage is 4-byte aligned, on both sides; rows that never are go one by one.
+    const GLOBAL char* xp = (const GLOBAL char*)A.x.p + ((long long)r * A.x.cols + A.v0) * (xh ? 2 : 4);
+    const GLOBAL char* op = (const GLOBAL char*)A.out.p + ((long long)r * A.out.cols + A.v0) * (oh ? 2 : 4);
+    const int px = xh ? (int)((uintptr_t)xp >> 1) & 1 : 0, po = oh ? (int)((uintptr_t)op >> 1) & 1 : 0;
+    const int peel = min(len, max(px, po)), nv = (!mask && A.out.p == A.x.p) || (xh && oh && px != po) ? 0 : (len - peel) / 4;
+    u32x4_t x[NB];                                                     // (bf16: the first half)
+    uint32_t m0[NB], m1[NB];
+    auto request = [&](int u, int base) {
+      const int i = peel + 4 * min(base + tid() + u * KVM_THREADS, nv - 1), v = A.v0 + i;
+      if (xh) { const u32x2_t t = *(const GLOBAL u32x2a4*)(xp + 2ll * i); x[u].x = t.x; x[u].y = t.y; }
+      else x[u] = *(const GLOBAL u32x4a4*)(xp + 4ll * i);
+      m0[u] = m1[u] = ~0u;
+      if (mask) { m0[u] = mask[v >> 5]; m1[u] = mask[(v + 3) >> 5]; }  // a vector's bits may lie in two words
+    };
+    // The tokens of this thread, four at a time: of the history, and (fewer than four, and the token chosen last) behind it.
     u32x4_t h[NH];
     auto tokens = [&](int k0) {
 #pragma unroll
       for (int u = 0; u < NH; ++u) if (k0 + 4 * u * KVM_THREADS < n / 4 * 4) h[u] = *(const GLOBAL u32x4a4*)(hist + k0 + 4 * u * KVM_THREADS);
     };
-    auto visit = [&](auto f) {
+    auto visit = [&](auto f) {                                         // f(position, token)
       for (int k0 = 4 * tid(); k0 < n / 4 * 4; k0 += 4 * NH * KVM_THREADS) {
         if (n >= 4 * NH * KVM_THREADS) tokens(k0);                     // else they are there
 #pragma unroll
-        for (int u = 0; u < NH; ++u) {
-          const int k = k0 + 4 * u * KVM_THREADS;
-          const int t[4] = {(int)h[u].x, (int)h[u].y, (int)h[u].z, (int)h[u].w};
-          if (k < n / 4 * 4) f(k, t);
-        }
+        for (int u = 0; u < NH; ++u)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) if (k0 + 4 * u * KVM_THREADS < n / 4 * 4) f(k0 + 4 * u * KVM_THREADS + e, (int)h[u][e]);
       }
       const int rest = n / 4 * 4 + tid();
-      const int t[4] = {rest < n ? hist[rest] : rest == n ? last : -1, -1, -1, -1};
-      if (rest <= n) f(rest, t);
+      if (rest <= n) f(rest, rest < n ? hist[rest] : last);
     };
-    auto count = [&](int c0, int most) {
-      __syncthreads();
-      for (int i = tid(); i < (most + 3) / 4; i += KVM_THREADS) ((LDS u32x4_t*)cnt)[i] = u32x4_t{0, 0, 0, 0};
-      __syncthreads();
-      if (nb) {
-        for (int j = tid(); j < nb; j += KVM_THREADS) {
-          const int v = bidx[j] - c0;
-          bsum[j] = bval[j];
-          if (v >= 0 && v < most) __hip_atomic_fetch_max(&cnt[v], (uint32_t)(ADJ_BIAS - j) << 20, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-        }
-        __syncthreads();
-        bool many = false;
-        for (int j = tid(); j < nb; j += KVM_THREADS) {
-          const int v = bidx[j] - c0, one = v >= 0 && v < most ? ADJ_BIAS - (int)(cnt[v] >> 20) : j;
-          later[j] = one == j ? -1 : one;
-          many = many || one != j;
-        }
-        if (__syncthreads_or(many) && wave() == 0)                     // entries of one token, in list order
-          for (int j0 = 0; j0 < nb; j0 += 64) {
-            const int mine = j0 + lane() < nb ? later[j0 + lane()] : -1;
-            for (uint64_t left = __ballot(mine >= 0); left; left &= left - 1) {
-              const int j = __ffsll((long long)left) - 1, to = __builtin_amdgcn_readlane(mine, j);
-              if (lane() == 0) bsum[to] += bsum[j0 + j];
-            }
-          }
-      }
-      visit([&](int k, const int (&t)[4]) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int v = t[e] - c0;
-          if (t[e] < 0 || v < 0 || v >= most) continue;
-          if (k + e < pl) lds_or(&cnt[v], 0x80000000u);
-          else __hip_atomic_fetch_add(&cnt[v], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-        }
-      });
-    };
-    auto first = [&] {
-      if (n && n < 4 * NH * KVM_THREADS) tokens(4 * tid());
-      if (named) count(A.v0, min(len, ADJ_CHUNK));
-    };
-    const GLOBAL char* xp = (const GLOBAL char*)A.x.p + ((long long)r * A.x.cols + A.v0) * (xh ? 2 : 4);
-    const GLOBAL char* op = (const GLOBAL char*)A.out.p + ((long long)r * A.out.cols + A.v0) * (oh ? 2 : 4);
-    if (!mask && A.out.p == A.x.p) first();
-    else if (xh) { if (oh) adjust_stream<true, true>(xp, op, mask, A.v0, len, first); else adjust_stream<true, false>(xp, op, mask, A.v0, len, first); }
-    else { if (oh) adjust_stream<false, true>(xp, op, mask, A.v0, len, first); else adjust_stream<false, false>(xp, op, mask, A.v0, len, first); }
-    for (int c0 = A.v0; c0 < A.v1 && named; c0 += ADJ_CHUNK) {         // the named tokens again
+    if (n && n < 4 * NH * KVM_THREADS) tokens(4 * tid());
+    for (int c0 = A.v0; c0 < A.v1 && (named || c0 == A.v0); c0 += ADJ_CHUNK) {
       const int most = min(A.v1 - c0, ADJ_CHUNK);
-      if (c0 > A.v0) count(c0, most);
-      wait_stores();                                                   // the stream's values of these logits are out
-      __syncthreads();
-      auto again = [&](const int (&t)[4]) {
-        uint32_t w[4];
-        float x[4];
-        bool ok[4];
+      if (c0 == A.v0 && nv) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int v = t[e] - c0;
-          w[e] = t[e] >= 0 && v >= 0 && v < most ? __hip_atomic_exchange(&cnt[v], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP) : 0u;
-          if (w[e]) { x[e] = A.x.at(r, t[e]); ok[e] = !mask || ((mask[t[e] >> 5] >> (t[e] & 31)) & 1); }
+        for (int u = 0; u < NB; ++u) request(u, 0);
+      }
+      if (named) {                                                     // counts and bias slots of the chunk's tokens
+        __syncthreads();
+        for (int i = tid(); i < (most + 3) / 4; i += KVM_THREADS) ((LDS u32x4_t*)cnt)[i] = u32x4_t{0, 0, 0, 0};
+        __syncthreads();
+        if (nb) {
+          for (int j = tid(); j < nb; j += KVM_THREADS) {
+            const int v = bidx[j] - c0;
+            bsum[j] = bval[j];
+            if (v >= 0 && v < most) __hip_atomic_fetch_max(&cnt[v], (uint32_t)(ADJ_BIAS - j) << 20, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+          }
+          __syncthreads();
+          bool many = false;
+          for (int j = tid(); j < nb; j += KVM_THREADS) {
+            const int v = bidx[j] - c0, one = v >= 0 && v < most ? ADJ_BIAS - (int)(cnt[v] >> 20) : j;
+            later[j] = one == j ? -1 : one;
+            many = many || one != j;
+          }
+          if (__syncthreads_or(many) && wave() == 0)                   // entries of one token, in list order
+            for (int j0 = 0; j0 < nb; j0 += 64) {
+              const int mine = j0 + lane() < nb ? later[j0 + lane()] : -1;
+              for (uint64_t left = __ballot(mine >= 0); left; left &= left - 1) {
+                const int j = __ffsll((long long)left) - 1, to = __builtin_amdgcn_readlane(mine, j);
+                if (lane() == 0) bsum[to] += bsum[j0 + j];
+              }
+            }
         }
+        visit([&](int k, int t) {
+          const unsigned v = (unsigned)(t - c0);
+          if (t < 0 || v >= (unsigned)most) return;
+          if (k < pl) lds_or(&cnt[v], 0x80000000u);
+          else __hip_atomic_fetch_add(&cnt[v], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+        });
+      }
+      if (c0 == A.v0 && (mask || A.out.p != A.x.p)) {
+        for (int base = 0; base < nv; base += NB * KVM_THREADS) {
+          // a descriptor for the round's vectors: what lies past the last one is out of its range and not stored
+          const __amdgpu_buffer_rsrc_t ro = wt_rsrc((const char*)op + (peel + 4ll * base) * (oh ? 2 : 4), (long long)min(4 * NB * KVM_THREADS, 4 * (nv - base)) * (oh ? 2 : 4));
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (w[e]) A.out.st((long long)r * A.out.cols + t[e], ok[e] ? adjusted(x[e], w[e], rep, freq, pres, bsum) : -INFINITY);
-      };
-      visit([&](int, const int (&t)[4]) { again(t); });
-      for (int j = tid(); j < nb; j += KVM_THREADS) { const int t[4] = {bidx[j], -1, -1, -1}; again(t); }
+          for (int u = 0; u < NB; ++u) {
+            const int i = 4 * (tid() + u * KVM_THREADS);
+            const uint32_t bits = (uint32_t)((((uint64_t)m1[u] << 32) | m0[u]) >> ((A.v0 + peel + 4 * base + i) & 31));
+            f32x4n y;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              y[e] = __uint_as_float(!xh ? x[u][e] : e & 1 ? x[u][e / 2] & 0xffff0000u : x[u][e / 2] << 16);
+              if (!((bits >> e) & 1)) y[e] = -INFINITY;
+            }
+            if (oh) stwt_bf4_buf(ro, 2 * i, y); else stwt_buf(ro, 4 * i, y);
+            if (base + NB * KVM_THREADS < nv) request(u, base + NB * KVM_THREADS);
+          }
+        }
+        for (int k = tid(); k < len - 4 * nv; k += KVM_THREADS) {       // before the first vector and behind the last
+          const int v = A.v0 + (k < peel ? k : k + 4 * nv);
+          A.out.st((long long)r * A.out.cols + v, !mask || ((mask[v >> 5] >> (v & 31)) & 1) ? A.x.at(r, v) : -INFINITY);
+        }
+      }
+      for (bool more = named; more;) {                                 // the named tokens again; those that the list cannot hold stay for a next round
+        wait_stores();                                                 // the stream's values of these logits are out
+        if (tid() == 0) *listed = 0;
+        __syncthreads();
+        auto take = [&](int t) {
+          const unsigned v = (unsigned)(t - c0);
+          if (t < 0 || v >= (unsigned)most) return;
+          const uint32_t w = __hip_atomic_exchange(&cnt[v], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+          if (!w) return;
+          const int k = __hip_atomic_fetch_add(listed, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+          if (k < ADJ_LIST) { list[2 * k] = (uint32_t)t; list[2 * k + 1] = w; }
+          else __hip_atomic_store(&cnt[v], w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+        };
+        visit([&](int, int t) { take(t); });
+        for (int j = tid(); j < nb; j += KVM_THREADS) take(bidx[j]);
+        __syncthreads();
+        const int found = min(*listed, ADJ_LIST);
+        more = *listed > ADJ_LIST;
+        for (int k0 = tid(); k0 < found; k0 += 4 * KVM_THREADS) {      // four logits of a thread in flight
+          float z[4];
+          uint32_t m[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int t = (int)list[2 * min(k0 + i * KVM_THREADS, found - 1)];
+            z[i] = A.x.at(r, t); m[i] = mask ? (uint32_t)mask[t >> 5] : ~0u;
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int k = k0 + i * KVM_THREADS, t = (int)list[2 * min(k, found - 1)];
+            if (k < found) A.out.st((long long)r * A.out.cols + t, (m[i] >> (t & 31)) & 1 ? adjusted(z[i], list[2 * k + 1], rep, freq, pres, bsum) : -INFINITY);
+          }
+        }
+        if (more) __syncthreads();
+      }
     }
     if (A.last.ok() && A.v0 == 0 && tid() == 0) stwt32i(A.hist.i() + ((long long)r * A.hist.cols + n), last);
   }
