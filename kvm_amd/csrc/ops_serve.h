@@ -533,7 +533,7 @@ __device__ __noinline__ void op_attn_decode_q8(const Ctx& c) {
 // tokens of its whole blocks; the pairs in order, by sequence and head, are cut into equal shares, in the tasks alike from the
 // lengths. A cut within Q8_SNAP of a pair's end moves there: a small piece costs more than it balances. A pair that is cut has one piece in
 // each of consecutive tasks; the first has the unfinished block.
-constexpr int Q8_PAIR = 8, Q8_SNAP = 12, Q8_SHARE = 24, Q8_SEQS = 1024;
+constexpr int Q8_PAIR = 12, Q8_SNAP = 14, Q8_SHARE = 16, Q8_SEQS = 1024;
 // (32 bits are enough: a unit is 4 KB and more of cache, whose buffers hold less than 2^33 bytes.)
 struct WorkQ8 {
   const LDS int* pre;          // [seqs + 1] cost of the sequences before, for one head
