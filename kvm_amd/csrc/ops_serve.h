@@ -247,9 +247,9 @@ __device__ __noinline__ void op_kv_append_q8(const Ctx& c) {
 // The tail rows of all pairs of the task go in one range, a row to HD / 8 lanes; blocks that become full (of single tokens one call in
 // blk) are a function of their own, whose registers the tail rows' callers need not save.
 // A full block is in registers as a whole, all its loads requested before any is used, K and V together with one reduction of both
-// maxima (of the largest blocks one after the other: their registers would be most of a worker's scratch).
-// Keys to be normalised or rotated
-// go through LDS first, row by row. Keys are stored as they lie, 8 bytes a lane; values turn through LDS.
+// maxima (of the largest blocks one after the other: their registers would be most of a worker's scratch). Keys to be normalised or
+// rotated go through LDS first, row by row. Keys are stored as they lie, 8 bytes a lane; values turn through LDS. One token of a
+// sequence: 4 us a task; a block of 64 tokens of 128 dims: 5 us.
 template <int HD> struct AppendLds {
   LDS double* freq; LDS float* red; LDS float* keys; LDS float* angs; LDS unsigned char* turn;
   __device__ explicit AppendLds(LDS char* p)
@@ -533,6 +533,8 @@ __device__ __noinline__ void op_attn_decode_q8(const Ctx& c) {
 // tokens of its whole blocks; the pairs in order, by sequence and head, are cut into equal shares, in the tasks alike from the
 // lengths. A cut within Q8_SNAP of a pair's end moves there: a small piece costs more than it balances. A pair that is cut has one piece in
 // each of consecutive tasks; the first has the unfinished block.
+// Measured (pair, snap, smallest share), us of a launch: one sequence of 32,000 tokens 50 (12, 14, 16), 55 (8, 12, 24), 57 (16, 20, 32),
+// 71 (24, 28, 56); 24 sequences of up to 4,096 tokens 69, 72, 70, 77; 6 sequences of 1,531, four tokens each 40, 42, 42, 41.
 constexpr int Q8_PAIR = 12, Q8_SNAP = 14, Q8_SHARE = 16, Q8_SEQS = 1024;
 // (32 bits are enough: a unit is 4 KB and more of cache, whose buffers hold less than 2^33 bytes.)
 struct WorkQ8 {
@@ -664,7 +666,9 @@ __device__ __forceinline__ void q8_arrive(const Ctx& c, const DecodeQ8& D, int b
 }
 
 // Decode attention over the 8-bit cache at head sizes 64 and 128, on the matrix units. Bound: streaming the cache's bytes, and
-// where few workers stream at once the ~550 vector instructions of a unit.
+// where few workers stream at once the 421 vector instructions and 56 products of a unit. 128 sequences of 8,000 tokens, 8 kv heads
+// of 128: 2.1 GB in 476 us (4.4 TB/s, a copy reaches 4.8). A piece costs 9 to 12 us beside its units (dependent loads: lengths, rows,
+// first unit; the unfinished block; the waves' sum), a unit about 0.5.
 // Each wave takes units of 64 tokens in turn, K and V straight from memory into registers in the layout of the operands, one to two
 // units ahead:
 //   scores  v_mfma_i32_16x16x64_i8, A = 16 keys as they lie, B = up to 16 query rows (NT such tiles) as three signed bytes of a
@@ -1034,15 +1038,18 @@ __device__ __noinline__ bool op_attn_decode_q8_fast(const Ctx& c) {
 // ---------------------------------------------------------------------------------------------- logits
 // Adjusted logits (op 314). Bound: the bytes of the logits, and per task the history, which every task of a row reads as a whole (a few
 // KB, from the L2). The task's logits go through as a stream that knows only the mask, in vectors of 4 from any element (a bf16
-// row from its first aligned one), 32 KB requested before the ones before are used (vectors of 8 bf16 logits have stores of 16 bytes 32
-// apart: 33 -> 40 us a task of 50257); rows in place without a mask
-// have no stream. The few tokens that the history or the biases name meet in LDS, one word of counts per logit of a chunk
-// (generated: bits 0..19, bias slot: bits 20..30, prompt: bit 31), before the first vectors of the stream have come; behind the stream
-// the words are taken out of there (by an exchange against 0, each once) into a list, whose logits are written again. A token's entries in the bias list meet by an
-// atomic maximum of (2047 - entry), which leaves the slot of the first; the others are added to it in list order, one after another
-// (they are few). Adjusting in the stream itself ran its divisions for every wave that met one named token: 256 rows of 50257
-// logits 47 us a task.
-constexpr int ADJ_CHUNK = 22528, ADJ_BIAS = 2047, ADJ_LIST = 2048;
+// row from its first aligned one), NB of a thread requested ahead (64 KB of f32, 32 KB of bf16), each again as soon as it is stored;
+// vectors of 8 bf16 logits have stores of 16 bytes 32 apart: 33 -> 40 us a task of 50,257 logits. Rows in place without a mask have
+// no stream.
+// The few tokens that the history or the biases name meet in LDS, one word each (generated: bits 0..19, bias slot: bits 20..30,
+// prompt: bit 31), before the first vectors of the stream have come; behind the stream their logits are written again, each once, four
+// of a thread in flight. The words lie at the tokens themselves where the range fits (22,528 logits) and are taken out of there by an
+// exchange against 0 into a list; a longer range has them in an open-addressed table while it names at most 6,144 tokens, and is
+// done in chunks otherwise: 256 rows of 50,257 bf16 logits, 777 tokens each, 49 us in three chunks, 42.6 with the table.
+// A token's entries in the bias list meet by an atomic maximum of (2047 - entry), which leaves the slot of the first; the others are
+// added to it in list order, one after another (they are few). Adjusting in the stream itself ran its divisions for every wave that
+// met one named token: a task of 50,257 logits 47 us, now 22.
+constexpr int ADJ_CHUNK = 22528, ADJ_BIAS = 2047, ADJ_LIST = 2048, ADJ_SLOTS = 8192, ADJ_NAMED = 6144;
 struct AdjustArgs {
   View x, out, par, hist, plen, hlen, last, bidx, bval, mask, mrow;
   int r0, r1, v0, v1, V;
@@ -1079,6 +1086,9 @@ __device__ __noinline__ void op_logits_adjust(const Ctx& c) {
   LDS int* later = (LDS int*)(bsum + ADJ_BIAS + 1);                    // [ADJ_BIAS + 1] first entry of the same token, or -1
   LDS uint32_t* list = (LDS uint32_t*)(later + ADJ_BIAS + 1);          // [ADJ_LIST][2] tokens and words taken out of cnt, then how many
   LDS int* listed = (LDS int*)(list + 2 * ADJ_LIST);
+  // a longer range of a row that names at most ADJ_NAMED tokens: an open-addressed table over cnt, and its slots in use
+  LDS uint32_t *keys = cnt, *words = cnt + ADJ_SLOTS, *used = words + ADJ_SLOTS;
+  static_assert(2 * ADJ_SLOTS + ADJ_NAMED <= ADJ_CHUNK && ADJ_NAMED < ADJ_SLOTS && (ADJ_SLOTS & (ADJ_SLOTS - 1)) == 0, "logits table");
   static_assert((ADJ_CHUNK + 2 * (ADJ_BIAS + 1) + 2 * ADJ_LIST + 1) * 4 <= KVM_LDS_BYTES, "logits LDS map");
   constexpr int NH = 4, NB = 16;                                       // vectors of tokens, and of logits, in flight
   const int nb = A.bidx.ok() ? A.bidx.cols : 0, len = A.v1 - A.v0;
@@ -1093,7 +1103,7 @@ __device__ __noinline__ void op_logits_adjust(const Ctx& c) {
     const GLOBAL int* bidx = nb ? A.bidx.i() + (long long)r * A.bidx.cols : nullptr;
     const GLOBAL float* bval = nb ? A.bval.f() + (long long)r * A.bval.cols : nullptr;
     const GLOBAL int* mask = mr >= 0 ? A.mask.i() + (long long)mr * A.mask.cols : nullptr;
-    const bool named = n || nb || last >= 0;
+    const bool named = n || nb || last >= 0, table = len > ADJ_CHUNK && n + nb < ADJ_NAMED;
     // The stream: vectors start where bf16 storage is 4-byte aligned, on both sides; rows that never are go one by one.
     const GLOBAL char* xp = (const GLOBAL char*)A.x.p + ((long long)r * A.x.cols + A.v0) * (xh ? 2 : 4);
     const GLOBAL char* op = (const GLOBAL char*)A.out.p + ((long long)r * A.out.cols + A.v0) * (oh ? 2 : 4);
@@ -1126,26 +1136,44 @@ __device__ __noinline__ void op_logits_adjust(const Ctx& c) {
       if (rest <= n) f(rest, rest < n ? hist[rest] : last);
     };
     if (n && n < 4 * NH * KVM_THREADS) tokens(4 * tid());
-    for (int c0 = A.v0; c0 < A.v1 && (named || c0 == A.v0); c0 += ADJ_CHUNK) {
-      const int most = min(A.v1 - c0, ADJ_CHUNK);
+    for (int c0 = A.v0, most; c0 < A.v1 && (named || c0 == A.v0); c0 += most) {
+      most = table ? len : min(len - (c0 - A.v0), ADJ_CHUNK);
+      // the word of token c0 + v (a token that is not in the table goes in: its slots are never all in use)
+      auto word = [&](uint32_t v) {
+        if (!table) return cnt + v;
+        uint32_t s = v * 2654435769u >> (32 - __builtin_ctz(ADJ_SLOTS));
+        for (;; s = (s + 1) & (ADJ_SLOTS - 1)) {
+          uint32_t old = ~0u;
+          if (__hip_atomic_compare_exchange_strong(keys + s, &old, v, __ATOMIC_RELAXED, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP)) {
+            used[__hip_atomic_fetch_add(listed, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP)] = s;
+            break;
+          }
+          if (old == v) break;
+        }
+        return words + s;
+      };
       if (c0 == A.v0 && nv) {
 #pragma unroll
         for (int u = 0; u < NB; ++u) request(u, 0);
       }
       if (named) {                                                     // counts and bias slots of the chunk's tokens
         __syncthreads();
-        for (int i = tid(); i < (most + 3) / 4; i += KVM_THREADS) ((LDS u32x4_t*)cnt)[i] = u32x4_t{0, 0, 0, 0};
+        if (table) {
+          for (int i = tid(); i < 2 * ADJ_SLOTS / 4; i += KVM_THREADS) ((LDS u32x4_t*)cnt)[i] = i < ADJ_SLOTS / 4 ? u32x4_t{~0u, ~0u, ~0u, ~0u} : u32x4_t{0, 0, 0, 0};
+          if (tid() == 0) *listed = 0;
+        } else
+          for (int i = tid(); i < (most + 3) / 4; i += KVM_THREADS) ((LDS u32x4_t*)cnt)[i] = u32x4_t{0, 0, 0, 0};
         __syncthreads();
         if (nb) {
           for (int j = tid(); j < nb; j += KVM_THREADS) {
             const int v = bidx[j] - c0;
             bsum[j] = bval[j];
-            if (v >= 0 && v < most) __hip_atomic_fetch_max(&cnt[v], (uint32_t)(ADJ_BIAS - j) << 20, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+            if (v >= 0 && v < most) __hip_atomic_fetch_max(word(v), (uint32_t)(ADJ_BIAS - j) << 20, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
           }
           __syncthreads();
           bool many = false;
           for (int j = tid(); j < nb; j += KVM_THREADS) {
-            const int v = bidx[j] - c0, one = v >= 0 && v < most ? ADJ_BIAS - (int)(cnt[v] >> 20) : j;
+            const int v = bidx[j] - c0, one = v >= 0 && v < most ? ADJ_BIAS - (int)(*word(v) >> 20) : j;
             later[j] = one == j ? -1 : one;
             many = many || one != j;
           }
@@ -1161,8 +1189,9 @@ __device__ __noinline__ void op_logits_adjust(const Ctx& c) {
         visit([&](int k, int t) {
           const unsigned v = (unsigned)(t - c0);
           if (t < 0 || v >= (unsigned)most) return;
-          if (k < pl) lds_or(&cnt[v], 0x80000000u);
-          else __hip_atomic_fetch_add(&cnt[v], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+          LDS uint32_t* w = word(v);
+          if (k < pl) lds_or(w, 0x80000000u);
+          else __hip_atomic_fetch_add(w, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
         });
       }
       if (c0 == A.v0 && (mask || A.out.p != A.x.p)) {
@@ -1188,37 +1217,41 @@ __device__ __noinline__ void op_logits_adjust(const Ctx& c) {
           A.out.st((long long)r * A.out.cols + v, !mask || ((mask[v >> 5] >> (v & 31)) & 1) ? A.x.at(r, v) : -INFINITY);
         }
       }
-      for (bool more = named; more;) {                                 // the named tokens again; those that the list cannot hold stay for a next round
+      // The named tokens again, each once: the table's, or those taken out of the counts (what the list cannot hold stays for a next round).
+      for (bool more = named; more;) {
         wait_stores();                                                 // the stream's values of these logits are out
-        if (tid() == 0) *listed = 0;
+        if (!table && tid() == 0) *listed = 0;
         __syncthreads();
-        auto take = [&](int t) {
-          const unsigned v = (unsigned)(t - c0);
-          if (t < 0 || v >= (unsigned)most) return;
-          const uint32_t w = __hip_atomic_exchange(&cnt[v], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-          if (!w) return;
-          const int k = __hip_atomic_fetch_add(listed, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-          if (k < ADJ_LIST) { list[2 * k] = (uint32_t)t; list[2 * k + 1] = w; }
-          else __hip_atomic_store(&cnt[v], w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-        };
-        visit([&](int, int t) { take(t); });
-        for (int j = tid(); j < nb; j += KVM_THREADS) take(bidx[j]);
-        __syncthreads();
-        const int found = min(*listed, ADJ_LIST);
-        more = *listed > ADJ_LIST;
+        if (!table) {
+          auto take = [&](int t) {
+            const unsigned v = (unsigned)(t - c0);
+            if (t < 0 || v >= (unsigned)most) return;
+            const uint32_t w = __hip_atomic_exchange(&cnt[v], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+            if (!w) return;
+            const int k = __hip_atomic_fetch_add(listed, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+            if (k < ADJ_LIST) { list[2 * k] = v; list[2 * k + 1] = w; }
+            else __hip_atomic_store(&cnt[v], w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+          };
+          visit([&](int, int t) { take(t); });
+          for (int j = tid(); j < nb; j += KVM_THREADS) take(bidx[j]);
+          __syncthreads();
+        }
+        const int found = table ? *listed : min(*listed, ADJ_LIST);
+        more = !table && *listed > ADJ_LIST;
         for (int k0 = tid(); k0 < found; k0 += 4 * KVM_THREADS) {      // four logits of a thread in flight
           float z[4];
-          uint32_t m[4];
+          uint32_t m[4], w[4];
+          int t[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const int t = (int)list[2 * min(k0 + i * KVM_THREADS, found - 1)];
-            z[i] = A.x.at(r, t); m[i] = mask ? (uint32_t)mask[t >> 5] : ~0u;
+            const int k = min(k0 + i * KVM_THREADS, found - 1);
+            const uint32_t s = table ? used[k] : 0;
+            t[i] = c0 + (int)(table ? keys[s] : list[2 * k]); w[i] = table ? words[s] : list[2 * k + 1];
+            z[i] = A.x.at(r, t[i]); m[i] = mask ? (uint32_t)mask[t[i] >> 5] : ~0u;
           }
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int k = k0 + i * KVM_THREADS, t = (int)list[2 * min(k, found - 1)];
-            if (k < found) A.out.st((long long)r * A.out.cols + t, (m[i] >> (t & 31)) & 1 ? adjusted(z[i], list[2 * k + 1], rep, freq, pres, bsum) : -INFINITY);
-          }
+          for (int i = 0; i < 4; ++i)
+            if (k0 + i * KVM_THREADS < found) A.out.st((long long)r * A.out.cols + t[i], (m[i] >> (t[i] & 31)) & 1 ? adjusted(z[i], w[i], rep, freq, pres, bsum) : -INFINITY);
         }
         if (more) __syncthreads();
       }

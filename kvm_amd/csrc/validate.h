@@ -64,6 +64,12 @@ struct Check {
     if (!((long long)b->rows * b->cols >= cnt)) need(false, (std::string("buffer '") + n + "' too small: needs " + std::to_string(cnt) + " elements").c_str());
   }
   void range(long long lo, long long hi) { need(0 <= lo && lo <= hi, "bad range"); }
+  // buffer n, which the operator writes, is none of its other buffers (but `same`, where the two may be one)
+  void own(const char* n, const char* same = "") {
+    const int w = a[idx(n)];
+    for (size_t i = 0; i < args.size(); ++i)
+      if (w >= 0 && a[i] == w && args[i].type == 0 && args[i].name != n && args[i].name != same) need(false, (std::string("'") + n + "' must be a buffer of its own").c_str());
+  }
 };
 
 // dtype classes of buffer arguments: 'i' int32, 'a' any (f32 / bf16 storage; i32 where the op moves raw words), else f32
@@ -137,7 +143,7 @@ static void cache_q8(Check& k, long long B, int Hkv, int hd, const char* gamma) 
   k.ext("kq", pairs * Tmax, 0); k.ext("vq", pairs * Tmax, 0); k.ext("ks", pairs, 0); k.ext("vs", pairs, 0);
   k.ext("kt", pairs * blk, hd); k.ext("vt", pairs * blk, hd); k.extn("lens", B); k.extn(gamma, hd);
   const float theta = k.F("theta"), eps = k.F("eps");
-  k.need(std::isfinite(theta) && theta >= 0.f && std::isfinite(eps) && eps >= 0.f, "theta and eps must be finite and not negative");
+  k.need(std::isfinite(theta) && (theta == 0.f || theta >= 1.f) && std::isfinite(eps) && eps >= 0.f, "theta must be 0 or at least 1, eps not negative, both finite");
 }
 
 // Operand extents of one task; mirrors the reference's extent functions for the ops implemented here.
@@ -323,7 +329,9 @@ static void extents(int op, Check& k) {
     case 312: { const int b0 = k.I("b0"), b1 = k.I("b1"), h0 = k.I("h0"), h1 = k.I("h1"), p = k.I("p"), P = k.I("P"), nn = k.I("n_new"), Hkv = k.I("Hkv"), hd = k.I("hd");
       k.range(b0, b1); k.need(0 <= h0 && h0 <= h1 && h1 <= Hkv && Hkv > 0 && 0 <= p && p < P && nn > 0, "bad h0/h1/Hkv/p/P/n_new");
       cache_q8(k, b1, Hkv, hd, "kgamma");
-      k.ext("knew", (long long)b1 * nn, (long long)Hkv * hd); k.ext("vnew", (long long)b1 * nn, (long long)Hkv * hd); break; }
+      k.ext("knew", (long long)b1 * nn, (long long)Hkv * hd); k.ext("vnew", (long long)b1 * nn, (long long)Hkv * hd);
+      for (const char* x : {"kq", "ks", "vq", "vs", "kt", "vt"}) k.own(x);
+      break; }
     case 313: { const int b0 = k.I("b0"), b1 = k.I("b1"), s = k.I("s"), S = k.I("S"), nn = k.I("n_new"), H = k.I("H"), Hkv = k.I("Hkv"), hd = k.I("hd");
       k.range(b0, b1); k.need((long long)b1 - b0 <= 1024, "at most 1024 sequences a call");
       k.need(Hkv > 0 && H > 0 && H % Hkv == 0 && 0 <= s && s < S && S <= (1 << 20), "bad s/S/H/Hkv");
@@ -332,6 +340,7 @@ static void extents(int op, Check& k) {
       k.ext("q", (long long)b1 * nn, (long long)H * hd); k.ext("o", (long long)b1 * nn, (long long)H * hd); k.extn("cnt", (long long)b1 * Hkv);
       if (Hkv > 0) k.ext("part", 2ll * S * nn * (H / Hkv), (long long)hd + 2);
       k.need(k.a[k.idx("o")] != k.a[k.idx("q")], "o must not be q");
+      for (const char* x : {"o", "part", "cnt"}) k.own(x);
       k.need(std::isfinite(k.F("scale")), "scale must be finite"); break; }
     case 314: { const int r0 = k.I("r0"), r1 = k.I("r1"), v0 = k.I("v0"), v1 = k.I("v1"), V = k.I("V"); k.range(r0, r1);
       k.need(V > 0 && 0 <= v0 && v0 <= v1 && v1 <= V, "bad v0/v1/V");
@@ -342,7 +351,9 @@ static void extents(int op, Check& k) {
       k.need(k.B("mask") || !k.B("mrow"), "mrow needs mask");
       k.need(!h || h->cols < (1 << 20), "hist holds less than 2^20 tokens a row");
       k.ext("hist", r1, 0); k.extn("plen", r1); k.extn("hlen", r1); k.extn("last", r1); k.ext("bidx", r1, 0); k.ext("bval", r1, 0);
-      k.ext("mask", k.B("mrow") ? 1 : r1, ((long long)V + 31) / 32); k.extn("mrow", r1); break; }
+      k.ext("mask", k.B("mrow") ? 1 : r1, ((long long)V + 31) / 32); k.extn("mrow", r1);
+      k.own("out", "logits"); if (k.B("last")) k.own("hist");
+      break; }
     default: k.need(false, "no extent rule");
   }
 }

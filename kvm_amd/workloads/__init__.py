@@ -54,6 +54,9 @@ class Builder:
         self.buffers.append(d)
         return name
 
+    def has(self, name) -> bool:
+        return name in self._names
+
     def normal(self, name, rows, cols=1, dtype='f32', scale=0.02, seed_name=None):
         """Seeded N(0, scale) (Irwin-Hall(4), the reference's `normal`); bf16 buffers get it as an executor override.
         `seed_name`: draw the values of that buffer instead (a bf16 buffer then holds the other one's values rounded)."""

@@ -57,17 +57,22 @@ def attn_decode_q8(b: Builder, c: CacheQ8, q: str, o: str, lens: str, heads: int
                    qgamma: str | None = None, theta: float = 0.0, eps: float = 0.0, part: str | None = None, cnt: str | None = None,
                    tasks: int = 256) -> list[str]:
     """Attention of the n_new newest tokens of every sequence over the cache, in `tasks` tasks that share the work evenly (a call of the
-    operator for every 1,024 sequences). `part`, `cnt`: the workspace, declared here (o + '.part', o + '.cnt') when absent; calls
-    that follow each other (the layers of a model) may share one, calls that may run side by side not."""
+    operator for every 1,024 sequences, with parts of their own: `part` + '.1' and so on). `part`, `cnt`: the workspace, declared here
+    (o + '.part', o + '.cnt') when absent; calls that follow each other (the layers of a model) may share one, calls that may run
+    side by side not."""
     rows = n_new * (heads // c.kv_heads)
     if rows > 32:
         raise ValueError(f'n_new * heads / kv_heads must be at most 32: {n_new} * {heads} / {c.kv_heads}')
     calls = [(b0, min(c.batch, b0 + 1024)) for b0 in range(0, c.batch, 1024)]
-    part = [part or b.fill(o + '.part', 2 * tasks * rows, c.hd + 2)] + [b.fill(f'{o}.part{i}', 2 * tasks * rows, c.hd + 2) for i in range(1, len(calls))]
+    part = part or b.fill(o + '.part', 2 * tasks * rows, c.hd + 2)
+    parts = [part] + [f'{part}.{i}' for i in range(1, len(calls))]
+    for x in parts[1:]:
+        if not b.has(x):
+            b.fill(x, 2 * tasks * rows, c.hd + 2)
     cnt = cnt or b.fill(o + '.cnt', c.batch * c.kv_heads, 1, 'i32')
     kw = dict(q=q, lens=lens, o=o, cnt=cnt, qgamma=qgamma, S=tasks, n_new=n_new, H=heads, scale=1 / math.sqrt(c.hd) if scale is None else scale,
               theta=theta, eps=eps, **c.args())
-    return [b.task('attn_decode_q8', after=after, b0=b0, b1=b1, s=s, part=p, **kw) for (b0, b1), p in zip(calls, part) for s in range(tasks)]
+    return [b.task('attn_decode_q8', after=after, b0=b0, b1=b1, s=s, part=p, **kw) for (b0, b1), p in zip(calls, parts) for s in range(tasks)]
 
 
 def logits_adjust(b: Builder, logits: str, out: str, par: str, rows: int, V: int, after=(), hist: str | None = None, plen: str | None = None,

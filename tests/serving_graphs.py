@@ -151,6 +151,9 @@ ADJUSTS = [
     (2, 32000, 'f32', 'f32', 5000, 300, 1, True, False),
     (2, 53300, 'bf16', 'bf16', 100, 2047, 2, False, True),      # more than two chunks, the largest list of biases
     (300, 257, 'f32', 'f32', 17, 3, 3, True, True),
+    (2, 50001, 'f32', 'f32', 6001, 143, 2, True, True),          # a long range: as many named tokens as the table takes, one more
+    (2, 50001, 'f32', 'f32', 6002, 143, 2, True, True),
+    (1, 45057, 'bf16', 'bf16', 9000, 5, 0, False, True),
 ]
 
 

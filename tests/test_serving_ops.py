@@ -161,6 +161,35 @@ def test_builder_refusals():
         serving.attn_decode_q8(b, c, 'q', 'o', 'lens', 16, n_new=3)
 
 
+@pytest.mark.parametrize('make,op,change', [
+    (_append, 'kv_append_q8', {'knew': 'kt', 'kt.cols': 256}), (_append, 'kv_append_q8', {'vnew': 'vt', 'vt.cols': 256}),
+    (_attend, 'attn_decode_q8', {'o': 'kt', 'kt.cols': 4096, 'kt.rows': 99999}), (_attend, 'attn_decode_q8', {'o': 'o.part', 'o.part.cols': 4096}),
+    (_attend, 'attn_decode_q8', {'q': 'o.part', 'o.part.cols': 4096}), (_attend, 'attn_decode_q8', {'cnt': 'lens', 'lens.rows': 4096}),
+    (_adjust, 'logits_adjust', {'hist': 'bidx'}), (_adjust, 'logits_adjust', {'mask': 'hist'}), (_adjust, 'logits_adjust', {'out': 'par', 'par.cols': 9999})],
+    ids=str)
+def test_written_buffers_are_no_inputs(make, op, change):
+    _refused(make, op, change, 'a buffer of its own')
+
+
+@pytest.mark.parametrize('theta', [0.5, 1e-30, float('inf')])
+def test_rotation_bases_below_one(theta):
+    _refused(_append, 'kv_append_q8', {'theta': theta}, 'theta')
+    _refused(_attend, 'attn_decode_q8', {'theta': theta}, 'theta')
+
+
+def test_more_sequences_than_a_call():
+    """Two layers of 1,500 sequences share a workspace: two calls each, with a part each."""
+    b = Builder(0)
+    c = serving.kv_q8_buffers(b, 'c', 1500, 1, 64, 64)
+    b.fill('q', 1500, 64), b.fill('o', 1500, 64), b.fill('lens', 1500, 1, 'i32'), b.fill('p', 8, 66), b.fill('n', 1500, 1, 'i32')
+    for _ in range(2):
+        ids = serving.attn_decode_q8(b, c, 'q', 'o', 'lens', 1, part='p', cnt='n', tasks=4)
+    tasks = [t['args'] for t in b.spec()['graphs'][0]['tasks']]
+    assert len(ids) == 8 and sorted({(t['b0'], t['b1'], t['part']) for t in tasks}) == [(0, 1024, 'p'), (1024, 1500, 'p.1')]
+    lb, _ = sg.compiled(b, {})
+    assert executor.validate(lb) is None
+
+
 @pytest.mark.parametrize('lens', [[63 - 64 * 2], [-2], [128]])
 def test_lengths_out_of_range(lens):
     case = sg.APPENDS[0]
