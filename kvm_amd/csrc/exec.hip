@@ -545,6 +545,36 @@ __device__ __forceinline__ const KvmDevState& fresh_state() {
   return *(const KvmDevState*)p;
 }
 
+// One workgroup: the counters and the workers' task counts of a launch into pinned host memory, `seq` behind them (the host waits for
+// it: a copy to the host and a stream synchronisation cost a small graph as much as its tasks). The stores are write-through to the
+// system, so `seq` follows them once every wave has waited for its own; no L2 is written back. clear: the static path's state as
+// kvm_reset_kernel leaves it, so that the next launch of a graph without version variables needs no reset of its own, and the
+// launch's ticks in `began`.
+__device__ __forceinline__ void report_and_clear(const KvmDevState& S, int* out, int seq, bool clear) {
+  const int words = KVM_CNT_BYTES / (int)sizeof(int) + S.grid;
+  for (int k = threadIdx.x; k < words; k += KVM_THREADS) {
+    int* const p = (int*)S.cnt + k;
+    int v = ld_relaxed(p);
+    if (clear) {
+      if (p == &S.cnt->began) v = (int)((unsigned)wall_clock64() - (unsigned)v);
+      st_relaxed(p, 0);
+    }
+    __hip_atomic_store(out + k, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+  }
+  if (clear) for (int k = threadIdx.x; k < S.grid; k += KVM_THREADS) st_relaxed(&S.sprogress[k * S.pstride], 0);
+  wait_stores();
+  __syncthreads();
+  if (threadIdx.x == 0) __hip_atomic_store(out + words, seq, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+}
+// End of a workgroup of a launch that reports itself, its stores waited for: the last one to come here reports. Nothing of the launch's
+// state is read or written by the others any more.
+__device__ __noinline__ void end_and_report(const KvmDevState& S, LDS int* flag) {
+  __syncthreads();
+  if (threadIdx.x == 0) *flag = add_relaxed(&S.cnt->ended, 1);
+  __syncthreads();
+  if (*flag == S.grid - 1) report_and_clear(S, S.rep, S.rep_seq, true);
+}
+
 __device__ void dispatch(int op, const Ctx& c) {
   switch (op) {
     case 0: break;
@@ -662,7 +692,7 @@ __device__ bool static_wait(const KvmDevState& S, const int* ent, int cnt, int s
       if ((polls & 1023) == 1023 && wall_clock64() - since > S.timeout_ticks) {
         int z = 0;
         if (l == 0 && __hip_atomic_compare_exchange_strong(&S.cnt->err_code, &z, (int)KVM_ERR_TIMEOUT, __ATOMIC_RELAXED, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) {
-          S.cnt->err_slot = slot; S.cnt->err_a = ww[0]; S.cnt->err_b = need[0];
+          st_relaxed(&S.cnt->err_slot, slot); st_relaxed(&S.cnt->err_a, ww[0]); st_relaxed(&S.cnt->err_b, need[0]);   // (read in this launch)
         }
         bad = true;
         break;
@@ -693,6 +723,7 @@ __global__ __launch_bounds__(KVM_THREADS, 1) void kvm_static_kernel(KvmDevState 
   const int p0 = S0.sprog_off[w], p1 = S0.sprog_off[w + 1];
   if (p0 < p1 && t < KVM_REC_VEC_OPS) ((LDS u32x4_t*)&s_recs[0])[t] = ((const u32x4_t*)(S0.recs + S0.sprog[p0]))[t];
   int next = p0 < p1 ? S0.sprog[p0] : -1;
+  if (w == 0 && t == 0 && S0.rep_seq) st_relaxed(&S0.cnt->began, (int)(unsigned)wall_clock64());
   __syncthreads();
   for (int i = p0; i < p1; ++i) {
     const KvmDevState& S = fresh_state();
@@ -784,6 +815,8 @@ __global__ __launch_bounds__(KVM_THREADS, 1) void kvm_static_kernel(KvmDevState 
     }
   }
   wait_stores();   // after an early exit: no direct-to-LDS load of a prefetch is still in flight when the workgroup ends
+  const KvmDevState& S = fresh_state();
+  if (S.rep_seq) end_and_report(S, (LDS int*)&s_go);
 }
 
 // Roots (tasks with no predecessors). Roots without a version wait go to fixed cells computed on the host (queue
@@ -1048,20 +1081,8 @@ __global__ void kvm_seed_kernel(KvmDevState S, const int* roots, const int* root
     for (int r = nfixed; r < nroots; ++r) release(S, roots[r], false);
 }
 
-// The counters and the workers' task counts of a launch, into pinned host memory, `seq` behind them (the host waits for it: a copy to
-// the host and a stream synchronisation cost a small graph as much as its tasks). clear: the static path's state as kvm_reset_kernel
-// leaves it, so that the next launch of a graph without version variables needs no reset of its own.
-__global__ void kvm_report_kernel(KvmDevState S, int* out, int seq, int clear) {
-  const int words = KVM_CNT_BYTES / (int)sizeof(int) + S.grid;
-  for (int k = threadIdx.x; k < words; k += blockDim.x) {
-    __hip_atomic_store(out + k, ((const int*)S.cnt)[k], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
-    if (clear) st_relaxed((int*)S.cnt + k, 0);
-  }
-  if (clear) for (int k = threadIdx.x; k < S.grid; k += blockDim.x) st_relaxed(&S.sprogress[k * S.pstride], 0);
-  __threadfence_system();
-  __syncthreads();
-  if (threadIdx.x == 0) __hip_atomic_store(out + words, seq, __ATOMIC_RELEASE, __HIP_MEMORY_SCOPE_SYSTEM);
-}
+// The counters and the workers' task counts of a launch that is collected, for launches that do not report themselves.
+__global__ void kvm_report_kernel(KvmDevState S, int* out, int seq) { report_and_clear(S, out, seq, false); }
 
 // ---------------------------------------------------------------------------------------------- init kernels
 __device__ __forceinline__ float seeded_u(unsigned long long seed, unsigned long long j) {
@@ -1125,6 +1146,7 @@ struct KvmExec {
   int* rep = nullptr;                      // pinned: counters, task counts, sequence number of the last reported launch
   int rep_seq = 0;
   bool reported = false;                   // the last launch's report is on its way
+  bool self_timed = false;                 // the last launch has its own time in its report
   bool clean = false;                      // the device state is as a reset leaves it (untraced static launches)
   bool versioned = false;                  // some task waits for or publishes a version
   std::string err;
@@ -2072,15 +2094,15 @@ static void launch_graph(const KvmDevState& S, const LaunchArgs& L, int grid, hi
   if (after_exec) hipEventRecord(after_exec, st);
 }
 
-static void launch_report(KvmExec* ex, bool clear) {
-  hipLaunchKernelGGL(kvm_report_kernel, dim3(1), dim3(256), 0, ex->stream, ex->S, ex->rep, ++ex->rep_seq, clear ? 1 : 0);
+static void launch_report(KvmExec* ex) {
+  hipLaunchKernelGGL(kvm_report_kernel, dim3(1), dim3(KVM_THREADS), 0, ex->stream, ex->S, ex->rep, ++ex->rep_seq);
   ex->reported = true;
 }
 
-// Untraced static launches of graphs without version variables end with the report that also clears their state, in place of the
-// reset in front of the next one; the others report when the launch is collected. One MLP step 123 -> 106 us of wall clock, a graph of
-// a few short tasks 40 -> 23.
-static int launch_once(KvmExec* ex, hipEvent_t before_exec = nullptr, hipEvent_t after_exec = nullptr) {
+// Untraced static launches of graphs without version variables are one kernel: its last workgroup reports, with the launch's time by the
+// device's clock, and clears the state in place of the reset in front of the next one. The others report when the launch is collected.
+// `one`: a launch to be collected by itself, between events where it does not time itself.
+static int launch_once(KvmExec* ex, hipEvent_t before_exec = nullptr, hipEvent_t after_exec = nullptr, bool one = false) {
   // The versions a launch starts from go over when they have changed since the last one. With the counters and the
   // workers' task counts read back by one copy: one MLP step, 135 -> 121 us of wall clock.
   if (!ex->base_sent) {
@@ -2095,10 +2117,13 @@ static int launch_once(KvmExec* ex, hipEvent_t before_exec = nullptr, hipEvent_t
     ex->last_dissolved = D.dissolved;
   }
   const bool light = ex->path == KVM_PATH_STATIC && !ex->S.trace_on && !ex->versioned;
-  launch_graph(ex->S, ex->L, ex->grid, ex->stream, before_exec, after_exec, ex->path == KVM_PATH_STATIC, !(light && ex->clean));
-  ex->clean = light;
-  ex->reported = false;
-  if (light) launch_report(ex, true);
+  if (one && !light) { HIPCK(hipEventRecord(ex->ev0, ex->stream)); after_exec = ex->ev1; }
+  KvmDevState S = ex->S;
+  S.rep = ex->rep;
+  S.rep_seq = light ? ++ex->rep_seq : 0;
+  launch_graph(S, ex->L, ex->grid, ex->stream, before_exec, after_exec, ex->path == KVM_PATH_STATIC, !(light && ex->clean));
+  ex->clean = ex->reported = light;
+  ex->self_timed = light && one;
   HIPCK(hipGetLastError());
   return 0;
 }
@@ -2118,8 +2143,7 @@ int kvm_start(KvmExec* ex) {
   }
   if (!ex->uploaded) { int rc = do_upload(ex); if (rc) return rc; }
   HIPCK(hipStreamSynchronize(ex->stream));   // buffer initialisation done
-  HIPCK(hipEventRecord(ex->ev0, ex->stream));
-  int rc = launch_once(ex, nullptr, ex->ev1);
+  int rc = launch_once(ex, nullptr, nullptr, true);
   if (rc) return rc;
   ex->launched = true;
   return 0;
@@ -2129,8 +2153,7 @@ int kvm_relaunch(KvmExec* ex) {
   if (ex->streaming) { ex->err = "kvm_relaunch: stream mode runs one launch (submit more bundles instead)"; return KVM_STATUS_INVALID; }
   if (!ex->uploaded) return kvm_start(ex);
   hipSetDevice(ex->dev);
-  HIPCK(hipEventRecord(ex->ev0, ex->stream));
-  int rc = launch_once(ex, nullptr, ex->ev1);
+  int rc = launch_once(ex, nullptr, nullptr, true);
   if (rc) return rc;
   ex->launched = true;
   return 0;
@@ -2181,7 +2204,7 @@ int kvm_finish(KvmExec* ex, KvmResult* res) {
   KvmCounters c{};
   int done = 0;
   if (ex->rep && ex->launched) {   // wait for the report: the stream's last word, with every task's stores behind it
-    if (!ex->reported) launch_report(ex, false);
+    if (!ex->reported) launch_report(ex);
     HIPCK(hipGetLastError());
     const int words = KVM_CNT_BYTES / sizeof(int) + ex->grid;
     const auto give_up = std::chrono::steady_clock::now() + std::chrono::microseconds(500);
@@ -2202,7 +2225,8 @@ int kvm_finish(KvmExec* ex, KvmResult* res) {
     if (!c.err_code) done += ex->last_dissolved;   // dissolved no-ops have no work: done once the run completes
   }
   float ms = 0.f;
-  if (ex->launched) hipEventElapsedTime(&ms, ex->ev0, ex->ev1);
+  if (ex->self_timed) ms = (float)(unsigned)c.began * 1e-5f;   // ticks of 10 ns
+  else if (ex->launched) hipEventElapsedTime(&ms, ex->ev0, ex->ev1);
   if (res) {
     res->err_code = c.err_code; res->err_slot = c.err_slot; res->err_a = c.err_a; res->err_b = c.err_b;
     res->done = done; res->admitted = ex->streaming ? (int)ex->stream_tasks : (int)ex->tasks.size(); res->grid = ex->grid; res->kernel_ms = ms;
@@ -2410,7 +2434,7 @@ int kvm_run_noalloc(const MvmTaskDesc* tasks, int ntasks, const int32_t* succ, i
     used = at + bytes;
     return base + at;
   };
-  KvmDevState S; LaunchArgs L;
+  KvmDevState S{}; LaunchArgs L;
   hipStream_t st = (hipStream_t)stream;
   int rc = place_graph(g, tv, nvars, grid, false, 0, timeout_us, bump, st, S, L, err, false);   // sizing pass
   if (rc == KVM_STATUS_TOO_BIG) {
