@@ -698,7 +698,7 @@ __device__ __forceinline__ f16x8 q8_half(uint32_t w0, uint32_t w1) {
 }
 template <int HD> struct KeysQ8 { u32x4_t k[4][HD / 64]; float s; };
 template <int HD> struct ValuesQ8 { u32x4_t v[HD / 16]; float s; };
-// LDS of a task. The work and the frequencies stay through its pieces; the tail's scores and values give way to the waves' P V.
+// LDS of a task. The work stays through its pieces; the tail's scores and values give way to the waves' P V.
 template <int HD> struct DecodeLds {
   LDS int* pre; LDS int* len; LDS double* freq; LDS float* qs; LDS float* to; LDS float* st; LDS float* cr; LDS float* ts; LDS float* tv;
   __device__ explicit DecodeLds(LDS char* p)
@@ -766,6 +766,8 @@ template <int HD, int NT> __device__ __noinline__ void attn_q8_piece(const Ctx& 
   ValuesQ8<HD> U;
   if (u0 + w < u1) { load_keys(keys[0], u0 + w); load_values(U, u0 + w); }
   if (NK > 1 && u0 + w + KVM_WAVES < u1) load_keys(keys[NK - 1], u0 + w + KVM_WAVES);
+  if (D.theta > 0.f && tid() < HD / 2) M.freq[tid()] = q8_freq(tid(), HD, log((double)D.theta));
+  __syncthreads();                                                     // frequencies; the work and the piece before are out of LDS
   // query rows: norm, rotation, then scaled by a power of two to magnitudes below 2^22
 #pragma unroll
   for (int i = 0; i < QP; ++i) {
@@ -1013,7 +1015,6 @@ template <int HD> __device__ __forceinline__ void attn_q8_t(const Ctx& c) {
   const DecodeQ8 D(c);
   WorkQ8 W;
   if (D.b0 == D.b1 || !q8_work(c, D, M.pre, M.len, (LDS int*)M.st, W)) return;
-  if (D.theta > 0.f && tid() < HD / 2) M.freq[tid()] = q8_freq(tid(), HD, log((double)D.theta));
   const int stop = W.cut(D.s + 1);
   for (int at = W.cut(D.s); at < stop;) {
     const WorkQ8::At P = W.find(at);
@@ -1022,7 +1023,6 @@ template <int HD> __device__ __forceinline__ void attn_q8_t(const Ctx& c) {
     if (L < 0) { D.zeros(b, P.h); continue; }
     const bool cut = off > 0 || end < P.cost;
     const int u0 = max(0, off - Q8_PAIR), u1 = max(0, end - Q8_PAIR), i0 = cut ? W.first_inside(P) : 0, live = cut ? W.inside(P) + 1 : 1;
-    __syncthreads();                                                   // frequencies; the piece before is out of LDS
     if (D.R > 16) attn_q8_piece<HD, 2>(c, b, P.h, L, u0, u1, off == 0, i0, live);
     else attn_q8_piece<HD, 1>(c, b, P.h, L, u0, u1, off == 0, i0, live);
   }
@@ -1045,7 +1045,7 @@ __device__ __noinline__ bool op_attn_decode_q8_fast(const Ctx& c) {
 // prompt: bit 31), before the first vectors of the stream have come; behind the stream their logits are written again, each once, four
 // of a thread in flight. The words lie at the tokens themselves where the range fits (22,528 logits) and are taken out of there by an
 // exchange against 0 into a list; a longer range has them in an open-addressed table while it names at most 6,144 tokens, and is
-// done in chunks otherwise: 256 rows of 50,257 bf16 logits, 777 tokens each, 49 us in three chunks, 42.6 with the table.
+// done in chunks otherwise: 256 rows of 50,257 bf16 logits, 777 tokens each, 31 us in three chunks, 25 with the table (tasks alone).
 // A token's entries in the bias list meet by an atomic maximum of (2047 - entry), which leaves the slot of the first; the others are
 // added to it in list order, one after another (they are few). Adjusting in the stream itself ran its divisions for every wave that
 // met one named token: a task of 50,257 logits 47 us, now 22.
