@@ -42,7 +42,7 @@ enum KvmErr {
 
 struct KvmCounters {
   int err_code, err_slot, err_a, err_b;
-  int ended, began;                // launches that report themselves: workgroups that have ended; low word of the clock at the start (then: ticks)
+  int ended, began;                // launches that report themselves: workgroups that have ended; low word of the clock at the start
   int pad[2];
 };
 #define KVM_CNT_BYTES 256        // KvmDevState::done_blk follows cnt at this distance
@@ -173,7 +173,7 @@ struct KvmDevState {
   int ntasks, nvars, trace_on, nq, qcap, grid, nb, ncells;
   unsigned long long timeout_ticks;   // stall timeout in wall_clock64 ticks (100 MHz)
   unsigned long long aging_ticks;     // wall_clock64 ticks of waiting worth one priority level (0: strict priority)
-  int* rep;                           // pinned host memory of the launch's report (see report_and_clear)
+  int* rep;                           // pinned host memory of the launch's report (see end_and_report)
   int rep_seq;                        // != 0: the static kernel's last workgroup reports, with this sequence number behind the counters
 };
 

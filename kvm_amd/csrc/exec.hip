@@ -545,34 +545,42 @@ __device__ __forceinline__ const KvmDevState& fresh_state() {
   return *(const KvmDevState*)p;
 }
 
-// One workgroup: the counters and the workers' task counts of a launch into pinned host memory, `seq` behind them (the host waits for
-// it: a copy to the host and a stream synchronisation cost a small graph as much as its tasks). The stores are write-through to the
-// system, so `seq` follows them once every wave has waited for its own; no L2 is written back. clear: the static path's state as
-// kvm_reset_kernel leaves it, so that the next launch of a graph without version variables needs no reset of its own, and the
-// launch's ticks in `began`.
-__device__ __forceinline__ void report_and_clear(const KvmDevState& S, int* out, int seq, bool clear) {
-  const int words = KVM_CNT_BYTES / (int)sizeof(int) + S.grid;
-  for (int k = threadIdx.x; k < words; k += KVM_THREADS) {
-    int* const p = (int*)S.cnt + k;
-    int v = ld_relaxed(p);
-    if (clear) {
-      if (p == &S.cnt->began) v = (int)((unsigned)wall_clock64() - (unsigned)v);
-      st_relaxed(p, 0);
-    }
-    __hip_atomic_store(out + k, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
-  }
-  if (clear) for (int k = threadIdx.x; k < S.grid; k += KVM_THREADS) st_relaxed(&S.sprogress[k * S.pstride], 0);
-  wait_stores();
+// A launch's report to the host, which waits for it (a copy to the host and a stream synchronisation cost a small graph as much as its
+// tasks), in pinned memory: the counters and the workers' task counts (word by word), then two pairs of words at KVM_REP_PAIRS, {seq,
+// tasks done} and {seq, ticks of the launch}, 8 bytes stored at once. Tasks done -1: the words before the pairs say it.
+#define KVM_REP_PAIRS(grid) (KVM_CNT_BYTES / (int)sizeof(int) + (((grid) + 1) & ~1))
+__device__ __forceinline__ void report_words(const KvmDevState& S, int* out) {
+  for (int k = threadIdx.x; k < KVM_CNT_BYTES / (int)sizeof(int) + S.grid; k += KVM_THREADS)
+    __hip_atomic_store(out + k, ld_relaxed((const int*)S.cnt + k), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+  wait_stores();                           // written through to the system: the pairs follow them
   __syncthreads();
-  if (threadIdx.x == 0) __hip_atomic_store(out + words, seq, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
 }
-// End of a workgroup of a launch that reports itself, its stores waited for: the last one to come here reports. Nothing of the launch's
-// state is read or written by the others any more.
-__device__ __noinline__ void end_and_report(const KvmDevState& S, LDS int* flag) {
+__device__ __forceinline__ void report_pairs(const KvmDevState& S, int* out, int seq, int done, unsigned ticks) {
+  unsigned long long* const p = (unsigned long long*)(out + KVM_REP_PAIRS(S.grid));
+  __hip_atomic_store(p, ((unsigned long long)(unsigned)done << 32) | (unsigned)seq, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+  __hip_atomic_store(p + 1, ((unsigned long long)ticks << 32) | (unsigned)seq, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+}
+// End of a workgroup of a launch that reports itself, its stores waited for: the last one to come here reports and leaves the static
+// path's state as kvm_reset_kernel does, so that the next launch of a graph without version variables needs no reset of its own.
+// Nothing of the state is read or written by the others any more.
+__device__ __noinline__ void end_and_report(const KvmDevState& S, LDS int* word) {
   __syncthreads();
-  if (threadIdx.x == 0) *flag = add_relaxed(&S.cnt->ended, 1);
+  if (threadIdx.x == 0) *word = add_relaxed(&S.cnt->ended, 1);
   __syncthreads();
-  if (*flag == S.grid - 1) report_and_clear(S, S.rep, S.rep_seq, true);
+  if (*word != S.grid - 1) return;
+  const int err = ld_relaxed(&S.cnt->err_code);
+  const unsigned began = (unsigned)ld_relaxed(&S.cnt->began);
+  int done = 0;
+  for (int k = threadIdx.x; k < S.grid; k += KVM_THREADS) done += ld_relaxed(S.done_blk + k);
+  if (err) report_words(S, S.rep);
+#pragma unroll
+  for (int m = 32; m; m >>= 1) done += __shfl_xor(done, m, 64);
+  __syncthreads();
+  if (lane() == 0) word[wave()] = done;
+  __syncthreads();
+  if (threadIdx.x == 0) report_pairs(S, S.rep, S.rep_seq, err ? -1 : word[0] + word[1] + word[2] + word[3], (unsigned)wall_clock64() - began);
+  for (int k = threadIdx.x; k < KVM_CNT_BYTES / (int)sizeof(int) + S.grid; k += KVM_THREADS) st_relaxed((int*)S.cnt + k, 0);
+  for (int k = threadIdx.x; k < S.grid; k += KVM_THREADS) st_relaxed(&S.sprogress[k * S.pstride], 0);
 }
 
 __device__ void dispatch(int op, const Ctx& c) {
@@ -816,7 +824,7 @@ __global__ __launch_bounds__(KVM_THREADS, 1) void kvm_static_kernel(KvmDevState 
   }
   wait_stores();   // after an early exit: no direct-to-LDS load of a prefetch is still in flight when the workgroup ends
   const KvmDevState& S = fresh_state();
-  if (S.rep_seq) end_and_report(S, (LDS int*)&s_go);
+  if (S.rep_seq) end_and_report(S, (LDS int*)smem);
 }
 
 // Roots (tasks with no predecessors). Roots without a version wait go to fixed cells computed on the host (queue
@@ -1081,8 +1089,11 @@ __global__ void kvm_seed_kernel(KvmDevState S, const int* roots, const int* root
     for (int r = nfixed; r < nroots; ++r) release(S, roots[r], false);
 }
 
-// The counters and the workers' task counts of a launch that is collected, for launches that do not report themselves.
-__global__ void kvm_report_kernel(KvmDevState S, int* out, int seq) { report_and_clear(S, out, seq, false); }
+// The report of a launch that does not report itself, when it is collected.
+__global__ void kvm_report_kernel(KvmDevState S, int* out, int seq) {
+  report_words(S, out);
+  if (threadIdx.x == 0) report_pairs(S, out, seq, -1, 0);
+}
 
 // ---------------------------------------------------------------------------------------------- init kernels
 __device__ __forceinline__ float seeded_u(unsigned long long seed, unsigned long long j) {
@@ -1143,7 +1154,7 @@ struct KvmExec {
   std::vector<int> base_versions;
   bool base_sent = false;                  // the device's copy (LaunchArgs::base) holds base_versions
   bool uploaded = false, launched = false;
-  int* rep = nullptr;                      // pinned: counters, task counts, sequence number of the last reported launch
+  int* rep = nullptr;                      // pinned: the last launch's report
   int rep_seq = 0;
   bool reported = false;                   // the last launch's report is on its way
   bool self_timed = false;                 // the last launch has its own time in its report
@@ -2049,7 +2060,7 @@ static int do_upload(KvmExec* ex) {
   if (rc) return rc == KVM_STATUS_TOO_BIG ? KVM_STATUS_HIP_ERROR : rc;
   ex->S.trace_on = ex->cfg.trace_on && ex->trace_req ? 1 : 0;   // a kvm_set_trace before the first launch holds
   for (const MvmTaskDesc& d : ex->tasks) ex->versioned = ex->versioned || d.wait_var >= 0 || d.pub_var >= 0;
-  const size_t rep_bytes = KVM_CNT_BYTES + (ex->grid + 1) * sizeof(int);
+  const size_t rep_bytes = (KVM_REP_PAIRS(ex->grid) + 4) * sizeof(int);
   if (hipHostMalloc((void**)&ex->rep, rep_bytes, 0) != hipSuccess) { ex->rep = nullptr; ex->err = "pinned memory for the report"; return KVM_STATUS_HIP_ERROR; }
   std::memset(ex->rep, 0, rep_bytes);
   ex->path = KVM_PATH_DYNAMIC;
@@ -2203,15 +2214,22 @@ int kvm_finish(KvmExec* ex, KvmResult* res) {
   if (ex->streaming && !ex->closed) { if (int rc = kvm_close(ex)) return rc; }
   KvmCounters c{};
   int done = 0;
+  unsigned ticks = 0;
   if (ex->rep && ex->launched) {   // wait for the report: the stream's last word, with every task's stores behind it
     if (!ex->reported) launch_report(ex);
     HIPCK(hipGetLastError());
-    const int words = KVM_CNT_BYTES / sizeof(int) + ex->grid;
+    const unsigned long long* pair = (const unsigned long long*)(ex->rep + KVM_REP_PAIRS(ex->grid));
+    auto seq = [&](int i) { return (int)(unsigned)__atomic_load_n(pair + i, __ATOMIC_ACQUIRE); };
     const auto give_up = std::chrono::steady_clock::now() + std::chrono::microseconds(500);
-    while (__atomic_load_n(ex->rep + words, __ATOMIC_ACQUIRE) != ex->rep_seq)
+    while (seq(0) != ex->rep_seq || seq(1) != ex->rep_seq)
       if (std::chrono::steady_clock::now() > give_up) { HIPCK(hipStreamSynchronize(ex->stream)); break; }   // long runs, and faults
-    std::memcpy(&c, ex->rep, sizeof c);
-    for (int k = KVM_CNT_BYTES / sizeof(int); k < words; ++k) done += ex->rep[k];
+    done = (int)(pair[0] >> 32);
+    ticks = (unsigned)(pair[1] >> 32);
+    if (done < 0) {
+      std::memcpy(&c, ex->rep, sizeof c);
+      done = 0;
+      for (int k = 0; k < ex->grid; ++k) done += ex->rep[KVM_CNT_BYTES / sizeof(int) + k];
+    }
   } else {
     std::vector<int> back(ex->S.cnt ? KVM_CNT_BYTES / sizeof(int) + ex->grid : 0);
     if (ex->S.cnt) HIPCK(hipMemcpyAsync(back.data(), ex->S.cnt, back.size() * sizeof(int), hipMemcpyDeviceToHost, ex->stream));
@@ -2225,7 +2243,7 @@ int kvm_finish(KvmExec* ex, KvmResult* res) {
     if (!c.err_code) done += ex->last_dissolved;   // dissolved no-ops have no work: done once the run completes
   }
   float ms = 0.f;
-  if (ex->self_timed) ms = (float)(unsigned)c.began * 1e-5f;   // ticks of 10 ns
+  if (ex->self_timed) ms = (float)ticks * 1e-5f;   // of 10 ns
   else if (ex->launched) hipEventElapsedTime(&ms, ex->ev0, ex->ev1);
   if (res) {
     res->err_code = c.err_code; res->err_slot = c.err_slot; res->err_a = c.err_a; res->err_b = c.err_b;
