@@ -2061,7 +2061,7 @@ static int do_upload(KvmExec* ex) {
   ex->S.trace_on = ex->cfg.trace_on && ex->trace_req ? 1 : 0;   // a kvm_set_trace before the first launch holds
   for (const MvmTaskDesc& d : ex->tasks) ex->versioned = ex->versioned || d.wait_var >= 0 || d.pub_var >= 0;
   const size_t rep_bytes = (KVM_REP_PAIRS(ex->grid) + 4) * sizeof(int);
-  if (hipHostMalloc((void**)&ex->rep, rep_bytes, 0) != hipSuccess) { ex->rep = nullptr; ex->err = "pinned memory for the report"; return KVM_STATUS_HIP_ERROR; }
+  if (hipHostMalloc((void**)&ex->rep, rep_bytes, hipHostMallocCoherent | hipHostMallocMapped) != hipSuccess) { ex->rep = nullptr; ex->err = "pinned memory for the report"; return KVM_STATUS_HIP_ERROR; }
   std::memset(ex->rep, 0, rep_bytes);
   ex->path = KVM_PATH_DYNAMIC;
   if (ncls) { if (int r = upload_classes(ex, alloc, has_dl.data(), has_bw.data(), pubcls, tbw, false)) return r; }
@@ -2223,6 +2223,7 @@ int kvm_finish(KvmExec* ex, KvmResult* res) {
     const auto give_up = std::chrono::steady_clock::now() + std::chrono::microseconds(500);
     while (seq(0) != ex->rep_seq || seq(1) != ex->rep_seq)
       if (std::chrono::steady_clock::now() > give_up) { HIPCK(hipStreamSynchronize(ex->stream)); break; }   // long runs, and faults
+    if (seq(0) != ex->rep_seq || seq(1) != ex->rep_seq) { ex->err = "the launch ended without its report"; return KVM_STATUS_HIP_ERROR; }
     done = (int)(pair[0] >> 32);
     ticks = (unsigned)(pair[1] >> 32);
     if (done < 0) {
