@@ -678,10 +678,12 @@ __device__ __forceinline__ void q8_arrive(const Ctx& c, const DecodeQ8& D, int b
 //           this too is a 16-byte load), B = P. Tokens go to the rows of the score tiles (row m of tile a: token 16 (m / 4) + 4 a +
 //           m % 4) such that the scores' output registers are the B operand, in the loads' order.
 // A byte of V becomes an f16 by two instructions for two of them (0x6400 | (v + 128) is 1024 + v + 128), exactly. Probabilities are
-// f16 pairs, the value and its remainder (22 bits; scaled to 2^12, so that no remainder that matters falls below f16's
-// numbers), two products each, summed in f32. A block's key scale multiplies its scores; its value scale the probabilities, relative
-// to the largest so far (vref, a power of two). Each unit's P V is summed on its own and added to the running one in f32 (the
-// units' chained sums round towards -inf). The unfinished block, at most blk - 1 tokens, is f32 work
+// f16 pairs, the value and its remainder, two products each, summed in f32. A block's key scale multiplies its scores; its value
+// scale the probabilities, and the pairs hold these products relative to a power of two above the row's largest so far (vtop, which
+// shrinks with the row's running maximum; the running P V is in its units), times 2^12: 22 bits of a product, none closer than 2^-36
+// of the largest. (Relative to the largest scale alone, a block without weight left 12 bits of the others at scales 2^26 apart and
+// nothing at 2^36.) Each unit's P V is summed on its own and added to the running one in f32 (the units' chained sums round
+// towards -inf). The unfinished block, at most blk - 1 tokens, is f32 work
 // of all lanes (a wave to a row, the tail in its registers and no barrier, was slower: 24 ragged sequences 52 -> 67 us).
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
@@ -864,7 +866,7 @@ template <int HD, int NT> __device__ __noinline__ void attn_q8_piece(const Ctx& 
   LDS i32x4_t* ql = (LDS i32x4_t*)ts + l;                              // [NT][KH][3][64]
   auto query = [&](int g, int h, int p) { return NT == 1 ? qb[NT == 1 ? h : 0][p] : ql[((g * KH + h) * 3 + p) * 64]; };
   if (NT > 1 && tail) __syncthreads();                                 // the scores have been read
-  float mrun[NT], lrun[NT], crow[NT];
+  float mrun[NT], lrun[NT], crow[NT], vtop[NT];                        // vtop: largest probability times value scale so far
   int lim[NT];
   f32x4n o[NT][VT];
 #pragma unroll
@@ -886,12 +888,13 @@ template <int HD, int NT> __device__ __noinline__ void attn_q8_piece(const Ctx& 
 #pragma unroll
       for (int p = 0; p < 3; ++p) { if (NT == 1) qb[h][p] = q[p]; else ql[((g * KH + h) * 3 + p) * 64] = q[p]; }
     }
-    crow[g] = cr[r]; mrun[g] = -INFINITY; lrun[g] = 0.f;
+    crow[g] = cr[r]; mrun[g] = -INFINITY; lrun[g] = vtop[g] = 0.f;
     lim[g] = r < D.R ? min(whole, L + r / D.G + 1) : 0;
 #pragma unroll
     for (int d = 0; d < VT; ++d) o[g][d] = f32x4n{0.f, 0.f, 0.f, 0.f};
   }
-  float vref = 1.17549435e-38f;
+  auto above = [](float x) { return __uint_as_float((__float_as_uint(x) & 0x7f800000u) + 0x00800000u); };   // a power of two, and 1 / it
+  auto one_over = [](float p) { return __uint_as_float(0x7f000000u - __float_as_uint(p)); };
   // one unit, its keys in C: the keys of this wave's unit after the next (of its next) are requested into C once the scores are there,
   // the next unit's values once the P V is
   auto unit = [&](int u, KeysQ8<HD>& C) {
@@ -915,32 +918,26 @@ template <int HD, int NT> __device__ __noinline__ void attn_q8_piece(const Ctx& 
         for (int i = 0; i < 4; ++i) sc[g][4 * a + i] = fmaf((float)((s[g][2][i] << 8) + s[g][1][i]), 256.f, (float)s[g][0][i]) * (crow[g] * C.s);
     }
     if (u + NK * KVM_WAVES < u1) load_keys(C, u + NK * KVM_WAVES);
-    const float vm = rows_max(U.s == U.s ? U.s : 0.f);
-    float fv = 1.f;
-    if (vm > vref) {                                                   // uniform: the four lane groups hold the unit's scales
-      const float nv = __uint_as_float((__float_as_uint(vm) & 0x7f800000u) + 0x00800000u);
-      fv = vref * __uint_as_float(0x7f000000u - __float_as_uint(nv));
-      vref = nv;
-    }
-    const float pv = U.s * __uint_as_float(0x7f000000u - __float_as_uint(vref)) * PS;
     const bool all = 64 * (u + 1) <= min(whole, L + 1);                // every row sees every token
     f16x8 ph[NT][2], pl[NT][2];
     float fo[NT];
 #pragma unroll
     for (int g = 0; g < NT; ++g) {
-      float pg = pv;
+      float sg = U.s, ml = -INFINITY;
       if (!all) {
         const int seen = lim[g] - 64 * u - 16 * qq;                    // of this lane's 16 tokens, which lie in one block
 #pragma unroll
         for (int i = 0; i < 16; ++i) sc[g][i] = i < seen ? sc[g][i] : -INFINITY;
-        pg = seen > 0 ? pv : 0.f;                                      // the scale of a block that is not seen does not count, NaN neither
+        sg = seen > 0 ? sg : 0.f;                                      // the scale of a block that is not seen does not count, NaN neither
       }
-      float m = mrun[g];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) m = fmaxf(m, sc[g][i]);
-      m = rows_max(m);
+      for (int i = 0; i < 16; ++i) ml = fmaxf(ml, sc[g][i]);
+      const float m = rows_max(fmaxf(mrun[g], ml));
       const float base = m == -INFINITY ? 0.f : m;                     // nothing seen yet (or NaN, which stays)
-      const float f = __builtin_amdgcn_exp2f(mrun[g] - base);
+      const float f = __builtin_amdgcn_exp2f(mrun[g] - base), el = __builtin_amdgcn_exp2f(ml - base);
+      sg = el > 0.f ? sg : 0.f * sg;                                   // no weight: the scale does not count (but NaN)
+      const float top = fmaxf(vtop[g] * f, rows_max(fmaxf(el, 0x1p-112f) * sg));   // (2^-112: sg / top stays below 2^113)
+      const float pg = sg * one_over(above(top)) * PS;
       float z = 0.f;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
@@ -951,7 +948,8 @@ template <int HD, int NT> __device__ __noinline__ void attn_q8_piece(const Ctx& 
       }
       lrun[g] = lrun[g] * f + z;
       mrun[g] = m;
-      fo[g] = f * fv;
+      fo[g] = f * above(vtop[g]) * one_over(above(top));
+      vtop[g] = top;
     }
 #pragma unroll
     for (int d = 0; d < VT; ++d) {
@@ -984,7 +982,7 @@ template <int HD, int NT> __device__ __noinline__ void attn_q8_piece(const Ctx& 
 #pragma unroll
       for (int d = 0; d < VT; ++d)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) ow[(w * D.R + r) * HD + 16 * d + 4 * qq + i] = o[g][d][i] * (vref * (1.f / PS));
+        for (int i = 0; i < 4; ++i) ow[(w * D.R + r) * HD + 16 * d + 4 * qq + i] = o[g][d][i] * (1.f / PS) * above(vtop[g]);
       if (qq == 0) { st[64 * w + r] = mrun[g]; st[64 * w + 32 + r] = z; }
     }
   }
