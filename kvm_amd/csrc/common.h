@@ -109,6 +109,9 @@ struct KvmSchedDev {
 };
 
 struct KvmRec;
+// Counts that the tasks of a launch leave at 0 when all of them have run (the arrivals of ops 310 and 313).
+struct KvmCountRange { int* p; long long n; };
+
 struct KvmDevState {
   const MvmTaskDesc* tasks;   // [ntasks]
   const KvmRec* recs;         // [ntasks] dispatch records (descriptor, argument words, buffer views)
@@ -173,6 +176,8 @@ struct KvmDevState {
   int ntasks, nvars, trace_on, nq, qcap, grid, nb, ncells;
   unsigned long long timeout_ticks;   // stall timeout in wall_clock64 ticks (100 MHz)
   unsigned long long aging_ticks;     // wall_clock64 ticks of waiting worth one priority level (0: strict priority)
+  const KvmCountRange* counts;        // [ncounts] set back to 0 after a launch that an error stopped between two arrivals
+  int ncounts;
   int* rep;                           // pinned host memory of the launch's report (see end_and_report)
   int rep_seq;                        // != 0: the static kernel's last workgroup reports, with this sequence number behind the counters
 };

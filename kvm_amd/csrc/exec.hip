@@ -560,6 +560,11 @@ __device__ __forceinline__ void report_pairs(const KvmDevState& S, int* out, int
   __hip_atomic_store(p, ((unsigned long long)(unsigned)done << 32) | (unsigned)seq, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
   __hip_atomic_store(p + 1, ((unsigned long long)ticks << 32) | (unsigned)seq, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
 }
+// After a launch that an error stopped: the counts of pieces that arrived for a merge which did not come to run. By one workgroup.
+__device__ __forceinline__ void clear_counts(const KvmDevState& S) {
+  for (int r = 0; r < S.ncounts; ++r)
+    for (long long k = threadIdx.x; k < S.counts[r].n; k += blockDim.x) st_relaxed(S.counts[r].p + k, 0);
+}
 // End of a workgroup of a launch that reports itself, its stores waited for: the last one to come here reports and leaves the static
 // path's state as kvm_reset_kernel does, so that the next launch of a graph without version variables needs no reset of its own.
 // Nothing of the state is read or written by the others any more.
@@ -572,7 +577,7 @@ __device__ __noinline__ void end_and_report(const KvmDevState& S, LDS int* word)
   const unsigned began = (unsigned)ld_relaxed(&S.cnt->began);
   int done = 0;
   for (int k = threadIdx.x; k < S.grid; k += KVM_THREADS) done += ld_relaxed(S.done_blk + k);
-  if (err) report_words(S, S.rep);
+  if (err) { report_words(S, S.rep); clear_counts(S); }
 #pragma unroll
   for (int m = 32; m; m >>= 1) done += __shfl_xor(done, m, 64);
   __syncthreads();
@@ -1059,7 +1064,11 @@ __global__ void kvm_reset_kernel(KvmDevState S, const int* base_versions) {
   for (int k = i; k < S.nvars; k += stride) { S.version[k] = base_versions[k]; S.park_head[k] = -1; }
   for (int k = i; k < S.grid; k += stride) { S.done_blk[k] = 0; if (S.sprogress) S.sprogress[k * S.pstride] = 0; }
   for (int k = i; k < S.nq * S.nb * (S.ncls ? S.ncls : 1); k += stride) { KvmQueue z = {}; S.queues[k] = z; }
-  if (i == 0) { KvmCounters z = {}; *S.cnt = z; }
+  if (blockIdx.x == 0) {
+    if (S.cnt->err_code) clear_counts(S);   // the launch before
+    __syncthreads();
+    if (i == 0) { KvmCounters z = {}; *S.cnt = z; }
+  }
   if (S.ncls && i < S.ncls) {   // class hot and statistics lines; the parameter line stays as uploaded
     KvmClsDev& k = S.sched->cls[i];
     k.running = 0; k.bw_running = 0; k.vtime = 0; k.est = 200;   // 2 us until measured
@@ -1201,6 +1210,7 @@ struct GraphPlan {
   std::vector<int32_t> succ_dev;
   std::vector<KvmRec> recs;
   std::vector<int> qcount, qoff, tq, prios, roots, root_cell, fixed_tail;
+  std::vector<KvmCountRange> counts;
 };
 
 // Buffer-argument positions of every registry operator (bit k: argument k is a buffer).
@@ -1232,6 +1242,23 @@ static void make_rec(const MvmTaskDesc& d, const int32_t* a, const std::vector<M
   }
 }
 
+// The counts of the graph's tasks (arguments: mvm_ops_kvm.def), each once.
+static std::vector<KvmCountRange> count_ranges(const std::vector<MvmTaskDesc>& tasks, const std::vector<int32_t>& args, const std::vector<MvmBuf>& table) {
+  std::vector<KvmCountRange> r;
+  for (const MvmTaskDesc& d : tasks) {
+    const int32_t* a = args.data() + d.args_off;
+    if (d.op_id == 310) r.push_back({(int*)table[a[22]].p + (long long)a[7] * a[12] + a[8], 1});
+    if (d.op_id == 313) r.push_back({(int*)table[a[10]].p + (long long)a[12] * a[18], (long long)(a[13] - a[12]) * a[18]});
+  }
+  std::sort(r.begin(), r.end(), [](const KvmCountRange& x, const KvmCountRange& y) { return x.p != y.p ? x.p < y.p : x.n > y.n; });
+  std::vector<KvmCountRange> out;
+  for (const KvmCountRange& x : r) {
+    if (!out.empty() && x.p <= out.back().p + out.back().n) out.back().n = std::max(out.back().n, (long long)(x.p - out.back().p) + x.n);
+    else out.push_back(x);
+  }
+  return out;
+}
+
 // ncls > 0: scheduler classes, the buckets split per class (task t's class is its workload_id); one_group: a single
 // queue group (the class-partitioned mode, whose workers of one class must all see its buckets).
 static void plan_graph(const std::vector<MvmTaskDesc>& tasks, const std::vector<int32_t>& succ, const std::vector<int32_t>& args,
@@ -1240,6 +1267,7 @@ static void plan_graph(const std::vector<MvmTaskDesc>& tasks, const std::vector<
   const int n = (int)tasks.size();
   g.n = n;
   g.succ_dev = succ;
+  g.counts = count_ranges(tasks, args, table);
   for (auto& e : g.succ_dev) e |= edge_flags(tasks[e]);
   g.recs.assign(n, KvmRec{});
   for (int i = 0; i < n; ++i) {
@@ -1319,7 +1347,11 @@ static int place_graph(const GraphPlan& g, const std::vector<MvmTaskDesc>& tasks
     S.bucket_prio = (const int*)vec(g.prios);
     if (aging_us > 0) S.ready_ts = (unsigned long long*)put(nullptr, n * sizeof(unsigned long long));
   }
+  const std::vector<char> none(KVM_CNT_BYTES, 0);                          // the first reset finds no error
   S.cnt = (KvmCounters*)put(nullptr, KVM_CNT_BYTES + grid * sizeof(int));   // one block: read back by one copy
+  if (copy && S.cnt && e == hipSuccess) e = hipMemcpyAsync(S.cnt, none.data(), none.size(), hipMemcpyHostToDevice, st);
+  S.counts = (const KvmCountRange*)vec(g.counts);
+  S.ncounts = (int)g.counts.size();
   S.done_blk = (int*)((char*)S.cnt + KVM_CNT_BYTES);
   S.state = (int*)put(nullptr, n * sizeof(int));
   S.park_next = (int*)put(nullptr, n * sizeof(int));
@@ -2471,6 +2503,11 @@ int kvm_run_noalloc(const MvmTaskDesc* tasks, int ntasks, const int32_t* succ, i
   if (e == hipSuccess) e = hipMemcpyAsync(per.data(), S.done_blk, grid * sizeof(int), hipMemcpyDeviceToHost, st);
   if (e == hipSuccess) e = hipMemcpyAsync(versions, S.version, nvars * sizeof(int), hipMemcpyDeviceToHost, st);
   if (e == hipSuccess) e = hipStreamSynchronize(st);
+  if (e == hipSuccess && c.err_code && S.ncounts) {   // the caller's next call may be another graph over the same counts
+    hipLaunchKernelGGL(kvm_reset_kernel, dim3(1), dim3(256), 0, st, S, (const int*)L.base);
+    e = hipGetLastError();
+    if (e == hipSuccess) e = hipStreamSynchronize(st);
+  }
   if (e != hipSuccess) { err = std::string("kvm_run_noalloc: ") + hipGetErrorString(e); return fail(KVM_STATUS_HIP_ERROR); }
   int done = 0;
   for (int d : per) done += d;
