@@ -521,11 +521,13 @@ __device__ __forceinline__ void attn_q8_pair(const Ctx& c, const DecodeQ8& D, in
 }
 __device__ __noinline__ void op_attn_decode_q8(const Ctx& c) {
   const DecodeQ8 D(c);
+  bool bad = false;                                                    // all lengths of the call are checked before anything is written
+  for (int b = D.b0 + tid(); b < D.b1; b += KVM_THREADS) bad = bad || !D.length_ok(c, b, D.lens.i()[b]);
+  if (__syncthreads_or(bad)) return;
   for (int p = D.s; p < (D.b1 - D.b0) * D.Hkv; p += D.S) {
     const int b = D.b0 + p / D.Hkv, h = p % D.Hkv, L = D.lens.i()[b];
     if (L == -1) D.zeros(b, h);
-    else if (L >= -1 && (long long)L + D.n <= (long long)D.blk * D.ks.cols) attn_q8_pair(c, D, b, h, L);
-    else { if (tid() == 0) D.length_ok(c, b, L); return; }
+    else attn_q8_pair(c, D, b, h, L);
   }
 }
 

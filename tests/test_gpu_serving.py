@@ -227,6 +227,22 @@ def test_bad_lengths_are_refused_whole(make):
             assert not any(got[n].any() for n in sg.CACHE)
 
 
+@pytest.mark.parametrize('hd', [128, 64, 100])
+@pytest.mark.parametrize('batch', [3, 100])
+def test_attention_with_a_bad_length_writes_nothing(hd, batch):
+    """In the form of whole vectors and in the general one: the tasks of a call check every length before they write."""
+    print(f'attention refused hd {hd} batch {batch}', flush=True)
+    c = f64.empty_cache(2 * batch, 2, 64, hd)
+    x = np.ones((batch, 2 * hd), np.float32)
+    for bad in (-2, 128, 2 ** 31 - 1):
+        for tasks in (1, 16):
+            lens = np.full(batch, 70, np.int64)
+            lens[0], lens[-1] = -1, bad
+            lb, init = sg.attend_graph(c, x, lens.astype(np.int32), 2, 2, 1, 1.0, tasks=tasks)
+            err, got = _error(lb, init)
+            assert err == 'OP_KVLEN' and (got['o'] == 7).all() and not got['o.cnt'].any()
+
+
 def _shifted(lb, init, skip):
     """The graph on buffers that begin `skip` elements into an allocation of the caller's; returns all contents."""
     meta = lb.metadata['buffers']
