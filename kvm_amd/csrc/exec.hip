@@ -40,6 +40,7 @@
 #include "ops_serve.h"
 #include "validate.h"
 #include "static_plan.h"
+#include "launch_state.h"
 
 using namespace kvm;
 
@@ -1164,10 +1165,7 @@ struct KvmExec {
   bool base_sent = false;                  // the device's copy (LaunchArgs::base) holds base_versions
   bool uploaded = false, launched = false;
   int* rep = nullptr;                      // pinned: the last launch's report
-  int rep_seq = 0;
-  bool reported = false;                   // the last launch's report is on its way
-  bool self_timed = false;                 // the last launch has its own time in its report
-  bool clean = false;                      // the device state is as a reset leaves it (untraced static launches)
+  LaunchState run;
   bool versioned = false;                  // some task waits for or publishes a version
   std::string err;
   // device memory of the placed graph (one hipMalloc each, freed by kvm_destroy)
@@ -2138,8 +2136,8 @@ static void launch_graph(const KvmDevState& S, const LaunchArgs& L, int grid, hi
 }
 
 static void launch_report(KvmExec* ex) {
-  hipLaunchKernelGGL(kvm_report_kernel, dim3(1), dim3(KVM_THREADS), 0, ex->stream, ex->S, ex->rep, ++ex->rep_seq);
-  ex->reported = true;
+  hipLaunchKernelGGL(kvm_report_kernel, dim3(1), dim3(KVM_THREADS), 0, ex->stream, ex->S, ex->rep, ex->run.next_seq());
+  ex->run.reported = true;
 }
 
 // Untraced static launches of graphs without version variables are one kernel: its last workgroup reports, with the launch's time by the
@@ -2151,7 +2149,7 @@ static int launch_once(KvmExec* ex, hipEvent_t before_exec = nullptr, hipEvent_t
   if (!ex->base_sent) {
     HIPCK(hipMemcpyAsync(ex->L.base, ex->base_versions.data(), ex->base_versions.size() * sizeof(int), hipMemcpyHostToDevice, ex->stream));
     ex->base_sent = true;
-    ex->clean = false;
+    ex->run.clean = false;
   }
   ex->last_dissolved = 0;
   if (ex->path == KVM_PATH_STATIC) {   // traced launches run every task; untraced ones the plan with the no-ops dissolved
@@ -2163,10 +2161,10 @@ static int launch_once(KvmExec* ex, hipEvent_t before_exec = nullptr, hipEvent_t
   if (one && !light) { HIPCK(hipEventRecord(ex->ev0, ex->stream)); after_exec = ex->ev1; }
   KvmDevState S = ex->S;
   S.rep = ex->rep;
-  S.rep_seq = light ? ++ex->rep_seq : 0;
-  launch_graph(S, ex->L, ex->grid, ex->stream, before_exec, after_exec, ex->path == KVM_PATH_STATIC, !(light && ex->clean));
-  ex->clean = ex->reported = light;
-  ex->self_timed = light && one;
+  S.rep_seq = light ? ex->run.next_seq() : 0;
+  launch_graph(S, ex->L, ex->grid, ex->stream, before_exec, after_exec, ex->path == KVM_PATH_STATIC, !(light && ex->run.clean));
+  ex->run.clean = ex->run.reported = light;
+  ex->run.self_timed = light && one;
   HIPCK(hipGetLastError());
   return 0;
 }
@@ -2248,14 +2246,14 @@ int kvm_finish(KvmExec* ex, KvmResult* res) {
   int done = 0;
   unsigned ticks = 0;
   if (ex->rep && ex->launched) {   // wait for the report: the stream's last word, with every task's stores behind it
-    if (!ex->reported) launch_report(ex);
+    if (!ex->run.reported) launch_report(ex);
     HIPCK(hipGetLastError());
     const unsigned long long* pair = (const unsigned long long*)(ex->rep + KVM_REP_PAIRS(ex->grid));
     auto seq = [&](int i) { return (int)(unsigned)__atomic_load_n(pair + i, __ATOMIC_ACQUIRE); };
     const auto give_up = std::chrono::steady_clock::now() + std::chrono::microseconds(500);
-    while (seq(0) != ex->rep_seq || seq(1) != ex->rep_seq)
+    while (seq(0) != ex->run.seq || seq(1) != ex->run.seq)
       if (std::chrono::steady_clock::now() > give_up) { HIPCK(hipStreamSynchronize(ex->stream)); break; }   // long runs, and faults
-    if (seq(0) != ex->rep_seq || seq(1) != ex->rep_seq) { ex->err = "the launch ended without its report"; return KVM_STATUS_HIP_ERROR; }
+    if (seq(0) != ex->run.seq || seq(1) != ex->run.seq) { ex->err = "the launch ended without its report"; return KVM_STATUS_HIP_ERROR; }
     done = (int)(pair[0] >> 32);
     ticks = (unsigned)(pair[1] >> 32);
     if (done < 0) {
@@ -2276,7 +2274,7 @@ int kvm_finish(KvmExec* ex, KvmResult* res) {
     if (!c.err_code) done += ex->last_dissolved;   // dissolved no-ops have no work: done once the run completes
   }
   float ms = 0.f;
-  if (ex->self_timed) ms = (float)ticks * 1e-5f;   // of 10 ns
+  if (ex->run.self_timed) ms = (float)ticks * 1e-5f;   // of 10 ns
   else if (ex->launched) hipEventElapsedTime(&ms, ex->ev0, ex->ev1);
   if (res) {
     res->err_code = c.err_code; res->err_slot = c.err_slot; res->err_a = c.err_a; res->err_b = c.err_b;

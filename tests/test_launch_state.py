@@ -1,0 +1,26 @@
+"""The host's bookkeeping of launches (kvm_amd/csrc/launch_state.h), compiled alone. No GPU needed."""
+import subprocess
+
+import pytest
+
+from kvm_amd import build as kb
+
+
+@pytest.fixture(scope='module')
+def run(tmp_path_factory):
+    """run(statements): a program of them, with `L` a LaunchState; CHECK ends it with the line that does not hold."""
+    def go(body):
+        d = tmp_path_factory.mktemp('ls')
+        (d / 'a.cpp').write_text('#include "launch_state.h"\n#include <cstdio>\n#include <cstdlib>\n'
+                                 '#define CHECK(x) do { if (!(x)) { std::printf("%s\\n", #x); std::exit(1); } } while (0)\n'
+                                 'using namespace kvm;\nint main() {\n  LaunchState L;\n' + body + '\n}\n')
+        subprocess.run([kb.CXX, '-std=c++17', '-O1', f'-I{kb.CSRC}', str(d / 'a.cpp'), '-o', str(d / 'a')], check=True)
+        r = subprocess.run([str(d / 'a')], capture_output=True, text=True)
+        assert r.returncode == 0, r.stdout
+    return go
+
+
+def test_sequence_numbers_are_never_zero(run):
+    run('CHECK(L.next_seq() == 1 && L.next_seq() == 2 && L.seq == 2);'
+        'L.seq = 0x7fffffff; CHECK(L.next_seq() == (int)0x80000000u);'
+        'L.seq = -1; CHECK(L.next_seq() == 1 && L.seq == 1);')
