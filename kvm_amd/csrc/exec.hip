@@ -2149,7 +2149,7 @@ static int launch_once(KvmExec* ex, hipEvent_t before_exec = nullptr, hipEvent_t
   if (!ex->base_sent) {
     HIPCK(hipMemcpyAsync(ex->L.base, ex->base_versions.data(), ex->base_versions.size() * sizeof(int), hipMemcpyHostToDevice, ex->stream));
     ex->base_sent = true;
-    ex->run.clean = false;
+    ex->run.lost();
   }
   ex->last_dissolved = 0;
   if (ex->path == KVM_PATH_STATIC) {   // traced launches run every task; untraced ones the plan with the no-ops dissolved
@@ -2162,10 +2162,10 @@ static int launch_once(KvmExec* ex, hipEvent_t before_exec = nullptr, hipEvent_t
   KvmDevState S = ex->S;
   S.rep = ex->rep;
   S.rep_seq = light ? ex->run.next_seq() : 0;
-  launch_graph(S, ex->L, ex->grid, ex->stream, before_exec, after_exec, ex->path == KVM_PATH_STATIC, !(light && ex->run.clean));
-  ex->run.clean = ex->run.reported = light;
+  launch_graph(S, ex->L, ex->grid, ex->stream, before_exec, after_exec, ex->path == KVM_PATH_STATIC, ex->run.begin(light));
   ex->run.self_timed = light && one;
   HIPCK(hipGetLastError());
+  ex->run.enqueued(light);
   return 0;
 }
 
@@ -2252,8 +2252,13 @@ int kvm_finish(KvmExec* ex, KvmResult* res) {
     auto seq = [&](int i) { return (int)(unsigned)__atomic_load_n(pair + i, __ATOMIC_ACQUIRE); };
     const auto give_up = std::chrono::steady_clock::now() + std::chrono::microseconds(500);
     while (seq(0) != ex->run.seq || seq(1) != ex->run.seq)
-      if (std::chrono::steady_clock::now() > give_up) { HIPCK(hipStreamSynchronize(ex->stream)); break; }   // long runs, and faults
-    if (seq(0) != ex->run.seq || seq(1) != ex->run.seq) { ex->err = "the launch ended without its report"; return KVM_STATUS_HIP_ERROR; }
+      if (std::chrono::steady_clock::now() > give_up) {                // long runs, and faults
+        const hipError_t e = hipStreamSynchronize(ex->stream);
+        if (e != hipSuccess) ex->run.lost();
+        HIPCK(e);
+        break;
+      }
+    if (seq(0) != ex->run.seq || seq(1) != ex->run.seq) { ex->run.lost(); ex->err = "the launch ended without its report"; return KVM_STATUS_HIP_ERROR; }
     done = (int)(pair[0] >> 32);
     ticks = (unsigned)(pair[1] >> 32);
     if (done < 0) {

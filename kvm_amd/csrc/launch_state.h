@@ -14,6 +14,16 @@ struct LaunchState {
     const unsigned s = (unsigned)seq + 1u;
     return seq = (int)(s ? s : 1u);
   }
+  // Around the enqueueing of a launch: whether a reset goes in front of it; it is enqueued; something about it failed. The state is
+  // clean for the next launch only once a launch that clears it is known to be on its way.
+  bool begin(bool light) {
+    const bool reset = !(light && clean);
+    clean = false;
+    reported = light;
+    return reset;
+  }
+  void enqueued(bool light) { clean = light; }
+  void lost() { clean = false; }
 };
 
 }  // namespace kvm

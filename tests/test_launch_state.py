@@ -24,3 +24,10 @@ def test_sequence_numbers_are_never_zero(run):
     run('CHECK(L.next_seq() == 1 && L.next_seq() == 2 && L.seq == 2);'
         'L.seq = 0x7fffffff; CHECK(L.next_seq() == (int)0x80000000u);'
         'L.seq = -1; CHECK(L.next_seq() == 1 && L.seq == 1);')
+
+
+def test_a_reset_goes_in_front_after_anything_that_failed(run):
+    run('CHECK(L.begin(true)); L.enqueued(true); CHECK(!L.begin(true)); L.enqueued(true);'        # the first one, the next one
+        'CHECK(!L.begin(true)); CHECK(L.begin(true));'                                            # one that was not enqueued
+        'L.enqueued(true); L.lost(); CHECK(L.begin(true)); L.enqueued(true);'                     # one without its report
+        'CHECK(L.begin(false)); L.enqueued(false); CHECK(!L.reported && L.begin(true) && L.reported);')   # a traced one between
