@@ -101,6 +101,15 @@ template <class F> __device__ __forceinline__ float rows_all(float v, F f) {
 }
 __device__ __forceinline__ float rows_sum(float v) { return rows_all(v, [](float a, float b) { return a + b; }); }
 __device__ __forceinline__ float rows_max(float v) { return rows_all(v, [](float a, float b) { return fmaxf(a, b); }); }
+// Between LDS stores of a wave's lanes and loads of the same words by others of them: one wave's LDS operations are carried out in order,
+// the fences keep them in order in the program. Not behind a loop that lanes leave one by one: where such a loop ends an `if`, the compiler
+// (LLVM 22) drops the restore of EXEC between the loop and the barrier, and registers that it reloads there come back in no lane.
+// With angles by sincosf and registers short, that left query rows of NaN. Loops in front of it have the same rounds for all lanes.
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
 // A head of HD values spread over HD / 8 neighbouring lanes, 8 each: RMS norm (gamma: the gains, or none) and rotation of
 // position t (freq: the HD / 2 frequencies in LDS, or none), in f32. The other half of a pair is HD / 16 lanes away; the lanes
 // share out the row's angles through `ang`, HD floats of LDS for each row in flight (HD / 8 lanes of one wave).
@@ -109,8 +118,12 @@ template <int HD> __device__ __forceinline__ void head8_turn(float (&v)[8], cons
   const int ln = lane() % LPR;
   if (freq) {
 #pragma unroll 1
-    for (int i = ln; i < HD / 2; i += LPR) { float sn, co; q8_turn(t, freq[i], sn, co); ang[i] = sn; ang[HD / 2 + i] = co; }
-    __builtin_amdgcn_wave_barrier();                                   // one wave's LDS operations stay in order
+    for (int j = 0; j < HD / 2 / LPR; ++j) {
+      const int i = ln + j * LPR;
+      float sn, co; q8_turn(t, freq[i], sn, co);
+      ang[i] = sn; ang[HD / 2 + i] = co;
+    }
+    wave_sync();
   }
   if (gamma) {
     float ss = 0.f;
@@ -127,7 +140,7 @@ template <int HD> __device__ __forceinline__ void head8_turn(float (&v)[8], cons
       const int k = 8 * (ln % (LPR / 2)) + i;
       v[i] = v[i] * ang[HD / 2 + k] + sign * __shfl_xor(v[i], LPR / 2, 64) * ang[k];
     }
-    __builtin_amdgcn_wave_barrier();
+    wave_sync();
   }
 }
 
@@ -588,7 +601,7 @@ __device__ __forceinline__ bool q8_work(const Ctx& c, const DecodeQ8& D, LDS int
     const int cost = lane() < seqs ? cost_of(L) : 0, upto = wave_scan(cost);
     if (lane() < seqs) { len[lane()] = L; pre[lane()] = upto - cost; }
     if (lane() == seqs - 1) pre[seqs] = upto;
-    __builtin_amdgcn_wave_barrier();                                   // one wave's LDS operations stay in order
+    wave_sync();
   } else {
     int cost[PER], sum = 0;
     bool bad = false;

@@ -77,6 +77,58 @@ def test_every_dispatch_case_is_a_function(asm):
     assert not missing, f'operators inlined into the kernel (mark them __noinline__): {missing}'
 
 
+def _under_no_lanes(text):
+    """Vector instructions between the end of a loop that lanes leave one by one (EXEC is 0 there) and the next change of EXEC."""
+    lines = [t.split(';')[0].strip() for t in text.split('\n')]
+    at = {t[:-1]: i for i, t in enumerate(lines) if t.endswith(':')}
+    def walk(i):
+        out = []
+        for _ in range(200):
+            s = lines[i] if i < len(lines) else 's_endpgm'
+            i += 1
+            if not s or s.endswith(':') or s.startswith('.'):
+                continue
+            op = s.split()[0]
+            if re.search(r'\bexec\b', s.split(',')[0]) or 'saveexec' in op:
+                break
+            if op in ('s_cbranch_execz', 's_branch'):
+                i = at[s.split()[1]]
+            elif op != 's_cbranch_execnz' and re.match(r's_(cbranch|setpc|swappc|endpgm)', op):
+                break
+            elif re.match(r'(v_(?!readlane|writelane|readfirstlane|mfma)|ds_|global_|scratch_|flat_|buffer_(?!wbl2|inv))', op):
+                out.append(s)
+        return out
+    bad = []
+    code = [(i, s) for i, s in enumerate(lines) if s and not s.endswith(':') and not s.startswith('.')]
+    for (_, a), (i, b) in zip(code, code[1:]):
+        if a.startswith('s_andn2_b64 exec, exec,') and b.startswith('s_cbranch_exec'):
+            bad += walk(i + 1 if b.split()[0] == 's_cbranch_execnz' else at[b.split()[1]])
+    return bad, len(code)
+
+
+def test_nothing_is_reloaded_behind_a_loop_without_lanes(asm):
+    """Registers that the compiler kept elsewhere over a loop and reloads behind it, before EXEC is restored, come back in no lane.
+    It does so where a wave barrier stands between such a loop and the end of the `if` around it."""
+    loop = '''
+f:
+  v_accvgpr_write_b32 a7, v120
+.L1:
+  v_add_u32_e32 v120, 1, v120
+  s_andn2_b64 exec, exec, s[6:7]
+  s_cbranch_execz .L2
+  s_branch .L1
+.L2:
+%s  v_accvgpr_read_b32 v120, a7
+.L3:
+  s_or_b64 exec, exec, s[4:5]
+  s_endpgm
+'''
+    assert _under_no_lanes(loop % '')[0] == ['v_accvgpr_read_b32 v120, a7']
+    assert _under_no_lanes(loop % '  s_or_b64 exec, exec, s[6:7]\n')[0] == []
+    bad, n = _under_no_lanes(asm)
+    assert n > 100000 and not bad, bad[:10]
+
+
 def test_kernel_private_segments_stay_below_the_residency_guard(asm):
     """kvm_create refuses a build whose persistent kernels need more than KVM_MAX_PRIVATE_BYTES (2,048) of private
     segment per lane; the compiled kernels stay below it (a 2,096-byte build stopped before its first task)."""
