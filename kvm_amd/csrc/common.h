@@ -42,8 +42,8 @@ enum KvmErr {
 
 struct KvmCounters {
   int err_code, err_slot, err_a, err_b;
-  int ended, began;                // launches that report themselves: workgroups that have ended; low word of the clock at the start
-  int pad[2];
+  int ended, pad;                  // launches that report themselves: workgroups that have ended
+  long long began;                 // and the clock when worker 0 started
 };
 #define KVM_CNT_BYTES 256        // KvmDevState::done_blk follows cnt at this distance
 

@@ -556,10 +556,10 @@ __device__ __forceinline__ void report_words(const KvmDevState& S, int* out) {
   wait_stores();                           // written through to the system: the pairs follow them
   __syncthreads();
 }
-__device__ __forceinline__ void report_pairs(const KvmDevState& S, int* out, int seq, int done, unsigned ticks) {
+__device__ __forceinline__ void report_pairs(const KvmDevState& S, int* out, int seq, int done, unsigned long long ticks) {
   unsigned long long* const p = (unsigned long long*)(out + KVM_REP_PAIRS(S.grid));
   __hip_atomic_store(p, ((unsigned long long)(unsigned)done << 32) | (unsigned)seq, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
-  __hip_atomic_store(p + 1, ((unsigned long long)ticks << 32) | (unsigned)seq, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+  __hip_atomic_store(p + 1, report_time(seq, ticks), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
 }
 // After a launch that an error stopped: the counts of pieces that arrived for a merge which did not come to run. By one workgroup.
 __device__ __forceinline__ void clear_counts(const KvmDevState& S) {
@@ -575,7 +575,7 @@ __device__ __noinline__ void end_and_report(const KvmDevState& S, LDS int* word)
   __syncthreads();
   if (*word != S.grid - 1) return;
   const int err = ld_relaxed(&S.cnt->err_code);
-  const unsigned began = (unsigned)ld_relaxed(&S.cnt->began);
+  const long long began = __hip_atomic_load(&S.cnt->began, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   int done = 0;
   for (int k = threadIdx.x; k < S.grid; k += KVM_THREADS) done += ld_relaxed(S.done_blk + k);
   if (err) { report_words(S, S.rep); clear_counts(S); }
@@ -584,7 +584,7 @@ __device__ __noinline__ void end_and_report(const KvmDevState& S, LDS int* word)
   __syncthreads();
   if (lane() == 0) word[wave()] = done;
   __syncthreads();
-  if (threadIdx.x == 0) report_pairs(S, S.rep, S.rep_seq, err ? -1 : word[0] + word[1] + word[2] + word[3], (unsigned)wall_clock64() - began);
+  if (threadIdx.x == 0) report_pairs(S, S.rep, S.rep_seq, err ? -1 : word[0] + word[1] + word[2] + word[3], (unsigned long long)(wall_clock64() - began));
   for (int k = threadIdx.x; k < KVM_CNT_BYTES / (int)sizeof(int) + S.grid; k += KVM_THREADS) st_relaxed((int*)S.cnt + k, 0);
   for (int k = threadIdx.x; k < S.grid; k += KVM_THREADS) st_relaxed(&S.sprogress[k * S.pstride], 0);
 }
@@ -737,7 +737,7 @@ __global__ __launch_bounds__(KVM_THREADS, 1) void kvm_static_kernel(KvmDevState 
   const int p0 = S0.sprog_off[w], p1 = S0.sprog_off[w + 1];
   if (p0 < p1 && t < KVM_REC_VEC_OPS) ((LDS u32x4_t*)&s_recs[0])[t] = ((const u32x4_t*)(S0.recs + S0.sprog[p0]))[t];
   int next = p0 < p1 ? S0.sprog[p0] : -1;
-  if (w == 0 && t == 0 && S0.rep_seq) st_relaxed(&S0.cnt->began, (int)(unsigned)wall_clock64());
+  if (w == 0 && t == 0 && S0.rep_seq) stwt64((GLOBAL void*)&S0.cnt->began, (uint64_t)wall_clock64());
   __syncthreads();
   for (int i = p0; i < p1; ++i) {
     const KvmDevState& S = fresh_state();
@@ -2244,23 +2244,25 @@ int kvm_finish(KvmExec* ex, KvmResult* res) {
   if (ex->streaming && !ex->closed) { if (int rc = kvm_close(ex)) return rc; }
   KvmCounters c{};
   int done = 0;
-  unsigned ticks = 0;
+  float ms = 0.f;
   if (ex->rep && ex->launched) {   // wait for the report: the stream's last word, with every task's stores behind it
     if (!ex->run.reported) launch_report(ex);
     HIPCK(hipGetLastError());
     const unsigned long long* pair = (const unsigned long long*)(ex->rep + KVM_REP_PAIRS(ex->grid));
-    auto seq = [&](int i) { return (int)(unsigned)__atomic_load_n(pair + i, __ATOMIC_ACQUIRE); };
+    auto here = [&] {
+      return (int)(unsigned)__atomic_load_n(pair, __ATOMIC_ACQUIRE) == ex->run.seq && report_time_is(__atomic_load_n(pair + 1, __ATOMIC_ACQUIRE), ex->run.seq);
+    };
     const auto give_up = std::chrono::steady_clock::now() + std::chrono::microseconds(500);
-    while (seq(0) != ex->run.seq || seq(1) != ex->run.seq)
+    while (!here())
       if (std::chrono::steady_clock::now() > give_up) {                // long runs, and faults
         const hipError_t e = hipStreamSynchronize(ex->stream);
         if (e != hipSuccess) ex->run.lost();
         HIPCK(e);
         break;
       }
-    if (seq(0) != ex->run.seq || seq(1) != ex->run.seq) { ex->run.lost(); ex->err = "the launch ended without its report"; return KVM_STATUS_HIP_ERROR; }
+    if (!here()) { ex->run.lost(); ex->err = "the launch ended without its report"; return KVM_STATUS_HIP_ERROR; }
     done = (int)(pair[0] >> 32);
-    ticks = (unsigned)(pair[1] >> 32);
+    ms = report_ms(pair[1]);
     if (done < 0) {
       std::memcpy(&c, ex->rep, sizeof c);
       done = 0;
@@ -2278,9 +2280,7 @@ int kvm_finish(KvmExec* ex, KvmResult* res) {
   if (ex->S.cnt) {
     if (!c.err_code) done += ex->last_dissolved;   // dissolved no-ops have no work: done once the run completes
   }
-  float ms = 0.f;
-  if (ex->run.self_timed) ms = (float)ticks * 1e-5f;   // of 10 ns
-  else if (ex->launched) hipEventElapsedTime(&ms, ex->ev0, ex->ev1);
+  if (!ex->run.self_timed && ex->launched) hipEventElapsedTime(&ms, ex->ev0, ex->ev1);
   if (res) {
     res->err_code = c.err_code; res->err_slot = c.err_slot; res->err_a = c.err_a; res->err_b = c.err_b;
     res->done = done; res->admitted = ex->streaming ? (int)ex->stream_tasks : (int)ex->tasks.size(); res->grid = ex->grid; res->kernel_ms = ms;

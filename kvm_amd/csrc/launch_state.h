@@ -3,6 +3,13 @@
 
 namespace kvm {
 
+// The second word of a launch's report: 16 bits of its sequence number (enough to know it from the report before) and 48 bits of the
+// launch's time in ticks of 10 ns, a month of them. (32 bits, beside the whole number, are 43 seconds, and the timeout bounds only how
+// long no task ends.)
+constexpr unsigned long long report_time(int seq, unsigned long long ticks) { return (ticks << 16) | ((unsigned)seq & 0xffffu); }
+constexpr bool report_time_is(unsigned long long word, int seq) { return (word & 0xffffu) == ((unsigned)seq & 0xffffu); }
+constexpr float report_ms(unsigned long long word) { return (float)((double)(word >> 16) * 1e-5); }
+
 struct LaunchState {
   int seq = 0;                // sequence number of the last report asked for
   bool reported = false;      // the last launch's report is on its way

@@ -6,6 +6,7 @@ import pytest
 import serving_fp64 as f64
 import serving_graphs as sg
 from kvm_amd.executor import PATH_STATIC, Executor
+from kvm_amd.workloads import Builder
 
 pytestmark = pytest.mark.gpu
 
@@ -61,4 +62,19 @@ def test_launches_collected_at_once_and_traced_between():
     got = sg.cache_of(ex.read, c)
     for n in sg.CACHE:
         np.testing.assert_array_equal(got[n], want[n], err_msg=n)
+    ex.close()
+
+
+@pytest.mark.parametrize('trace', [False, True])
+def test_the_time_of_a_launch(trace):
+    """A launch whose only task waits for 20 ms: its time is that, by the report's clock and by events."""
+    print(f'report time trace {trace}', flush=True)
+    b = Builder(0)
+    b.task('spin', us=20000)
+    lb, init = sg.compiled(b, {})
+    ex = Executor.from_bundle(lb, buffers=init, path=PATH_STATIC, trace=trace)
+    ex.run()
+    for _ in range(3):
+        ex.relaunch()
+        assert 20 <= ex.finish()['kernel_ms'] < 25
     ex.close()
