@@ -2135,9 +2135,12 @@ static void launch_graph(const KvmDevState& S, const LaunchArgs& L, int grid, hi
   if (after_exec) hipEventRecord(after_exec, st);
 }
 
-static void launch_report(KvmExec* ex) {
-  hipLaunchKernelGGL(kvm_report_kernel, dim3(1), dim3(KVM_THREADS), 0, ex->stream, ex->S, ex->rep, ex->run.next_seq());
-  ex->run.reported = true;
+static hipError_t launch_report(KvmExec* ex) {
+  int seq = ex->run.next_seq();
+  void* args[] = {&ex->S, &ex->rep, &seq};
+  const hipError_t e = hipLaunchKernel((const void*)kvm_report_kernel, dim3(1), dim3(KVM_THREADS), args, 0, ex->stream);   // its own status
+  ex->run.reported = e == hipSuccess;
+  return e;
 }
 
 // Untraced static launches of graphs without version variables are one kernel: its last workgroup reports, with the launch's time by the
@@ -2246,8 +2249,7 @@ int kvm_finish(KvmExec* ex, KvmResult* res) {
   int done = 0;
   float ms = 0.f;
   if (ex->rep && ex->launched) {   // wait for the report: the stream's last word, with every task's stores behind it
-    if (!ex->run.reported) launch_report(ex);
-    HIPCK(hipGetLastError());
+    if (!ex->run.reported) HIPCK(launch_report(ex));
     const unsigned long long* pair = (const unsigned long long*)(ex->rep + KVM_REP_PAIRS(ex->grid));
     auto here = [&] {
       return (int)(unsigned)__atomic_load_n(pair, __ATOMIC_ACQUIRE) == ex->run.seq && report_time_is(__atomic_load_n(pair + 1, __ATOMIC_ACQUIRE), ex->run.seq);

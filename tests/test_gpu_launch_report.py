@@ -5,7 +5,8 @@ import pytest
 
 import serving_fp64 as f64
 import serving_graphs as sg
-from kvm_amd.executor import PATH_STATIC, Executor
+from kvm_amd import executor
+from kvm_amd.executor import PATH_DYNAMIC, PATH_STATIC, Executor
 from kvm_amd.workloads import Builder
 
 pytestmark = pytest.mark.gpu
@@ -77,4 +78,22 @@ def test_the_time_of_a_launch(trace):
     for _ in range(3):
         ex.relaunch()
         assert 20 <= ex.finish()['kernel_ms'] < 25
+    ex.close()
+
+
+@pytest.mark.parametrize('path,trace', [(PATH_STATIC, False), (PATH_STATIC, True), (PATH_DYNAMIC, False)])
+def test_an_error_of_another_call_is_not_the_launchs(path, trace):
+    """A HIP call of the program that fails between a launch and its collection (a device number that is not there) leaves its error with
+    the thread; the launch is collected all the same."""
+    print(f'report foreign error path {path} trace {trace}', flush=True)
+    c, k, v, lb, init = _graph()
+    ex = Executor.from_bundle(lb, buffers=init, path=path, trace=trace)
+    L = executor.lib()
+    ex.relaunch()
+    assert L.hipSetDevice(1 << 20) != 0
+    res = ex.finish(check=False)
+    assert res['err_code'] == 0 and res['done'] == lb.ntasks
+    L.hipGetLastError()                                                # the program takes its error
+    ex.relaunch()
+    assert ex.finish()['done'] == lb.ntasks
     ex.close()
