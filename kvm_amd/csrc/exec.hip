@@ -2091,7 +2091,7 @@ static int do_upload(KvmExec* ex) {
   ex->S.trace_on = ex->cfg.trace_on && ex->trace_req ? 1 : 0;   // a kvm_set_trace before the first launch holds
   for (const MvmTaskDesc& d : ex->tasks) ex->versioned = ex->versioned || d.wait_var >= 0 || d.pub_var >= 0;
   const size_t rep_bytes = (KVM_REP_PAIRS(ex->grid) + 4) * sizeof(int);
-  if (hipHostMalloc((void**)&ex->rep, rep_bytes, hipHostMallocCoherent | hipHostMallocMapped) != hipSuccess) { ex->rep = nullptr; ex->err = "pinned memory for the report"; return KVM_STATUS_HIP_ERROR; }
+  if (!ex->rep && hipHostMalloc((void**)&ex->rep, rep_bytes, hipHostMallocCoherent | hipHostMallocMapped) != hipSuccess) { ex->rep = nullptr; ex->err = "pinned memory for the report"; return KVM_STATUS_HIP_ERROR; }
   std::memset(ex->rep, 0, rep_bytes);
   ex->path = KVM_PATH_DYNAMIC;
   if (ncls) { if (int r = upload_classes(ex, alloc, has_dl.data(), has_bw.data(), pubcls, tbw, false)) return r; }
@@ -2282,7 +2282,10 @@ int kvm_finish(KvmExec* ex, KvmResult* res) {
   if (ex->S.cnt) {
     if (!c.err_code) done += ex->last_dissolved;   // dissolved no-ops have no work: done once the run completes
   }
-  if (!ex->run.self_timed && ex->launched) hipEventElapsedTime(&ms, ex->ev0, ex->ev1);
+  if (!ex->run.self_timed && ex->launched) {   // the report comes behind the event; that the event is marked may take longer
+    HIPCK(hipEventSynchronize(ex->ev1));
+    HIPCK(hipEventElapsedTime(&ms, ex->ev0, ex->ev1));
+  }
   if (res) {
     res->err_code = c.err_code; res->err_slot = c.err_slot; res->err_a = c.err_a; res->err_b = c.err_b;
     res->done = done; res->admitted = ex->streaming ? (int)ex->stream_tasks : (int)ex->tasks.size(); res->grid = ex->grid; res->kernel_ms = ms;

@@ -97,3 +97,17 @@ def test_an_error_of_another_call_is_not_the_launchs(path, trace):
     ex.relaunch()
     assert ex.finish()['done'] == lb.ntasks
     ex.close()
+
+
+@pytest.mark.parametrize('path,trace', [(PATH_STATIC, True), (PATH_DYNAMIC, False)])
+def test_every_launch_between_events_has_a_time(path, trace):
+    print(f'report event times path {path} trace {trace}', flush=True)
+    c, k, v, lb, init = _graph()
+    ex = Executor.from_bundle(lb, buffers=init, path=path, trace=trace)
+    ex.run()
+    for _ in range(500):
+        ex.relaunch()
+        assert 0 < ex.finish()['kernel_ms'] < 50
+    ms = ex.run_timed(20)                                              # its events hold 20 launches
+    assert ms > 0 and abs(ex.finish()['kernel_ms'] - ms) < 1e-3
+    ex.close()
