@@ -44,7 +44,8 @@ def kv_q8_buffers(b: Builder, name: str, batch: int, kv_heads: int, hd: int, tma
 def kv_append_q8(b: Builder, c: CacheQ8, knew: str, vnew: str, lens: str, n_new: int = 1, after=(), kgamma: str | None = None, theta: float = 0.0,
                  eps: float = 0.0, tasks: int = 256) -> list[str]:
     """Appends n_new tokens to every sequence in about `tasks` tasks: (sequence, head) pairs, and with fewer pairs than tasks
-    also shares of a long n_new."""
+    also shares of a long n_new. Tokens that may be taken back (drafted ones) must not finish a block: a length can be set back
+    within the unfinished block or to where a block starts, not into a block that has become full."""
     pairs = c.batch * c.kv_heads
     P = max(1, min(tasks // pairs, n_new // c.blk))
     kw = dict(knew=knew, vnew=vnew, lens=lens, kgamma=kgamma, theta=theta, eps=eps, n_new=n_new, P=P, **c.args())

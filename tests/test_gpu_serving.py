@@ -117,6 +117,34 @@ def test_append_token_by_token():
             np.testing.assert_array_equal(have[x + 't'][:, :75 % 32], want[x + 't'][:, :75 % 32])
 
 
+@pytest.mark.parametrize('hd', [128, 100])
+@pytest.mark.parametrize('first,drafted,kept', [(10, 7, 0), (10, 21, 5), (0, 31, 30), (32, 31, 0), (30, 2, 2), (20, 44, 44), (20, 12, 12), (25, 20, 7)], ids=str)
+def test_lengths_set_back(first, drafted, kept, hd):
+    """Drafted tokens are appended, attended to and all but `kept` taken back (to within the unfinished block, or to where a block
+    starts); the tokens and the attention that follow are as if only the kept ones had been there."""
+    print(f'set back {first} {drafted} {kept} hd {hd}', flush=True)
+    rng = np.random.default_rng(6)
+    have = f64.empty_cache(2, 3, 32, hd)
+    rows = lambda n: tuple(bl.bf16_round(rng.standard_normal((n, 2 * hd)).astype(np.float32)) for _ in range(2))   # noqa: E731
+    step = lambda c, x, at: sg.cache_of(_run(*sg.append_graph(c, *x, [at], 2, len(x[0]))).__getitem__, c)   # noqa: E731
+    begin, draft, after = rows(first), rows(drafted), rows(9)
+    if first:
+        have = step(have, begin, 0)
+    have = step(have, draft, first)
+    L = first + kept
+    have = step(have, after, L)
+    k, v = (np.concatenate([begin[i], draft[i][:kept], after[i]]) for i in range(2))
+    want = f64.append(f64.empty_cache(2, 3, 32, hd), k, v, [0], 2, L + 9, True)
+    n = L + 9
+    for x in 'kv':
+        np.testing.assert_array_equal(have[x + 'q'][:, :n // 32], want[x + 'q'][:, :n // 32])
+        np.testing.assert_array_equal(have[x + 's'][:, :n // 32], want[x + 's'][:, :n // 32])
+        np.testing.assert_array_equal(have[x + 't'][:, :n % 32], want[x + 't'][:, :n % 32])
+    q = bl.bf16_round(rng.standard_normal((1, 4 * hd)).astype(np.float32))
+    o, bound = f64.attend(want, q, [n - 1], 2, 4, 1, np.float32(0.1))
+    sg.near(_run(*sg.attend_graph(have, q, [n - 1], 2, 4, 1, 0.1))['o'], o, bound, 'bf16')
+
+
 @pytest.mark.parametrize('rope', [False, True])
 @pytest.mark.parametrize('tasks', [1, 7, 256])
 @pytest.mark.parametrize('case', sg.ATTENDS, ids=lambda c: str(c)[:60])
