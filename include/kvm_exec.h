@@ -84,6 +84,9 @@ typedef struct KvmTrace {
 typedef struct KvmResult {
   int err_code, err_slot, err_a, err_b;   // first device error (0 none)
   int done, admitted, grid;
+  // The last launch's time in ms. Untraced launches of the static path without version variables: the device's clock from worker 0's
+  // start to the last worker's end, without the launch itself. Other launches: between events, the reset in front included
+  // (after kvm_run_timed and kvm_run_timed_split: between their events, all launches together).
   float kernel_ms;
 } KvmResult;
 
@@ -136,7 +139,10 @@ int kvm_window_done(KvmExec* ex, long long wid);
 // mvm_exec.cu:830-889).
 int kvm_submit_stream(KvmExec* ex, const MvmTaskDesc* tasks, int ntasks, const int32_t* succ, int nedges,
                       const int32_t* args, int nargs, int max_window_tasks, int timeout_ms);
-// Waits for the launch, then fills `res` (reference: close/finish, mvm_exec.cu:1505-1540).
+// Waits for the launch, then fills `res` (reference: close/finish, mvm_exec.cu:1505-1540). Every task's stores are out by then, the
+// kernel itself may still be ending (work on the executor's stream comes behind it). The calling thread polls the launch's report
+// for up to 500 us, after that it waits with the stream. HIP errors that other calls left with the thread are not looked at. After a device
+// error the next launch starts clean, the arrival counts of ops 310 and 313 included.
 int kvm_finish(KvmExec* ex, KvmResult* res);
 // Runs the whole submitted graph again on the current buffer contents (versions restart from their set values):
 // reset + launch, asynchronous. Used for repeated training steps / decode tokens; kvm_finish collects it.

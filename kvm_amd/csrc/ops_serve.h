@@ -197,7 +197,8 @@ __device__ __forceinline__ void q8_new_key(const AppendQ8& A, LDS float* x, long
   }
 }
 
-// KV append in 8 bits, any alignment and head size: token by token into an f32 copy of the block in LDS, which is quantised
+// KV append in 8 bits, any alignment and head size (16-byte vectors need aligned rows and 64 or 128 dims; this form is the plain one,
+// 4,001 tokens of 8 heads of 96 dims 175 us where 128 dims take 32): token by token into an f32 copy of the block in LDS, which is quantised
 // when it is full and stored to the tail otherwise.
 __device__ __noinline__ void op_kv_append_q8(const Ctx& c) {
   const AppendQ8 A(c);
@@ -262,7 +263,7 @@ __device__ __noinline__ void op_kv_append_q8(const Ctx& c) {
 // A full block is in registers as a whole, all its loads requested before any is used, K and V together with one reduction of both
 // maxima (of the largest blocks one after the other: their registers would be most of a worker's scratch). Keys to be normalised or
 // rotated go through LDS first, row by row. Keys are stored as they lie, 8 bytes a lane; values turn through LDS. One token of a
-// sequence: 4 us a task; a block of 64 tokens of 128 dims: 5 us.
+// sequence: 4 us a task, 5 with norm and rotation; a block of 64 tokens of 128 dims: 6 us, 8 with them.
 template <int HD> struct AppendLds {
   LDS double* freq; LDS float* red; LDS float* keys; LDS float* angs; LDS unsigned char* turn;
   __device__ explicit AppendLds(LDS char* p)
@@ -452,7 +453,8 @@ struct DecodeQ8 {
   __device__ void zeros(int b, int h) const { for (int e = tid(); e < R * hd; e += KVM_THREADS) o.st(at(o, b, h, e / hd) + e % hd, 0.f); }
 };
 
-// Decode attention over the 8-bit cache, any alignment and head size: whole pairs, every S-th one; 256 tokens at a time, a thread
+// Decode attention over the 8-bit cache, any alignment and head size (a byte a load: 24 sequences of up to 4,096 tokens 2.6 ms at 96
+// dims, 62 us at 128): whole pairs, every S-th one; 256 tokens at a time, a thread
 // to a token for the scores and to an output element for P V, each row with its running maximum and sum.
 __device__ __forceinline__ void attn_q8_pair(const Ctx& c, const DecodeQ8& D, int b, int kvh, int L) {
   constexpr float LOG2E = 1.44269504088896340736f;
@@ -548,8 +550,8 @@ __device__ __noinline__ void op_attn_decode_q8(const Ctx& c) {
 // tokens of its whole blocks; the pairs in order, by sequence and head, are cut into equal shares, in the tasks alike from the
 // lengths. A cut within Q8_SNAP of a pair's end moves there: a small piece costs more than it balances. A pair that is cut has one piece in
 // each of consecutive tasks; the first has the unfinished block.
-// Measured (pair, snap, smallest share), us of a launch: one sequence of 32,000 tokens 50 (12, 14, 16), 55 (8, 12, 24), 57 (16, 20, 32),
-// 71 (24, 28, 56); 24 sequences of up to 4,096 tokens 69, 72, 70, 77; 6 sequences of 1,531, four tokens each 40, 42, 42, 41.
+// Measured (pair, snap, smallest share), us of a launch in a row of them: one sequence of 32,000 tokens 38 (12, 14, 16), 44 (8, 12, 24),
+// 45 (16, 20, 32), 59 (24, 28, 56); 24 sequences of up to 4,096 tokens 57, 60, 61, 65; 6 sequences of 1,531, four tokens each 30, 32, 31, 30.
 constexpr int Q8_PAIR = 12, Q8_SNAP = 14, Q8_SHARE = 16, Q8_SEQS = 1024;
 // (32 bits are enough: a unit is 4 KB and more of cache, whose buffers hold less than 2^33 bytes.)
 struct WorkQ8 {
@@ -681,8 +683,8 @@ __device__ __forceinline__ void q8_arrive(const Ctx& c, const DecodeQ8& D, int b
 }
 
 // Decode attention over the 8-bit cache at head sizes 64 and 128, on the matrix units. Bound: streaming the cache's bytes, and
-// where few workers stream at once the 421 vector instructions and 56 products of a unit. 128 sequences of 8,000 tokens, 8 kv heads
-// of 128: 2.1 GB in 476 us (4.4 TB/s, a copy reaches 4.8). A piece costs 9 to 12 us beside its units (dependent loads: lengths, rows,
+// where few workers stream at once the 415 vector instructions and 56 products of a unit. 128 sequences of 8,000 tokens, 8 kv heads
+// of 128: 2.1 GB in 470 us (4.5 TB/s, a copy reaches 4.8). A piece costs 9 to 12 us beside its units (dependent loads: lengths, rows,
 // first unit; the unfinished block; the waves' sum), a unit about 0.5.
 // Each wave takes units of 64 tokens in turn, K and V straight from memory into registers in the layout of the operands, one to two
 // units ahead:
@@ -699,7 +701,7 @@ __device__ __forceinline__ void q8_arrive(const Ctx& c, const DecodeQ8& D, int b
 // of the largest. (Relative to the largest scale alone, a block without weight left 12 bits of the others at scales 2^26 apart and
 // nothing at 2^36.) Each unit's P V is summed on its own and added to the running one in f32 (the units' chained sums round
 // towards -inf). The unfinished block, at most blk - 1 tokens, is f32 work
-// of all lanes (a wave to a row, the tail in its registers and no barrier, was slower: 24 ragged sequences 52 -> 67 us).
+// of all lanes (a wave to a row, the tail in its registers and no barrier, was 15 us slower for 24 ragged sequences).
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 // Eight signed bytes (two words) as f16.
@@ -1052,8 +1054,8 @@ __device__ __noinline__ bool op_attn_decode_q8_fast(const Ctx& c) {
 // Adjusted logits (op 314). Bound: the bytes of the logits, and per task the history, which every task of a row reads as a whole (a few
 // KB, from the L2). The task's logits go through as a stream that knows only the mask, in vectors of 4 from any element (a bf16
 // row from its first aligned one), NB of a thread requested ahead (64 KB of f32, 32 KB of bf16), each again as soon as it is stored;
-// vectors of 8 bf16 logits have stores of 16 bytes 32 apart: 33 -> 40 us a task of 50,257 logits. Rows in place without a mask have
-// no stream.
+// vectors of 8 bf16 logits have stores of 16 bytes 32 apart, 7 us more for a task of 50,257 logits. Rows in place without a mask
+// have no stream.
 // The few tokens that the history or the biases name meet in LDS, one word each (generated: bits 0..19, bias slot: bits 20..30,
 // prompt: bit 31), before the first vectors of the stream have come; behind the stream their logits are written again, each once, four
 // of a thread in flight. The words lie at the tokens themselves where the range fits (22,528 logits) and are taken out of there by an
