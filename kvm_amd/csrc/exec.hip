@@ -38,6 +38,8 @@
 #include "ops_decode.h"
 #include "ops_stream.h"
 #include "ops_serve.h"
+#include "ops_quant.h"
+#include "ops_paged.h"
 #include "validate.h"
 #include "static_plan.h"
 #include "launch_state.h"
@@ -672,6 +674,11 @@ __device__ void dispatch(int op, const Ctx& c) {
     case 312: if (!op_kv_append_q8_fast(c)) op_kv_append_q8(c); break;
     case 313: if (!op_attn_decode_q8_fast(c)) op_attn_decode_q8(c); break;
     case 314: op_logits_adjust(c); break;
+    case 315: op_rows_q8(c); break;
+    case 316: op_matmul_q8(c); break;
+    case 317: op_gemv_q8(c); break;
+    case 318: if (!op_qkv_append_paged_fast(c)) op_qkv_append_paged(c); break;
+    case 319: op_attn_paged(c); break;
     default: if (threadIdx.x == 0) c.fail(KVM_ERR_BAD_OP, op, 0);
   }
 }
@@ -755,6 +762,7 @@ __global__ __launch_bounds__(KVM_THREADS, 1) void kvm_static_kernel(KvmDevState 
     if (sf & KVM_SF_PRE) {
       const int op = s_rec.desc.op_id;
       if (op == 134 || op == 301 || op == 311) gemv_prefetch(c, op);
+      else if (op == 317) gemv_q8_prefetch(c);
       else attn_prefetch(c, op);
       c.pre = 1;
     }
@@ -1247,6 +1255,7 @@ static std::vector<KvmCountRange> count_ranges(const std::vector<MvmTaskDesc>& t
     const int32_t* a = args.data() + d.args_off;
     if (d.op_id == 310) r.push_back({(int*)table[a[22]].p + (long long)a[7] * a[12] + a[8], 1});
     if (d.op_id == 313) r.push_back({(int*)table[a[10]].p + (long long)a[12] * a[18], (long long)(a[13] - a[12]) * a[18]});
+    if (d.op_id == 319) r.push_back({(int*)table[a[8]].p, a[10]});
   }
   std::sort(r.begin(), r.end(), [](const KvmCountRange& x, const KvmCountRange& y) { return x.p != y.p ? x.p < y.p : x.n > y.n; });
   std::vector<KvmCountRange> out;
@@ -1915,7 +1924,7 @@ static std::vector<int> static_flags(const KvmExec* ex, const kvms::Plan& P) {
     if (sigs[op].empty()) if (const kvmv::OpSig* o = kvmv::find_op(op)) sigs[op] = kvmv::parse_sig(o->sig);
     const int32_t* a = ex->args.data() + d.args_off;
     for (size_t k = 0; k < sigs[op].size() && (int)k < d.args_words; ++k)
-      if (sigs[op][k].type == 0 && a[k] >= 0 && a[k] < nb && !((op == 134 || op == 301) && k == 3) && !(op == 311 && (k == 2 || k == 3)) &&
+      if (sigs[op][k].type == 0 && a[k] >= 0 && a[k] < nb && !((op == 134 || op == 301 || op == 317) && k == 3) && !(op == 311 && (k == 2 || k == 3)) &&
           !((op == 135 || op == 306 || op == 310) && (k == 1 || k == 2)))
         other_use[a[k]] = 1;
   }
@@ -1923,7 +1932,7 @@ static std::vector<int> static_flags(const KvmExec* ex, const kvms::Plan& P) {
   for (int i = 0; i < n; ++i) {
     const MvmTaskDesc& d = ex->tasks[i];
     if (P.publishes[i]) f[i] |= KVM_SF_PUB;
-    if ((d.op_id == 134 || d.op_id == 301) && d.args_words > 3) {
+    if ((d.op_id == 134 || d.op_id == 301 || d.op_id == 317) && d.args_words > 3) {
       const int wb = ex->args[d.args_off + 3];
       if (wb >= 0 && wb < nb && !other_use[wb] && !getenv("KVM_NO_PREFETCH")) f[i] |= KVM_SF_PRE;
     }

@@ -1,0 +1,536 @@
+// A KV cache in pages: append of new tokens with head norm and rotation (op 318) and their attention (op 319). Semantics: mvm_ops_kvm.def.
+#pragma once
+#include "common.h"
+#include "ops_basic.h"
+#include "ops_attn.h"
+#include "ops_serve.h"
+
+namespace kvm {
+
+constexpr int PG_SEQS = 1024;
+
+// What both operators check before they write: row numbers that do not fall and end within the buffers, lengths within the table. All
+// threads of the workgroup call it; the row numbers are in LDS afterwards (cu: B + 1 words).
+__device__ __forceinline__ bool paged_call_ok(const Ctx& c, const View& cu, const View& lens, int B, int rows, long long room, LDS int* scu) {
+  bool bad = false;
+  for (int b = tid(); b <= B; b += KVM_THREADS) {
+    const int r = cu.i()[b], p = b ? cu.i()[b - 1] : 0, L = b ? lens.i()[b - 1] : 0;
+    scu[b] = r;
+    if (r < p || p < 0 || r > rows || (r > p && b && (L < 0 || (long long)L + (r - p) > room))) { bad = true; c.fail(KVM_ERR_OP_KVLEN, b - 1, L); }
+  }
+  return !__syncthreads_or(bad);
+}
+// The sequence of row r < scu[B]: the last one that starts at or before it (ones without rows start where the next does).
+__device__ __forceinline__ int paged_owner(const LDS int* scu, int B, int r) {
+  int lo = 0, hi = B;                                                  // scu[lo] <= r < scu[hi]
+  while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (scu[mid] <= r) lo = mid; else hi = mid; }
+  return lo;
+}
+
+// ---------------------------------------------------------------------------------------------- append
+struct AppendPaged {
+  View q, k, v, qo, kc, vc, table, lens, cu, qg, kg; int r0, r1, B, H, Hkv, hd, page, lp; float theta, eps; int pages;
+  __device__ explicit AppendPaged(const Ctx& c)
+      : q(uview(c, 0)), k(uview(c, 1)), v(uview(c, 2)), qo(uview(c, 3)), kc(uview(c, 4)), vc(uview(c, 5)), table(uview(c, 6)), lens(uview(c, 7)), cu(uview(c, 8)), qg(uview(c, 9)),
+        kg(uview(c, 10)), r0(rfl(c.i(11))), r1(rfl(c.i(12))), B(rfl(c.i(13))), H(rfl(c.i(14))), Hkv(rfl(c.i(15))), hd(rfl(c.i(16))), page(rfl(c.i(17))), theta(c.f(18)), eps(c.f(19)) {
+    lp = 31 - __clz(page);
+    pages = (int)((unsigned)kc.rows / (unsigned)(Hkv * page));
+    if (!q.ok()) H = 0;
+  }
+  __device__ int rows() const { return q.ok() ? min(min(q.rows, qo.rows), min(k.rows, v.rows)) : min(k.rows, v.rows); }
+  // Position of row r and its place in the pages (of head 0); the page is checked.
+  __device__ bool place(const LDS int* scu, int r, int& t, long long& at) const {
+    const int b = paged_owner(scu, B, r);
+    t = lens.i()[b] + (r - scu[b]);
+    const int p = table.i()[(long long)b * table.cols + (t >> lp)];
+    at = (((long long)p * Hkv) << lp) + (t & (page - 1));
+    return (unsigned)p < (unsigned)pages;
+  }
+};
+// LDS of a task: rows in flight with their positions, places and angles.
+constexpr int AP_ROWS = 32;
+struct AppendPagedLds {
+  LDS double* freq; LDS long long* at; LDS int* pos; LDS int* cu; LDS float* ang;
+  __device__ explicit AppendPagedLds(LDS char* p) : freq((LDS double*)p), at((LDS long long*)(freq + 128)), pos((LDS int*)(at + AP_ROWS)), cu(pos + AP_ROWS), ang((LDS float*)(cu + PG_SEQS + 4)) {}
+  static constexpr int BYTES = 128 * 8 + AP_ROWS * 12 + (PG_SEQS + 4) * 4 + AP_ROWS * 256 * 4;
+};
+static_assert(AppendPagedLds::BYTES <= KVM_LDS_BYTES, "LDS");
+// Checks the call and the task's own pages (nothing is written before), then the frequencies; the rows that have a token end at `end`.
+__device__ __forceinline__ bool append_paged_begin(const Ctx& c, const AppendPaged& A, const AppendPagedLds& M, int& end) {
+  if (!paged_call_ok(c, A.cu, A.lens, A.B, A.rows(), (long long)A.table.cols << A.lp, M.cu)) return false;
+  end = min(A.r1, rfl(M.cu[A.B]));
+  bool bad = false;
+  for (int r = max(A.r0, rfl(M.cu[0])) + tid(); r < end; r += KVM_THREADS) {
+    int t; long long at;
+    if (!A.place(M.cu, r, t, at)) { bad = true; c.fail(KVM_ERR_OP_RANGE, r, t); }
+  }
+  if (A.theta > 0.f && tid() < A.hd / 2) M.freq[tid()] = q8_freq(tid(), A.hd, log((double)A.theta));
+  return !__syncthreads_or(bad);
+}
+// Positions, places and angles of rows [r, r + nr).
+__device__ __forceinline__ void append_paged_rows(const AppendPaged& A, const AppendPagedLds& M, int r, int nr) {
+  const int half = A.hd / 2;
+  __syncthreads();
+  if (tid() < nr) {
+    int t; long long at;
+    A.place(M.cu, r + tid(), t, at);
+    M.pos[tid()] = t; M.at[tid()] = at;
+  }
+  __syncthreads();
+  if (A.theta > 0.f) {
+    for (int e = tid(); e < nr * half; e += KVM_THREADS) {
+      const int u = e / half, i = e % half;
+      float sn, co; q8_turn(M.pos[u], M.freq[i], sn, co);
+      M.ang[u * A.hd + i] = sn; M.ang[u * A.hd + half + i] = co;
+    }
+    __syncthreads();
+  }
+}
+// Any head size and alignment: a wave to a (row, head), a lane to pairs of dims.
+__device__ __noinline__ void op_qkv_append_paged(const Ctx& c) {
+  const AppendPaged A(c);
+  const AppendPagedLds M(c.smem);
+  int end;
+  if (!append_paged_begin(c, A, M, end)) return;
+  const int half = A.hd / 2, heads = A.H + 2 * A.Hkv, l = lane();
+  for (int r = max(A.r0, rfl(M.cu[0])); r < end; r += AP_ROWS) {
+    const int nr = min(AP_ROWS, end - r);
+    append_paged_rows(A, M, r, nr);
+    for (int u = wave(); u < nr * heads; u += KVM_WAVES) {
+      const int row = u / heads, s = u % heads, what = s < A.H ? 0 : s < A.H + A.Hkv ? 1 : 2, h = what == 0 ? s : what == 1 ? s - A.H : s - A.H - A.Hkv;
+      const View src = what == 0 ? A.q : what == 1 ? A.k : A.v, dst = what == 0 ? A.qo : what == 1 ? A.kc : A.vc, g = what == 0 ? A.qg : what == 1 ? A.kg : View{nullptr, 0, 0, 0, 0};
+      const long long from = (long long)(r + row) * src.cols + (long long)h * A.hd;
+      const long long to = what == 0 ? (long long)(r + row) * dst.cols + (long long)h * A.hd : (M.at[row] + ((long long)h << A.lp)) * dst.cols;
+      float x[2][2], ss = 0.f;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int i = l + 64 * j;
+        x[j][0] = i < half ? src.ld(from + i) : 0.f; x[j][1] = i < half ? src.ld(from + half + i) : 0.f;
+        ss += x[j][0] * x[j][0] + x[j][1] * x[j][1];
+      }
+      const float rs = g.ok() ? 1.f / sqrtf(wave_sum(ss) / A.hd + A.eps) : 1.f;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int i = l + 64 * j;
+        if (i >= half) continue;
+        float a = x[j][0], b = x[j][1];
+        if (g.ok()) { a = a * rs * g.f()[i]; b = b * rs * g.f()[half + i]; }
+        if (what < 2 && A.theta > 0.f) {
+          const float sn = M.ang[row * A.hd + i], co = M.ang[row * A.hd + half + i], y = a * co - b * sn;
+          b = a * sn + b * co; a = y;
+        }
+        dst.st(to + i, a); dst.st(to + half + i, b);
+      }
+    }
+  }
+}
+// Head sizes 64 and 128, rows in whole vectors. Bound: bytes for prompts, a few dependent loads (row numbers, length, page, row) and the
+// launch for single tokens. A (row, head) is HD / 8 lanes of 8 values; a row's angles are computed once for all its heads; four items'
+// loads are requested together.
+template <int HD> __device__ __noinline__ void append_paged_t(const Ctx& c) {
+  constexpr int LPR = HD / 8, RPP = KVM_THREADS / LPR, NR = 4;
+  const AppendPaged A(c);
+  const AppendPagedLds M(c.smem);
+  int end;
+  if (!append_paged_begin(c, A, M, end)) return;
+  const int ln = tid() % LPR, rw = tid() / LPR, heads = A.H + 2 * A.Hkv;
+  const float sign = ln >= LPR / 2 ? 1.f : -1.f;
+  for (int r = max(A.r0, rfl(M.cu[0])); r < end; r += AP_ROWS) {
+    const int nr = min(AP_ROWS, end - r), items = nr * heads;
+    append_paged_rows(A, M, r, nr);
+    for (int u0 = rw; u0 < items; u0 += NR * RPP) {
+      Raw8 raw[NR];
+#pragma unroll
+      for (int i = 0; i < NR; ++i) {
+        const int u = min(u0 + i * RPP, items - 1), row = u / heads, s = u % heads;
+        const View& X = s < A.H ? A.q : s < A.H + A.Hkv ? A.k : A.v;
+        const int h = s < A.H ? s : s < A.H + A.Hkv ? s - A.H : s - A.H - A.Hkv;
+        raw[i].load(X, (long long)(r + row) * X.cols + h * HD + 8 * ln);
+      }
+#pragma unroll
+      for (int i = 0; i < NR; ++i) {
+        const int u = u0 + i * RPP;
+        if (u >= items) break;
+        const int row = u / heads, s = u % heads, what = s < A.H ? 0 : s < A.H + A.Hkv ? 1 : 2, h = what == 0 ? s : what == 1 ? s - A.H : s - A.H - A.Hkv;
+        float x[8];
+        raw[i].get((what == 0 ? A.q.dtype : what == 1 ? A.k.dtype : A.v.dtype) == 2, x);
+        const View& g = what == 0 ? A.qg : A.kg;
+        if (what < 2 && g.ok()) {
+          float ss = 0.f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) ss += x[e] * x[e];
+          const float rs = 1.f / sqrtf(lanes_sum<LPR>(ss) / HD + A.eps);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = x[e] * rs * g.f()[8 * ln + e];
+        }
+        if (what < 2 && A.theta > 0.f) {
+          const LDS float* ang = M.ang + row * HD + 8 * (ln % (LPR / 2));
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = x[e] * ang[HD / 2 + e] + sign * __shfl_xor(x[e], LPR / 2, 64) * ang[e];
+        }
+        const View& Y = what == 0 ? A.qo : what == 1 ? A.kc : A.vc;
+        st8(Y, what == 0 ? (long long)(r + row) * Y.cols + h * HD + 8 * ln : (M.at[row] + ((long long)h << A.lp)) * Y.cols + 8 * ln, x);
+      }
+    }
+  }
+}
+__device__ __noinline__ bool op_qkv_append_paged_fast(const Ctx& c) {
+  const View q = c.buf(0), qo = c.buf(3);
+  if ((q.ok() && (!rows8_ok(q) || !rows8_ok(qo))) || !rows8_ok(c.buf(1)) || !rows8_ok(c.buf(2)) || !rows8_ok(c.buf(4)) || !rows8_ok(c.buf(5))) return false;
+  if (c.i(16) == 128) append_paged_t<128>(c);
+  else if (c.i(16) == 64) append_paged_t<64>(c);
+  else return false;
+  return true;
+}
+
+// ---------------------------------------------------------------------------------------------- attention
+struct AttnPaged {
+  View q, kc, vc, table, lens, cu, part, o, cnt; int s, S, B, H, Hkv, hd, page, tile, G, lp, pages; float sl2;
+  __device__ explicit AttnPaged(const Ctx& c)
+      : q(uview(c, 0)), kc(uview(c, 1)), vc(uview(c, 2)), table(uview(c, 3)), lens(uview(c, 4)), cu(uview(c, 5)), part(uview(c, 6)), o(uview(c, 7)), cnt(uview(c, 8)),
+        s(rfl(c.i(9))), S(rfl(c.i(10))), B(rfl(c.i(11))), H(rfl(c.i(12))), Hkv(rfl(c.i(13))), hd(rfl(c.i(14))), page(rfl(c.i(15))), tile(rfl(c.i(16))) {
+    G = H / Hkv;
+    lp = 31 - __clz(page);
+    pages = (int)((unsigned)kc.rows / (unsigned)(Hkv * page));
+    sl2 = __int_as_float(rfl(__float_as_int(c.f(17) * 1.44269504088896340736f)));
+  }
+  // bf16 storage at head sizes 64 and 128 in whole vectors: the matrix units
+  __device__ bool fast() const {
+    return q.dtype == 2 && kc.dtype == 2 && vc.dtype == 2 && o.dtype == 2 && (hd == 64 || hd == 128) && rows8_ok(q) && rows8_ok(kc) && rows8_ok(vc) && rows8_ok(o) &&
+           (long long)Hkv * page * max(kc.cols, vc.cols) * 2 < 0x7fffff00ll;
+  }
+};
+// A tile's rows: row r is token tok0 + r / G of the sequence's new ones, head h * G + r % G; it sees keys 0 .. L + tok0 + r / G.
+struct TilePaged { int b, h, L, row0, tok0, ntok; long long start, cost; };
+// A piece of a tile: keys [k0, k1), k0 a multiple of 64; piece k of `live`, the second of which falls to task i0.
+struct PiecePaged { int k0, k1, k, live, i0; };
+
+// The work of a call over its tasks: a tile costs PG_TILE and one per key up to the last that it sees; tiles in order of sequence, kv head
+// and token are cut into equal shares, in all tasks alike from the lengths. A cut within PG_SNAP of a tile's end moves there: a small piece
+// costs more than it balances. Tiles of up to 32 rows are a sequence's new tokens as a whole (the waves share the keys); longer ones have `tile`
+// rows (the waves share the rows).
+constexpr int PG_TILE = 256, PG_SNAP = 320, PG_SHARE = 512;
+struct WorkPaged {
+  const LDS long long* pre;    // [B + 1] cost of the sequences before
+  const LDS int *cu, *len;
+  int B, Hkv, G, rows;
+  long long share, total;
+  __device__ __forceinline__ int tokens(int n) const { return (long long)n * G <= 32 ? n : max(1, rows / G); }   // of a tile
+  // cost of the first j tiles of TT tokens of one head, none of them the last, ragged one
+  __device__ __forceinline__ static long long upto(long long j, long long L, long long TT) { return j * (PG_TILE + L) + TT * (j * (j + 1) / 2); }
+  __device__ __forceinline__ long long head_cost(int n, int L) const {
+    if (n <= 0) return 0;
+    const int TT = tokens(n), nt = (n + TT - 1) / TT;
+    return upto(nt - 1, L, TT) + PG_TILE + L + n;
+  }
+  __device__ __forceinline__ TilePaged find(long long x) const {
+    int b = 0;
+    for (int j0 = 0; j0 < B; j0 += 64) b += __popcll(__ballot(j0 + lane() < B && pre[min(j0 + lane(), B)] <= x));
+    b = rfl(b) - 1;
+    const int L = rfl(len[b]), r0 = rfl(cu[b]), n = rfl(cu[b + 1]) - r0, TT = tokens(n), nt = (n + TT - 1) / TT;
+    const long long p0 = pre[b], hc = head_cost(n, L);
+    const int h = rfl((int)((x - p0) / hc));
+    const long long rest = x - p0 - h * hc;
+    int lo = 0, hi = nt;                                               // upto(lo) <= rest, rest < upto(hi) or hi is the end
+    while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (upto(mid, L, TT) <= rest) lo = mid; else hi = mid; }
+    lo = rfl(lo);
+    TilePaged t;
+    t.b = b; t.h = h; t.L = L; t.row0 = r0 + lo * TT; t.tok0 = lo * TT; t.ntok = min(TT, n - lo * TT);
+    t.start = p0 + h * hc + upto(lo, L, TT);
+    t.cost = PG_TILE + (long long)L + t.tok0 + t.ntok;
+    return t;
+  }
+  __device__ __forceinline__ long long cut(int i) const {
+    const long long x = min(i * share, total);
+    if (x == total) return total;
+    const TilePaged t = find(x);
+    const long long off = x - t.start;
+    return off < PG_SNAP ? t.start : t.cost - off < PG_SNAP ? t.start + t.cost : x;
+  }
+  // The piece [x, end) of a tile: its keys, and which of how many pieces it is.
+  __device__ __forceinline__ PiecePaged piece(const TilePaged& t, long long x, long long end) const {
+    auto key = [&](long long off) { return (int)(max(0ll, off - PG_TILE) & ~63ll); };
+    PiecePaged p;
+    p.k0 = x == t.start ? 0 : key(x - t.start);
+    p.k1 = end == t.start + t.cost ? t.L + t.tok0 + t.ntok : key(end - t.start);
+    const long long first = (t.start + PG_SNAP + share - 1) / share, last = (t.start + t.cost - PG_SNAP) / share;
+    const int inside = t.cost < 2 * PG_SNAP ? 0 : (int)max(0ll, last - first + 1);
+    p.i0 = rfl((int)first); p.live = rfl(inside + 1);
+    p.k = x == t.start ? 0 : rfl((int)(x / share - first + 1));
+    p.k0 = rfl(p.k0); p.k1 = rfl(p.k1);
+    return p;
+  }
+};
+// LDS that stays over a task's pieces: the work; the forms' own memory begins behind it.
+constexpr int PG_WORK = (PG_SEQS + 2) * 8 + (PG_SEQS + 4) * 4 + PG_SEQS * 4 + 128;
+
+// Where piece k of a tile keeps its partial rows: the second half of the task in front of i0 for the first one, the first half of its own task
+// for the others (a task has at most one piece of each kind).
+__device__ __forceinline__ GLOBAL float* paged_partial(const AttnPaged& D, const PiecePaged& p, int k, int r) {
+  return D.part.f() + ((long long)(2 * p.i0 - 2 + (k ? 2 * k : 1)) * D.tile + r) * D.part.cols;
+}
+__device__ __forceinline__ long long paged_out(const AttnPaged& D, const TilePaged& t, int r) {
+  return (long long)(t.row0 + r / D.G) * D.o.cols + (long long)(t.h * D.G + r % D.G) * D.hd;
+}
+// The piece that counts itself last merges the tile's rows; maxima are in units of log2. Weights: all pieces' maxima and sums go through LDS,
+// up to 8192 at a time; then a thread has four dims of a row, or a share of the pieces of them where there are threads enough.
+__device__ __noinline__ void paged_merge(const Ctx& c, int row0_, int h_, int ntok_, int live_, int i0_) {
+  const AttnPaged D(c);
+  const int live = rfl(live_), R = rfl(ntok_) * D.G, hd = D.hd;
+  const TilePaged t{0, rfl(h_), 0, rfl(row0_), 0, rfl(ntok_), 0, 0};
+  const PiecePaged p{0, 0, 0, live, rfl(i0_)};
+  LDS float* M = (LDS float*)(c.smem + PG_WORK);                       // [128] maxima, [128] sums
+  LDS float* Z = M + 128;
+  LDS float* ml = Z + 128;                                             // [pieces][R][2]
+  const int PB = 8192 / R;
+  for (int k0 = 0; k0 < live; k0 += PB) {
+    const int n = min(PB, live - k0);
+    __syncthreads();
+    for (int e = tid(); e < n * R; e += KVM_THREADS) {
+      const GLOBAL float* y = paged_partial(D, p, k0 + e / R, e % R) + hd;
+      ml[2 * e] = y[0]; ml[2 * e + 1] = y[1];
+    }
+    __syncthreads();
+    if (tid() < R) {
+      float m = k0 ? M[tid()] : -INFINITY, z = k0 ? Z[tid()] : 0.f, top = m;
+      for (int k = 0; k < n; ++k) top = fmaxf(top, ml[2 * (k * R + tid())]);
+      const float base = top == -INFINITY ? 0.f : top;
+      z *= exp2f(m - base);
+      for (int k = 0; k < n; ++k) z += exp2f(ml[2 * (k * R + tid())] - base) * ml[2 * (k * R + tid()) + 1];
+      M[tid()] = top; Z[tid()] = z;
+    }
+  }
+  __syncthreads();
+  const int C4 = (hd + 3) >> 2, items = R * C4, split = items >= KVM_THREADS ? 1 : min(live, KVM_THREADS / items);
+  for (int e0 = 0; e0 < items; e0 += KVM_THREADS) {
+    const int e = split > 1 ? tid() % items : e0 + tid(), g = split > 1 ? tid() / items : 0;
+    const bool on = e < items && g < split;
+    const int r = on ? e / C4 : 0, d = on ? 4 * (e % C4) : 0, nd = min(4, hd - d);
+    float a[4] = {0.f, 0.f, 0.f, 0.f};
+    constexpr int U = 8;
+    for (int k0 = on ? g : live; k0 < live; k0 += U * split) {
+      float m[U], x[U][4];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const GLOBAL float* y = paged_partial(D, p, min(k0 + u * split, live - 1), r);
+        m[u] = y[hd];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[u][i] = y[d + min(i, nd - 1)];
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const float w = k0 + u * split < live && m[u] != -INFINITY ? exp2f(m[u] - M[r]) : 0.f;
+        if (w != 0.f)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) a[i] += w * x[u][i];
+      }
+    }
+    if (split > 1) {
+      __syncthreads();
+      if (on)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) ml[4 * tid() + i] = a[i];
+      __syncthreads();
+      if (on && g == 0)
+        for (int s = 1; s < split; ++s)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) a[i] += ml[4 * (tid() + s * items) + i];
+    }
+    if (on && g == 0)
+      for (int i = 0; i < nd; ++i) D.o.st(paged_out(D, t, r) + d + i, a[i] / Z[r]);
+  }
+}
+__device__ __forceinline__ void paged_arrive(const Ctx& c, const AttnPaged& D, const TilePaged& t, const PiecePaged& p, LDS int* flag) {
+  wait_stores();
+  __syncthreads();
+  if (tid() == 0) *flag = add_relaxed((int*)D.cnt.i() + p.i0, 1);
+  __syncthreads();
+  const int old = rfl(*flag);
+  if (old < 0 || old >= p.live) { if (tid() == 0) c.fail(KVM_ERR_OP_RANGE, p.i0, old); return; }
+  if (old != p.live - 1) return;
+  fence_acquire();                                                     // the other pieces' partials, stored before their counts
+  paged_merge(c, t.row0, t.h, t.ntok, p.live, p.i0);
+  if (tid() == 0) st_relaxed((int*)D.cnt.i() + p.i0, 0);
+}
+
+// Any storage, head size and alignment, in f32, and pieces of the other forms with results that are not finite (a key that a row does not see
+// has weight 0 there, which an infinity or NaN in its value would turn into NaN; here it is skipped): 32 rows by 32 keys at a time in LDS, the
+// next keys' loads in flight; scores a thread to a key and four rows, eight threads to a row for the softmax and its P V.
+__device__ __noinline__ void attn_paged_general(const Ctx& c, int b_, int h_, int L_, int row0_, int tok0_, int ntok_, int k0_, int k1_, int k_, int live_, int i0_) {
+  const AttnPaged D(c);
+  const TilePaged t{rfl(b_), rfl(h_), rfl(L_), rfl(row0_), rfl(tok0_), rfl(ntok_), 0, 0};
+  const PiecePaged p{rfl(k0_), rfl(k1_), rfl(k_), rfl(live_), rfl(i0_)};
+  constexpr int KB = 32, NF = 8;                                       // keys a step; vectors of 4 a thread at 256 dims
+  const int hd = D.hd, C4 = (hd + 3) >> 2, HP = 4 * C4 + 4, R = t.ntok * D.G;
+  LDS float* qs = (LDS float*)(c.smem + PG_WORK);                      // [32][HP]
+  LDS float* ks = qs + 32 * HP;                                        // [KB][HP]
+  LDS float* vs = ks + KB * HP;
+  LDS float* ps = vs + KB * HP;                                        // [32][KB + 4]; below 0: not seen
+  const bool vec = (hd & 3) == 0 && rows8_ok(D.kc) && rows8_ok(D.vc);
+  const GLOBAL int* tb = D.table.i() + (long long)t.b * D.table.cols;
+  bool bad = false;
+  f32x4n kr[NF], vr[NF];
+  auto at4 = [&](const View& X, long long o, int d) {
+    if (vec) return ld4(X, o + d);
+    return f32x4n{X.ld(o + d), d + 1 < hd ? X.ld(o + d + 1) : 0.f, d + 2 < hd ? X.ld(o + d + 2) : 0.f, d + 3 < hd ? X.ld(o + d + 3) : 0.f};
+  };
+  auto fetch = [&](int kb) {
+#pragma unroll
+    for (int i = 0; i < NF; ++i) {
+      const int e = tid() + i * KVM_THREADS;
+      if (e >= KB * C4) break;
+      const int key = min(kb + e / C4, p.k1 - 1), d = 4 * (e % C4);
+      int id = tb[key >> D.lp];
+      if ((unsigned)id >= (unsigned)D.pages) { bad = true; id = 0; }
+      const long long row = ((((long long)id * D.Hkv) + t.h) << D.lp) + (key & (D.page - 1));
+      kr[i] = at4(D.kc, row * D.kc.cols, d);
+      vr[i] = at4(D.vc, row * D.vc.cols, d);
+    }
+  };
+  for (int rg = 0; rg < R; rg += 32) {
+    __syncthreads();
+    for (int e = tid(); e < 32 * C4; e += KVM_THREADS) {
+      const int r = rg + e / C4, d = 4 * (e % C4);
+      const long long o = (long long)(t.row0 + min(r, R - 1) / D.G) * D.q.cols + (long long)(t.h * D.G + min(r, R - 1) % D.G) * hd;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) qs[(e / C4) * HP + d + i] = d + i < hd ? D.q.ld(o + d + i) : 0.f;
+    }
+    fetch(p.k0);
+    const int row = tid() >> 3, sub = tid() & 7, rr = min(rg + row, R - 1), lim = t.L + t.tok0 + rr / D.G;
+    float m = -INFINITY, lsum = 0.f;
+    f32x4n acc[NF];
+#pragma unroll
+    for (int i = 0; i < NF; ++i) acc[i] = f32x4n{0.f, 0.f, 0.f, 0.f};
+    for (int kb = p.k0; kb < p.k1; kb += KB) {
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < NF; ++i) {
+        const int e = tid() + i * KVM_THREADS;
+        if (e >= KB * C4) break;
+        *(LDS f32x4n*)(ks + (e / C4) * HP + 4 * (e % C4)) = kr[i];
+        *(LDS f32x4n*)(vs + (e / C4) * HP + 4 * (e % C4)) = vr[i];
+      }
+      __syncthreads();
+      if (kb + KB < p.k1) fetch(kb + KB);
+      {
+        const int key = tid() & 31, r4 = 4 * (tid() >> 5);
+        float a[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int d = 0; d < 4 * C4; d += 4) {
+          const f32x4n kk = *(const LDS f32x4n*)(ks + key * HP + d);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const f32x4n qq = *(const LDS f32x4n*)(qs + (r4 + i) * HP + d);
+            a[i] += qq.x * kk.x; a[i] += qq.y * kk.y; a[i] += qq.z * kk.z; a[i] += qq.w * kk.w;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) ps[(r4 + i) * (KB + 4) + key] = a[i] * D.sl2;
+      }
+      __syncthreads();
+      float x[4], mx = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int key = kb + 4 * sub + i;
+        const bool on = key <= lim && key < p.k1;
+        x[i] = on ? ps[row * (KB + 4) + 4 * sub + i] : -INFINITY;
+        mx = fmaxf(mx, x[i]);
+        if (on && x[i] != x[i]) mx = x[i];                             // a NaN score stays one (fmaxf drops it)
+      }
+      mx = lanes_all<8>(mx, [](float a, float b) { return a != a ? a : b != b ? b : fmaxf(a, b); });
+      const float top = mx != mx ? mx : fmaxf(m, mx), f = m == -INFINITY ? 0.f : exp2f(m - top);
+      float sum = 0.f;
+      __syncthreads();                                                 // scores are read before weights overwrite them
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int key = kb + 4 * sub + i;
+        const bool on = key <= lim && key < p.k1;
+        const float e = on ? exp2f(x[i] - top) : -1.f;
+        if (on) sum += e;
+        ps[row * (KB + 4) + 4 * sub + i] = e;
+      }
+      sum = lanes_sum<8>(sum);
+      lsum = lsum * f + sum;
+      m = top;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < NF; ++i) acc[i] *= f;
+      const int n = min(KB, p.k1 - kb);
+      for (int u = 0; u < n; ++u) {
+        const float e = ps[row * (KB + 4) + u];
+        if (e < 0.f) continue;
+#pragma unroll
+        for (int i = 0; i < NF; ++i)
+          if (sub + 8 * i < C4) acc[i] += e * *(const LDS f32x4n*)(vs + u * HP + 4 * (sub + 8 * i));
+      }
+    }
+    if (__syncthreads_or(bad)) { if (tid() == 0) c.fail(KVM_ERR_OP_RANGE, t.b, p.k0); return; }
+    if (rg + row < R) {
+#pragma unroll
+      for (int i = 0; i < NF; ++i)
+        for (int e = 0; e < 4; ++e) {
+          const int d = 4 * (sub + 8 * i) + e;
+          if (d >= hd) break;
+          if (p.live == 1) D.o.st(paged_out(D, t, rg + row) + d, acc[i][e] / lsum);
+          else stwt32(paged_partial(D, p, p.k, rg + row) + d, acc[i][e]);
+        }
+      if (p.live > 1 && sub == 0) { GLOBAL float* y = paged_partial(D, p, p.k, rg + row) + hd; stwt32(y, m); stwt32(y + 1, lsum); }
+    }
+  }
+}
+
+__device__ __noinline__ void op_attn_paged(const Ctx& c) {
+  const AttnPaged D(c);
+  LDS long long* pre = (LDS long long*)c.smem;                         // [PG_SEQS + 2]
+  LDS int* scu = (LDS int*)(pre + PG_SEQS + 2);                        // [PG_SEQS + 4]
+  LDS int* len = scu + PG_SEQS + 4;                                    // [PG_SEQS]
+  LDS int* flag = len + PG_SEQS;                                       // [4], then four sums of 8 bytes
+  LDS long long* tot = (LDS long long*)(flag + 4);
+  if (!paged_call_ok(c, D.cu, D.lens, D.B, min(D.q.rows, D.o.rows), (long long)D.table.cols << D.lp, scu)) return;
+  WorkPaged W;
+  W.pre = pre; W.cu = scu; W.len = len; W.B = D.B; W.Hkv = D.Hkv; W.G = D.G;
+  const bool fast = D.fast();
+  W.rows = fast ? D.tile : min(D.tile, max(32, D.G));                  // (the general form takes 32 rows at a time)
+  {
+    constexpr int PER = PG_SEQS / KVM_THREADS;
+    long long cost[PER], sum = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int b = tid() * PER + i;
+      cost[i] = 0;
+      if (b < D.B) {
+        const int L = D.lens.i()[b];
+        len[b] = L;
+        cost[i] = W.head_cost(scu[b + 1] - scu[b], L) * D.Hkv;
+        sum += cost[i];
+      }
+    }
+    long long upto = sum;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) { const long long y = __shfl_up(upto, d, 64); if (lane() >= d) upto += y; }
+    if (lane() == 63) tot[wave()] = upto;
+    __syncthreads();
+    long long at = upto - sum;
+    for (int w = 0; w < wave(); ++w) at += tot[w];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int b = tid() * PER + i;
+      if (b < D.B) { pre[b] = at; at += cost[i]; if (b == D.B - 1) pre[D.B] = at; }
+    }
+    __syncthreads();
+  }
+  W.total = pre[D.B];
+  W.share = max((W.total + D.S - 1) / D.S, (long long)PG_SHARE);
+  long long x = W.cut(D.s);
+  const long long end = W.cut(D.s + 1);
+  while (x < end) {
+    const TilePaged t = W.find(x);
+    const long long stop = min(end, t.start + t.cost);
+    const PiecePaged p = W.piece(t, x, stop);
+    attn_paged_general(c, t.b, t.h, t.L, t.row0, t.tok0, t.ntok, p.k0, p.k1, p.k, p.live, p.i0);
+    if (p.live > 1) paged_arrive(c, D, t, p, flag);
+    __syncthreads();
+    x = stop;
+  }
+}
+
+}  // namespace kvm

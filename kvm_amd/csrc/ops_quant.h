@@ -1,0 +1,559 @@
+// Products in 8-bit integers with a scale for each row of activations and of weights (ops 315-317). Semantics: mvm_ops_kvm.def.
+#pragma once
+#include "common.h"
+#include "ops_basic.h"
+#include "ops_gemm.h"
+#include "ops_decode.h"
+#include "ops_serve.h"
+
+namespace kvm {
+
+typedef int i32x16_t __attribute__((ext_vector_type(16)));
+
+// ---------------------------------------------------------------------------------------------- rows in 8 bits
+// v of a row (x, RMS-normalised x, silu(x) * x2) in vectors of 8: thread t has vectors t, t + 256, ..
+struct RowsSrc {
+  View x, x2, g; int K, pro; float eps;
+  __device__ bool vec() const { return rows8_ok(x) && (pro != 2 || rows8_ok(x2)) && (pro != 1 || vec_base(g)); }
+  template <bool VEC> __device__ __forceinline__ void load(const View& X, long long row, int j, float (&v)[8]) const {
+    const int n = K - 8 * j;                                           // values from here on
+    const long long o = row * X.cols + 8 * j;
+    if (VEC) {
+      Raw8 w;
+      w.load(X, o); w.get(X.dtype == 2, v);
+      if (n < 8)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = e < n ? v[e] : 0.f;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = e < n ? X.ld(o + e) : 0.f;
+    }
+  }
+  // x * rstd * gamma, or silu(x) * x2: rounded after each product
+  template <bool VEC> __device__ __forceinline__ void shape(float (&v)[8], long long row, int j, float rstd) const {
+    float y[8];
+    if (pro == 1) {
+      load<VEC>(g, 0, j, y);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) { const float t = v[e] * rstd; v[e] = t * y[e]; }
+    } else if (pro == 2) {
+      load<VEC>(x2, row, j, y);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = silu_f(v[e]) * y[e];
+    }
+  }
+};
+__device__ __forceinline__ uint32_t q8_big(const float (&v)[8], uint32_t big) {   // magnitudes by their bits: what is not finite is largest
+#pragma unroll
+  for (int e = 0; e < 8; ++e) big = max(big, __float_as_uint(v[e]) & 0x7fffffffu);
+  return big;
+}
+// One sum or maximum per row over the workgroup, the waves' in order; red: 4 * RB of LDS.
+template <int RB> __device__ __forceinline__ void q8_rows_sum(double (&s)[RB], LDS double* red) {
+#pragma unroll
+  for (int i = 0; i < RB; ++i) s[i] = wave_sum_d(s[i]);
+  __syncthreads();
+  if (lane() == 0)
+#pragma unroll
+    for (int i = 0; i < RB; ++i) red[4 * i + wave()] = s[i];
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < RB; ++i) s[i] = (red[4 * i] + red[4 * i + 1]) + (red[4 * i + 2] + red[4 * i + 3]);
+}
+template <int RB> __device__ __forceinline__ void q8_rows_max(uint32_t (&b)[RB], LDS double* red_) {
+  LDS uint32_t* red = (LDS uint32_t*)red_ + 8 * RB;
+#pragma unroll
+  for (int i = 0; i < RB; ++i) b[i] = __float_as_uint(rows_max(lanes_max<16>(__uint_as_float(min(b[i], 0x7f800000u)))));
+  __syncthreads();
+  if (lane() == 0)
+#pragma unroll
+    for (int i = 0; i < RB; ++i) red[4 * i + wave()] = b[i];
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < RB; ++i) b[i] = max(max(red[4 * i], red[4 * i + 1]), max(red[4 * i + 2], red[4 * i + 3]));
+}
+constexpr int Q8_RED = 12;     // doubles of LDS per row in flight
+// nr <= RB rows from r0 on, K <= 2048 NV, held in registers: one read of x, all its loads in flight together, one reduction for the norm
+// and one for the scale whatever RB is. put(i, j, w0, w1): vector j of row r0 + i as bytes; scaled(i, s). Sums of squares in double, so
+// that rstd is the f32 nearest to the exact one whatever the order.
+template <bool VEC, int NV, int RB, class Put, class Scaled>
+__device__ __forceinline__ void q8_rows(const RowsSrc& S, long long r0, int nr, LDS double* red, Put put, Scaled scaled) {
+  const int nvec = (S.K + 7) >> 3;
+  float v[RB][NV][8];
+#pragma unroll
+  for (int i = 0; i < RB; ++i)
+#pragma unroll
+    for (int u = 0; u < NV; ++u) S.load<VEC>(S.x, r0 + min(i, nr - 1), min(tid() + u * KVM_THREADS, nvec - 1), v[i][u]);
+  double ss[RB] = {};
+  if (S.pro == 1) {
+#pragma unroll
+    for (int i = 0; i < RB; ++i)
+#pragma unroll
+      for (int u = 0; u < NV; ++u)
+        if (tid() + u * KVM_THREADS < nvec)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) ss[i] += (double)v[i][u][e] * (double)v[i][u][e];
+    q8_rows_sum<RB>(ss, red);
+  }
+  uint32_t big[RB] = {};
+#pragma unroll
+  for (int i = 0; i < RB; ++i) {
+    const float rstd = (float)(1.0 / sqrt(ss[i] / S.K + (double)S.eps));
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+      S.shape<VEC>(v[i][u], r0 + min(i, nr - 1), min(tid() + u * KVM_THREADS, nvec - 1), rstd);
+      big[i] = q8_big(v[i][u], big[i]);
+    }
+  }
+  q8_rows_max<RB>(big, red);
+#pragma unroll
+  for (int i = 0; i < RB; ++i) {
+    if (i >= nr) break;
+    const float s = q8_scale(__uint_as_float(big[i])), inv = s > 0.f ? 1.f / s : 0.f;
+    if (tid() == 0) scaled(i, s);
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+      uint32_t w0, w1;
+      q8_pack(v[i][u], s, inv, w0, w1);
+      if (tid() + u * KVM_THREADS < nvec) put(i, tid() + u * KVM_THREADS, w0, w1);
+    }
+  }
+}
+// A row of any length, read three times.
+template <bool VEC, class Put, class Scaled>
+__device__ __forceinline__ void q8_row_long(const RowsSrc& S, long long r, LDS double* red, Put put, Scaled scaled) {
+  const int nvec = (S.K + 7) >> 3;
+  double ss[1] = {};
+  float v[8];
+  if (S.pro == 1) {
+    for (int j = tid(); j < nvec; j += KVM_THREADS) {
+      S.load<VEC>(S.x, r, j, v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) ss[0] += (double)v[e] * (double)v[e];
+    }
+    q8_rows_sum<1>(ss, red);
+  }
+  const float rstd = (float)(1.0 / sqrt(ss[0] / S.K + (double)S.eps));
+  uint32_t big[1] = {};
+  for (int j = tid(); j < nvec; j += KVM_THREADS) { S.load<VEC>(S.x, r, j, v); S.shape<VEC>(v, r, j, rstd); big[0] = q8_big(v, big[0]); }
+  q8_rows_max<1>(big, red);
+  const float s = q8_scale(__uint_as_float(big[0])), inv = s > 0.f ? 1.f / s : 0.f;
+  if (tid() == 0) scaled(0, s);
+  for (int j = tid(); j < nvec; j += KVM_THREADS) {
+    uint32_t w0, w1;
+    S.load<VEC>(S.x, r, j, v); S.shape<VEC>(v, r, j, rstd);
+    q8_pack(v, s, inv, w0, w1);
+    put(0, j, w0, w1);
+  }
+}
+
+// Op 315. Bound: bytes (K * (2 to 8) read, K written a row). Four rows of up to 4,096 values at once, one of up to 16,384, so that the two
+// reductions' waits are shared.
+template <bool VEC, int NV> __device__ __noinline__ void rows_q8_t(const Ctx& c) {
+  constexpr int RB = NV == 2 ? 4 : 1;
+  const RowsSrc S{uview(c, 0), uview(c, 1), uview(c, 2), rfl(c.i(7)), rfl(c.i(8)), c.f(9)};
+  const View q = uview(c, 3), qs = uview(c, 4);
+  const int r0 = rfl(c.i(5)), r1 = rfl(c.i(6)), words = min(q.cols, ((S.K + 15) >> 4) << 2), nvec = (S.K + 7) >> 3;
+  const bool pair = (q.cols & 1) == 0 && ((uintptr_t)q.p & 7) == 0;
+  LDS double* red = (LDS double*)c.smem;
+  for (int r = r0; r < r1; r += RB) {
+    auto word = [&](GLOBAL int* p, int k, uint32_t w) { if (k < words) stwt32i(p + k, (int)w); };
+    auto put = [&](int i, int j, uint32_t w0, uint32_t w1) {
+      GLOBAL int* p = q.i() + (long long)(r + i) * q.cols;
+      if (pair && 2 * j + 1 < words) stwt64(p + 2 * j, (uint64_t)w0 | ((uint64_t)w1 << 32));
+      else { word(p, 2 * j, w0); word(p, 2 * j + 1, w1); }
+      if (j == nvec - 1 && (nvec & 1)) { word(p, 2 * nvec, 0); word(p, 2 * nvec + 1, 0); }   // up to the multiple of 16 bytes
+    };
+    auto scaled = [&](int i, float s) { stwt32(qs.f() + (r + i), s); };
+    if constexpr (NV > 0) q8_rows<VEC, NV, RB>(S, r, min(RB, r1 - r), red, put, scaled);
+    else q8_row_long<VEC>(S, r, red, put, scaled);
+  }
+}
+__device__ __noinline__ void op_rows_q8(const Ctx& c) {
+  const RowsSrc S{c.buf(0), c.buf(1), c.buf(2), c.i(7), c.i(8), c.f(9)};
+  if (S.vec()) { if (S.K <= 4096) rows_q8_t<true, 2>(c); else if (S.K <= 16384) rows_q8_t<true, 8>(c); else rows_q8_t<true, 0>(c); }
+  else if (S.K <= 4096) rows_q8_t<false, 2>(c); else rows_q8_t<false, 0>(c);
+}
+
+// ---------------------------------------------------------------------------------------------- product tiles
+// Arguments of op 316 (a, sa, w, sw, out, bias, res, m0, n0, M, N, K, tile), wave-uniform.
+struct TileQ8 {
+  View a, sa, w, sw, out, bias, res; int m0, n0, M, N, K;
+  __device__ explicit TileQ8(const Ctx& c)
+      : a(uview(c, 0)), sa(uview(c, 1)), w(uview(c, 2)), sw(uview(c, 3)), out(uview(c, 4)), bias(uview(c, 5)), res(uview(c, 6)),
+        m0(rfl(c.i(7))), n0(rfl(c.i(8))), M(rfl(c.i(9))), N(rfl(c.i(10))), K(rfl(c.i(11))) {}
+  __device__ float scaled(int sum, float s, float t) const { const float y = (float)sum * s; return y * t; }
+  __device__ void put(int m, int n, int sum, float s) const {
+    float y = scaled(sum, s, sw.f()[n]);
+    if (bias.ok()) y += bias.f()[n];
+    if (res.ok()) y += res.at(m, n);
+    out.st((long long)m * out.cols + n, y);
+  }
+};
+// The staged tile [TM][TN] of sums (16-byte pieces swizzled by row as in gemm_store): a lane has 4 columns, the waves take rows in turn, the
+// residual of 8 rows requested together.
+template <int TM, int TN, bool OBF> __device__ __noinline__ void q8_epilogue(const Ctx& c) {
+  constexpr int LPR = TN / 4, RPI = 64 / LPR < 1 ? 1 : 64 / LPR, NI = TM / KVM_WAVES / RPI, NB = NI < 8 ? NI : 8;
+  const TileQ8 g(c);
+  const LDS int* et = (const LDS int*)c.smem;
+  const int l = lane(), w = wave(), ch = l % LPR, n = g.n0 + 4 * ch;
+  const long long lim = 0x7fffffffll;
+  const bool vec = n + 4 <= g.N && (g.out.cols & 3) == 0 && vec_base(g.out) && (!g.res.ok() || ((g.res.cols & 3) == 0 && vec_base(g.res))) &&
+                   (long long)TM * g.res.cols * 4 < lim && (long long)TM * g.out.cols * 4 < lim;
+  float sw4[4], b4[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    sw4[i] = n + i < g.N ? g.sw.f()[n + i] : 0.f;
+    b4[i] = g.bias.ok() && n + i < g.N ? g.bias.f()[n + i] : 0.f;
+  }
+  const bool res = g.res.ok();
+  const View ov{(char*)g.out.p + (long long)g.m0 * g.out.cols * (OBF ? 2 : 4), g.out.rows - g.m0, g.out.cols, g.out.dtype, 0};
+  const int re = g.res.dtype == 2 ? 2 : 4;
+  const View rv{res ? (char*)g.res.p + (long long)g.m0 * g.res.cols * re : nullptr, g.res.rows - g.m0, g.res.cols, g.res.dtype, 0};
+  Ld4 lr;
+  lr.init(rv, res && vec);
+  const __amdgpu_buffer_rsrc_t orsrc = wt_rsrc(ov.p, (long long)min(TM, g.M - g.m0) * ov.cols * (OBF ? 2 : 4));
+  for (int k0 = 0; k0 < NI; k0 += NB) {
+    u32x4_t raw[NB];
+    float sa[NB];
+#pragma unroll
+    for (int u = 0; u < NB; ++u) {
+      const int r = ((k0 + u) * KVM_WAVES + w) * RPI + l / LPR;
+      raw[u] = lr.raw(vec ? min(r, g.M - 1 - g.m0) * rv.cols + n : 0);
+      sa[u] = g.sa.f()[min(g.m0 + r, g.M - 1)];
+    }
+#pragma unroll
+    for (int u = 0; u < NB; ++u) {
+      const int r = ((k0 + u) * KVM_WAVES + w) * RPI + l / LPR, m = g.m0 + r;
+      if (m >= g.M) continue;
+      const i32x4_t s = *(const LDS i32x4_t*)(et + r * TN + 4 * (ch ^ epi_swz<TN>(r)));
+      if (vec) {
+        f32x4n y = {g.scaled(s.x, sa[u], sw4[0]), g.scaled(s.y, sa[u], sw4[1]), g.scaled(s.z, sa[u], sw4[2]), g.scaled(s.w, sa[u], sw4[3])};
+        if (g.bias.ok()) y += f32x4n{b4[0], b4[1], b4[2], b4[3]};
+        if (res) y += lr.cvt(raw[u]);
+        if constexpr (OBF) stwt_bf4_buf(orsrc, (r * ov.cols + n) * 2, y);
+        else stwt_buf(orsrc, (r * ov.cols + n) * 4, y);
+      } else {
+        const int x[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) if (n + i < g.N) g.put(m, n + i, x[i], sa[u]);
+      }
+    }
+  }
+}
+// The first n bytes of a lane's 16, the others 0.
+__device__ __forceinline__ bf16x8 first_bytes(bf16x8 f, int n) {
+  u32x4_t x = __builtin_bit_cast(u32x4_t, f);
+#pragma unroll
+  for (int d = 0; d < 4; ++d) x[d] &= n >= 4 * d + 4 ? 0xffffffffu : n <= 4 * d ? 0u : 0xffffffffu >> (8 * (4 - (n & 3)));
+  return __builtin_bit_cast(bf16x8, x);
+}
+// A tile on the matrix units, v_mfma_i32_32x32x32_i8: a row of bytes moves like a row of half as many bf16 values (DOp: HBM straight into
+// LDS, NS stages of 64 bytes a row, fragments of 16 bytes a lane), and the schedule is gemm_lds_b's: fragments of the next half under the products
+// of this one, constant waits, the last stage peeled. The sums are exact, so nothing depends on the tile's shape. K's tail is cut off in A
+// alone: a byte of B meets a 0.
+template <int TM, int TN> __device__ __noinline__ void q8_tile(const Ctx& c) {
+  constexpr int WM = TM / 2, WN = TN / 2, BM = WM / 32, BN = WN / 32, SA = TM * DK, SB = TN * DK, ST = SA + SB;
+  constexpr int NS = 4 * ST * 2 * 2 <= KVM_LDS_BYTES ? 8 : 4;
+  static_assert(NS * ST * 2 <= KVM_LDS_BYTES && TM * TN * 4 <= KVM_LDS_BYTES, "LDS");
+  const TileQ8 g(c);
+  const View A{g.a.p, g.a.rows, 2 * g.a.cols, 2, 0}, B{g.w.p, g.w.rows, 2 * g.w.cols, 2, 0};
+  LDS uint16_t* lds = (LDS uint16_t*)c.smem;
+  const int wm0 = (wave() >> 1) * WM, wn0 = (wave() & 1) * WN;
+  DOp<TM, true> da;
+  DOp<TN, true> db;
+  da.init(A, g.m0, g.M);
+  db.init(B, g.n0, g.N);
+  i32x16_t acc[BM][BN];
+#pragma unroll
+  for (int i = 0; i < BM; ++i)
+#pragma unroll
+    for (int j = 0; j < BN; ++j) acc[i][j] = i32x16_t{};
+  const int nst = (g.K + 2 * DK - 1) / (2 * DK);
+  constexpr int NLA = DOp<TM, true>::NL, NLS = NLA + DOp<TN, true>::NL, NF = BM + BN, NM = BM * BN, PF = (NF + NM - 1) / NM, PX = (NF + NLS + NM - 1) / NM;
+  __syncthreads();                                 // the previous task may still read this LDS
+  const unsigned lb = (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(uintptr_t)lds);
+#pragma unroll
+  for (int p = 0; p < NS - 1; ++p) { da.issue(lb + p * ST * 2, p, nst); db.issue(lb + (p * ST + SA) * 2, p, nst); }
+  bf16x8 fa0[BM], fb0[BN], fa1[BM], fb1[BN];
+  auto read_one = [&](const LDS uint16_t* st, int kk, int f, bf16x8 (&fa)[BM], bf16x8 (&fb)[BN]) {
+    if (f < BM) fa[f] = da.frag(st, wm0 + f * 32, kk);
+    else fb[f - BM] = db.frag(st + SA, wn0 + (f - BM) * 32, kk);
+  };
+  auto mfma_one = [&](int m, const bf16x8 (&fa)[BM], const bf16x8 (&fb)[BN]) {
+    const int i = m / BN, j = m % BN;
+    acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4_t, fb[j]), __builtin_bit_cast(i32x4_t, fa[i]), acc[i][j], 0, 0, 0);
+  };
+  wait_vm_c<(NS - 2) * NLS>();
+  __syncthreads();
+#pragma unroll
+  for (int f = 0; f < NF; ++f) read_one(lds, 0, f, fa0, fb0);
+  for (int s = 0; s + 1 < nst; ++s) {
+    const LDS uint16_t* la = lds + (s % NS) * ST;
+#pragma unroll
+    for (int m = 0; m < NM; ++m) {
+      mfma_one(m, fa0, fb0);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int f = m * PF; f < (m + 1) * PF && f < NF; ++f) read_one(la, 1, f, fa1, fb1);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    wait_vm_c<(NS - 3) * NLS>();                 // this thread's loads of stage s + 1 have landed
+    asm volatile("s_barrier" ::: "memory");        // ... everyone's, and every wave is past stage s - 1
+    const int sn = s + NS - 1;
+    const unsigned nb = lb + ((s + NS - 1) % NS) * ST * 2;
+    const LDS uint16_t* ln = lds + ((s + 1) % NS) * ST;
+#pragma unroll
+    for (int m = 0; m < NM; ++m) {
+      mfma_one(m, fa1, fb1);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int x = m * PX; x < (m + 1) * PX && x < NF + NLS; ++x) {
+        if (x < NF) read_one(ln, 0, x, fa0, fb0);
+        else if (x - NF < NLA) da.issue_one(nb, sn, x - NF, nst);
+        else db.issue_one(nb + SA * 2, sn, x - NF - NLA, nst);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+  {
+    const LDS uint16_t* la = lds + ((nst - 1) % NS) * ST;
+#pragma unroll
+    for (int f = 0; f < NF; ++f) read_one(la, 1, f, fa1, fb1);
+    const int kr = g.K - (nst - 1) * 2 * DK;       // bytes of the last stage
+    if (kr < 2 * DK) {
+      const int k0 = kr - 16 * (lane() >> 5);
+#pragma unroll
+      for (int i = 0; i < BM; ++i) { fa0[i] = first_bytes(fa0[i], k0); fa1[i] = first_bytes(fa1[i], k0 - 32); }
+    }
+#pragma unroll
+    for (int m = 0; m < NM; ++m) mfma_one(m, fa0, fb0);
+#pragma unroll
+    for (int m = 0; m < NM; ++m) mfma_one(m, fa1, fb1);
+  }
+  wait_vm_c<0>();                                  // the placeholder loads have written their LDS bytes
+  __syncthreads();
+  LDS int* et = (LDS int*)c.smem;                  // D^T: lane has row l % 32 of block i, columns 8 q + 4 (l / 32) .. + 3 of block j
+  const int l = lane();
+#pragma unroll
+  for (int i = 0; i < BM; ++i) {
+    const int r = wm0 + i * 32 + (l & 31);
+#pragma unroll
+    for (int j = 0; j < BN; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int chunk = (wn0 + j * 32 + 8 * q) / 4 + (l >> 5);
+        *(LDS i32x4_t*)(et + r * TN + 4 * (chunk ^ epi_swz<TN>(r))) = i32x4_t{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+      }
+  }
+  __syncthreads();
+  if (g.out.dtype == 2) q8_epilogue<TM, TN, true>(c);
+  else q8_epilogue<TM, TN, false>(c);
+}
+// Rows of bytes that do not lie in whole 16-byte vectors: an output at a time, four products an instruction.
+__device__ __forceinline__ int q8_dot(const GLOBAL int* a, const GLOBAL int* w, int K) {
+  int s = 0;
+  for (int k = 0; k < K >> 2; ++k) s = __builtin_amdgcn_sdot4(a[k], w[k], s, false);
+  if (K & 3) s = __builtin_amdgcn_sdot4((int)((uint32_t)a[K >> 2] & (0xffffffffu >> (8 * (4 - (K & 3))))), w[K >> 2], s, false);
+  return s;
+}
+__device__ __noinline__ void matmul_q8_simt(const Ctx& c, int tm, int tn) {
+  const TileQ8 g(c);
+  const int rows = min(rfl(tm), g.M - g.m0), cols = min(rfl(tn), g.N - g.n0);
+  for (int e = tid(); e < rows * cols; e += KVM_THREADS) {
+    const int m = g.m0 + e / cols, n = g.n0 + e % cols;
+    g.put(m, n, q8_dot(g.a.i() + (long long)m * g.a.cols, g.w.i() + (long long)n * g.w.cols, g.K), g.sa.f()[m]);
+  }
+}
+// Whether rows r0 .. of X lie in whole vectors that a descriptor from row r0 on reaches in 31 bits.
+__device__ __forceinline__ bool q8_fast(const View& X, int R, int K) {
+  return (X.cols & 3) == 0 && vec_base(X) && (long long)R * X.cols * 4 + K < 0x7fffff00ll;
+}
+__device__ __noinline__ void op_matmul_q8(const Ctx& c) {
+  const int tile = rfl(c.i(12)), tm = tile == 2 ? 64 : 128, tn = tile == 0 ? 256 : tile == 1 ? 128 : 64;
+  if (!q8_fast(c.buf(0), tm, c.i(11)) || !q8_fast(c.buf(2), tn, c.i(11))) matmul_q8_simt(c, tm, tn);
+  else if (tile == 0) q8_tile<128, 256>(c);
+  else if (tile == 1) q8_tile<128, 128>(c);
+  else q8_tile<64, 64>(c);
+}
+
+// ---------------------------------------------------------------------------------------------- rows of weights, streamed
+// Op 317. Bound: the weights' bytes (N * K), as the bf16 stream of ops 134 and 301, whose ring and cursor it uses (a row of bytes is a row of
+// half as many bf16 values); K is rounded up to whole steps of all waves, the bytes behind K are 0 in the staged rows. A step of a wave is two
+// v_mfma_i32_16x16x64_i8.
+struct GemvQ8 {
+  View x, x2, g, w, sw, out, bias, res, sx; int n0, n1, K, M, pro, Ke;
+  __device__ explicit GemvQ8(const Ctx& c)
+      : x(uview(c, 0)), x2(uview(c, 1)), g(uview(c, 2)), w(uview(c, 3)), sw(uview(c, 4)), out(uview(c, 5)), bias(uview(c, 6)), res(uview(c, 7)), sx(uview(c, 8)),
+        n0(rfl(c.i(9))), n1(rfl(c.i(10))), K(rfl(c.i(11))), M(rfl(c.i(12))), pro(rfl(c.i(13))) { Ke = ((K + 511) >> 9) << 8; }
+  __device__ View stream() const { return View{w.p, w.rows, 2 * w.cols, 2, 0}; }
+  __device__ bool fast() const { return q8_fast(w, n1 - n0 + 16, 2 * Ke); }
+  __device__ void put(int m, int n, int sum, float s) const {
+    float y = (float)sum * s;
+    y *= sw.f()[n];
+    if (bias.ok()) y += bias.f()[n];
+    if (res.ok()) y += res.at(m, n);
+    out.st((long long)m * out.cols + n, y);
+  }
+};
+// Row m's bytes [lo, lo + n) (n a multiple of 16, zeros behind K) to LDS at vs + m * pitch and the scales, for all rows.
+template <bool VEC, int NV> __device__ __noinline__ void gemv_q8_stage(const Ctx& c, LDS char* vs_, int pitch_, int lo_, int n_, LDS float* scale, LDS double* red) {
+  const int pitch = rfl(pitch_), lo = rfl(lo_), n = rfl(n_);
+  const GemvQ8 G(c);
+  const RowsSrc S{G.x, G.x2, G.g, G.K, G.pro, c.f(14)};
+  for (int m = 0; m < G.M; ++m) {
+    LDS char* const vs = vs_ + m * pitch;
+    auto put = [&](int, int j, uint32_t w0, uint32_t w1) {
+      const int o = 8 * j - lo;
+      if (o >= 0 && o < n) { *(LDS uint32_t*)(vs + o) = w0; *(LDS uint32_t*)(vs + o + 4) = w1; }
+    };
+    auto scaled = [&](int, float s) { scale[m] = s; };
+    if constexpr (NV > 0) q8_rows<VEC, NV, 1>(S, m, 1, red, put, scaled);
+    else q8_row_long<VEC>(S, m, red, put, scaled);
+    for (int o = max(0, ((G.K + 7) & ~7) - lo) + 4 * tid(); o < n; o += 4 * KVM_THREADS) *(LDS int*)(vs + o) = 0;
+  }
+}
+__device__ __forceinline__ void gemv_q8_rows(const Ctx& c, const GemvQ8& G, LDS char* vs, int pitch, int lo, int n, LDS float* scale, LDS double* red) {
+  if (G.pro == 3) {                                // words that are there already
+    for (int m = 0; m < G.M; ++m)
+      for (int o = 4 * tid(); o < n; o += 4 * KVM_THREADS) {
+        const int k = lo + o;
+        int v = k < G.K ? G.x.i()[(long long)m * G.x.cols + (k >> 2)] : 0;
+        if (G.K - k < 4 && k < G.K) v &= (int)(0xffffffffu >> (8 * (4 - (G.K - k))));
+        *(LDS int*)(vs + m * pitch + o) = v;
+      }
+    if (tid() < G.M) scale[tid()] = G.sx.f()[tid()];
+    return;
+  }
+  const RowsSrc S{G.x, G.x2, G.g, G.K, G.pro, 0.f};
+  if (S.vec()) {
+    if (G.K <= 4096) gemv_q8_stage<true, 2>(c, vs, pitch, lo, n, scale, red);
+    else if (G.K <= 16384) gemv_q8_stage<true, 8>(c, vs, pitch, lo, n, scale, red);
+    else gemv_q8_stage<true, 0>(c, vs, pitch, lo, n, scale, red);
+  } else if (G.K <= 4096) gemv_q8_stage<false, 2>(c, vs, pitch, lo, n, scale, red);
+  else gemv_q8_stage<false, 0>(c, vs, pitch, lo, n, scale, red);
+}
+// LDS of one call with a ring of R steps a wave: [ring][rows: M x (2 KC + 16) bytes][scales][reductions][sums: 4 x GV_GRP x M x 16]. KC (pairs of
+// bytes): all of K when it fits, else the largest power of two from 4096 to 256 that divides K and does.
+struct GqGeo { int KC, pitch, vs, scale, red, part; };
+__device__ __forceinline__ GqGeo gq_geo(int Ke, int M, int R) {
+  const int rest = R * KVM_WAVES * GV_STEP + 64 + Q8_RED * 8 + KVM_WAVES * GV_GRP * M * 16 * 4;
+  int KC = Ke;
+  if (rest + M * (2 * Ke + 16) > KVM_LDS_BYTES)
+    for (KC = 4096; KC > 256 && (Ke % KC || rest + M * (2 * KC + 16) > KVM_LDS_BYTES); KC >>= 1) {}
+  GqGeo g;
+  g.KC = KC; g.pitch = 2 * KC + 16;
+  g.vs = R * KVM_WAVES * GV_STEP;
+  g.scale = g.vs + M * g.pitch;
+  g.red = g.scale + 64;
+  g.part = g.red + Q8_RED * 8;
+  return g;
+}
+template <int R> __device__ __forceinline__ void gemv_q8_prefetch_r(const GemvQ8& G, LDS char* smem) {
+  GvStream<> ws;
+  ws.init(G.stream(), G.n0, G.n1, G.Ke, gq_geo(G.Ke, G.M, R).KC);
+  LDS char* ring = smem + wave() * R * GV_STEP;
+#pragma unroll
+  for (int j = 0; j < R; ++j) ws.template issue<R>(ring);
+}
+__device__ __noinline__ void gemv_q8_prefetch(const Ctx& c) {
+  const GemvQ8 G(c);
+  if (!G.fast()) return;
+  if (gv_pre_ring(G.M) == 12) gemv_q8_prefetch_r<12>(G, c.smem);
+  else gemv_q8_prefetch_r<4>(G, c.smem);
+}
+template <int R> __device__ __noinline__ void gemv_q8_stream(const Ctx& c) {
+  const GemvQ8 G(c);
+  const int M = G.M, K = G.Ke, PM = 16 * M;                                     // K in pairs of bytes
+  const GqGeo geo = gq_geo(K, M, R);
+  const int KC = geo.KC;
+  LDS char* vs = c.smem + geo.vs;
+  LDS float* scale = (LDS float*)(c.smem + geo.scale);
+  LDS int* part = (LDS int*)(c.smem + geo.part);
+  const int l = lane(), wv = wave(), nrb = (G.n1 - G.n0 + 15) / 16;
+  LDS char* ring = c.smem + wv * R * GV_STEP;
+  GvStream<> ws;
+  ws.init(G.stream(), G.n0, G.n1, K, KC);
+  if (rfl(c.pre)) {
+#pragma unroll
+    for (int j = 0; j < R; ++j) ws.template skip<R>();                           // issued before the dependency wait
+  } else {
+#pragma unroll
+    for (int j = 0; j < R; ++j) ws.template issue<R>(ring);
+  }
+  const bool arow = (l & 15) < M;
+  const LDS char* va = vs + (arow ? (l & 15) : 0) * geo.pitch + 16 * (l >> 4);
+  const LDS char* rl = ring + 16 * l;
+  int cslot = 0;
+  for (int g0 = 0; g0 < nrb; g0 += GV_GRP) {
+    const int ng = min(GV_GRP, nrb - g0);
+    for (int e = l; e < ng * PM; e += 64) part[wv * GV_GRP * PM + e] = 0;
+    for (int kc = 0; kc < K; kc += KC) {
+      const int kq = KC / 2, ns = KC / 256;                                      // bytes of a wave's quarter, its steps
+      __syncthreads();
+      if (KC != K || g0 == 0) gemv_q8_rows(c, G, vs, geo.pitch, 2 * kc, 2 * KC, scale, (LDS double*)(c.smem + geo.red));
+      __syncthreads();
+      const LDS char* vk = va + wv * kq;
+      i32x4_t acc = {0, 0, 0, 0};
+      int rb = 0, st = 0;
+      for (int tt = 0; tt < ng * ns; ++tt) {                                     // one flat loop: no full wait at an inner loop's head
+        wait_vm_c<2 * (R - 1)>();
+        const LDS char* slot = rl + cslot * GV_STEP;
+        const i32x4_t w0 = *(const LDS i32x4_t*)slot, w1 = *(const LDS i32x4_t*)(slot + 1024);
+        const i32x4_t a0 = *(const LDS i32x4_t*)(vk + st * 128), a1 = *(const LDS i32x4_t*)(vk + st * 128 + 64);
+        acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(arow ? a0 : i32x4_t{}, w0, acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(arow ? a1 : i32x4_t{}, w1, acc, 0, 0, 0);
+        wait_lds();
+        ws.template issue<R>(ring);
+        cslot = cslot + 1 == R ? 0 : cslot + 1;
+        if (++st == ns) {                                                        // D[m][n]: lane holds m = 4 (l / 16) + i, n = l % 16
+          LDS int* pp = part + (wv * GV_GRP + rb) * PM + (l & 15);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int m = 4 * (l >> 4) + i;
+            if (m < M) pp[m * 16] += acc[i];
+          }
+          acc = i32x4_t{0, 0, 0, 0};
+          st = 0; ++rb;
+        }
+      }
+    }
+    __syncthreads();
+    for (int e = tid(); e < ng * PM; e += KVM_THREADS) {
+      const int rb = e / PM, m = (e / 16) % M, n = G.n0 + (g0 + rb) * 16 + e % 16;
+      if (n < G.n1) G.put(m, n, part[e] + part[GV_GRP * PM + e] + part[2 * GV_GRP * PM + e] + part[3 * GV_GRP * PM + e], scale[m]);
+    }
+    __syncthreads();                                                            // read before the next group clears them
+  }
+  wait_vm_c<0>();                                                               // the ring's trailing loads have landed
+}
+// Weights that do not lie in whole 16-byte vectors: rows in LDS 4,096 bytes at a time, an output to a thread.
+__device__ __noinline__ void gemv_q8_simt(const Ctx& c) {
+  const GemvQ8 G(c);
+  constexpr int CH = 4096;
+  LDS char* vs = c.smem;                                                        // [16][CH + 16]
+  LDS float* scale = (LDS float*)(vs + 16 * (CH + 16));
+  LDS double* red = (LDS double*)(scale + 16);
+  for (int e0 = 0; e0 < (G.n1 - G.n0) * G.M; e0 += KVM_THREADS) {
+    const int e = e0 + tid(), m = e % G.M, n = G.n0 + e / G.M;
+    int s = 0;
+    for (int k0 = 0; k0 < G.K; k0 += CH) {
+      __syncthreads();
+      gemv_q8_rows(c, G, vs, CH + 16, k0, CH, scale, red);
+      __syncthreads();
+      const int nw = (min(CH, G.K - k0) + 3) >> 2;
+      if (n < G.n1)
+        for (int k = 0; k < nw; ++k) s = __builtin_amdgcn_sdot4(*(const LDS int*)(vs + m * (CH + 16) + 4 * k), G.w.i()[(long long)n * G.w.cols + (k0 >> 2) + k], s, false);
+    }
+    if (n < G.n1) G.put(m, n, s, scale[m]);
+  }
+}
+__device__ __noinline__ void op_gemv_q8(const Ctx& c) {
+  const GemvQ8 G(c);
+  if (G.n0 >= G.n1) return;
+  if (!G.fast()) gemv_q8_simt(c);
+  else if (rfl(c.pre) && gv_pre_ring(G.M) == 12) gemv_q8_stream<12>(c);
+  else gemv_q8_stream<4>(c);
+}
+
+}  // namespace kvm

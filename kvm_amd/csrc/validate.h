@@ -42,7 +42,7 @@ static const OpSig* find_op(int id) { for (const OpSig& o : kRegistry) if (o.id 
 static bool implemented(int id) {
   static const int ids[] = {0, 1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 32, 33, 34, 35, 36, 37, 38, 39, 40, 41, 42, 43, 44, 45, 46, 47, 48, 49, 50,
                             51, 52, 53, 54, 55, 56, 57, 58, 59, 60, 61, 62, 63, 96, 97, 98, 99, 100, 101, 102, 103, 104, 113, 114, 115,
-                            116, 117, 118, 120, 121, 122, 123, 126, 127, 134, 135, 136, 300, 301, 302, 303, 304, 305, 306, 308, 309, 310, 311, 312, 313, 314};
+                            116, 117, 118, 120, 121, 122, 123, 126, 127, 134, 135, 136, 300, 301, 302, 303, 304, 305, 306, 308, 309, 310, 311, 312, 313, 314, 315, 316, 317, 318, 319};
   for (int i : ids) if (i == id) return true;
   return false;
 }
@@ -122,6 +122,11 @@ static char arg_class(int op, const std::string& n) {
     case 312: return in({"kq", "vq", "lens"}) ? 'i' : in({"ks", "vs", "kgamma"}) ? 'f' : 'a';
     case 313: return in({"kq", "vq", "lens", "cnt"}) ? 'i' : in({"ks", "vs", "qgamma", "part"}) ? 'f' : 'a';
     case 314: return in({"logits", "out"}) ? 'a' : in({"par", "bval"}) ? 'f' : 'i';
+    case 315: return in({"q"}) ? 'i' : in({"qs", "gamma"}) ? 'f' : 'a';
+    case 316: return in({"a", "w"}) ? 'i' : in({"out", "res"}) ? 'a' : 'f';
+    case 317: return in({"w"}) ? 'i' : in({"x"}) ? 'x' : in({"x2", "out", "res"}) ? 'a' : 'f';   // x: by `pro`, among the extents
+    case 318: return in({"table", "lens", "cu"}) ? 'i' : in({"qgamma", "kgamma"}) ? 'f' : 'a';
+    case 319: return in({"table", "lens", "cu", "cnt"}) ? 'i' : in({"part"}) ? 'f' : 'a';
     default: return 'f';
   }
 }
@@ -144,6 +149,26 @@ static void cache_q8(Check& k, long long B, int Hkv, int hd, const char* gamma) 
   k.ext("kt", pairs * blk, hd); k.ext("vt", pairs * blk, hd); k.extn("lens", B); k.extn(gamma, hd);
   const float theta = k.F("theta"), eps = k.F("eps");
   k.need(std::isfinite(theta) && (theta == 0.f || theta >= 1.f) && std::isfinite(eps) && eps >= 0.f, "theta must be 0 or at least 1, eps not negative, both finite");
+}
+
+// What stands in front of 8-bit rows (ops 315, 317): its operands for M rows of K values.
+static void rows_q8(Check& k, int pro, long long M, int K) {
+  k.need(K > 0 && K <= 131071, "K must be 1 .. 131071");
+  k.need((k.B("gamma") != nullptr) == (pro == 1) && (k.B("x2") != nullptr) == (pro == 2), "gamma goes with pro 1, x2 with pro 2");
+  k.need(std::isfinite(k.F("eps")) && k.F("eps") >= 0.f, "eps must be finite and not negative");
+  k.ext("x", M, pro == 3 ? (K + 3) / 4 : K); k.ext("x2", M, K); k.extn("gamma", K);
+}
+// The paged cache of ops 318 and 319 (layout: mvm_ops_kvm.def).
+static void cache_paged(Check& k) {
+  const int B = k.I("B"), Hkv = k.I("Hkv"), hd = k.I("hd"), page = k.I("page");
+  k.need(page == 16 || page == 32 || page == 64 || page == 128, "page must be 16, 32, 64 or 128");
+  k.need(hd > 0 && hd <= 256 && hd % 2 == 0, "hd must be even, up to 256");
+  k.need(B > 0 && B <= 1024 && Hkv > 0, "B must be 1 .. 1024, Hkv positive");
+  const MvmBuf *kc = k.B("kc"), *vc = k.B("vc"), *tb = k.B("table");
+  if (!kc || !vc || !tb || !k.err.empty()) return;
+  k.need(kc->rows == vc->rows && kc->rows >= (long long)Hkv * page, "kc and vc must have the same rows, a page at least");
+  k.need((long long)tb->cols * page < 0x7fffff00ll && tb->cols > 0, "table must have 1 .. (2^31 - 256) / page columns");
+  k.ext("kc", 0, hd); k.ext("vc", 0, hd); k.ext("table", B, 1); k.extn("lens", B); k.extn("cu", (long long)B + 1);
 }
 
 // Operand extents of one task; mirrors the reference's extent functions for the ops implemented here.
@@ -354,6 +379,39 @@ static void extents(int op, Check& k) {
       k.ext("mask", k.B("mrow") ? 1 : r1, ((long long)V + 31) / 32); k.extn("mrow", r1);
       k.own("out", "logits"); if (k.B("last")) k.own("hist");
       break; }
+    case 315: { const int r1 = k.I("r1"), K = k.I("K"), pro = k.I("pro"); k.range(k.I("r0"), r1);
+      k.need(pro >= 0 && pro <= 2, "pro must be 0, 1 or 2");
+      rows_q8(k, pro, r1, K); k.ext("q", r1, ((long long)K + 3) / 4); k.extn("qs", r1); k.own("q"); k.own("qs"); break; }
+    case 316: { const int m0 = k.I("m0"), n0 = k.I("n0"), M = k.I("M"), N = k.I("N"), K = k.I("K"), tile = k.I("tile");
+      k.need(M > 0 && N > 0 && 0 <= m0 && m0 < M && 0 <= n0 && n0 < N, "bad m0/n0/M/N");
+      k.need(K > 0 && K <= 131071 && tile >= 0 && tile <= 2, "K must be 1 .. 131071, tile 0, 1 or 2");
+      const long long kw = ((long long)K + 3) / 4;
+      k.ext("a", M, kw); k.ext("w", N, kw); k.extn("sa", M); k.extn("sw", N); k.ext("out", M, N); k.extn("bias", N); k.ext("res", M, N);
+      k.own("out", "res"); break; }
+    case 317: { const int n0 = k.I("n0"), n1 = k.I("n1"), K = k.I("K"), M = k.I("M"), pro = k.I("pro"); k.range(n0, n1);
+      k.need(M >= 1 && M <= 16 && pro >= 0 && pro <= 3, "M must be 1 .. 16, pro 0 .. 3");
+      k.need(!k.B("x") || (k.B("x")->dtype == 1) == (pro == 3), "x must be i32 for pro 3, f32 or bf16 otherwise");
+      k.need((k.B("sx") != nullptr) == (pro == 3), "sx goes with pro 3");
+      rows_q8(k, pro, M, K); k.extn("sx", M);
+      k.ext("w", n1, ((long long)K + 3) / 4); k.extn("sw", n1); k.ext("out", M, n1); k.extn("bias", n1); k.ext("res", M, n1);
+      k.own("out", "res"); break; }
+    case 318: { const int r1 = k.I("r1"), H = k.I("H"), Hkv = k.I("Hkv"), hd = k.I("hd"); k.range(k.I("r0"), r1);
+      cache_paged(k);
+      k.need(!k.B("q") == !k.B("qo") && (!k.B("q") ? !k.B("qgamma") : H > 0), "q and qo go together, H positive with them, qgamma needs them");
+      const float theta = k.F("theta"), eps = k.F("eps");
+      k.need(std::isfinite(theta) && (theta == 0.f || theta >= 1.f) && std::isfinite(eps) && eps >= 0.f, "theta must be 0 or at least 1, eps not negative, both finite");
+      k.ext("q", r1, (long long)H * hd); k.ext("qo", r1, (long long)H * hd); k.ext("k", r1, (long long)Hkv * hd); k.ext("v", r1, (long long)Hkv * hd);
+      k.extn("qgamma", hd); k.extn("kgamma", hd);
+      if (k.B("qo")) k.own("qo", "q");
+      k.own("kc"); k.own("vc"); break; }
+    case 319: { const int s = k.I("s"), S = k.I("S"), H = k.I("H"), Hkv = k.I("Hkv"), hd = k.I("hd"), tile = k.I("tile");
+      cache_paged(k);
+      k.need(H > 0 && Hkv > 0 && H % Hkv == 0 && 0 <= s && s < S && S <= (1 << 16), "bad s/S/H/Hkv");
+      k.need(tile <= 128 && (Hkv <= 0 || tile >= H / Hkv), "tile must be H / Hkv .. 128");
+      k.ext("q", 1, (long long)H * hd); k.ext("o", 1, (long long)H * hd); k.extn("cnt", S); k.ext("part", 2ll * S * tile, (long long)hd + 2);
+      if (k.B("q") && k.B("o")) k.need(k.B("q")->rows == k.B("o")->rows, "q and o must have the same rows");
+      for (const char* x : {"o", "part", "cnt"}) k.own(x);
+      k.need(std::isfinite(k.F("scale")) && k.F("scale") > 0.f, "scale must be finite and positive"); break; }
     default: k.need(false, "no extent rule");
   }
 }

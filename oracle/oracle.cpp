@@ -908,6 +908,131 @@ void op_logits_adjust(const Ctx& c) {
   }
 }
 
+// Ops 315-317: a row in 8 bits, v in f32 as the definition rounds it, the byte the exact quotient rounded to nearest even.
+static void q8_row(const V& x, const V& x2, const V& g, long long r, int K, int pro, float eps, std::vector<int>& q, float& scale) {
+  std::vector<float> v(K);
+  float rstd = 0.f;
+  if (pro == 1) {
+    double ss = 0; for (int k = 0; k < K; ++k) ss += x.at(r, k) * x.at(r, k);
+    rstd = f32(1.0 / std::sqrt(ss / K + eps));
+  }
+  float amax = 0.f; bool finite = true;
+  for (int k = 0; k < K; ++k) {
+    const float y = f32(x.at(r, k));
+    if (pro == 1) { volatile float t = y * rstd; v[k] = t * g.f[k]; }
+    else v[k] = pro == 2 ? f32((double)y / (1.0 + std::exp(-(double)y)) * x2.at(r, k)) : y;
+    if (std::isfinite(v[k])) amax = std::max(amax, std::fabs(v[k])); else finite = false;
+  }
+  scale = f32((double)amax * (double)f32(1.0 / 127.0));
+  if (scale < 1.17549435e-38f) scale = 0.f;
+  q.assign(K, 0);
+  if (finite && scale > 0.f)
+    for (int k = 0; k < K; ++k) q[k] = (int)std::max(-127.0, std::min(127.0, std::nearbyint((double)v[k] / (double)scale)));
+  if (!finite) scale = NAN;
+}
+static void q8_out(const V& out, const V& bias, const V& res, long long m, long long n, long long sum, float sa, float sw) {
+  double y = (double)(f32(f32(f32((double)sum) * (double)sa) * (double)sw));
+  if (bias.ok()) y = f32(y + bias.f[n]);
+  if (res.ok()) y = f32(y + res.at(m, n));
+  out.st(m * out.cols + n, y);
+}
+void op_rows_q8(const Ctx& c) {
+  V x = c.buf(0), x2 = c.buf(1, true), g = c.buf(2, true), q = c.buf(3), qs = c.buf(4);
+  const int K = c.i(7), pad = std::min<long long>((K + 15) / 16 * 16, 4ll * q.cols);
+  for (int r = c.i(5); r < c.i(6); ++r) {
+    std::vector<int> b; q8_row(x, x2, g, r, K, c.i(8), c.fl(9), b, qs.f[r]);
+    signed char* p = (signed char*)(q.i + (long long)r * q.cols);
+    for (int k = 0; k < pad; ++k) p[k] = (signed char)(k < K ? b[k] : 0);
+  }
+}
+void op_matmul_q8(const Ctx& c) {
+  V a = c.buf(0), sa = c.buf(1), w = c.buf(2), sw = c.buf(3), out = c.buf(4), bias = c.buf(5, true), res = c.buf(6, true);
+  const int m0 = c.i(7), n0 = c.i(8), M = c.i(9), N = c.i(10), K = c.i(11), tile = c.i(12), tm = tile == 2 ? 64 : 128, tn = tile == 0 ? 256 : tile == 1 ? 128 : 64;
+  for (int m = m0; m < std::min(M, m0 + tm); ++m) for (int n = n0; n < std::min(N, n0 + tn); ++n) {
+    const signed char *x = (const signed char*)(a.i + (long long)m * a.cols), *y = (const signed char*)(w.i + (long long)n * w.cols);
+    long long s = 0; for (int k = 0; k < K; ++k) s += x[k] * y[k];
+    q8_out(out, bias, res, m, n, s, sa.f[m], sw.f[n]);
+  }
+}
+void op_gemv_q8(const Ctx& c) {
+  V x = c.buf(0), x2 = c.buf(1, true), g = c.buf(2, true), w = c.buf(3), sw = c.buf(4), out = c.buf(5), bias = c.buf(6, true), res = c.buf(7, true), sx = c.buf(8, true);
+  const int n0 = c.i(9), n1 = c.i(10), K = c.i(11), M = c.i(12), pro = c.i(13);
+  for (int m = 0; m < M; ++m) {
+    std::vector<int> b; float s = 0.f;
+    if (pro == 3) { b.resize(K); for (int k = 0; k < K; ++k) b[k] = ((const signed char*)(x.i + (long long)m * x.cols))[k]; s = sx.f[m]; }
+    else q8_row(x, x2, g, m, K, pro, c.fl(14), b, s);
+    for (int n = n0; n < n1; ++n) {
+      const signed char* y = (const signed char*)(w.i + (long long)n * w.cols);
+      long long sum = 0; for (int k = 0; k < K; ++k) sum += b[k] * y[k];
+      q8_out(out, bias, res, m, n, sum, s, sw.f[n]);
+    }
+  }
+}
+
+// Ops 318 and 319: a cache in pages.
+struct PagedSeqs {
+  const V &table, &lens, &cu; int B, Hkv, page; long long pages;
+  void check(const char* who, int rows) const {
+    for (int b = 0; b < B; ++b) {
+      const long long n = (long long)cu.i[b + 1] - cu.i[b];
+      if (cu.i[b] < 0 || n < 0 || cu.i[b + 1] > rows) fail(std::string(who) + ": rows");
+      if (n > 0 && (lens.i[b] < 0 || lens.i[b] + n > (long long)table.cols * page)) fail(std::string(who) + ": length");
+    }
+  }
+  long long row(int b, int h, long long t) const {
+    const int p = table.i[(long long)b * table.cols + t / page];
+    if (p < 0 || p >= pages) fail("page outside the cache");
+    return ((long long)p * Hkv + h) * page + t % page;
+  }
+};
+void op_qkv_append_paged(const Ctx& c) {
+  V q = c.buf(0, true), k = c.buf(1), v = c.buf(2), qo = c.buf(3, true), kc = c.buf(4), vc = c.buf(5), table = c.buf(6), lens = c.buf(7), cu = c.buf(8), qg = c.buf(9, true), kg = c.buf(10, true);
+  const int r0 = c.i(11), r1 = c.i(12), B = c.i(13), H = c.i(14), Hkv = c.i(15), hd = c.i(16), page = c.i(17);
+  const float theta = c.fl(18), eps = c.fl(19);
+  const PagedSeqs P{table, lens, cu, B, Hkv, page, kc.rows / ((long long)Hkv * page)};
+  P.check("qkv_append_paged", q.ok() ? std::min({q.rows, qo.rows, k.rows, v.rows}) : std::min(k.rows, v.rows));
+  for (int b = 0; b < B; ++b) for (int r = std::max(r0, cu.i[b]); r < std::min(r1, cu.i[b + 1]); ++r) P.row(b, 0, (long long)lens.i[b] + r - cu.i[b]);
+  for (int b = 0; b < B; ++b) for (int r = std::max(r0, cu.i[b]); r < std::min(r1, cu.i[b + 1]); ++r) {
+    const long long t = (long long)lens.i[b] + r - cu.i[b];
+    std::vector<double> x(hd);
+    for (int h = 0; h < (q.ok() ? H : 0); ++h) {
+      for (int d = 0; d < hd; ++d) x[d] = q.at(r, (long long)h * hd + d);
+      q8_turned(x, qg, eps, theta, t);
+      for (int d = 0; d < hd; ++d) qo.st((long long)r * qo.cols + h * hd + d, x[d]);
+    }
+    for (int h = 0; h < Hkv; ++h) {
+      const long long at = P.row(b, h, t);
+      for (int d = 0; d < hd; ++d) x[d] = k.at(r, (long long)h * hd + d);
+      q8_turned(x, kg, eps, theta, t);
+      for (int d = 0; d < hd; ++d) { kc.st(at * kc.cols + d, x[d]); vc.st(at * vc.cols + d, v.at(r, (long long)h * hd + d)); }
+    }
+  }
+}
+void op_attn_paged(const Ctx& c) { // every S-th (row, head): how the device cuts the work is its matter
+  V q = c.buf(0), kc = c.buf(1), vc = c.buf(2), table = c.buf(3), lens = c.buf(4), cu = c.buf(5), o = c.buf(7);
+  const int s = c.i(9), S = c.i(10), B = c.i(11), H = c.i(12), Hkv = c.i(13), hd = c.i(14), page = c.i(15), G = H / Hkv;
+  const double scale = c.fl(17);
+  const PagedSeqs P{table, lens, cu, B, Hkv, page, kc.rows / ((long long)Hkv * page)};
+  P.check("attn_paged", std::min(q.rows, o.rows));
+  for (int b = 0; b < B; ++b) for (int r = cu.i[b]; r < cu.i[b + 1]; ++r) for (int h = 0; h < H; ++h) {
+    if (((long long)r * H + h) % S != s) continue;
+    const long long n = (long long)lens.i[b] + r - cu.i[b] + 1;
+    std::vector<double> p(n);
+    std::vector<long long> at(n);
+    double m = -INFINITY, l = 0;
+    for (long long t = 0; t < n; ++t) {
+      at[t] = P.row(b, h / G, t);
+      double a = 0; for (int d = 0; d < hd; ++d) a += q.at(r, (long long)h * hd + d) * kc.at(at[t], d);
+      p[t] = a * scale; m = std::max(m, p[t]);
+    }
+    for (double& x : p) { x = std::exp(x - m); l += x; }
+    for (int d = 0; d < hd; ++d) {
+      double a = 0; for (long long t = 0; t < n; ++t) a += p[t] * vc.at(at[t], d);
+      o.st((long long)r * o.cols + h * hd + d, a / l);
+    }
+  }
+}
+
 typedef void (*OpFn)(const Ctx&);
 struct OpEnt { int id; OpFn fn; };
 const OpEnt kOps[] = {
@@ -926,6 +1051,7 @@ const OpEnt kOps[] = {
   {135, op_attn_decode_part}, {136, op_attn_decode_merge}, {115, op_adamw_lr}, {116, op_lr_schedule}, {117, op_scale_flat},
   {118, op_add_rowtile}, {120, op_matmul_tile_silu_mul}, {121, op_matmul_tile_silu_mul_bwd}, {300, op_head_rmsnorm}, {301, op_gemv_bf16_rows}, {311, op_gemv_swiglu}, {302, op_matmul_mma_bf16_kr}, {303, op_splitk_reduce}, {304, op_matmul_mma_bf16_256}, {305, op_adamw_bf16}, {306, op_attn_decode_part_qkn}, {310, op_attn_decode_part_merge}, {308, op_matmul_mma_bf16_delta},
   {312, op_kv_append_q8}, {313, op_attn_decode_q8}, {314, op_logits_adjust},
+  {315, op_rows_q8}, {316, op_matmul_q8}, {317, op_gemv_q8}, {318, op_qkv_append_paged}, {319, op_attn_paged},
 };
 OpFn find_op(int id) { for (const OpEnt& e : kOps) if (e.id == id) return e.fn; return nullptr; }
 
