@@ -47,6 +47,11 @@ struct AppendPaged {
     return (unsigned)p < (unsigned)pages;
   }
 };
+// One of three values by `what` (values, not references: a choice between fields would put the arguments into scratch memory).
+template <class T> __device__ __forceinline__ T pick(int what, T a, T b, T c) { return what == 0 ? a : what == 1 ? b : c; }
+__device__ __forceinline__ View pick_view(int what, const View& a, const View& b, const View& c) {
+  return View{pick<void*>(what, a.p, b.p, c.p), 0, pick<int>(what, a.cols, b.cols, c.cols), pick<int>(what, a.dtype, b.dtype, c.dtype), 0};
+}
 // LDS of a task: rows in flight with their positions, places and angles.
 constexpr int AP_ROWS = 32;
 struct AppendPagedLds {
@@ -98,7 +103,7 @@ __device__ __noinline__ void op_qkv_append_paged(const Ctx& c) {
     append_paged_rows(A, M, r, nr);
     for (int u = wave(); u < nr * heads; u += KVM_WAVES) {
       const int row = u / heads, s = u % heads, what = s < A.H ? 0 : s < A.H + A.Hkv ? 1 : 2, h = what == 0 ? s : what == 1 ? s - A.H : s - A.H - A.Hkv;
-      const View src = what == 0 ? A.q : what == 1 ? A.k : A.v, dst = what == 0 ? A.qo : what == 1 ? A.kc : A.vc, g = what == 0 ? A.qg : what == 1 ? A.kg : View{nullptr, 0, 0, 0, 0};
+      const View src = pick_view(what, A.q, A.k, A.v), dst = pick_view(what, A.qo, A.kc, A.vc), g = pick_view(what, A.qg, A.kg, View{nullptr, 0, 0, 0, 0});
       const long long from = (long long)(r + row) * src.cols + (long long)h * A.hd;
       const long long to = what == 0 ? (long long)(r + row) * dst.cols + (long long)h * A.hd : (M.at[row] + ((long long)h << A.lp)) * dst.cols;
       float x[2][2], ss = 0.f;
@@ -124,59 +129,75 @@ __device__ __noinline__ void op_qkv_append_paged(const Ctx& c) {
     }
   }
 }
-// Head sizes 64 and 128, rows in whole vectors. Bound: bytes for prompts, a few dependent loads (row numbers, length, page, row) and the
-// launch for single tokens. A (row, head) is HD / 8 lanes of 8 values; a row's angles are computed once for all its heads; four items'
-// loads are requested together.
+// Head sizes 64 and 128, rows in whole vectors, one type for the new rows and one for where they go. Bound: bytes for prompts, a few dependent
+// loads (row numbers, length, page, row) and the launch for single tokens. A (row, head) is HD / 8 lanes of 8 values; a row's angles are
+// computed once for all its heads; four items' loads are requested together.
 template <int HD> __device__ __noinline__ void append_paged_t(const Ctx& c) {
   constexpr int LPR = HD / 8, RPP = KVM_THREADS / LPR, NR = 4;
   const AppendPaged A(c);
   const AppendPagedLds M(c.smem);
   int end;
   if (!append_paged_begin(c, A, M, end)) return;
-  const int ln = tid() % LPR, rw = tid() / LPR, heads = A.H + 2 * A.Hkv;
+  const int ln = tid() % LPR, rw = tid() / LPR;
+  const unsigned heads = A.H + 2 * A.Hkv;
+  const bool from16 = A.k.dtype == 2, to16 = A.kc.dtype == 2, qn = A.qg.ok(), kn = A.kg.ok(), turn = A.theta > 0.f;
   const float sign = ln >= LPR / 2 ? 1.f : -1.f;
+  float qg[8], kg[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) { qg[e] = qn ? A.qg.f()[8 * ln + e] : 1.f; kg[e] = kn ? A.kg.f()[8 * ln + e] : 1.f; }
+  // the row and head of item u of this range: what it is (0 query, 1 key, 2 value) and its head
+  struct Item { int row, what, h; };
+  auto item = [&](int u) {
+    const int row = (int)((unsigned)u / heads), s = u - row * (int)heads, what = s < A.H ? 0 : s < A.H + A.Hkv ? 1 : 2;
+    return Item{row, what, s - (what == 0 ? 0 : what == 1 ? A.H : A.H + A.Hkv)};
+  };
   for (int r = max(A.r0, rfl(M.cu[0])); r < end; r += AP_ROWS) {
-    const int nr = min(AP_ROWS, end - r), items = nr * heads;
-    append_paged_rows(A, M, r, nr);
-    for (int u0 = rw; u0 < items; u0 += NR * RPP) {
-      Raw8 raw[NR];
+    const int nr = min(AP_ROWS, end - r), items = nr * (int)heads;
+    Raw8 raw[NR];
+    auto request = [&](int u0) {
 #pragma unroll
       for (int i = 0; i < NR; ++i) {
-        const int u = min(u0 + i * RPP, items - 1), row = u / heads, s = u % heads;
-        const View& X = s < A.H ? A.q : s < A.H + A.Hkv ? A.k : A.v;
-        const int h = s < A.H ? s : s < A.H + A.Hkv ? s - A.H : s - A.H - A.Hkv;
-        raw[i].load(X, (long long)(r + row) * X.cols + h * HD + 8 * ln);
+        const Item t = item(min(u0 + i * RPP, items - 1));
+        const View x = pick_view(t.what, A.q, A.k, A.v);
+        raw[i].load(View{x.p, 0, x.cols, from16 ? 2 : 0, 0}, (long long)(r + t.row) * x.cols + t.h * HD + 8 * ln);
       }
+    };
+    request(rw);                                                       // under the positions and angles
+    append_paged_rows(A, M, r, nr);
+    for (int u0 = rw; u0 < items; u0 += NR * RPP) {
+      if (u0 != rw) request(u0);
 #pragma unroll
       for (int i = 0; i < NR; ++i) {
         const int u = u0 + i * RPP;
         if (u >= items) break;
-        const int row = u / heads, s = u % heads, what = s < A.H ? 0 : s < A.H + A.Hkv ? 1 : 2, h = what == 0 ? s : what == 1 ? s - A.H : s - A.H - A.Hkv;
+        const Item t = item(u);
         float x[8];
-        raw[i].get((what == 0 ? A.q.dtype : what == 1 ? A.k.dtype : A.v.dtype) == 2, x);
-        const View& g = what == 0 ? A.qg : A.kg;
-        if (what < 2 && g.ok()) {
+        raw[i].get(from16, x);
+        if (t.what == 0 ? qn : t.what == 1 && kn) {
           float ss = 0.f;
 #pragma unroll
           for (int e = 0; e < 8; ++e) ss += x[e] * x[e];
           const float rs = 1.f / sqrtf(lanes_sum<LPR>(ss) / HD + A.eps);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] = x[e] * rs * g.f()[8 * ln + e];
+          for (int e = 0; e < 8; ++e) x[e] = x[e] * rs * (t.what == 0 ? qg[e] : kg[e]);
         }
-        if (what < 2 && A.theta > 0.f) {
-          const LDS float* ang = M.ang + row * HD + 8 * (ln % (LPR / 2));
+        if (turn && t.what < 2) {
+          const LDS float* ang = M.ang + t.row * HD + 8 * (ln % (LPR / 2));
 #pragma unroll
           for (int e = 0; e < 8; ++e) x[e] = x[e] * ang[HD / 2 + e] + sign * __shfl_xor(x[e], LPR / 2, 64) * ang[e];
         }
-        const View& Y = what == 0 ? A.qo : what == 1 ? A.kc : A.vc;
-        st8(Y, what == 0 ? (long long)(r + row) * Y.cols + h * HD + 8 * ln : (M.at[row] + ((long long)h << A.lp)) * Y.cols + 8 * ln, x);
+        const View y = pick_view(t.what, A.qo, A.kc, A.vc);
+        const long long at = (t.what == 0 ? (long long)(r + t.row) : M.at[t.row] + ((long long)t.h << A.lp)) * y.cols + (t.what == 0 ? t.h * HD : 0) + 8 * ln;
+        if (to16) { stwt_bf4(y.h() + at, x[0], x[1], x[2], x[3]); stwt_bf4(y.h() + at + 4, x[4], x[5], x[6], x[7]); }
+        else { stwt_f4(y.f() + at, f32x4n{x[0], x[1], x[2], x[3]}); stwt_f4(y.f() + at + 4, f32x4n{x[4], x[5], x[6], x[7]}); }
       }
     }
   }
 }
 __device__ __noinline__ bool op_qkv_append_paged_fast(const Ctx& c) {
-  const View q = c.buf(0), qo = c.buf(3);
-  if ((q.ok() && (!rows8_ok(q) || !rows8_ok(qo))) || !rows8_ok(c.buf(1)) || !rows8_ok(c.buf(2)) || !rows8_ok(c.buf(4)) || !rows8_ok(c.buf(5))) return false;
+  const View q = c.buf(0), k = c.buf(1), v = c.buf(2), qo = c.buf(3), kc = c.buf(4), vc = c.buf(5);
+  if ((q.ok() && (!rows8_ok(q) || !rows8_ok(qo) || q.dtype != k.dtype || qo.dtype != kc.dtype)) || v.dtype != k.dtype || vc.dtype != kc.dtype) return false;
+  if (!rows8_ok(k) || !rows8_ok(v) || !rows8_ok(kc) || !rows8_ok(vc)) return false;
   if (c.i(16) == 128) append_paged_t<128>(c);
   else if (c.i(16) == 64) append_paged_t<64>(c);
   else return false;
@@ -194,10 +215,11 @@ struct AttnPaged {
     pages = (int)((unsigned)kc.rows / (unsigned)(Hkv * page));
     sl2 = __int_as_float(rfl(__float_as_int(c.f(17) * 1.44269504088896340736f)));
   }
-  // bf16 storage at head sizes 64 and 128 in whole vectors: the matrix units
-  __device__ bool fast() const {
-    return q.dtype == 2 && kc.dtype == 2 && vc.dtype == 2 && o.dtype == 2 && (hd == 64 || hd == 128) && rows8_ok(q) && rows8_ok(kc) && rows8_ok(vc) && rows8_ok(o) &&
-           (long long)Hkv * page * max(kc.cols, vc.cols) * 2 < 0x7fffff00ll;
+  // Storage of one type throughout at head sizes 64 and 128 in whole vectors: the matrix units (0 no, 1 f32, 2 bf16)
+  __device__ int fast() const {
+    const int t = q.dtype;
+    if (kc.dtype != t || vc.dtype != t || o.dtype != t || (hd != 64 && hd != 128) || !rows8_ok(q) || !rows8_ok(kc) || !rows8_ok(vc) || !rows8_ok(o)) return 0;
+    return (long long)Hkv * page * max(kc.cols, vc.cols) * 4 >= 0x7fffff00ll ? 0 : t == 2 ? 2 : 1;
   }
 };
 // A tile's rows: row r is token tok0 + r / G of the sequence's new ones, head h * G + r % G; it sees keys 0 .. L + tok0 + r / G.
@@ -353,10 +375,12 @@ __device__ __forceinline__ void paged_arrive(const Ctx& c, const AttnPaged& D, c
   if (tid() == 0) st_relaxed((int*)D.cnt.i() + p.i0, 0);
 }
 
+enum { PG_DONE, PG_AGAIN, PG_FAILED };   // a piece is written; is to be done by the general form; has a page that is none
+
 // Any storage, head size and alignment, in f32, and pieces of the other forms with results that are not finite (a key that a row does not see
 // has weight 0 there, which an infinity or NaN in its value would turn into NaN; here it is skipped): 32 rows by 32 keys at a time in LDS, the
 // next keys' loads in flight; scores a thread to a key and four rows, eight threads to a row for the softmax and its P V.
-__device__ __noinline__ void attn_paged_general(const Ctx& c, int b_, int h_, int L_, int row0_, int tok0_, int ntok_, int k0_, int k1_, int k_, int live_, int i0_) {
+__device__ __noinline__ int attn_paged_general(const Ctx& c, int b_, int h_, int L_, int row0_, int tok0_, int ntok_, int k0_, int k1_, int k_, int live_, int i0_) {
   const AttnPaged D(c);
   const TilePaged t{rfl(b_), rfl(h_), rfl(L_), rfl(row0_), rfl(tok0_), rfl(ntok_), 0, 0};
   const PiecePaged p{rfl(k0_), rfl(k1_), rfl(k_), rfl(live_), rfl(i0_)};
@@ -463,7 +487,7 @@ __device__ __noinline__ void attn_paged_general(const Ctx& c, int b_, int h_, in
           if (sub + 8 * i < C4) acc[i] += e * *(const LDS f32x4n*)(vs + u * HP + 4 * (sub + 8 * i));
       }
     }
-    if (__syncthreads_or(bad)) { if (tid() == 0) c.fail(KVM_ERR_OP_RANGE, t.b, p.k0); return; }
+    if (__syncthreads_or(bad)) { if (tid() == 0) c.fail(KVM_ERR_OP_RANGE, t.b, p.k0); return PG_FAILED; }
     if (rg + row < R) {
 #pragma unroll
       for (int i = 0; i < NF; ++i)
@@ -476,8 +500,509 @@ __device__ __noinline__ void attn_paged_general(const Ctx& c, int b_, int h_, in
       if (p.live > 1 && sub == 0) { GLOBAL float* y = paged_partial(D, p, p.k, rg + row) + hd; stwt32(y, m); stwt32(y + 1, lsum); }
     }
   }
+  return PG_DONE;
 }
 
+// The end of a piece whose waves have keys of their own: their states (maxima m and sums ls of row l % 16 of each tile, ls a share for each quarter
+// of the wave, P V in acc: dims DPL (4 (l / 16) + q) + i) meet in LDS; the rows go out, or to the piece's partials.
+template <int HD, int NT, bool HALF>
+__device__ __forceinline__ int paged_waves(const Ctx& c, const AttnPaged& D, const TilePaged& t, const PiecePaged& p, const f32x4_t (&acc)[NT][HD / 16], const float (&m)[NT],
+                                           const float (&ls)[NT], bool bad) {
+  constexpr int DPL = HD / 16, RW = 16 * NT;
+  const int l = lane(), w = rfl(wave()), m16 = l & 15, qq = l >> 4, R = t.ntok * D.G;
+  LDS float* st = (LDS float*)(c.smem + PG_WORK);                      // [4][2][32] maxima and sums
+  LDS float* ol = st + 256;                                            // [4][RW][HD + 4]
+  __syncthreads();
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const float z = rows_sum(ls[n]);
+    if (qq == 0) { st[64 * w + 16 * n + m16] = m[n]; st[64 * w + 32 + 16 * n + m16] = z; }
+  }
+  __syncthreads();
+  float nf = 0.f;
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int r = 16 * n + m16;
+    const float top = fmaxf(fmaxf(st[r], st[64 + r]), fmaxf(st[128 + r], st[192 + r]));
+    const float f = m[n] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[n] - top);
+    float z = 0.f;
+#pragma unroll
+    for (int v = 0; v < 4; ++v) z += (st[64 * v + r] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st[64 * v + r] - top)) * st[64 * v + 32 + r];
+    nf += z * 0.f + (top == -INFINITY ? 0.f : top * 0.f);
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+#pragma unroll
+      for (int i = 0; i < DPL; ++i) {
+        const float y = acc[n][i][q] * f;
+        nf += y * 0.f;
+        ol[(w * RW + r) * (HD + 4) + DPL * (4 * qq + q) + i] = y;
+      }
+  }
+  const int again = __syncthreads_or(nf != 0.f ? 1 : 0), out = __syncthreads_or(bad ? 1 : 0);
+  if (out) { if (tid() == 0) c.fail(KVM_ERR_OP_RANGE, t.b, p.k0); return PG_FAILED; }
+  if (again) return PG_AGAIN;                                            // something is not finite: by the general form
+  for (int e = tid(); e < R * (HD / 4); e += KVM_THREADS) {
+    const int r = e / (HD / 4), d = 4 * (e % (HD / 4));
+    f32x4n a = *(const LDS f32x4n*)(ol + r * (HD + 4) + d);
+#pragma unroll
+    for (int v = 1; v < 4; ++v) a += *(const LDS f32x4n*)(ol + (v * RW + r) * (HD + 4) + d);
+    const float top = fmaxf(fmaxf(st[r], st[64 + r]), fmaxf(st[128 + r], st[192 + r]));
+    float z = 0.f;
+#pragma unroll
+    for (int v = 0; v < 4; ++v) z += (st[64 * v + r] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st[64 * v + r] - top)) * st[64 * v + 32 + r];
+    if (p.live == 1) {
+      a *= 1.f / z;
+      if constexpr (HALF) stwt_bf4(D.o.h() + paged_out(D, t, r) + d, a.x, a.y, a.z, a.w);
+      else stwt_f4(D.o.f() + paged_out(D, t, r) + d, a);
+    }
+    else {
+      GLOBAL float* y = paged_partial(D, p, p.k, r);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) stwt32(y + d + i, a[i]);
+      if (d == 0) { stwt32(y + HD, top); stwt32(y + HD + 1, z); }
+    }
+  }
+  return PG_DONE;
+}
+
+// ---- The matrix units: bf16 storage, head sizes 64 and 128.
+// Tiles of up to 32 rows (single tokens, drafted ones): bound by the bytes of keys and values. The four waves take units of 32 keys in turn,
+// each for itself, K and V straight from the pages into registers, a unit ahead, the page numbers two:
+//   scores  v_mfma_f32_16x16x32_bf16, A = 16 keys (row m of tile a: key 8 (m / 4) + 4 a + m % 4), B = 16 query rows (NT such tiles). A lane's
+//           16-byte load of a key is its part of the operand, and the rows' order makes the scores' registers the B operand of
+//   P V     the same instruction, A = V transposed: a lane loads HD / 16 dims of 8 keys, whole rows of the page to 16 lanes, and turns them
+//           in registers (one byte permute for two values), dims DPL m + i to row m of product i.
+// Probabilities are bf16; the running maximum moves only when a row's grows by more than 2^8. The waves' states
+// meet in LDS.
+// The sum of eight bf16 weights onto s: what the second product weighs with is what the row is divided by, so that the rounding of a large weight
+// cancels.
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ float sum_bf16(bf16x8 p, float s) {
+  const bf16x2 one = {(__bf16)1.f, (__bf16)1.f};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) s = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{p[2 * i], p[2 * i + 1]}, one, s, false);
+  return s;
+}
+template <int HD, int NT> __device__ __noinline__ int attn_paged_keys(const Ctx& c, int b_, int h_, int L_, int row0_, int tok0_, int ntok_, int k0_, int k1_, int k_, int live_, int i0_) {
+  constexpr int NK = HD / 32, DPL = HD / 16, RW = 16 * NT;
+  const AttnPaged D(c);
+  const TilePaged t{rfl(b_), rfl(h_), rfl(L_), rfl(row0_), rfl(tok0_), rfl(ntok_), 0, 0};
+  const PiecePaged p{rfl(k0_), rfl(k1_), rfl(k_), rfl(live_), rfl(i0_)};
+  const int l = lane(), w = rfl(wave()), m16 = l & 15, qq = l >> 4, R = t.ntok * D.G, klast = p.k1 - 1;
+  const GLOBAL int* tb = D.table.i() + (long long)t.b * D.table.cols;
+  const GLOBAL char* kb = (const GLOBAL char*)D.kc.p + (((long long)t.h << D.lp) * D.kc.cols) * 2;
+  const GLOBAL char* vb = (const GLOBAL char*)D.vc.p + (((long long)t.h << D.lp) * D.vc.cols) * 2;
+  const unsigned kpage = (unsigned)(D.Hkv << D.lp) * D.kc.cols * 2, vpage = (unsigned)(D.Hkv << D.lp) * D.vc.cols * 2;   // bytes (below 2^31)
+  const int pm = D.page - 1, kpitch = D.kc.cols * 2, vpitch = D.vc.cols * 2;
+  bf16x8 qf[NT][NK];
+  int lim[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int r = min(16 * n + m16, R - 1);
+    lim[n] = t.L + t.tok0 + r / D.G;
+    const GLOBAL uint16_t* q = D.q.h() + (long long)(t.row0 + r / D.G) * D.q.cols + (long long)(t.h * D.G + r % D.G) * HD + 8 * qq;
+#pragma unroll
+    for (int kk = 0; kk < NK; ++kk) qf[n][kk] = *(const GLOBAL bf16x8*)(q + 32 * kk);
+  }
+  struct Ids { int k, v; };
+  struct Unit { u32x4_t k[2][NK]; u32x4_t v[8]; };                     // (HD 64: the first half of v)
+  bool bad = false;
+  const int nu = (p.k1 - p.k0 + 31) >> 5;                              // units of the piece; this wave: w, w + 4, ..
+  auto ids = [&](Ids& I, int u) {
+    const int key0 = p.k0 + 32 * u;
+    I.k = tb[min(key0 + 8 * (m16 >> 2), klast) >> D.lp];
+    I.v = tb[min(key0 + 8 * qq, klast) >> D.lp];
+  };
+  auto load = [&](Unit& U, const Ids& I, int u) {
+    const int key0 = p.k0 + 32 * u;
+    bad = bad || (unsigned)I.k >= (unsigned)D.pages || (unsigned)I.v >= (unsigned)D.pages;
+    const unsigned ik = (unsigned)I.k < (unsigned)D.pages ? I.k : 0u, iv = (unsigned)I.v < (unsigned)D.pages ? I.v : 0u;
+    const GLOBAL char* kp = kb + (unsigned long long)ik * kpage;
+    const GLOBAL char* vp = vb + (unsigned long long)iv * vpage;
+#pragma unroll
+    for (int a = 0; a < 2; ++a) {
+      const GLOBAL char* y = kp + ((min(key0 + 8 * (m16 >> 2) + 4 * a + (m16 & 3), klast) & pm) * kpitch + 16 * qq);
+#pragma unroll
+      for (int kk = 0; kk < NK; ++kk) U.k[a][kk] = *(const GLOBAL u32x4_t*)(y + 64 * kk);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const GLOBAL char* y = vp + ((min(key0 + 8 * qq + j, klast) & pm) * vpitch + 2 * DPL * m16);
+      if constexpr (DPL == 8) U.v[j] = *(const GLOBAL u32x4_t*)y;
+      else { const u32x2_t x = *(const GLOBAL u32x2_t*)y; U.v[j].x = x.x; U.v[j].y = x.y; }
+    }
+  };
+  f32x4_t acc[NT][DPL];
+  float m[NT], ls[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    m[n] = -INFINITY; ls[n] = 0.f;
+#pragma unroll
+    for (int i = 0; i < DPL; ++i) acc[n][i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  }
+  auto compute = [&](const Unit& U, int u) {
+    const int key0 = p.k0 + 32 * u;
+    bf16x8 vt[DPL];
+#pragma unroll
+    for (int d = 0; d < DPL / 2; ++d) {
+      u32x4_t lo, hi;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        lo[j] = __builtin_amdgcn_perm(U.v[2 * j + 1][d], U.v[2 * j][d], 0x05040100u);
+        hi[j] = __builtin_amdgcn_perm(U.v[2 * j + 1][d], U.v[2 * j][d], 0x07060302u);
+      }
+      vt[2 * d] = __builtin_bit_cast(bf16x8, lo); vt[2 * d + 1] = __builtin_bit_cast(bf16x8, hi);
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      f32x4_t s[2];
+#pragma unroll
+      for (int a = 0; a < 2; ++a) {
+        s[a] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kk = 0; kk < NK; ++kk) s[a] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, U.k[a][kk]), qf[n][kk], s[a], 0, 0, 0);
+      }
+      float x[8], mx = -INFINITY;
+      const bool edge = key0 + 31 > t.L + t.tok0;                      // some row does not see the whole unit
+#pragma unroll
+      for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float y = s[a][r] * D.sl2;
+          x[4 * a + r] = edge && key0 + 8 * qq + 4 * a + r > lim[n] ? -INFINITY : y;
+          mx = fmaxf(mx, x[4 * a + r]);
+        }
+      mx = rows_max(mx);
+      if (__ballot(mx > m[n] + 8.f)) {
+        const float top = fmaxf(m[n], mx), f = m[n] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[n] - top);
+        ls[n] *= f;
+#pragma unroll
+        for (int i = 0; i < DPL; ++i) acc[n][i] *= f;
+        m[n] = top;
+      }
+      const float base = m[n] == -INFINITY ? 0.f : m[n];
+      float pv[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) pv[i] = __builtin_amdgcn_exp2f(x[i] - base);
+      const bf16x8 pb = pack_bf16(pv);
+      ls[n] = sum_bf16(pb, ls[n]);
+#pragma unroll
+      for (int i = 0; i < DPL; ++i) acc[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vt[i], pb, acc[n][i], 0, 0, 0);
+    }
+  };
+  if (w < nu) {
+    Ids i0, i1;
+    Unit u0, u1;
+    ids(i0, w); ids(i1, min(w + 4, nu - 1));
+    load(u0, i0, w);
+    int u = w;
+    for (; u + 8 < nu; u += 8) {                                       // (no branch between a unit's loads and the products of the one before)
+      ids(i0, u + 8);
+      load(u1, i1, u + 4);
+      compute(u0, u);
+      ids(i1, min(u + 12, nu - 1));
+      load(u0, i0, u + 8);
+      compute(u1, u + 4);
+    }
+    if (u + 4 < nu) {
+      load(u1, i1, u + 4);
+      compute(u0, u);
+      compute(u1, u + 4);
+    } else compute(u0, u);
+  }
+  return paged_waves<HD, NT, true>(c, D, t, p, acc, m, ls, bad);
+}
+
+// The same tiles in f32 storage, v_mfma_f32_16x16x4_f32 (exact products): units of 16 keys; a lane's 16-byte load of a key is four dims of it, of
+// which product i takes the i-th from all lanes (k = l / 16), and the scores' registers r are, row by row, P's operand for the keys 4 k + r,
+// whose values the lane has loaded.
+template <int HD, int NT> __device__ __noinline__ int attn_paged_keys_f32(const Ctx& c, int b_, int h_, int L_, int row0_, int tok0_, int ntok_, int k0_, int k1_, int k_, int live_, int i0_) {
+  constexpr int NK = HD / 16, DPL = HD / 16, NV = DPL / 4;
+  const AttnPaged D(c);
+  const TilePaged t{rfl(b_), rfl(h_), rfl(L_), rfl(row0_), rfl(tok0_), rfl(ntok_), 0, 0};
+  const PiecePaged p{rfl(k0_), rfl(k1_), rfl(k_), rfl(live_), rfl(i0_)};
+  const int l = lane(), w = rfl(wave()), m16 = l & 15, qq = l >> 4, R = t.ntok * D.G, klast = p.k1 - 1;
+  const GLOBAL int* tb = D.table.i() + (long long)t.b * D.table.cols;
+  const GLOBAL char* kb = (const GLOBAL char*)D.kc.p + (((long long)t.h << D.lp) * D.kc.cols) * 4;
+  const GLOBAL char* vb = (const GLOBAL char*)D.vc.p + (((long long)t.h << D.lp) * D.vc.cols) * 4;
+  const unsigned kpage = (unsigned)(D.Hkv << D.lp) * D.kc.cols * 4, vpage = (unsigned)(D.Hkv << D.lp) * D.vc.cols * 4;
+  const int pm = D.page - 1, kpitch = D.kc.cols * 4, vpitch = D.vc.cols * 4;
+  f32x4n qf[NT][NK];
+  int lim[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int r = min(16 * n + m16, R - 1);
+    lim[n] = t.L + t.tok0 + r / D.G;
+    const GLOBAL float* q = D.q.f() + (long long)(t.row0 + r / D.G) * D.q.cols + (long long)(t.h * D.G + r % D.G) * HD + 4 * qq;
+#pragma unroll
+    for (int kk = 0; kk < NK; ++kk) qf[n][kk] = *(const GLOBAL f32x4n*)(q + 16 * kk);
+  }
+  struct Unit { f32x4n k[NK], v[4][NV]; };
+  bool bad = false;
+  const int nu = (p.k1 - p.k0 + 15) >> 4;
+  auto ids = [&](int u) { return tb[min(p.k0 + 16 * u, klast) >> D.lp]; };   // (a unit lies within a page)
+  auto load = [&](Unit& U, int id, int u) {
+    const int key0 = p.k0 + 16 * u;
+    bad = bad || (unsigned)id >= (unsigned)D.pages;
+    const unsigned i = (unsigned)id < (unsigned)D.pages ? id : 0u;
+    const GLOBAL char* kp = kb + (unsigned long long)i * kpage + ((min(key0 + m16, klast) & pm) * kpitch + 16 * qq);
+    const GLOBAL char* vp = vb + (unsigned long long)i * vpage + 4 * DPL * m16;
+#pragma unroll
+    for (int kk = 0; kk < NK; ++kk) U.k[kk] = *(const GLOBAL f32x4n*)(kp + 64 * kk);
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int j = 0; j < NV; ++j) U.v[r][j] = *(const GLOBAL f32x4n*)(vp + ((min(key0 + 4 * qq + r, klast) & pm) * vpitch + 16 * j));
+  };
+  f32x4_t acc[NT][DPL];
+  float m[NT], ls[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    m[n] = -INFINITY; ls[n] = 0.f;
+#pragma unroll
+    for (int i = 0; i < DPL; ++i) acc[n][i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  }
+  auto compute = [&](const Unit& U, int u) {
+    const int key0 = p.k0 + 16 * u;
+    const bool edge = key0 + 15 > t.L + t.tok0;                        // some row does not see the whole unit
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      f32x4_t s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};      // (two chains: a product waits for the one before the last)
+#pragma unroll
+      for (int kk = 0; kk < NK; ++kk)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[i & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(U.k[kk][i], qf[n][kk][i], s[i & 1], 0, 0, 0);
+      float x[4], mx = -INFINITY;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float y = (s[0][r] + s[1][r]) * D.sl2;
+        x[r] = edge && key0 + 4 * qq + r > lim[n] ? -INFINITY : y;
+        mx = fmaxf(mx, x[r]);
+      }
+      mx = rows_max(mx);
+      if (__ballot(mx > m[n] + 8.f)) {
+        const float top = fmaxf(m[n], mx), f = m[n] == -INFINITY ? 0.f : exp2f(m[n] - top);
+        ls[n] *= f;
+#pragma unroll
+        for (int i = 0; i < DPL; ++i) acc[n][i] *= f;
+        m[n] = top;
+      }
+      const float base = m[n] == -INFINITY ? 0.f : m[n];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float e = exp2f(x[r] - base);
+        ls[n] += e;
+#pragma unroll
+        for (int i = 0; i < DPL; ++i) acc[n][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(U.v[r][i >> 2][i & 3], e, acc[n][i], 0, 0, 0);
+      }
+    }
+  };
+  if (w < nu) {
+    Unit u0, u1;
+    int i0 = ids(w), i1 = ids(w + 4), u = w;
+    load(u0, i0, w);
+    for (; u + 8 < nu; u += 8) {
+      i0 = ids(u + 8);
+      load(u1, i1, u + 4);
+      compute(u0, u);
+      i1 = ids(u + 12);
+      load(u0, i0, u + 8);
+      compute(u1, u + 4);
+    }
+    if (u + 4 < nu) {
+      load(u1, i1, u + 4);
+      compute(u0, u);
+      compute(u1, u + 4);
+    } else compute(u0, u);
+  }
+  return paged_waves<HD, NT, false>(c, D, t, p, acc, m, ls, bad);
+}
+
+// Tiles of up to 128 rows (chunks of prompts): bound by the matrix units and the vector work of the softmax. A wave has 32 rows; blocks of 64 keys
+// come from the pages straight into LDS for all of them, three stages, the page numbers of up to PG_IDS pages in LDS. In transposed space as
+// attn_fwd_mfma: S^T = K Q^T (a lane owns a query row), O^T += V^T P^T with P^T's registers as they are; the scores of the next block under the
+// softmax of this one.
+constexpr int PG_IDS = 2048, PG_NS = 3;
+__device__ __forceinline__ void dma16_at(const GLOBAL char* src, const LDS void* dst) {   // 16 bytes a lane from its own address to dst + 16 * lane
+  const int m = __builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)dst);
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" :: "s"(m), "v"(src) : "memory", "m0");
+}
+template <int HD> __device__ __noinline__ int attn_paged_rows(const Ctx& c, int b_, int h_, int L_, int row0_, int tok0_, int ntok_, int k0_, int k1_, int k_, int live_, int i0_) {
+  typedef FaL<HD> FL;
+  constexpr int NKK = HD / 16, NDB = HD / 32, ST = 2 * FA_KB * HD;
+  static_assert(PG_WORK + PG_IDS * 4 + PG_NS * ST * 2 <= KVM_LDS_BYTES, "LDS");
+  const AttnPaged D(c);
+  const TilePaged t{rfl(b_), rfl(h_), rfl(L_), rfl(row0_), rfl(tok0_), rfl(ntok_), 0, 0};
+  const PiecePaged p{rfl(k0_), rfl(k1_), rfl(k_), rfl(live_), rfl(i0_)};
+  const int w = rfl(wave()), l = lane(), g = l >> 5, qi = l & 31, R = t.ntok * D.G, row = 32 * w + qi, rr = min(row, R - 1), klast = p.k1 - 1;
+  const bool qok = row < R, wave_on = 32 * w < R;
+  const int lim = t.L + t.tok0 + rr / D.G;
+  const int wfirst = rfl(t.L + t.tok0 + min(32 * w, R - 1) / D.G), wlast = rfl(t.L + t.tok0 + min(32 * w + 31, R - 1) / D.G);
+  const GLOBAL int* tb = D.table.i() + (long long)t.b * D.table.cols;
+  const GLOBAL char* kb = (const GLOBAL char*)D.kc.p + (((long long)t.h << D.lp) * D.kc.cols) * 2;
+  const GLOBAL char* vb = (const GLOBAL char*)D.vc.p + (((long long)t.h << D.lp) * D.vc.cols) * 2;
+  const unsigned kpage = (unsigned)(D.Hkv << D.lp) * D.kc.cols * 2, vpage = (unsigned)(D.Hkv << D.lp) * D.vc.cols * 2;
+  const int pm = D.page - 1, kpitch = D.kc.cols * 2, vpitch = D.vc.cols * 2;
+  LDS int* sid = (LDS int*)(c.smem + PG_WORK);
+  LDS uint16_t* lds = (LDS uint16_t*)(sid + PG_IDS);
+  bf16x8 qf[NKK];
+  {
+    const GLOBAL uint16_t* q = D.q.h() + (long long)(t.row0 + rr / D.G) * D.q.cols + (long long)(t.h * D.G + rr % D.G) * HD + 8 * g;
+#pragma unroll
+    for (int kk = 0; kk < NKK; ++kk) qf[kk] = *(const GLOBAL bf16x8*)(q + 16 * kk);
+  }
+  f32x16 oacc[NDB];
+#pragma unroll
+  for (int d = 0; d < NDB; ++d) oacc[d] = f32x16{};
+  float m = -INFINITY, lsum = 0.f;
+  bool bad = false;
+  const int seg = (PG_IDS << D.lp) - 64;                               // (k0 is a multiple of 64, which may be the middle of a page)
+  for (long long s0_ = p.k0; s0_ < p.k1; s0_ += seg) {
+    const int s0 = (int)s0_, s1 = (int)min((long long)p.k1, s0_ + seg), pg0 = s0 >> D.lp, nkb = (s1 - s0 + 63) >> 6;
+    __syncthreads();                                                   // the stages and numbers before are read
+    for (int e = tid(); e <= ((s1 - 1) >> D.lp) - pg0; e += KVM_THREADS) {
+      int id = tb[pg0 + e];
+      if ((unsigned)id >= (unsigned)D.pages) { bad = true; id = 0; }
+      sid[e] = id;
+    }
+    __syncthreads();
+    auto issue = [&](int blk) {
+      LDS uint16_t* d = lds + (blk % PG_NS) * ST;
+#pragma unroll
+      for (int q = 0; q < FL::NL; ++q) {
+        const int b = q * KVM_WAVES + wave(), u = 64 * b + l, r = u / FL::UPR, ph = u % FL::UPR, key = min(s0 + blk * FA_KB + r, klast);
+        const unsigned id = (unsigned)sid[(key >> D.lp) - pg0];
+        const GLOBAL char* ka = kb + ((unsigned long long)id * kpage + (unsigned)((key & pm) * kpitch + 16 * (ph ^ FL::kswz(r))));
+        const GLOBAL char* va = vb + ((unsigned long long)id * vpage + (unsigned)((key & pm) * vpitch + 16 * (ph ^ FL::tswz(r))));
+        dma16_at(ka, d + b * 512);
+        dma16_at(va, d + FA_KB * HD + b * 512);
+      }
+    };
+    auto scores = [&](int blk, f32x16 (&s)[2]) {
+      const LDS uint16_t* Ks = lds + (blk % PG_NS) * ST;
+#pragma unroll
+      for (int sb = 0; sb < 2; ++sb) {
+        s[sb] = f32x16{};
+#pragma unroll
+        for (int kk = 0; kk < NKK; ++kk) s[sb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(FL::frag_kc(Ks, sb * 32, kk), qf[kk], s[sb], 0, 0, 0);
+      }
+    };
+    auto step = [&](int kb_, f32x16 (&sa)[2], f32x16 (&sn)[2]) {
+      if (kb_ + 1 < nkb) wait_vm_c<0>();                               // block kb + 1 has landed
+      __syncthreads();
+      if (kb_ + 2 < nkb) issue(kb_ + 2);
+      const int key0 = s0 + kb_ * FA_KB;
+      if (!wave_on || key0 > wlast) return;                            // no row of the wave sees a key of the block
+      if (key0 + FA_KB - 1 > wfirst) {
+#pragma unroll
+        for (int sb = 0; sb < 2; ++sb)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (key0 + sb * 32 + 8 * (r >> 2) + 4 * g + (r & 3) > lim) sa[sb][r] = -INFINITY;
+      }
+      float mx = sa[0][0];
+#pragma unroll
+      for (int sb = 0; sb < 2; ++sb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sa[sb][r]);
+      mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * D.sl2;
+      if (__ballot(mx > m + 8.f)) {
+        const float top = fmaxf(m, mx), f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
+        lsum *= f;
+#pragma unroll
+        for (int d = 0; d < NDB; ++d) oacc[d] *= f;
+        m = top;
+      }
+      const float base = m == -INFINITY ? 0.f : m;
+      const LDS uint16_t* Kn = lds + ((kb_ + 1) % PG_NS) * ST;
+      const LDS uint16_t* Vs = lds + (kb_ % PG_NS) * ST + FA_KB * HD;
+      bf16x8 kfr[2][NKK], vfr[NDB][2][2];
+#pragma unroll
+      for (int sb = 0; sb < 2; ++sb)
+#pragma unroll
+        for (int kk = 0; kk < NKK; ++kk) kfr[sb][kk] = FL::frag_kc(Kn, sb * 32, kk);
+#pragma unroll
+      for (int d = 0; d < NDB; ++d)
+#pragma unroll
+        for (int sb = 0; sb < 2; ++sb)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) vfr[d][sb][u] = FL::frag_tr(Vs, d * 32, sb * 32 + 16 * u);
+      float ps = 0.f;
+      bf16x8 pf[2][2];
+#pragma unroll
+      for (int sb = 0; sb < 2; ++sb)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          float pv[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) pv[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sa[sb][8 * u + i], D.sl2, -base));
+          pf[sb][u] = pack_bf16(pv);
+          ps = sum_bf16(pf[sb][u], ps);
+        }
+#pragma unroll
+      for (int sb = 0; sb < 2; ++sb) {
+        sn[sb] = f32x16{};
+#pragma unroll
+        for (int kk = 0; kk < NKK; ++kk) sn[sb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kfr[sb][kk], qf[kk], sn[sb], 0, 0, 0);
+      }
+      lsum += ps + __shfl_xor(ps, 32, 64);
+#pragma unroll
+      for (int d = 0; d < NDB; ++d)
+#pragma unroll
+        for (int sb = 0; sb < 2; ++sb)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) oacc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vfr[d][sb][u], pf[sb][u], oacc[d], 0, 0, 0);
+    };
+    issue(0);
+    if (nkb > 1) issue(1);
+    wait_vm(nkb > 1 ? 2 * FL::NL : 0);
+    __syncthreads();
+    f32x16 sa[2], sn[2];
+    scores(0, sa);
+    int kb_ = 0;
+    for (; kb_ + 1 < nkb; kb_ += 2) { step(kb_, sa, sn); step(kb_ + 1, sn, sa); }
+    if (kb_ < nkb) step(kb_, sa, sn);
+  }
+  float nf = 0.f;
+#pragma unroll
+  for (int d = 0; d < NDB; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) nf += oacc[d][r] * 0.f;
+  nf += lsum * 0.f + (m == -INFINITY ? 0.f : m * 0.f);
+  if (__syncthreads_or(bad ? 1 : 0)) { if (tid() == 0) c.fail(KVM_ERR_OP_RANGE, t.b, p.k0); return PG_FAILED; }
+  if (__syncthreads_or(qok && nf != 0.f ? 1 : 0)) return PG_AGAIN;
+  if (qok) {
+    if (p.live == 1) {
+      const float inv = 1.f / lsum;
+      GLOBAL uint16_t* o = D.o.h() + paged_out(D, t, row) + 4 * g;
+#pragma unroll
+      for (int d = 0; d < NDB; ++d)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) stwt_bf4(o + d * 32 + 8 * q, oacc[d][4 * q] * inv, oacc[d][4 * q + 1] * inv, oacc[d][4 * q + 2] * inv, oacc[d][4 * q + 3] * inv);
+    } else {
+      GLOBAL float* y = paged_partial(D, p, p.k, row);
+#pragma unroll
+      for (int d = 0; d < NDB; ++d)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) stwt32(y + d * 32 + 8 * q + 4 * g + i, oacc[d][4 * q + i]);
+      if (g == 0) { stwt32(y + HD, m); stwt32(y + HD + 1, lsum); }
+    }
+  }
+  return PG_DONE;
+}
+
+template <int HD> __device__ __forceinline__ int attn_paged_fast(const Ctx& c, const TilePaged& t, const PiecePaged& p, int R, int kind) {
+  if (kind == 1) {
+    if (R <= 16) return attn_paged_keys_f32<HD, 1>(c, t.b, t.h, t.L, t.row0, t.tok0, t.ntok, p.k0, p.k1, p.k, p.live, p.i0);
+    if (R <= 32) return attn_paged_keys_f32<HD, 2>(c, t.b, t.h, t.L, t.row0, t.tok0, t.ntok, p.k0, p.k1, p.k, p.live, p.i0);
+    return PG_AGAIN;
+  }
+  if (R <= 16) return attn_paged_keys<HD, 1>(c, t.b, t.h, t.L, t.row0, t.tok0, t.ntok, p.k0, p.k1, p.k, p.live, p.i0);
+  if (R <= 32) return attn_paged_keys<HD, 2>(c, t.b, t.h, t.L, t.row0, t.tok0, t.ntok, p.k0, p.k1, p.k, p.live, p.i0);
+  return attn_paged_rows<HD>(c, t.b, t.h, t.L, t.row0, t.tok0, t.ntok, p.k0, p.k1, p.k, p.live, p.i0);
+}
 __device__ __noinline__ void op_attn_paged(const Ctx& c) {
   const AttnPaged D(c);
   LDS long long* pre = (LDS long long*)c.smem;                         // [PG_SEQS + 2]
@@ -488,8 +1013,8 @@ __device__ __noinline__ void op_attn_paged(const Ctx& c) {
   if (!paged_call_ok(c, D.cu, D.lens, D.B, min(D.q.rows, D.o.rows), (long long)D.table.cols << D.lp, scu)) return;
   WorkPaged W;
   W.pre = pre; W.cu = scu; W.len = len; W.B = D.B; W.Hkv = D.Hkv; W.G = D.G;
-  const bool fast = D.fast();
-  W.rows = fast ? D.tile : min(D.tile, max(32, D.G));                  // (the general form takes 32 rows at a time)
+  const int fast = D.fast();
+  W.rows = fast == 2 ? D.tile : min(D.tile, max(32, D.G));             // (the other forms take 32 rows at a time)
   {
     constexpr int PER = PG_SEQS / KVM_THREADS;
     long long cost[PER], sum = 0;
@@ -526,7 +1051,9 @@ __device__ __noinline__ void op_attn_paged(const Ctx& c) {
     const TilePaged t = W.find(x);
     const long long stop = min(end, t.start + t.cost);
     const PiecePaged p = W.piece(t, x, stop);
-    attn_paged_general(c, t.b, t.h, t.L, t.row0, t.tok0, t.ntok, p.k0, p.k1, p.k, p.live, p.i0);
+    int r = !fast ? PG_AGAIN : D.hd == 128 ? attn_paged_fast<128>(c, t, p, t.ntok * D.G, fast) : attn_paged_fast<64>(c, t, p, t.ntok * D.G, fast);
+    if (rfl(r) == PG_AGAIN) r = attn_paged_general(c, t.b, t.h, t.L, t.row0, t.tok0, t.ntok, p.k0, p.k1, p.k, p.live, p.i0);
+    if (rfl(r) == PG_FAILED) return;
     if (p.live > 1) paged_arrive(c, D, t, p, flag);
     __syncthreads();
     x = stop;
