@@ -60,28 +60,35 @@ struct AppendPagedLds {
   static constexpr int BYTES = 128 * 8 + AP_ROWS * 12 + (PG_SEQS + 4) * 4 + AP_ROWS * 256 * 4;
 };
 static_assert(AppendPagedLds::BYTES <= KVM_LDS_BYTES, "LDS");
-// Checks the call and the task's own pages (nothing is written before), then the frequencies; the rows that have a token end at `end`.
-__device__ __forceinline__ bool append_paged_begin(const Ctx& c, const AppendPaged& A, const AppendPagedLds& M, int& end) {
-  if (!paged_call_ok(c, A.cu, A.lens, A.B, A.rows(), (long long)A.table.cols << A.lp, M.cu)) return false;
-  end = min(A.r1, rfl(M.cu[A.B]));
-  bool bad = false;
-  for (int r = max(A.r0, rfl(M.cu[0])) + tid(); r < end; r += KVM_THREADS) {
-    int t; long long at;
-    if (!A.place(M.cu, r, t, at)) { bad = true; c.fail(KVM_ERR_OP_RANGE, r, t); }
+// Checks the call and the task's own pages (nothing is written before); the rows that have a token begin at `r` and end at `end`. Frequencies, and
+// positions and places of the first AP_ROWS rows, are in LDS then.
+__device__ __forceinline__ bool append_paged_begin(const Ctx& c, const AppendPaged& A, const AppendPagedLds& M, int& r, int& end) {
+  if (A.theta > 0.f && tid() >= KVM_THREADS - A.hd / 2) {              // (under the loads of what follows)
+    const int i = KVM_THREADS - 1 - tid();
+    M.freq[i] = q8_freq(i, A.hd, log((double)A.theta));
   }
-  if (A.theta > 0.f && tid() < A.hd / 2) M.freq[tid()] = q8_freq(tid(), A.hd, log((double)A.theta));
+  if (!paged_call_ok(c, A.cu, A.lens, A.B, A.rows(), (long long)A.table.cols << A.lp, M.cu)) return false;
+  r = max(A.r0, rfl(M.cu[0])); end = min(A.r1, rfl(M.cu[A.B]));
+  bool bad = false;
+  for (int u = r + tid(); u < end; u += KVM_THREADS) {
+    int t; long long at;
+    if (!A.place(M.cu, u, t, at)) { bad = true; c.fail(KVM_ERR_OP_RANGE, u, t); }
+    if (u < r + AP_ROWS) { M.pos[u - r] = t; M.at[u - r] = at; }
+  }
   return !__syncthreads_or(bad);
 }
-// Positions, places and angles of rows [r, r + nr).
-__device__ __forceinline__ void append_paged_rows(const AppendPaged& A, const AppendPagedLds& M, int r, int nr) {
+// Positions, places (the first rows' are there) and angles of rows [r, r + nr).
+__device__ __forceinline__ void append_paged_rows(const AppendPaged& A, const AppendPagedLds& M, int r, int nr, bool first) {
   const int half = A.hd / 2;
-  __syncthreads();
-  if (tid() < nr) {
-    int t; long long at;
-    A.place(M.cu, r + tid(), t, at);
-    M.pos[tid()] = t; M.at[tid()] = at;
+  if (!first) {
+    __syncthreads();
+    if (tid() < nr) {
+      int t; long long at;
+      A.place(M.cu, r + tid(), t, at);
+      M.pos[tid()] = t; M.at[tid()] = at;
+    }
+    __syncthreads();
   }
-  __syncthreads();
   if (A.theta > 0.f) {
     for (int e = tid(); e < nr * half; e += KVM_THREADS) {
       const int u = e / half, i = e % half;
@@ -95,12 +102,12 @@ __device__ __forceinline__ void append_paged_rows(const AppendPaged& A, const Ap
 __device__ __noinline__ void op_qkv_append_paged(const Ctx& c) {
   const AppendPaged A(c);
   const AppendPagedLds M(c.smem);
-  int end;
-  if (!append_paged_begin(c, A, M, end)) return;
+  int begin, end;
+  if (!append_paged_begin(c, A, M, begin, end)) return;
   const int half = A.hd / 2, heads = A.H + 2 * A.Hkv, l = lane();
-  for (int r = max(A.r0, rfl(M.cu[0])); r < end; r += AP_ROWS) {
+  for (int r = begin; r < end; r += AP_ROWS) {
     const int nr = min(AP_ROWS, end - r);
-    append_paged_rows(A, M, r, nr);
+    append_paged_rows(A, M, r, nr, r == begin);
     for (int u = wave(); u < nr * heads; u += KVM_WAVES) {
       const int row = u / heads, s = u % heads, what = s < A.H ? 0 : s < A.H + A.Hkv ? 1 : 2, h = what == 0 ? s : what == 1 ? s - A.H : s - A.H - A.Hkv;
       const View src = pick_view(what, A.q, A.k, A.v), dst = pick_view(what, A.qo, A.kc, A.vc), g = pick_view(what, A.qg, A.kg, View{nullptr, 0, 0, 0, 0});
@@ -132,15 +139,13 @@ __device__ __noinline__ void op_qkv_append_paged(const Ctx& c) {
 // Head sizes 64 and 128, rows in whole vectors, one type for the new rows and one for where they go. Bound: bytes for prompts, a few dependent
 // loads (row numbers, length, page, row) and the launch for single tokens. A (row, head) is HD / 8 lanes of 8 values; a row's angles are
 // computed once for all its heads; four items' loads are requested together.
-template <int HD> __device__ __noinline__ void append_paged_t(const Ctx& c) {
+template <int HD, bool FROM16> __device__ __noinline__ void append_paged_t(const Ctx& c) {
   constexpr int LPR = HD / 8, RPP = KVM_THREADS / LPR, NR = 4;
   const AppendPaged A(c);
   const AppendPagedLds M(c.smem);
-  int end;
-  if (!append_paged_begin(c, A, M, end)) return;
   const int ln = tid() % LPR, rw = tid() / LPR;
   const unsigned heads = A.H + 2 * A.Hkv;
-  const bool from16 = A.k.dtype == 2, to16 = A.kc.dtype == 2, qn = A.qg.ok(), kn = A.kg.ok(), turn = A.theta > 0.f;
+  const bool to16 = A.kc.dtype == 2, qn = A.qg.ok(), kn = A.kg.ok(), turn = A.theta > 0.f;
   const float sign = ln >= LPR / 2 ? 1.f : -1.f;
   float qg[8], kg[8];
 #pragma unroll
@@ -151,28 +156,32 @@ template <int HD> __device__ __noinline__ void append_paged_t(const Ctx& c) {
     const int row = (int)((unsigned)u / heads), s = u - row * (int)heads, what = s < A.H ? 0 : s < A.H + A.Hkv ? 1 : 2;
     return Item{row, what, s - (what == 0 ? 0 : what == 1 ? A.H : A.H + A.Hkv)};
   };
-  for (int r = max(A.r0, rfl(M.cu[0])); r < end; r += AP_ROWS) {
-    const int nr = min(AP_ROWS, end - r), items = nr * (int)heads;
-    Raw8 raw[NR];
-    auto request = [&](int u0) {
+  Raw8 raw[NR];
+  auto request = [&](int r, int items, int u0) {
 #pragma unroll
       for (int i = 0; i < NR; ++i) {
         const Item t = item(min(u0 + i * RPP, items - 1));
         const View x = pick_view(t.what, A.q, A.k, A.v);
-        raw[i].load(View{x.p, 0, x.cols, from16 ? 2 : 0, 0}, (long long)(r + t.row) * x.cols + t.h * HD + 8 * ln);
+        raw[i].load(View{x.p, 0, x.cols, FROM16 ? 2 : 0, 0}, (long long)(r + t.row) * x.cols + t.h * HD + 8 * ln);
       }
-    };
-    request(rw);                                                       // under the positions and angles
-    append_paged_rows(A, M, r, nr);
+  };
+  if (A.r0 >= A.r1) return;
+  request(A.r0, min(AP_ROWS, A.r1 - A.r0) * (int)heads, rw);           // the first rows, before it is known whose they are
+  int begin, end;
+  if (!append_paged_begin(c, A, M, begin, end)) return;
+  for (int r = begin; r < end; r += AP_ROWS) {
+    const int nr = min(AP_ROWS, end - r), items = nr * (int)heads;
+    if (r != A.r0) request(r, items, rw);
+    append_paged_rows(A, M, r, nr, r == begin);
     for (int u0 = rw; u0 < items; u0 += NR * RPP) {
-      if (u0 != rw) request(u0);
+      if (u0 != rw) request(r, items, u0);
 #pragma unroll
       for (int i = 0; i < NR; ++i) {
         const int u = u0 + i * RPP;
         if (u >= items) break;
         const Item t = item(u);
         float x[8];
-        raw[i].get(from16, x);
+        raw[i].get(FROM16, x);
         if (t.what == 0 ? qn : t.what == 1 && kn) {
           float ss = 0.f;
 #pragma unroll
@@ -198,8 +207,9 @@ __device__ __noinline__ bool op_qkv_append_paged_fast(const Ctx& c) {
   const View q = c.buf(0), k = c.buf(1), v = c.buf(2), qo = c.buf(3), kc = c.buf(4), vc = c.buf(5);
   if ((q.ok() && (!rows8_ok(q) || !rows8_ok(qo) || q.dtype != k.dtype || qo.dtype != kc.dtype)) || v.dtype != k.dtype || vc.dtype != kc.dtype) return false;
   if (!rows8_ok(k) || !rows8_ok(v) || !rows8_ok(kc) || !rows8_ok(vc)) return false;
-  if (c.i(16) == 128) append_paged_t<128>(c);
-  else if (c.i(16) == 64) append_paged_t<64>(c);
+  const bool half = k.dtype == 2;
+  if (c.i(16) == 128) { if (half) append_paged_t<128, true>(c); else append_paged_t<128, false>(c); }
+  else if (c.i(16) == 64) { if (half) append_paged_t<64, true>(c); else append_paged_t<64, false>(c); }
   else return false;
   return true;
 }
@@ -219,7 +229,8 @@ struct AttnPaged {
   __device__ int fast() const {
     const int t = q.dtype;
     if (kc.dtype != t || vc.dtype != t || o.dtype != t || (hd != 64 && hd != 128) || !rows8_ok(q) || !rows8_ok(kc) || !rows8_ok(vc) || !rows8_ok(o)) return 0;
-    return (long long)Hkv * page * max(kc.cols, vc.cols) * 4 >= 0x7fffff00ll ? 0 : t == 2 ? 2 : 1;
+    if ((part.cols & 1) || ((uintptr_t)part.p & 7) || (long long)Hkv * page * max(kc.cols, vc.cols) * 4 >= 0x7fffff00ll) return 0;   // (partial rows as pairs of words)
+    return t == 2 ? 2 : 1;
   }
 };
 // A tile's rows: row r is token tok0 + r / G of the sequence's new ones, head h * G + r % G; it sees keys 0 .. L + tok0 + r / G.
@@ -294,73 +305,79 @@ __device__ __forceinline__ GLOBAL float* paged_partial(const AttnPaged& D, const
 __device__ __forceinline__ long long paged_out(const AttnPaged& D, const TilePaged& t, int r) {
   return (long long)(t.row0 + r / D.G) * D.o.cols + (long long)(t.h * D.G + r % D.G) * D.hd;
 }
-// The piece that counts itself last merges the tile's rows; maxima are in units of log2. Weights: all pieces' maxima and sums go through LDS,
-// up to 8192 at a time; then a thread has four dims of a row, or a share of the pieces of them where there are threads enough.
-__device__ __noinline__ void paged_merge(const Ctx& c, int row0_, int h_, int ntok_, int live_, int i0_) {
-  const AttnPaged D(c);
-  const int live = rfl(live_), R = rfl(ntok_) * D.G, hd = D.hd;
-  const TilePaged t{0, rfl(h_), 0, rfl(row0_), 0, rfl(ntok_), 0, 0};
-  const PiecePaged p{0, 0, 0, live, rfl(i0_)};
-  LDS float* M = (LDS float*)(c.smem + PG_WORK);                       // [128] maxima, [128] sums
-  LDS float* Z = M + 128;
-  LDS float* ml = Z + 128;                                             // [pieces][R][2]
-  const int PB = 8192 / R;
-  for (int k0 = 0; k0 < live; k0 += PB) {
-    const int n = min(PB, live - k0);
-    __syncthreads();
-    for (int e = tid(); e < n * R; e += KVM_THREADS) {
-      const GLOBAL float* y = paged_partial(D, p, k0 + e / R, e % R) + hd;
-      ml[2 * e] = y[0]; ml[2 * e + 1] = y[1];
-    }
-    __syncthreads();
-    if (tid() < R) {
-      float m = k0 ? M[tid()] : -INFINITY, z = k0 ? Z[tid()] : 0.f, top = m;
-      for (int k = 0; k < n; ++k) top = fmaxf(top, ml[2 * (k * R + tid())]);
-      const float base = top == -INFINITY ? 0.f : top;
-      z *= exp2f(m - base);
-      for (int k = 0; k < n; ++k) z += exp2f(ml[2 * (k * R + tid())] - base) * ml[2 * (k * R + tid()) + 1];
-      M[tid()] = top; Z[tid()] = z;
-    }
-  }
-  __syncthreads();
-  const int C4 = (hd + 3) >> 2, items = R * C4, split = items >= KVM_THREADS ? 1 : min(live, KVM_THREADS / items);
+// The piece that counts itself last merges the tile's rows; maxima are in units of log2. First the rows' maxima and sums, eight lanes to a row and
+// eight pieces at a time; then a thread has four dims of a row, or a share of the pieces of them where there are threads enough, the loads of U
+// pieces in flight.
+template <int U> __device__ __forceinline__ void paged_merge_dims(const AttnPaged& D, const TilePaged& t, const PiecePaged& p, int R, const LDS float* M, const LDS float* Z, LDS float* sum) {
+  const int hd = D.hd, C4 = (hd + 3) >> 2, items = R * C4, split = items >= KVM_THREADS ? 1 : min(p.live, KVM_THREADS / items);
   for (int e0 = 0; e0 < items; e0 += KVM_THREADS) {
     const int e = split > 1 ? tid() % items : e0 + tid(), g = split > 1 ? tid() / items : 0;
     const bool on = e < items && g < split;
     const int r = on ? e / C4 : 0, d = on ? 4 * (e % C4) : 0, nd = min(4, hd - d);
     float a[4] = {0.f, 0.f, 0.f, 0.f};
-    constexpr int U = 8;
-    for (int k0 = on ? g : live; k0 < live; k0 += U * split) {
+    for (int k0 = on ? g : p.live; k0 < p.live; k0 += U * split) {
       float m[U], x[U][4];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const GLOBAL float* y = paged_partial(D, p, min(k0 + u * split, live - 1), r);
+        const GLOBAL float* y = paged_partial(D, p, min(k0 + u * split, p.live - 1), r);
         m[u] = y[hd];
 #pragma unroll
         for (int i = 0; i < 4; ++i) x[u][i] = y[d + min(i, nd - 1)];
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const float w = k0 + u * split < live && m[u] != -INFINITY ? exp2f(m[u] - M[r]) : 0.f;
+        const float w = k0 + u * split < p.live && m[u] != -INFINITY ? exp2f(m[u] - M[r]) : 0.f;
         if (w != 0.f)
 #pragma unroll
           for (int i = 0; i < 4; ++i) a[i] += w * x[u][i];
       }
     }
     if (split > 1) {
-      __syncthreads();
       if (on)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) ml[4 * tid() + i] = a[i];
+        for (int i = 0; i < 4; ++i) sum[4 * tid() + i] = a[i];
       __syncthreads();
       if (on && g == 0)
         for (int s = 1; s < split; ++s)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) a[i] += ml[4 * (tid() + s * items) + i];
+          for (int i = 0; i < 4; ++i) a[i] += sum[4 * (tid() + s * items) + i];
     }
     if (on && g == 0)
       for (int i = 0; i < nd; ++i) D.o.st(paged_out(D, t, r) + d + i, a[i] / Z[r]);
   }
+}
+__device__ __noinline__ void paged_merge(const Ctx& c, int row0_, int h_, int ntok_, int live_, int i0_) {
+  const AttnPaged D(c);
+  const int live = rfl(live_), R = rfl(ntok_) * D.G;
+  const TilePaged t{0, rfl(h_), 0, rfl(row0_), 0, rfl(ntok_), 0, 0};
+  const PiecePaged p{0, 0, 0, live, rfl(i0_)};
+  LDS float* M = (LDS float*)(c.smem + PG_WORK);                       // [128] maxima, [128] sums, [1024]
+  LDS float* Z = M + 128;
+  for (int r0 = 0; r0 < R; r0 += KVM_THREADS / 8) {
+    const int r = r0 + (tid() >> 3), sub = tid() & 7;
+    float m = -INFINITY, z = 0.f;
+    for (int k0 = sub; k0 < live; k0 += 32) {
+      float x[4], y[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const GLOBAL float* v = paged_partial(D, p, min(k0 + 8 * u, live - 1), min(r, R - 1)) + D.hd;
+        x[u] = v[0]; y[u] = v[1];
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (k0 + 8 * u < live && x[u] != -INFINITY) {
+          const float top = x[u] > m || x[u] != x[u] ? x[u] : m;
+          z = (m == -INFINITY ? 0.f : z * exp2f(m - top)) + exp2f(x[u] - top) * y[u];
+          m = top;
+        }
+    }
+    const float top = lanes_max<8>(m), f = m == -INFINITY ? 0.f : exp2f(m - top);
+    z = lanes_sum<8>(f * z);
+    if (sub == 0 && r < R) { M[r] = top; Z[r] = z; }
+  }
+  __syncthreads();
+  if (live <= 4) paged_merge_dims<4>(D, t, p, R, M, Z, Z + 128);
+  else paged_merge_dims<16>(D, t, p, R, M, Z, Z + 128);
 }
 __device__ __forceinline__ void paged_arrive(const Ctx& c, const AttnPaged& D, const TilePaged& t, const PiecePaged& p, LDS int* flag) {
   wait_stores();
@@ -557,8 +574,7 @@ __device__ __forceinline__ int paged_waves(const Ctx& c, const AttnPaged& D, con
     }
     else {
       GLOBAL float* y = paged_partial(D, p, p.k, r);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) stwt32(y + d + i, a[i]);
+      stwt_f4(y + d, a);
       if (d == 0) { stwt32(y + HD, top); stwt32(y + HD + 1, z); }
     }
   }
@@ -818,15 +834,36 @@ template <int HD, int NT> __device__ __noinline__ int attn_paged_keys_f32(const 
   return paged_waves<HD, NT, false>(c, D, t, p, acc, m, ls, bad);
 }
 
-// Tiles of up to 128 rows (chunks of prompts): bound by the matrix units and the vector work of the softmax. A wave has 32 rows; blocks of 64 keys
-// come from the pages straight into LDS for all of them, three stages, the page numbers of up to PG_IDS pages in LDS. In transposed space as
-// attn_fwd_mfma: S^T = K Q^T (a lane owns a query row), O^T += V^T P^T with P^T's registers as they are; the scores of the next block under the
-// softmax of this one.
+// Tiles of up to 128 rows (chunks of prompts): bound by the matrix units, the vector work of the softmax and LDS alike. A wave has 32 rows; blocks of
+// 64 keys come from the pages straight into LDS for all of them, three stages, the places of up to PG_IDS pieces of pages in LDS. In transposed
+// space: S^T = K Q^T by v_mfma_f32_32x32x16_bf16 (a lane owns a query row), O^T += V^T P^T with P^T's registers as they are. V lies row by row;
+// a lane reads HD / 32 dims of 8 keys and turns them in registers (a byte permute for two values), dims HD / 32 * m + i to row m of product i:
+// transposing reads of LDS run at a third of the rate. 32 keys at a time, the scores of the next ones under the softmax of these: with 64 the
+// fragments and scores under way pass 256 registers.
 constexpr int PG_IDS = 2048, PG_NS = 3;
-__device__ __forceinline__ void dma16_at(const GLOBAL char* src, const LDS void* dst) {   // 16 bytes a lane from its own address to dst + 16 * lane
+__device__ __forceinline__ void dma16_at(unsigned long long src, const LDS void* dst) {   // 16 bytes a lane from its own address to dst + 16 * lane
   const int m = __builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)dst);
   asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" :: "s"(m), "v"(src) : "memory", "m0");
 }
+// 8 keys of HD / 32 dims each (HD 128: 4 in two words; 64: 2 in one) as HD / 32 operands of 8 keys.
+template <int HD> struct VTurn {
+  static constexpr int NW = HD / 64;
+  uint32_t w[8][NW];
+  __device__ __forceinline__ void read(const LDS uint16_t* v, int key0, int g, int m) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const LDS uint16_t* y = v + (key0 + 8 * (j >> 2) + 4 * g + (j & 3)) * HD + 2 * NW * m;
+      if constexpr (NW == 2) { const u32x2_t x = *(const LDS u32x2_t*)y; w[j][0] = x.x; w[j][1] = x.y; }
+      else w[j][0] = *(const LDS uint32_t*)y;
+    }
+  }
+  __device__ __forceinline__ bf16x8 turned(int d) const {
+    u32x4_t r;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) r[j] = __builtin_amdgcn_perm(w[2 * j + 1][d >> 1], w[2 * j][d >> 1], d & 1 ? 0x07060302u : 0x05040100u);
+    return __builtin_bit_cast(bf16x8, r);
+  }
+};
 template <int HD> __device__ __noinline__ int attn_paged_rows(const Ctx& c, int b_, int h_, int L_, int row0_, int tok0_, int ntok_, int k0_, int k1_, int k_, int live_, int i0_) {
   typedef FaL<HD> FL;
   constexpr int NKK = HD / 16, NDB = HD / 32, ST = 2 * FA_KB * HD;
@@ -834,15 +871,16 @@ template <int HD> __device__ __noinline__ int attn_paged_rows(const Ctx& c, int 
   const AttnPaged D(c);
   const TilePaged t{rfl(b_), rfl(h_), rfl(L_), rfl(row0_), rfl(tok0_), rfl(ntok_), 0, 0};
   const PiecePaged p{rfl(k0_), rfl(k1_), rfl(k_), rfl(live_), rfl(i0_)};
-  const int w = rfl(wave()), l = lane(), g = l >> 5, qi = l & 31, R = t.ntok * D.G, row = 32 * w + qi, rr = min(row, R - 1), klast = p.k1 - 1;
+  const int w = rfl(wave()), l = lane(), g = l >> 5, qi = l & 31, R = t.ntok * D.G, row = 32 * w + qi, rr = min(row, R - 1);
   const bool qok = row < R, wave_on = 32 * w < R;
   const int lim = t.L + t.tok0 + rr / D.G;
   const int wfirst = rfl(t.L + t.tok0 + min(32 * w, R - 1) / D.G), wlast = rfl(t.L + t.tok0 + min(32 * w + 31, R - 1) / D.G);
   const GLOBAL int* tb = D.table.i() + (long long)t.b * D.table.cols;
-  const GLOBAL char* kb = (const GLOBAL char*)D.kc.p + (((long long)t.h << D.lp) * D.kc.cols) * 2;
-  const GLOBAL char* vb = (const GLOBAL char*)D.vc.p + (((long long)t.h << D.lp) * D.vc.cols) * 2;
-  const unsigned kpage = (unsigned)(D.Hkv << D.lp) * D.kc.cols * 2, vpage = (unsigned)(D.Hkv << D.lp) * D.vc.cols * 2;
-  const int pm = D.page - 1, kpitch = D.kc.cols * 2, vpitch = D.vc.cols * 2;
+  // a piece of a page is up to 64 tokens: number v = (page * Hkv) * (pieces of a page) + piece lies v * (piece's bytes) behind kb and vb
+  const int lsub = min(D.lp, 6), kpitch = D.kc.cols * 2, vpitch = D.vc.cols * 2;
+  const unsigned ksub = (unsigned)kpitch << lsub, vsub = (unsigned)vpitch << lsub;
+  const unsigned long long kb = (unsigned long long)(uintptr_t)D.kc.p + ((unsigned long long)t.h << D.lp) * kpitch;
+  const unsigned long long vb = (unsigned long long)(uintptr_t)D.vc.p + ((unsigned long long)t.h << D.lp) * vpitch;
   LDS int* sid = (LDS int*)(c.smem + PG_WORK);
   LDS uint16_t* lds = (LDS uint16_t*)(sid + PG_IDS);
   bf16x8 qf[NKK];
@@ -856,55 +894,41 @@ template <int HD> __device__ __noinline__ int attn_paged_rows(const Ctx& c, int 
   for (int d = 0; d < NDB; ++d) oacc[d] = f32x16{};
   float m = -INFINITY, lsum = 0.f;
   bool bad = false;
-  const int seg = (PG_IDS << D.lp) - 64;                               // (k0 is a multiple of 64, which may be the middle of a page)
+  const int seg = PG_IDS << lsub;
   for (long long s0_ = p.k0; s0_ < p.k1; s0_ += seg) {
-    const int s0 = (int)s0_, s1 = (int)min((long long)p.k1, s0_ + seg), pg0 = s0 >> D.lp, nkb = (s1 - s0 + 63) >> 6;
-    __syncthreads();                                                   // the stages and numbers before are read
-    for (int e = tid(); e <= ((s1 - 1) >> D.lp) - pg0; e += KVM_THREADS) {
-      int id = tb[pg0 + e];
+    const int s0 = (int)s0_, s1 = (int)min((long long)p.k1, s0_ + seg), nkb = (s1 - s0 + 63) >> 6, last = s1 - 1 - s0;
+    __syncthreads();                                                   // the stages and places before are read
+    for (int e = tid(); e <= last >> lsub; e += KVM_THREADS) {
+      const int key = s0 + (e << lsub);
+      int id = tb[key >> D.lp];
       if ((unsigned)id >= (unsigned)D.pages) { bad = true; id = 0; }
-      sid[e] = id;
+      sid[e] = ((id * D.Hkv) << (D.lp - lsub)) + ((key & (D.page - 1)) >> lsub);
     }
     __syncthreads();
+    // (keys behind the last one: the last one again, not seen)
     auto issue = [&](int blk) {
       LDS uint16_t* d = lds + (blk % PG_NS) * ST;
+      const bool whole = blk * FA_KB + FA_KB - 1 <= last;
 #pragma unroll
       for (int q = 0; q < FL::NL; ++q) {
-        const int b = q * KVM_WAVES + wave(), u = 64 * b + l, r = u / FL::UPR, ph = u % FL::UPR, key = min(s0 + blk * FA_KB + r, klast);
-        const unsigned id = (unsigned)sid[(key >> D.lp) - pg0];
-        const GLOBAL char* ka = kb + ((unsigned long long)id * kpage + (unsigned)((key & pm) * kpitch + 16 * (ph ^ FL::kswz(r))));
-        const GLOBAL char* va = vb + ((unsigned long long)id * vpage + (unsigned)((key & pm) * vpitch + 16 * (ph ^ FL::tswz(r))));
-        dma16_at(ka, d + b * 512);
-        dma16_at(va, d + FA_KB * HD + b * 512);
+        const int b = q * KVM_WAVES + w, u = 64 * b + l, r = u / FL::UPR, ph = u % FL::UPR;
+        const int key = whole ? blk * FA_KB + r : min(blk * FA_KB + r, last), at = key & ((1 << lsub) - 1);
+        const unsigned v = (unsigned)sid[key >> lsub];
+        dma16_at((kb + (unsigned)(at * kpitch + 16 * (ph ^ FL::kswz(r)))) + (unsigned long long)v * ksub, d + b * 512);
+        dma16_at((vb + (unsigned)(at * vpitch + 16 * ph)) + (unsigned long long)v * vsub, d + FA_KB * HD + b * 512);
       }
     };
-    auto scores = [&](int blk, f32x16 (&s)[2]) {
-      const LDS uint16_t* Ks = lds + (blk % PG_NS) * ST;
+    // Keys [key0, key0 + 32): scores sa, values at Vs (keys of the block from vk on); the scores of the next 32, keys from nk on at Kn, to sn.
+    auto step = [&](int key0, const LDS uint16_t* Vs, int vk, const LDS uint16_t* Kn, int nk, f32x16& sa, f32x16& sn) {
+      if (!wave_on || key0 > wlast) return;                            // no row of the wave sees a key of these
+      if (key0 + 31 > wfirst) {
 #pragma unroll
-      for (int sb = 0; sb < 2; ++sb) {
-        s[sb] = f32x16{};
-#pragma unroll
-        for (int kk = 0; kk < NKK; ++kk) s[sb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(FL::frag_kc(Ks, sb * 32, kk), qf[kk], s[sb], 0, 0, 0);
+        for (int r = 0; r < 16; ++r)
+          if (key0 + 8 * (r >> 2) + 4 * g + (r & 3) > lim) sa[r] = -INFINITY;
       }
-    };
-    auto step = [&](int kb_, f32x16 (&sa)[2], f32x16 (&sn)[2]) {
-      if (kb_ + 1 < nkb) wait_vm_c<0>();                               // block kb + 1 has landed
-      __syncthreads();
-      if (kb_ + 2 < nkb) issue(kb_ + 2);
-      const int key0 = s0 + kb_ * FA_KB;
-      if (!wave_on || key0 > wlast) return;                            // no row of the wave sees a key of the block
-      if (key0 + FA_KB - 1 > wfirst) {
+      float mx = sa[0];
 #pragma unroll
-        for (int sb = 0; sb < 2; ++sb)
-#pragma unroll
-          for (int r = 0; r < 16; ++r)
-            if (key0 + sb * 32 + 8 * (r >> 2) + 4 * g + (r & 3) > lim) sa[sb][r] = -INFINITY;
-      }
-      float mx = sa[0][0];
-#pragma unroll
-      for (int sb = 0; sb < 2; ++sb)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sa[sb][r]);
+      for (int r = 1; r < 16; ++r) mx = fmaxf(mx, sa[r]);
       mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * D.sl2;
       if (__ballot(mx > m + 8.f)) {
         const float top = fmaxf(m, mx), f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
@@ -914,81 +938,75 @@ template <int HD> __device__ __noinline__ int attn_paged_rows(const Ctx& c, int 
         m = top;
       }
       const float base = m == -INFINITY ? 0.f : m;
-      const LDS uint16_t* Kn = lds + ((kb_ + 1) % PG_NS) * ST;
-      const LDS uint16_t* Vs = lds + (kb_ % PG_NS) * ST + FA_KB * HD;
-      bf16x8 kfr[2][NKK], vfr[NDB][2][2];
+      bf16x8 kfr[NKK];
+      VTurn<HD> vt[2];
 #pragma unroll
-      for (int sb = 0; sb < 2; ++sb)
+      for (int kk = 0; kk < NKK; ++kk) kfr[kk] = FL::frag_kc(Kn, nk, kk);
 #pragma unroll
-        for (int kk = 0; kk < NKK; ++kk) kfr[sb][kk] = FL::frag_kc(Kn, sb * 32, kk);
-#pragma unroll
-      for (int d = 0; d < NDB; ++d)
-#pragma unroll
-        for (int sb = 0; sb < 2; ++sb)
-#pragma unroll
-          for (int u = 0; u < 2; ++u) vfr[d][sb][u] = FL::frag_tr(Vs, d * 32, sb * 32 + 16 * u);
+      for (int u = 0; u < 2; ++u) vt[u].read(Vs, vk + 16 * u, g, qi);
+      bf16x8 pf[2];
       float ps = 0.f;
-      bf16x8 pf[2][2];
 #pragma unroll
-      for (int sb = 0; sb < 2; ++sb)
+      for (int u = 0; u < 2; ++u) {
+        float pv[8];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          float pv[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) pv[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sa[sb][8 * u + i], D.sl2, -base));
-          pf[sb][u] = pack_bf16(pv);
-          ps = sum_bf16(pf[sb][u], ps);
-        }
-#pragma unroll
-      for (int sb = 0; sb < 2; ++sb) {
-        sn[sb] = f32x16{};
-#pragma unroll
-        for (int kk = 0; kk < NKK; ++kk) sn[sb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kfr[sb][kk], qf[kk], sn[sb], 0, 0, 0);
+        for (int i = 0; i < 8; ++i) pv[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sa[8 * u + i], D.sl2, -base));
+        pf[u] = pack_bf16(pv);
+        ps = sum_bf16(pf[u], ps);
       }
-      lsum += ps + __shfl_xor(ps, 32, 64);
+      sn = f32x16{};
 #pragma unroll
-      for (int d = 0; d < NDB; ++d)
+      for (int kk = 0; kk < NKK; ++kk) sn = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kfr[kk], qf[kk], sn, 0, 0, 0);
+      lsum += ps;
 #pragma unroll
-        for (int sb = 0; sb < 2; ++sb)
+      for (int u = 0; u < 2; ++u)
 #pragma unroll
-          for (int u = 0; u < 2; ++u) oacc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vfr[d][sb][u], pf[sb][u], oacc[d], 0, 0, 0);
+        for (int d = 0; d < NDB; ++d) oacc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vt[u].turned(d), pf[u], oacc[d], 0, 0, 0);
     };
     issue(0);
     if (nkb > 1) issue(1);
     wait_vm(nkb > 1 ? 2 * FL::NL : 0);
     __syncthreads();
-    f32x16 sa[2], sn[2];
-    scores(0, sa);
-    int kb_ = 0;
-    for (; kb_ + 1 < nkb; kb_ += 2) { step(kb_, sa, sn); step(kb_ + 1, sn, sa); }
-    if (kb_ < nkb) step(kb_, sa, sn);
+    f32x16 sa = {}, sn;
+#pragma unroll
+    for (int kk = 0; kk < NKK; ++kk) sa = __builtin_amdgcn_mfma_f32_32x32x16_bf16(FL::frag_kc(lds, 0, kk), qf[kk], sa, 0, 0, 0);
+    for (int blk = 0; blk < nkb; ++blk) {
+      const LDS uint16_t* Ks = lds + (blk % PG_NS) * ST;
+      const LDS uint16_t* Kn = lds + ((blk + 1) % PG_NS) * ST;
+      step(s0 + blk * FA_KB, Ks + FA_KB * HD, 0, Ks, 32, sa, sn);
+      wait_vm_c<0>();                                                  // block blk + 1 has landed
+      __syncthreads();                                                 // ... everyone's, and every wave is past block blk - 1
+      if (blk + 2 < nkb) issue(blk + 2);
+      step(s0 + blk * FA_KB + 32, Ks + FA_KB * HD, 32, Kn, 0, sn, sa);
+    }
   }
-  float nf = 0.f;
+  lsum += __shfl_xor(lsum, 32, 64);
+  float nf = lsum * 0.f + (m == -INFINITY ? 0.f : m * 0.f);
 #pragma unroll
   for (int d = 0; d < NDB; ++d)
 #pragma unroll
     for (int r = 0; r < 16; ++r) nf += oacc[d][r] * 0.f;
-  nf += lsum * 0.f + (m == -INFINITY ? 0.f : m * 0.f);
   if (__syncthreads_or(bad ? 1 : 0)) { if (tid() == 0) c.fail(KVM_ERR_OP_RANGE, t.b, p.k0); return PG_FAILED; }
   if (__syncthreads_or(qok && nf != 0.f ? 1 : 0)) return PG_AGAIN;
-  if (qok) {
-    if (p.live == 1) {
-      const float inv = 1.f / lsum;
-      GLOBAL uint16_t* o = D.o.h() + paged_out(D, t, row) + 4 * g;
+  if (qok) {                                                           // registers r = 4 q .. 4 q + 3 of all products: 4 NDB dims in a row
+    const float inv = p.live == 1 ? 1.f / lsum : 1.f;
+    GLOBAL uint16_t* o = D.o.h() + paged_out(D, t, row);
+    GLOBAL float* y = paged_partial(D, p, p.k, row);
 #pragma unroll
-      for (int d = 0; d < NDB; ++d)
+    for (int q = 0; q < 4; ++q) {
+      const int d0 = NDB * (8 * q + 4 * g);
+      float x[4 * NDB];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) stwt_bf4(o + d * 32 + 8 * q, oacc[d][4 * q] * inv, oacc[d][4 * q + 1] * inv, oacc[d][4 * q + 2] * inv, oacc[d][4 * q + 3] * inv);
-    } else {
-      GLOBAL float* y = paged_partial(D, p, p.k, row);
+      for (int r = 0; r < 4; ++r)
 #pragma unroll
-      for (int d = 0; d < NDB; ++d)
+        for (int d = 0; d < NDB; ++d) x[NDB * r + d] = oacc[d][4 * q + r] * inv;
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) stwt32(y + d * 32 + 8 * q + 4 * g + i, oacc[d][4 * q + i]);
-      if (g == 0) { stwt32(y + HD, m); stwt32(y + HD + 1, lsum); }
+      for (int i = 0; i < 4 * NDB; i += 4) {
+        if (p.live == 1) stwt_bf4(o + d0 + i, x[i], x[i + 1], x[i + 2], x[i + 3]);
+        else stwt_f4(y + d0 + i, f32x4n{x[i], x[i + 1], x[i + 2], x[i + 3]});
+      }
     }
+    if (p.live > 1 && g == 0) { stwt32(y + HD, m); stwt32(y + HD + 1, lsum); }
   }
   return PG_DONE;
 }

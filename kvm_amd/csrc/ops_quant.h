@@ -14,30 +14,33 @@ typedef int i32x16_t __attribute__((ext_vector_type(16)));
 // v of a row (x, RMS-normalised x, silu(x) * x2) in vectors of 8: thread t has vectors t, t + 256, ..
 struct RowsSrc {
   View x, x2, g; int K, pro; float eps;
-  __device__ bool vec() const { return rows8_ok(x) && (pro != 2 || rows8_ok(x2)) && (pro != 1 || vec_base(g)); }
-  template <bool VEC> __device__ __forceinline__ void load(const View& X, long long row, int j, float (&v)[8]) const {
+  // How x (and x2) can be read: 1, 2 vectors of f32 and of bf16, 0 element by element. A form of its own for each: a branch on the type between
+  // two loads makes each wait for the one before (a prompt's rows 4,001 x 4,096 59 us a call in place of NEWQ).
+  __device__ int form() const {
+    return rows8_ok(x) && (pro != 2 || (rows8_ok(x2) && x2.dtype == x.dtype)) && (pro != 1 || vec_base(g)) ? x.dtype == 2 ? 2 : 1 : 0;
+  }
+  template <int FORM> __device__ __forceinline__ void load(const View& X, long long row, int j, float (&v)[8]) const {
     const int n = K - 8 * j;                                           // values from here on
     const long long o = row * X.cols + 8 * j;
-    if (VEC) {
+    if (FORM) {
       Raw8 w;
-      w.load(X, o); w.get(X.dtype == 2, v);
-      if (n < 8)
+      w.load(View{X.p, 0, 0, FORM == 2 ? 2 : 0, 0}, o); w.get(FORM == 2, v);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = e < n ? v[e] : 0.f;
+      for (int e = 0; e < 8; ++e) v[e] = e < n ? v[e] : 0.f;
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = e < n ? X.ld(o + e) : 0.f;
     }
   }
   // x * rstd * gamma, or silu(x) * x2: rounded after each product
-  template <bool VEC> __device__ __forceinline__ void shape(float (&v)[8], long long row, int j, float rstd) const {
+  template <int FORM> __device__ __forceinline__ void shape(float (&v)[8], long long row, int j, float rstd) const {
     float y[8];
     if (pro == 1) {
-      load<VEC>(g, 0, j, y);
+      load<FORM ? 1 : 0>(g, 0, j, y);
 #pragma unroll
       for (int e = 0; e < 8; ++e) { const float t = v[e] * rstd; v[e] = t * y[e]; }
     } else if (pro == 2) {
-      load<VEC>(x2, row, j, y);
+      load<FORM>(x2, row, j, y);
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = silu_f(v[e]) * y[e];
     }
@@ -76,14 +79,14 @@ constexpr int Q8_RED = 12;     // doubles of LDS per row in flight
 // nr <= RB rows from r0 on, K <= 2048 NV, held in registers: one read of x, all its loads in flight together, one reduction for the norm
 // and one for the scale whatever RB is. put(i, j, w0, w1): vector j of row r0 + i as bytes; scaled(i, s). Sums of squares in double, so
 // that rstd is the f32 nearest to the exact one whatever the order.
-template <bool VEC, int NV, int RB, class Put, class Scaled>
+template <int FORM, int NV, int RB, class Put, class Scaled>
 __device__ __forceinline__ void q8_rows(const RowsSrc& S, long long r0, int nr, LDS double* red, Put put, Scaled scaled) {
   const int nvec = (S.K + 7) >> 3;
   float v[RB][NV][8];
 #pragma unroll
   for (int i = 0; i < RB; ++i)
 #pragma unroll
-    for (int u = 0; u < NV; ++u) S.load<VEC>(S.x, r0 + min(i, nr - 1), min(tid() + u * KVM_THREADS, nvec - 1), v[i][u]);
+    for (int u = 0; u < NV; ++u) S.load<FORM>(S.x, r0 + min(i, nr - 1), min(tid() + u * KVM_THREADS, nvec - 1), v[i][u]);
   double ss[RB] = {};
   if (S.pro == 1) {
 #pragma unroll
@@ -101,7 +104,7 @@ __device__ __forceinline__ void q8_rows(const RowsSrc& S, long long r0, int nr, 
     const float rstd = (float)(1.0 / sqrt(ss[i] / S.K + (double)S.eps));
 #pragma unroll
     for (int u = 0; u < NV; ++u) {
-      S.shape<VEC>(v[i][u], r0 + min(i, nr - 1), min(tid() + u * KVM_THREADS, nvec - 1), rstd);
+      S.shape<FORM>(v[i][u], r0 + min(i, nr - 1), min(tid() + u * KVM_THREADS, nvec - 1), rstd);
       big[i] = q8_big(v[i][u], big[i]);
     }
   }
@@ -120,14 +123,14 @@ __device__ __forceinline__ void q8_rows(const RowsSrc& S, long long r0, int nr, 
   }
 }
 // A row of any length, read three times.
-template <bool VEC, class Put, class Scaled>
+template <int FORM, class Put, class Scaled>
 __device__ __forceinline__ void q8_row_long(const RowsSrc& S, long long r, LDS double* red, Put put, Scaled scaled) {
   const int nvec = (S.K + 7) >> 3;
   double ss[1] = {};
   float v[8];
   if (S.pro == 1) {
     for (int j = tid(); j < nvec; j += KVM_THREADS) {
-      S.load<VEC>(S.x, r, j, v);
+      S.load<FORM>(S.x, r, j, v);
 #pragma unroll
       for (int e = 0; e < 8; ++e) ss[0] += (double)v[e] * (double)v[e];
     }
@@ -135,13 +138,13 @@ __device__ __forceinline__ void q8_row_long(const RowsSrc& S, long long r, LDS d
   }
   const float rstd = (float)(1.0 / sqrt(ss[0] / S.K + (double)S.eps));
   uint32_t big[1] = {};
-  for (int j = tid(); j < nvec; j += KVM_THREADS) { S.load<VEC>(S.x, r, j, v); S.shape<VEC>(v, r, j, rstd); big[0] = q8_big(v, big[0]); }
+  for (int j = tid(); j < nvec; j += KVM_THREADS) { S.load<FORM>(S.x, r, j, v); S.shape<FORM>(v, r, j, rstd); big[0] = q8_big(v, big[0]); }
   q8_rows_max<1>(big, red);
   const float s = q8_scale(__uint_as_float(big[0])), inv = s > 0.f ? 1.f / s : 0.f;
   if (tid() == 0) scaled(0, s);
   for (int j = tid(); j < nvec; j += KVM_THREADS) {
     uint32_t w0, w1;
-    S.load<VEC>(S.x, r, j, v); S.shape<VEC>(v, r, j, rstd);
+    S.load<FORM>(S.x, r, j, v); S.shape<FORM>(v, r, j, rstd);
     q8_pack(v, s, inv, w0, w1);
     put(0, j, w0, w1);
   }
@@ -149,7 +152,7 @@ __device__ __forceinline__ void q8_row_long(const RowsSrc& S, long long r, LDS d
 
 // Op 315. Bound: bytes (K * (2 to 8) read, K written a row). Four rows of up to 4,096 values at once, one of up to 16,384, so that the two
 // reductions' waits are shared.
-template <bool VEC, int NV> __device__ __noinline__ void rows_q8_t(const Ctx& c) {
+template <int FORM, int NV> __device__ __noinline__ void rows_q8_t(const Ctx& c) {
   constexpr int RB = NV == 2 ? 4 : 1;
   const RowsSrc S{uview(c, 0), uview(c, 1), uview(c, 2), rfl(c.i(7)), rfl(c.i(8)), c.f(9)};
   const View q = uview(c, 3), qs = uview(c, 4);
@@ -165,14 +168,16 @@ template <bool VEC, int NV> __device__ __noinline__ void rows_q8_t(const Ctx& c)
       if (j == nvec - 1 && (nvec & 1)) { word(p, 2 * nvec, 0); word(p, 2 * nvec + 1, 0); }   // up to the multiple of 16 bytes
     };
     auto scaled = [&](int i, float s) { stwt32(qs.f() + (r + i), s); };
-    if constexpr (NV > 0) q8_rows<VEC, NV, RB>(S, r, min(RB, r1 - r), red, put, scaled);
-    else q8_row_long<VEC>(S, r, red, put, scaled);
+    if constexpr (NV > 0) q8_rows<FORM, NV, RB>(S, r, min(RB, r1 - r), red, put, scaled);
+    else q8_row_long<FORM>(S, r, red, put, scaled);
   }
 }
 __device__ __noinline__ void op_rows_q8(const Ctx& c) {
   const RowsSrc S{c.buf(0), c.buf(1), c.buf(2), c.i(7), c.i(8), c.f(9)};
-  if (S.vec()) { if (S.K <= 4096) rows_q8_t<true, 2>(c); else if (S.K <= 16384) rows_q8_t<true, 8>(c); else rows_q8_t<true, 0>(c); }
-  else if (S.K <= 4096) rows_q8_t<false, 2>(c); else rows_q8_t<false, 0>(c);
+  const int form = rfl(S.form());
+  if (form == 2) { if (S.K <= 4096) rows_q8_t<2, 2>(c); else if (S.K <= 16384) rows_q8_t<2, 8>(c); else rows_q8_t<2, 0>(c); }
+  else if (form == 1) { if (S.K <= 4096) rows_q8_t<1, 2>(c); else if (S.K <= 16384) rows_q8_t<1, 8>(c); else rows_q8_t<1, 0>(c); }
+  else if (S.K <= 4096) rows_q8_t<0, 2>(c); else rows_q8_t<0, 0>(c);
 }
 
 // ---------------------------------------------------------------------------------------------- product tiles
@@ -254,7 +259,7 @@ __device__ __forceinline__ bf16x8 first_bytes(bf16x8 f, int n) {
 // alone: a byte of B meets a 0.
 template <int TM, int TN> __device__ __noinline__ void q8_tile(const Ctx& c) {
   constexpr int WM = TM / 2, WN = TN / 2, BM = WM / 32, BN = WN / 32, SA = TM * DK, SB = TN * DK, ST = SA + SB;
-  constexpr int NS = 4 * ST * 2 * 2 <= KVM_LDS_BYTES ? 8 : 4;
+  constexpr int NS = KVM_LDS_BYTES / (ST * 2) < 8 ? KVM_LDS_BYTES / (ST * 2) : 8;
   static_assert(NS * ST * 2 <= KVM_LDS_BYTES && TM * TN * 4 <= KVM_LDS_BYTES, "LDS");
   const TileQ8 g(c);
   const View A{g.a.p, g.a.rows, 2 * g.a.cols, 2, 0}, B{g.w.p, g.w.rows, 2 * g.w.cols, 2, 0};
@@ -396,62 +401,91 @@ struct GemvQ8 {
     out.st((long long)m * out.cols + n, y);
   }
 };
-// Row m's bytes [lo, lo + n) (n a multiple of 16, zeros behind K) to LDS at vs + m * pitch and the scales, for all rows.
-template <bool VEC, int NV> __device__ __noinline__ void gemv_q8_stage(const Ctx& c, LDS char* vs_, int pitch_, int lo_, int n_, LDS float* scale, LDS double* red) {
+// Where byte o (a multiple of 4) of row m's staged range lies: its 16-byte pieces swizzled by row, so that 16 rows' reads of one piece touch every
+// bank once without padding between the rows, which direct loads could not leave.
+__device__ __forceinline__ int gq_at(int m, int pitch, int o) { return m * pitch + (o ^ (m << 4)); }
+// Row m's bytes [lo, lo + n) (n a multiple of 256, zeros behind K) to LDS and the scales, for all rows.
+template <int FORM, int NV> __device__ __noinline__ void gemv_q8_stage(const Ctx& c, LDS char* vs_, int pitch_, int lo_, int n_, LDS float* scale, LDS double* red) {
   const int pitch = rfl(pitch_), lo = rfl(lo_), n = rfl(n_);
   const GemvQ8 G(c);
   const RowsSrc S{G.x, G.x2, G.g, G.K, G.pro, c.f(14)};
   for (int m = 0; m < G.M; ++m) {
-    LDS char* const vs = vs_ + m * pitch;
     auto put = [&](int, int j, uint32_t w0, uint32_t w1) {
       const int o = 8 * j - lo;
-      if (o >= 0 && o < n) { *(LDS uint32_t*)(vs + o) = w0; *(LDS uint32_t*)(vs + o + 4) = w1; }
+      if (o >= 0 && o < n) { *(LDS uint32_t*)(vs_ + gq_at(m, pitch, o)) = w0; *(LDS uint32_t*)(vs_ + gq_at(m, pitch, o + 4)) = w1; }
     };
     auto scaled = [&](int, float s) { scale[m] = s; };
-    if constexpr (NV > 0) q8_rows<VEC, NV, 1>(S, m, 1, red, put, scaled);
-    else q8_row_long<VEC>(S, m, red, put, scaled);
-    for (int o = max(0, ((G.K + 7) & ~7) - lo) + 4 * tid(); o < n; o += 4 * KVM_THREADS) *(LDS int*)(vs + o) = 0;
+    if constexpr (NV > 0) q8_rows<FORM, NV, 1>(S, m, 1, red, put, scaled);
+    else q8_row_long<FORM>(S, m, red, put, scaled);
+    for (int o = max(0, ((G.K + 7) & ~7) - lo) + 4 * tid(); o < n; o += 4 * KVM_THREADS) *(LDS int*)(vs_ + gq_at(m, pitch, o)) = 0;
   }
 }
 __device__ __forceinline__ void gemv_q8_rows(const Ctx& c, const GemvQ8& G, LDS char* vs, int pitch, int lo, int n, LDS float* scale, LDS double* red) {
-  if (G.pro == 3) {                                // words that are there already
-    for (int m = 0; m < G.M; ++m)
-      for (int o = 4 * tid(); o < n; o += 4 * KVM_THREADS) {
-        const int k = lo + o;
-        int v = k < G.K ? G.x.i()[(long long)m * G.x.cols + (k >> 2)] : 0;
-        if (G.K - k < 4 && k < G.K) v &= (int)(0xffffffffu >> (8 * (4 - (G.K - k))));
-        *(LDS int*)(vs + m * pitch + o) = v;
+  if (G.pro == 3) {                                // bytes that are there already
+    if (q8_fast(G.x, G.M, lo + n) && pitch == n) { // direct loads, 1 KiB a wave; what lies behind K is cleared once they have landed
+      const i32x4_t rs = dma_rsrc(G.x.p, (long long)G.x.rows * G.x.cols * 4);
+      for (int b = wave(); b < G.M * n / 1024; b += KVM_WAVES) {
+        const int o = 1024 * b + 16 * lane(), m = o / pitch;
+        dma16(rs, m * G.x.cols * 4 + lo + ((o - m * pitch) ^ (m << 4)), 0, vs + 1024 * b);
       }
+      for (int o = (G.M * n & ~1023) + 4 * tid(); o < G.M * n; o += 4 * KVM_THREADS) {   // half a block may be left
+        const int m = o / pitch, k = lo + ((o - m * pitch) ^ (m << 4));
+        *(LDS int*)(vs + o) = k < G.K ? G.x.i()[(long long)m * G.x.cols + (k >> 2)] : 0;
+      }
+      wait_vm_c<0>();
+      __syncthreads();
+      const int k0 = max(0, (G.K - lo) & ~3);
+      for (int m = 0; m < G.M; ++m)
+        for (int o = k0 + 4 * tid(); o < n; o += 4 * KVM_THREADS) {
+          LDS int* y = (LDS int*)(vs + gq_at(m, pitch, o));
+          *y = G.K - lo - o > 0 ? *y & (int)(0xffffffffu >> (8 * (4 - (G.K - lo - o)))) : 0;
+        }
+    } else {
+      for (int m = 0; m < G.M; ++m)
+        for (int o = 4 * tid(); o < n; o += 4 * KVM_THREADS) {
+          const int k = lo + o;
+          int v = k < G.K ? G.x.i()[(long long)m * G.x.cols + (k >> 2)] : 0;
+          if (G.K - k < 4 && k < G.K) v &= (int)(0xffffffffu >> (8 * (4 - (G.K - k))));
+          *(LDS int*)(vs + gq_at(m, pitch, o)) = v;
+        }
+    }
     if (tid() < G.M) scale[tid()] = G.sx.f()[tid()];
     return;
   }
   const RowsSrc S{G.x, G.x2, G.g, G.K, G.pro, 0.f};
-  if (S.vec()) {
-    if (G.K <= 4096) gemv_q8_stage<true, 2>(c, vs, pitch, lo, n, scale, red);
-    else if (G.K <= 16384) gemv_q8_stage<true, 8>(c, vs, pitch, lo, n, scale, red);
-    else gemv_q8_stage<true, 0>(c, vs, pitch, lo, n, scale, red);
-  } else if (G.K <= 4096) gemv_q8_stage<false, 2>(c, vs, pitch, lo, n, scale, red);
-  else gemv_q8_stage<false, 0>(c, vs, pitch, lo, n, scale, red);
+  const int form = rfl(S.form());
+  if (form == 2) {
+    if (G.K <= 4096) gemv_q8_stage<2, 2>(c, vs, pitch, lo, n, scale, red);
+    else if (G.K <= 16384) gemv_q8_stage<2, 8>(c, vs, pitch, lo, n, scale, red);
+    else gemv_q8_stage<2, 0>(c, vs, pitch, lo, n, scale, red);
+  } else if (form == 1) {
+    if (G.K <= 4096) gemv_q8_stage<1, 2>(c, vs, pitch, lo, n, scale, red);
+    else if (G.K <= 16384) gemv_q8_stage<1, 8>(c, vs, pitch, lo, n, scale, red);
+    else gemv_q8_stage<1, 0>(c, vs, pitch, lo, n, scale, red);
+  } else if (G.K <= 4096) gemv_q8_stage<0, 2>(c, vs, pitch, lo, n, scale, red);
+  else gemv_q8_stage<0, 0>(c, vs, pitch, lo, n, scale, red);
 }
-// LDS of one call with a ring of R steps a wave: [ring][rows: M x (2 KC + 16) bytes][scales][reductions][sums: 4 x GV_GRP x M x 16]. KC (pairs of
-// bytes): all of K when it fits, else the largest power of two from 4096 to 256 that divides K and does.
-struct GqGeo { int KC, pitch, vs, scale, red, part; };
-__device__ __forceinline__ GqGeo gq_geo(int Ke, int M, int R) {
-  const int rest = R * KVM_WAVES * GV_STEP + 64 + Q8_RED * 8 + KVM_WAVES * GV_GRP * M * 16 * 4;
-  int KC = Ke;
-  if (rest + M * (2 * Ke + 16) > KVM_LDS_BYTES)
-    for (KC = 4096; KC > 256 && (Ke % KC || rest + M * (2 * KC + 16) > KVM_LDS_BYTES); KC >>= 1) {}
+// LDS of one call with a ring of R steps a wave: [ring][rows: M x 2 KC bytes][scales][reductions][sums: 4 x blocks x M x 16], blocks the 16-output
+// blocks of the task, at most GV_GRP. KC (pairs of bytes): the largest part of K in whole steps of all waves that fits.
+struct GqGeo { int KC, pitch, vs, scale, red, part, grp; };
+__device__ __forceinline__ GqGeo gq_geo(int Ke, int M, int R, int n) {
   GqGeo g;
-  g.KC = KC; g.pitch = 2 * KC + 16;
+  g.grp = min((n + 15) >> 4, GV_GRP);
+  const int rest = R * KVM_WAVES * GV_STEP + 64 + Q8_RED * 8 + KVM_WAVES * g.grp * M * 16 * 4, steps = Ke >> 8;
+  int parts = 1;
+  while (parts < steps && (steps % parts || rest + M * (2 * Ke / parts) > KVM_LDS_BYTES)) ++parts;
+  g.KC = Ke / parts; g.pitch = 2 * g.KC;
   g.vs = R * KVM_WAVES * GV_STEP;
   g.scale = g.vs + M * g.pitch;
   g.red = g.scale + 64;
   g.part = g.red + Q8_RED * 8;
   return g;
 }
+static_assert(4 * KVM_WAVES * GV_STEP + 64 + Q8_RED * 8 + KVM_WAVES * GV_GRP * 16 * 16 * 4 + 16 * 512 <= KVM_LDS_BYTES, "LDS");
+static_assert(12 * KVM_WAVES * GV_STEP + 64 + Q8_RED * 8 + KVM_WAVES * GV_GRP * 4 * 16 * 4 + 4 * 512 <= KVM_LDS_BYTES, "LDS");
 template <int R> __device__ __forceinline__ void gemv_q8_prefetch_r(const GemvQ8& G, LDS char* smem) {
   GvStream<> ws;
-  ws.init(G.stream(), G.n0, G.n1, G.Ke, gq_geo(G.Ke, G.M, R).KC);
+  ws.init(G.stream(), G.n0, G.n1, G.Ke, gq_geo(G.Ke, G.M, R, G.n1 - G.n0).KC);
   LDS char* ring = smem + wave() * R * GV_STEP;
 #pragma unroll
   for (int j = 0; j < R; ++j) ws.template issue<R>(ring);
@@ -465,7 +499,7 @@ __device__ __noinline__ void gemv_q8_prefetch(const Ctx& c) {
 template <int R> __device__ __noinline__ void gemv_q8_stream(const Ctx& c) {
   const GemvQ8 G(c);
   const int M = G.M, K = G.Ke, PM = 16 * M;                                     // K in pairs of bytes
-  const GqGeo geo = gq_geo(K, M, R);
+  const GqGeo geo = gq_geo(K, M, R, G.n1 - G.n0);
   const int KC = geo.KC;
   LDS char* vs = c.smem + geo.vs;
   LDS float* scale = (LDS float*)(c.smem + geo.scale);
@@ -482,32 +516,33 @@ template <int R> __device__ __noinline__ void gemv_q8_stream(const Ctx& c) {
     for (int j = 0; j < R; ++j) ws.template issue<R>(ring);
   }
   const bool arow = (l & 15) < M;
-  const LDS char* va = vs + (arow ? (l & 15) : 0) * geo.pitch + 16 * (l >> 4);
+  const int vm = arow ? l & 15 : 0, vx = vm << 4;
+  const LDS char* va = vs + vm * geo.pitch;
   const LDS char* rl = ring + 16 * l;
   int cslot = 0;
   for (int g0 = 0; g0 < nrb; g0 += GV_GRP) {
     const int ng = min(GV_GRP, nrb - g0);
-    for (int e = l; e < ng * PM; e += 64) part[wv * GV_GRP * PM + e] = 0;
+    for (int e = l; e < ng * PM; e += 64) part[wv * geo.grp * PM + e] = 0;
     for (int kc = 0; kc < K; kc += KC) {
       const int kq = KC / 2, ns = KC / 256;                                      // bytes of a wave's quarter, its steps
       __syncthreads();
       if (KC != K || g0 == 0) gemv_q8_rows(c, G, vs, geo.pitch, 2 * kc, 2 * KC, scale, (LDS double*)(c.smem + geo.red));
       __syncthreads();
-      const LDS char* vk = va + wv * kq;
+      const int vk = wv * kq + 16 * (l >> 4);
       i32x4_t acc = {0, 0, 0, 0};
       int rb = 0, st = 0;
       for (int tt = 0; tt < ng * ns; ++tt) {                                     // one flat loop: no full wait at an inner loop's head
         wait_vm_c<2 * (R - 1)>();
         const LDS char* slot = rl + cslot * GV_STEP;
         const i32x4_t w0 = *(const LDS i32x4_t*)slot, w1 = *(const LDS i32x4_t*)(slot + 1024);
-        const i32x4_t a0 = *(const LDS i32x4_t*)(vk + st * 128), a1 = *(const LDS i32x4_t*)(vk + st * 128 + 64);
+        const i32x4_t a0 = *(const LDS i32x4_t*)(va + ((vk + st * 128) ^ vx)), a1 = *(const LDS i32x4_t*)(va + ((vk + st * 128 + 64) ^ vx));
         acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(arow ? a0 : i32x4_t{}, w0, acc, 0, 0, 0);
         acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(arow ? a1 : i32x4_t{}, w1, acc, 0, 0, 0);
         wait_lds();
         ws.template issue<R>(ring);
         cslot = cslot + 1 == R ? 0 : cslot + 1;
         if (++st == ns) {                                                        // D[m][n]: lane holds m = 4 (l / 16) + i, n = l % 16
-          LDS int* pp = part + (wv * GV_GRP + rb) * PM + (l & 15);
+          LDS int* pp = part + (wv * geo.grp + rb) * PM + (l & 15);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int m = 4 * (l >> 4) + i;
@@ -521,7 +556,7 @@ template <int R> __device__ __noinline__ void gemv_q8_stream(const Ctx& c) {
     __syncthreads();
     for (int e = tid(); e < ng * PM; e += KVM_THREADS) {
       const int rb = e / PM, m = (e / 16) % M, n = G.n0 + (g0 + rb) * 16 + e % 16;
-      if (n < G.n1) G.put(m, n, part[e] + part[GV_GRP * PM + e] + part[2 * GV_GRP * PM + e] + part[3 * GV_GRP * PM + e], scale[m]);
+      if (n < G.n1) G.put(m, n, part[e] + part[geo.grp * PM + e] + part[2 * geo.grp * PM + e] + part[3 * geo.grp * PM + e], scale[m]);
     }
     __syncthreads();                                                            // read before the next group clears them
   }
@@ -531,19 +566,19 @@ template <int R> __device__ __noinline__ void gemv_q8_stream(const Ctx& c) {
 __device__ __noinline__ void gemv_q8_simt(const Ctx& c) {
   const GemvQ8 G(c);
   constexpr int CH = 4096;
-  LDS char* vs = c.smem;                                                        // [16][CH + 16]
-  LDS float* scale = (LDS float*)(vs + 16 * (CH + 16));
+  LDS char* vs = c.smem;                                                        // [16][CH]
+  LDS float* scale = (LDS float*)(vs + 16 * CH);
   LDS double* red = (LDS double*)(scale + 16);
   for (int e0 = 0; e0 < (G.n1 - G.n0) * G.M; e0 += KVM_THREADS) {
     const int e = e0 + tid(), m = e % G.M, n = G.n0 + e / G.M;
     int s = 0;
     for (int k0 = 0; k0 < G.K; k0 += CH) {
       __syncthreads();
-      gemv_q8_rows(c, G, vs, CH + 16, k0, CH, scale, red);
+      gemv_q8_rows(c, G, vs, CH, k0, CH, scale, red);
       __syncthreads();
       const int nw = (min(CH, G.K - k0) + 3) >> 2;
       if (n < G.n1)
-        for (int k = 0; k < nw; ++k) s = __builtin_amdgcn_sdot4(*(const LDS int*)(vs + m * (CH + 16) + 4 * k), G.w.i()[(long long)n * G.w.cols + (k0 >> 2) + k], s, false);
+        for (int k = 0; k < nw; ++k) s = __builtin_amdgcn_sdot4(*(const LDS int*)(vs + gq_at(m, CH, 4 * k)), G.w.i()[(long long)n * G.w.cols + (k0 >> 2) + k], s, false);
     }
     if (n < G.n1) G.put(m, n, s, scale[m]);
   }
