@@ -195,54 +195,55 @@ struct TileQ8 {
     out.st((long long)m * out.cols + n, y);
   }
 };
-// The staged tile [TM][TN] of sums (16-byte pieces swizzled by row as in gemm_store): a lane has 4 columns, the waves take rows in turn, the
-// residual of 8 rows requested together.
-template <int TM, int TN, bool OBF> __device__ __noinline__ void q8_epilogue(const Ctx& c) {
-  constexpr int LPR = TN / 4, RPI = 64 / LPR < 1 ? 1 : 64 / LPR, NI = TM / KVM_WAVES / RPI, NB = NI < 8 ? NI : 8;
-  const TileQ8 g(c);
-  const LDS int* et = (const LDS int*)c.smem;
+// The staged tile [TM][TN] of sums times their rows' scales (16-byte pieces swizzled by row as in gemm_store): a lane has 4 columns, whose scales
+// (and bias) it brings; the waves take rows in turn. Without a residual nothing is loaded; with one, those of 8 rows are requested together.
+template <int TM, int TN, bool OBF, bool RES> __device__ __forceinline__ void q8_rows_out(const TileQ8& g, const LDS float* et, f32x4n sw, f32x4n bias) {
+  constexpr int LPR = TN / 4, RPI = 64 / LPR, NI = TM / KVM_WAVES / RPI, NB = NI < 8 ? NI : 8;
   const int l = lane(), w = wave(), ch = l % LPR, n = g.n0 + 4 * ch;
-  const long long lim = 0x7fffffffll;
-  const bool vec = n + 4 <= g.N && (g.out.cols & 3) == 0 && vec_base(g.out) && (!g.res.ok() || ((g.res.cols & 3) == 0 && vec_base(g.res))) &&
-                   (long long)TM * g.res.cols * 4 < lim && (long long)TM * g.out.cols * 4 < lim;
-  float sw4[4], b4[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    sw4[i] = n + i < g.N ? g.sw.f()[n + i] : 0.f;
-    b4[i] = g.bias.ok() && n + i < g.N ? g.bias.f()[n + i] : 0.f;
-  }
-  const bool res = g.res.ok();
-  const View ov{(char*)g.out.p + (long long)g.m0 * g.out.cols * (OBF ? 2 : 4), g.out.rows - g.m0, g.out.cols, g.out.dtype, 0};
-  const int re = g.res.dtype == 2 ? 2 : 4;
-  const View rv{res ? (char*)g.res.p + (long long)g.m0 * g.res.cols * re : nullptr, g.res.rows - g.m0, g.res.cols, g.res.dtype, 0};
+  const int re = g.res.dtype == 2 ? 2 : 4, left = g.M - g.m0;
+  const View ov{(char*)g.out.p + (long long)g.m0 * g.out.cols * (OBF ? 2 : 4), left, g.out.cols, g.out.dtype, 0};
   Ld4 lr;
-  lr.init(rv, res && vec);
-  const __amdgpu_buffer_rsrc_t orsrc = wt_rsrc(ov.p, (long long)min(TM, g.M - g.m0) * ov.cols * (OBF ? 2 : 4));
+  if constexpr (RES) lr.init(View{(char*)g.res.p + (long long)g.m0 * g.res.cols * re, g.res.rows - g.m0, g.res.cols, g.res.dtype, 0});
+  const __amdgpu_buffer_rsrc_t orsrc = wt_rsrc(ov.p, (long long)min(TM, left) * ov.cols * (OBF ? 2 : 4));
   for (int k0 = 0; k0 < NI; k0 += NB) {
     u32x4_t raw[NB];
-    float sa[NB];
+    if constexpr (RES)
+#pragma unroll
+      for (int u = 0; u < NB; ++u) raw[u] = lr.raw(min(((k0 + u) * KVM_WAVES + w) * RPI + l / LPR, left - 1) * g.res.cols + n);
 #pragma unroll
     for (int u = 0; u < NB; ++u) {
       const int r = ((k0 + u) * KVM_WAVES + w) * RPI + l / LPR;
-      raw[u] = lr.raw(vec ? min(r, g.M - 1 - g.m0) * rv.cols + n : 0);
-      sa[u] = g.sa.f()[min(g.m0 + r, g.M - 1)];
+      if (r >= left) continue;
+      f32x4n y = *(const LDS f32x4n*)(et + r * TN + 4 * (ch ^ epi_swz<TN>(r)));
+      y.x *= sw.x; y.y *= sw.y; y.z *= sw.z; y.w *= sw.w;
+      if (g.bias.ok()) y += bias;
+      if constexpr (RES) y += lr.cvt(raw[u]);
+      if constexpr (OBF) stwt_bf4_buf(orsrc, (r * ov.cols + n) * 2, y);
+      else stwt_buf(orsrc, (r * ov.cols + n) * 4, y);
     }
+  }
+}
+// Rows of out or res that are no whole vectors, and the last columns of a ragged N: an element at a time, a row's neighbours in neighbouring lanes.
+template <int TM, int TN> __device__ __noinline__ void q8_elements_out(const Ctx& c) {
+  const TileQ8 g(c);
+  const LDS float* et = (const LDS float*)c.smem;
+  const int cols = min(TN, g.N - g.n0), rows = min(TM, g.M - g.m0), l = tid() % TN, r1 = KVM_THREADS / TN;
+  if (l >= cols) return;
+  const int n = g.n0 + l;
+  const float sw = g.sw.f()[n], bias = g.bias.ok() ? g.bias.f()[n] : 0.f;
+  constexpr int U = 4;
+  for (int r0 = tid() / TN; r0 < rows; r0 += U * r1) {
+    float x[U];
 #pragma unroll
-    for (int u = 0; u < NB; ++u) {
-      const int r = ((k0 + u) * KVM_WAVES + w) * RPI + l / LPR, m = g.m0 + r;
-      if (m >= g.M) continue;
-      const i32x4_t s = *(const LDS i32x4_t*)(et + r * TN + 4 * (ch ^ epi_swz<TN>(r)));
-      if (vec) {
-        f32x4n y = {g.scaled(s.x, sa[u], sw4[0]), g.scaled(s.y, sa[u], sw4[1]), g.scaled(s.z, sa[u], sw4[2]), g.scaled(s.w, sa[u], sw4[3])};
-        if (g.bias.ok()) y += f32x4n{b4[0], b4[1], b4[2], b4[3]};
-        if (res) y += lr.cvt(raw[u]);
-        if constexpr (OBF) stwt_bf4_buf(orsrc, (r * ov.cols + n) * 2, y);
-        else stwt_buf(orsrc, (r * ov.cols + n) * 4, y);
-      } else {
-        const int x[4] = {s.x, s.y, s.z, s.w};
+    for (int u = 0; u < U; ++u) x[u] = g.res.ok() ? g.res.at(g.m0 + min(r0 + u * r1, rows - 1), n) : 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) if (n + i < g.N) g.put(m, n + i, x[i], sa[u]);
-      }
+    for (int u = 0; u < U; ++u) {
+      const int r = r0 + u * r1;
+      if (r >= rows) break;
+      float y = et[r * TN + 4 * ((l >> 2) ^ epi_swz<TN>(r)) + (l & 3)] * sw;
+      if (g.bias.ok()) y += bias;
+      if (g.res.ok()) y += x[u];
+      g.out.st((long long)(g.m0 + r) * g.out.cols + n, y);
     }
   }
 }
@@ -274,6 +275,9 @@ template <int TM, int TN> __device__ __noinline__ void q8_tile(const Ctx& c) {
   for (int i = 0; i < BM; ++i)
 #pragma unroll
     for (int j = 0; j < BN; ++j) acc[i][j] = i32x16_t{};
+  float sa[BM];                                    // of the rows whose sums the lane gets
+#pragma unroll
+  for (int i = 0; i < BM; ++i) sa[i] = g.sa.f()[min(g.m0 + wm0 + i * 32 + (lane() & 31), g.M - 1)];
   const int nst = (g.K + 2 * DK - 1) / (2 * DK);
   constexpr int NLA = DOp<TM, true>::NL, NLS = NLA + DOp<TN, true>::NL, NF = BM + BN, NM = BM * BN, PF = (NF + NM - 1) / NM, PX = (NF + NLS + NM - 1) / NM;
   __syncthreads();                                 // the previous task may still read this LDS
@@ -336,10 +340,16 @@ template <int TM, int TN> __device__ __noinline__ void q8_tile(const Ctx& c) {
 #pragma unroll
     for (int m = 0; m < NM; ++m) mfma_one(m, fa1, fb1);
   }
+  const int l = lane(), n = g.n0 + 4 * (l % (TN / 4));
+  const bool vec = g.n0 + TN <= g.N && (g.out.cols & 3) == 0 && vec_base(g.out) && (!g.res.ok() || ((g.res.cols & 3) == 0 && vec_base(g.res))) &&
+                   (long long)TM * max(g.res.cols, g.out.cols) * 4 < 0x7fffffffll;
+  f32x4n sw = {0.f, 0.f, 0.f, 0.f}, bias = sw;
+  if (vec)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { sw[i] = g.sw.f()[n + i]; if (g.bias.ok()) bias[i] = g.bias.f()[n + i]; }
   wait_vm_c<0>();                                  // the placeholder loads have written their LDS bytes
   __syncthreads();
-  LDS int* et = (LDS int*)c.smem;                  // D^T: lane has row l % 32 of block i, columns 8 q + 4 (l / 32) .. + 3 of block j
-  const int l = lane();
+  LDS float* et = (LDS float*)c.smem;              // D^T: lane has row l % 32 of block i, columns 8 q + 4 (l / 32) .. + 3 of block j
 #pragma unroll
   for (int i = 0; i < BM; ++i) {
     const int r = wm0 + i * 32 + (l & 31);
@@ -348,12 +358,15 @@ template <int TM, int TN> __device__ __noinline__ void q8_tile(const Ctx& c) {
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const int chunk = (wn0 + j * 32 + 8 * q) / 4 + (l >> 5);
-        *(LDS i32x4_t*)(et + r * TN + 4 * (chunk ^ epi_swz<TN>(r))) = i32x4_t{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+        *(LDS f32x4n*)(et + r * TN + 4 * (chunk ^ epi_swz<TN>(r))) = f32x4n{(float)acc[i][j][4 * q] * sa[i], (float)acc[i][j][4 * q + 1] * sa[i], (float)acc[i][j][4 * q + 2] * sa[i],
+                                                                          (float)acc[i][j][4 * q + 3] * sa[i]};
       }
   }
   __syncthreads();
-  if (g.out.dtype == 2) q8_epilogue<TM, TN, true>(c);
-  else q8_epilogue<TM, TN, false>(c);
+  if (!vec) q8_elements_out<TM, TN>(c);
+  else if (g.out.dtype == 2) { if (g.res.ok()) q8_rows_out<TM, TN, true, true>(g, et, sw, bias); else q8_rows_out<TM, TN, true, false>(g, et, sw, bias); }
+  else if (g.res.ok()) q8_rows_out<TM, TN, false, true>(g, et, sw, bias);
+  else q8_rows_out<TM, TN, false, false>(g, et, sw, bias);
 }
 // Rows of bytes that do not lie in whole 16-byte vectors: an output at a time, four products an instruction.
 __device__ __forceinline__ int q8_dot(const GLOBAL int* a, const GLOBAL int* w, int K) {
