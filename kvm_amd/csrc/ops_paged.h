@@ -240,14 +240,16 @@ struct PiecePaged { int k0, k1, k, live, i0; };
 
 // The work of a call over its tasks: a tile costs PG_TILE and one per key up to the last that it sees; tiles in order of sequence, kv head
 // and token are cut into equal shares, in all tasks alike from the lengths. A cut within PG_SNAP of a tile's end moves there: a small piece
-// costs more than it balances. Tiles of up to 32 rows are a sequence's new tokens as a whole (the waves share the keys); longer ones have `tile`
+// costs more than it balances; where there is a task for every tile and none is longer than a share by PG_CUT, about what the partials and the
+// merge of a cut cost, no tile is cut. Tiles of up to 32 rows are a sequence's new tokens as a whole (the waves share the keys); longer ones have `tile`
 // rows (the waves share the rows).
-constexpr int PG_TILE = 256, PG_SNAP = 320, PG_SHARE = 512;
+constexpr int PG_TILE = 256, PG_SNAP = 320, PG_SHARE = 512, PG_CUT = 1024;
 struct WorkPaged {
   const LDS long long* pre;    // [B + 1] cost of the sequences before
   const LDS int *cu, *len;
   int B, Hkv, G, rows;
   long long share, total;
+  bool whole;                  // tiles are not cut
   __device__ __forceinline__ int tokens(int n) const { return (long long)n * G <= 32 ? n : max(1, rows / G); }   // of a tile
   // cost of the first j tiles of TT tokens of one head, none of them the last, ragged one
   __device__ __forceinline__ static long long upto(long long j, long long L, long long TT) { return j * (PG_TILE + L) + TT * (j * (j + 1) / 2); }
@@ -278,6 +280,7 @@ struct WorkPaged {
     if (x == total) return total;
     const TilePaged t = find(x);
     const long long off = x - t.start;
+    if (whole) return off < t.cost - off ? t.start : t.start + t.cost;
     return off < PG_SNAP ? t.start : t.cost - off < PG_SNAP ? t.start + t.cost : x;
   }
   // The piece [x, end) of a tile: its keys, and which of how many pieces it is.
@@ -287,7 +290,7 @@ struct WorkPaged {
     p.k0 = x == t.start ? 0 : key(x - t.start);
     p.k1 = end == t.start + t.cost ? t.L + t.tok0 + t.ntok : key(end - t.start);
     const long long first = (t.start + PG_SNAP + share - 1) / share, last = (t.start + t.cost - PG_SNAP) / share;
-    const int inside = t.cost < 2 * PG_SNAP ? 0 : (int)max(0ll, last - first + 1);
+    const int inside = whole || t.cost < 2 * PG_SNAP ? 0 : (int)max(0ll, last - first + 1);
     p.i0 = rfl((int)first); p.live = rfl(inside + 1);
     p.k = x == t.start ? 0 : rfl((int)(x / share - first + 1));
     p.k0 = rfl(p.k0); p.k1 = rfl(p.k1);
@@ -305,79 +308,176 @@ __device__ __forceinline__ GLOBAL float* paged_partial(const AttnPaged& D, const
 __device__ __forceinline__ long long paged_out(const AttnPaged& D, const TilePaged& t, int r) {
   return (long long)(t.row0 + r / D.G) * D.o.cols + (long long)(t.h * D.G + r % D.G) * D.hd;
 }
-// The piece that counts itself last merges the tile's rows; maxima are in units of log2. First the rows' maxima and sums, eight lanes to a row and
-// eight pieces at a time; then a thread has four dims of a row, or a share of the pieces of them where there are threads enough, the loads of U
-// pieces in flight.
-template <int U> __device__ __forceinline__ void paged_merge_dims(const AttnPaged& D, const TilePaged& t, const PiecePaged& p, int R, const LDS float* M, const LDS float* Z, LDS float* sum) {
-  const int hd = D.hd, C4 = (hd + 3) >> 2, items = R * C4, split = items >= KVM_THREADS ? 1 : min(p.live, KVM_THREADS / items);
-  for (int e0 = 0; e0 < items; e0 += KVM_THREADS) {
-    const int e = split > 1 ? tid() % items : e0 + tid(), g = split > 1 ? tid() / items : 0;
-    const bool on = e < items && g < split;
-    const int r = on ? e / C4 : 0, d = on ? 4 * (e % C4) : 0, nd = min(4, hd - d);
-    float a[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int k0 = on ? g : p.live; k0 < p.live; k0 += U * split) {
-      float m[U], x[U][4];
+// The piece that counts itself last merges the tile's rows, in the pieces' order whichever it is; maxima are in units of log2.
+// Few rows: a thread has four dims of a row and a share of the pieces, 16 of them requested at once with their maxima and sums; the shares meet
+// in LDS. Many rows: first the pieces' weights, to LDS, then four dims of four rows a thread at once.
+template <bool PAIRS> __device__ __forceinline__ f32x4n paged_dims(const GLOBAL float* y, int d, int hd) {
+  if (PAIRS) { const u32x2_t a = *(const GLOBAL u32x2_t*)(y + d), b = *(const GLOBAL u32x2_t*)(y + d + 2); return f32x4n{__uint_as_float(a.x), __uint_as_float(a.y), __uint_as_float(b.x), __uint_as_float(b.y)}; }
+  f32x4n x;
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const GLOBAL float* y = paged_partial(D, p, min(k0 + u * split, p.live - 1), r);
-        m[u] = y[hd];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[u][i] = y[d + min(i, nd - 1)];
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const float w = k0 + u * split < p.live && m[u] != -INFINITY ? exp2f(m[u] - M[r]) : 0.f;
-        if (w != 0.f)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) a[i] += w * x[u][i];
-      }
-    }
-    if (split > 1) {
-      if (on)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sum[4 * tid() + i] = a[i];
-      __syncthreads();
-      if (on && g == 0)
-        for (int s = 1; s < split; ++s)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) a[i] += sum[4 * (tid() + s * items) + i];
-    }
-    if (on && g == 0)
-      for (int i = 0; i < nd; ++i) D.o.st(paged_out(D, t, r) + d + i, a[i] / Z[r]);
-  }
+  for (int i = 0; i < 4; ++i) x[i] = y[min(d + i, hd - 1)];
+  return x;
 }
-__device__ __noinline__ void paged_merge(const Ctx& c, int row0_, int h_, int ntok_, int live_, int i0_) {
+__device__ __forceinline__ void paged_put(const AttnPaged& D, const TilePaged& t, int r, int d, f32x4n x, bool pairs) {
+  const long long o = paged_out(D, t, r) + d;
+  if (pairs && D.o.dtype == 2) stwt_bf4(D.o.h() + o, x.x, x.y, x.z, x.w);
+  else if (pairs) stwt_f4(D.o.f() + o, x);
+  else
+    for (int i = 0; i < min(4, D.hd - d); ++i) D.o.st(o + i, x[i]);
+}
+__device__ __forceinline__ float paged_top(float m, float x) { return x > m || x != x ? x : m; }              // a NaN stays
+__device__ __forceinline__ float paged_weight(float m, float top) { return m == -INFINITY ? 0.f : exp2f(m - top); }
+template <bool PAIRS> __device__ __noinline__ void paged_merge_few(const Ctx& c, int row0_, int h_, int ntok_, int live_, int i0_) {
   const AttnPaged D(c);
-  const int live = rfl(live_), R = rfl(ntok_) * D.G;
+  const int live = rfl(live_), R = rfl(ntok_) * D.G, hd = D.hd, C4 = (hd + 3) >> 2, items = R * C4, split = min(live, KVM_THREADS / items);
   const TilePaged t{0, rfl(h_), 0, rfl(row0_), 0, rfl(ntok_), 0, 0};
   const PiecePaged p{0, 0, 0, live, rfl(i0_)};
-  LDS float* M = (LDS float*)(c.smem + PG_WORK);                       // [128] maxima, [128] sums, [1024]
-  LDS float* Z = M + 128;
-  for (int r0 = 0; r0 < R; r0 += KVM_THREADS / 8) {
-    const int r = r0 + (tid() >> 3), sub = tid() & 7;
-    float m = -INFINITY, z = 0.f;
-    for (int k0 = sub; k0 < live; k0 += 32) {
-      float x[4], y[4];
+  const int e = tid() % items, g = tid() / items, r = e / C4, d = 4 * (e % C4);
+  f32x4n a = {0.f, 0.f, 0.f, 0.f};
+  float M = -INFINITY, z = 0.f;
+  constexpr int U = 16;
+  for (int k0 = g < split ? g : live; k0 < live; k0 += U * split) {
+    float m[U], s[U], top = M;
+    f32x4n x[U];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const GLOBAL float* v = paged_partial(D, p, min(k0 + 8 * u, live - 1), min(r, R - 1)) + D.hd;
-        x[u] = v[0]; y[u] = v[1];
-      }
+    for (int u = 0; u < U; ++u) {
+      const GLOBAL float* y = paged_partial(D, p, min(k0 + u * split, live - 1), r);
+      m[u] = y[hd]; s[u] = y[hd + 1];
+      x[u] = paged_dims<PAIRS>(y, d, hd);
+    }
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
-        if (k0 + 8 * u < live && x[u] != -INFINITY) {
-          const float top = x[u] > m || x[u] != x[u] ? x[u] : m;
-          z = (m == -INFINITY ? 0.f : z * exp2f(m - top)) + exp2f(x[u] - top) * y[u];
-          m = top;
+    for (int u = 0; u < U; ++u) {
+      m[u] = k0 + u * split < live ? m[u] : -INFINITY;
+      top = paged_top(top, m[u]);
+    }
+    const float f = paged_weight(M, top);
+    a *= f; z *= f; M = top;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const float w = paged_weight(m[u], top);
+      if (w != 0.f) { a += w * x[u]; z += w * s[u]; }
+    }
+  }
+  LDS float* sh = (LDS float*)(c.smem + PG_WORK);                      // [256][6]
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) sh[6 * tid() + i] = a[i];
+  sh[6 * tid() + 4] = M; sh[6 * tid() + 5] = z;
+  __syncthreads();
+  if (g == 0) {
+    float top = M;
+    for (int k = 1; k < split; ++k) top = paged_top(top, sh[6 * (tid() + k * items) + 4]);
+    const float f = paged_weight(M, top);
+    a *= f; z *= f;
+    for (int k = 1; k < split; ++k) {
+      const LDS float* y = sh + 6 * (tid() + k * items);
+      const float w = paged_weight(y[4], top);
+      a += w * f32x4n{y[0], y[1], y[2], y[3]}; z += w * y[5];
+    }
+    paged_put(D, t, r, d, f32x4n{a.x / z, a.y / z, a.z / z, a.w / z}, PAIRS);
+  }
+}
+constexpr int PG_WEIGHTS = 8192;   // weights of pieces in LDS; tiles cut into more take them as they go
+static_assert(PG_WORK + (256 + 2 * PG_WEIGHTS) * 4 <= KVM_LDS_BYTES, "LDS");
+// (forms of their own: a branch between two loads makes each wait for the one before; merging two pieces of 128 rows 50 us in place of MERGEUS)
+template <bool PAIRS, bool TABLE, int NI, int U> __device__ __forceinline__ void paged_sum_many(const AttnPaged& D, const TilePaged& t, const PiecePaged& p, int R, const LDS float* M, const LDS float* Z, const LDS float* W) {
+  const int hd = D.hd, C4 = (hd + 3) >> 2, items = R * C4;
+  for (int e0 = tid(); e0 < items; e0 += NI * KVM_THREADS) {
+    f32x4n a[NI];
+    int r[NI], d[NI];
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int e = min(e0 + i * KVM_THREADS, items - 1);
+      r[i] = e / C4; d[i] = 4 * (e - r[i] * C4);
+      a[i] = f32x4n{0.f, 0.f, 0.f, 0.f};
+    }
+    for (int k0 = 0; k0 < p.live; k0 += U) {
+      f32x4n x[NI][U];
+      float w[NI][U];
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const GLOBAL float* y = paged_partial(D, p, min(k0 + u, p.live - 1), r[i]);
+          x[i][u] = paged_dims<PAIRS>(y, d[i], hd);
+          if (!TABLE) w[i][u] = y[hd];
+        }
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const float v = TABLE ? W[min(k0 + u, p.live - 1) * R + r[i]] : paged_weight(w[i][u], M[r[i]]);
+          if (k0 + u < p.live && v != 0.f) a[i] += v * x[i][u];
         }
     }
-    const float top = lanes_max<8>(m), f = m == -INFINITY ? 0.f : exp2f(m - top);
-    z = lanes_sum<8>(f * z);
-    if (sub == 0 && r < R) { M[r] = top; Z[r] = z; }
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+      if (e0 + i * KVM_THREADS < items) { const float z = Z[r[i]]; paged_put(D, t, r[i], d[i], f32x4n{a[i].x / z, a[i].y / z, a[i].z / z, a[i].w / z}, PAIRS); }
   }
-  __syncthreads();
-  if (live <= 4) paged_merge_dims<4>(D, t, p, R, M, Z, Z + 128);
-  else paged_merge_dims<16>(D, t, p, R, M, Z, Z + 128);
+}
+template <bool PAIRS> __device__ __noinline__ void paged_merge_many(const Ctx& c, int row0_, int h_, int ntok_, int live_, int i0_) {
+  const AttnPaged D(c);
+  const int live = rfl(live_), R = rfl(ntok_) * D.G, hd = D.hd;
+  const TilePaged t{0, rfl(h_), 0, rfl(row0_), 0, rfl(ntok_), 0, 0};
+  const PiecePaged p{0, 0, 0, live, rfl(i0_)};
+  LDS float* M = (LDS float*)(c.smem + PG_WORK);                       // [128] maxima, [128] sums, [live][R] weights, the pieces' sums
+  LDS float* Z = M + 128;
+  LDS float* W = Z + 128;
+  const bool table = live * R <= PG_WEIGHTS;
+  if (table) {                                                         // maxima and sums of all pieces in one round of loads
+    LDS float* S = W + PG_WEIGHTS;
+    constexpr int NB = 8;
+    for (int e0 = tid(); e0 < live * R; e0 += NB * KVM_THREADS) {
+      float x[NB], y[NB];
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        const int e = min(e0 + i * KVM_THREADS, live * R - 1), k = e / R;
+        const GLOBAL float* v = paged_partial(D, p, k, e - k * R) + hd;
+        x[i] = v[0]; y[i] = v[1];
+      }
+#pragma unroll
+      for (int i = 0; i < NB; ++i) if (e0 + i * KVM_THREADS < live * R) { W[e0 + i * KVM_THREADS] = x[i]; S[e0 + i * KVM_THREADS] = y[i]; }
+    }
+    __syncthreads();
+    if (tid() < R) {
+      float top = -INFINITY, z = 0.f;
+      for (int k = 0; k < live; ++k) top = paged_top(top, W[k * R + tid()]);
+      for (int k = 0; k < live; ++k) {
+        const float w = paged_weight(W[k * R + tid()], top);
+        W[k * R + tid()] = w;
+        if (w != 0.f) z += w * S[k * R + tid()];
+      }
+      M[tid()] = top; Z[tid()] = z;
+    }
+    __syncthreads();
+  } else {
+    for (int r0 = 0; r0 < R; r0 += KVM_THREADS / 8) {                    // eight lanes to a row
+      const int r = r0 + (tid() >> 3), sub = tid() & 7;
+      float m = -INFINITY, z = 0.f;
+      for (int k0 = sub; k0 < live; k0 += 32) {
+        float x[4], y[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const GLOBAL float* v = paged_partial(D, p, min(k0 + 8 * u, live - 1), min(r, R - 1)) + hd;
+          x[u] = v[0]; y[u] = v[1];
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (k0 + 8 * u < live && x[u] != -INFINITY) {
+            const float top = paged_top(m, x[u]);
+            z = paged_weight(m, top) * z + exp2f(x[u] - top) * y[u];
+            m = top;
+          }
+      }
+      const float top = lanes_all<8>(m, [](float a, float b) { return a != a ? a : paged_top(a, b); }), f = paged_weight(m, top);
+      z = lanes_sum<8>(f * z);
+      if (sub == 0 && r < R) { M[r] = top; Z[r] = z; }
+    }
+    __syncthreads();
+  }
+  if (!table) paged_sum_many<PAIRS, false, 4, 4>(D, t, p, R, M, Z, W);
+  else if (live == 2) paged_sum_many<PAIRS, true, 8, 2>(D, t, p, R, M, Z, W);
+  else paged_sum_many<PAIRS, true, 4, 4>(D, t, p, R, M, Z, W);
 }
 __device__ __forceinline__ void paged_arrive(const Ctx& c, const AttnPaged& D, const TilePaged& t, const PiecePaged& p, LDS int* flag) {
   wait_stores();
@@ -388,7 +488,10 @@ __device__ __forceinline__ void paged_arrive(const Ctx& c, const AttnPaged& D, c
   if (old < 0 || old >= p.live) { if (tid() == 0) c.fail(KVM_ERR_OP_RANGE, p.i0, old); return; }
   if (old != p.live - 1) return;
   fence_acquire();                                                     // the other pieces' partials, stored before their counts
-  paged_merge(c, t.row0, t.h, t.ntok, p.live, p.i0);
+  const bool few = t.ntok * D.G * ((D.hd + 3) >> 2) <= KVM_THREADS / 2, pairs = rfl(D.fast()) != 0;
+  if (few) { if (pairs) paged_merge_few<true>(c, t.row0, t.h, t.ntok, p.live, p.i0); else paged_merge_few<false>(c, t.row0, t.h, t.ntok, p.live, p.i0); }
+  else if (pairs) paged_merge_many<true>(c, t.row0, t.h, t.ntok, p.live, p.i0);
+  else paged_merge_many<false>(c, t.row0, t.h, t.ntok, p.live, p.i0);
   if (tid() == 0) st_relaxed((int*)D.cnt.i() + p.i0, 0);
 }
 
@@ -841,9 +944,8 @@ template <int HD, int NT> __device__ __noinline__ int attn_paged_keys_f32(const 
 // transposing reads of LDS run at a third of the rate. 32 keys at a time, the scores of the next ones under the softmax of these: with 64 the
 // fragments and scores under way pass 256 registers.
 constexpr int PG_IDS = 2048, PG_NS = 3;
-__device__ __forceinline__ void dma16_at(unsigned long long src, const LDS void* dst) {   // 16 bytes a lane from its own address to dst + 16 * lane
-  const int m = __builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)dst);
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" :: "s"(m), "v"(src) : "memory", "m0");
+__device__ __forceinline__ void dma16_at(unsigned long long src, unsigned dst) {   // 16 bytes a lane from its own address to LDS byte dst (uniform) + 16 * lane
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" :: "s"(dst), "v"(src) : "memory", "m0");
 }
 // 8 keys of HD / 32 dims each (HD 128: 4 in two words; 64: 2 in one) as HD / 32 operands of 8 keys.
 template <int HD> struct VTurn {
@@ -864,6 +966,12 @@ template <int HD> struct VTurn {
     return __builtin_bit_cast(bf16x8, r);
   }
 };
+// Maximum over a lane and the one 32 away, in registers: through LDS it would wait for all reads of LDS under way (a block of 64 keys 2.8 us in place of
+// ROWSUS).
+__device__ __forceinline__ float halves_max(float v) {
+  auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
 template <int HD> __device__ __noinline__ int attn_paged_rows(const Ctx& c, int b_, int h_, int L_, int row0_, int tok0_, int ntok_, int k0_, int k1_, int k_, int live_, int i0_) {
   typedef FaL<HD> FL;
   constexpr int NKK = HD / 16, NDB = HD / 32, ST = 2 * FA_KB * HD;
@@ -894,6 +1002,15 @@ template <int HD> __device__ __noinline__ int attn_paged_rows(const Ctx& c, int 
   for (int d = 0; d < NDB; ++d) oacc[d] = f32x16{};
   float m = -INFINITY, lsum = 0.f;
   bool bad = false;
+  const unsigned lds0 = (unsigned)rfl((int)(unsigned)(uintptr_t)lds) + w * 1024u;   // where this wave's first KiB of stage 0 lies
+  int lrow[FL::NL];                                                    // rows of a block that the lane loads pieces of, and these within a piece of a page
+  unsigned koff[FL::NL], voff[FL::NL];
+#pragma unroll
+  for (int q = 0; q < FL::NL; ++q) {
+    const int u = 64 * (q * KVM_WAVES + w) + l, r = u / FL::UPR, ph = u % FL::UPR, at = r & ((1 << lsub) - 1);
+    lrow[q] = r;
+    koff[q] = (unsigned)(at * kpitch + 16 * (ph ^ FL::kswz(r))); voff[q] = (unsigned)(at * vpitch + 16 * ph);
+  }
   const int seg = PG_IDS << lsub;
   for (long long s0_ = p.k0; s0_ < p.k1; s0_ += seg) {
     const int s0 = (int)s0_, s1 = (int)min((long long)p.k1, s0_ + seg), nkb = (s1 - s0 + 63) >> 6, last = s1 - 1 - s0;
@@ -907,29 +1024,51 @@ template <int HD> __device__ __noinline__ int attn_paged_rows(const Ctx& c, int 
     __syncthreads();
     // (keys behind the last one: the last one again, not seen)
     auto issue = [&](int blk) {
-      LDS uint16_t* d = lds + (blk % PG_NS) * ST;
-      const bool whole = blk * FA_KB + FA_KB - 1 <= last;
+      const unsigned d = lds0 + (unsigned)((blk % PG_NS) * ST * 2);
+      const int first = (blk * FA_KB) >> lsub;
+      if (blk * FA_KB + FA_KB - 1 <= last) {
+        unsigned v[FL::NL];
 #pragma unroll
-      for (int q = 0; q < FL::NL; ++q) {
-        const int b = q * KVM_WAVES + w, u = 64 * b + l, r = u / FL::UPR, ph = u % FL::UPR;
-        const int key = whole ? blk * FA_KB + r : min(blk * FA_KB + r, last), at = key & ((1 << lsub) - 1);
-        const unsigned v = (unsigned)sid[key >> lsub];
-        dma16_at((kb + (unsigned)(at * kpitch + 16 * (ph ^ FL::kswz(r)))) + (unsigned long long)v * ksub, d + b * 512);
-        dma16_at((vb + (unsigned)(at * vpitch + 16 * ph)) + (unsigned long long)v * vsub, d + FA_KB * HD + b * 512);
+        for (int q = 0; q < FL::NL; ++q) v[q] = (unsigned)sid[first + (lrow[q] >> lsub)];
+#pragma unroll
+        for (int q = 0; q < FL::NL; ++q) {
+          dma16_at(kb + ((unsigned long long)v[q] * ksub + koff[q]), d + q * KVM_WAVES * 1024);
+          dma16_at(vb + ((unsigned long long)v[q] * vsub + voff[q]), d + FA_KB * HD * 2 + q * KVM_WAVES * 1024);
+        }
+      } else {
+#pragma unroll 1
+        for (int q = 0; q < FL::NL; ++q) {
+          const int u = 64 * (q * KVM_WAVES + w) + l, r = u / FL::UPR, ph = u % FL::UPR;
+          const int key = min(blk * FA_KB + r, last), at = key & ((1 << lsub) - 1);
+          const unsigned v = (unsigned)sid[key >> lsub];
+          dma16_at(kb + ((unsigned long long)v * ksub + (unsigned)(at * kpitch + 16 * (ph ^ FL::kswz(r)))), d + q * KVM_WAVES * 1024);
+          dma16_at(vb + ((unsigned long long)v * vsub + (unsigned)(at * vpitch + 16 * ph)), d + FA_KB * HD * 2 + q * KVM_WAVES * 1024);
+        }
       }
     };
-    // Keys [key0, key0 + 32): scores sa, values at Vs (keys of the block from vk on); the scores of the next 32, keys from nk on at Kn, to sn.
-    auto step = [&](int key0, const LDS uint16_t* Vs, int vk, const LDS uint16_t* Kn, int nk, f32x16& sa, f32x16& sn) {
+    bf16x8 kfr[NKK];                                                   // of the keys after the step's, and the step's own values
+    VTurn<HD> vt[2];
+    auto read = [&](const LDS uint16_t* K, int nk, const LDS uint16_t* V, int vk) {
+#pragma unroll
+      for (int kk = 0; kk < NKK; ++kk) kfr[kk] = FL::frag_kc(K, nk, kk);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) vt[u].read(V, vk + 16 * u, g, qi);
+    };
+    // Keys [key0, key0 + 32): scores sa; the scores of the next 32 to sn. Then what the next step needs is read: K of the keys after it (from
+    // nk on at Kn), V of its own (from vk on at Vn), under the last products and its maximum.
+    auto step = [&](int key0, f32x16& sa, f32x16& sn, const LDS uint16_t* Kn, int nk, const LDS uint16_t* Vn, int vk) {
       if (!wave_on || key0 > wlast) return;                            // no row of the wave sees a key of these
       if (key0 + 31 > wfirst) {
+        asm volatile("" ::: "memory");                                 // stays a branch: flattened, its selects run in every step
+        const int seen = lim - key0 - 4 * g;
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (key0 + 8 * (r >> 2) + 4 * g + (r & 3) > lim) sa[r] = -INFINITY;
+        for (int r = 0; r < 16; ++r) sa[r] = 8 * (r >> 2) + (r & 3) > seen ? -INFINITY : sa[r];
       }
-      float mx = sa[0];
+      float mx = fmaxf(fmaxf(sa[0], sa[1]), sa[2]);
 #pragma unroll
-      for (int r = 1; r < 16; ++r) mx = fmaxf(mx, sa[r]);
-      mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * D.sl2;
+      for (int r = 3; r + 1 < 16; r += 2) mx = fmaxf(fmaxf(mx, sa[r]), sa[r + 1]);
+      mx = fmaxf(mx, sa[15]);
+      mx = halves_max(mx) * D.sl2;
       if (__ballot(mx > m + 8.f)) {
         const float top = fmaxf(m, mx), f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
         lsum *= f;
@@ -938,14 +1077,11 @@ template <int HD> __device__ __noinline__ int attn_paged_rows(const Ctx& c, int 
         m = top;
       }
       const float base = m == -INFINITY ? 0.f : m;
-      bf16x8 kfr[NKK];
-      VTurn<HD> vt[2];
-#pragma unroll
-      for (int kk = 0; kk < NKK; ++kk) kfr[kk] = FL::frag_kc(Kn, nk, kk);
-#pragma unroll
-      for (int u = 0; u < 2; ++u) vt[u].read(Vs, vk + 16 * u, g, qi);
       bf16x8 pf[2];
       float ps = 0.f;
+      sn = f32x16{};
+      // a product of the next scores, two exponentials and what belongs to them, in turn; then the products of P, their operands and the reads
+      // between them
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         float pv[8];
@@ -954,7 +1090,6 @@ template <int HD> __device__ __noinline__ int attn_paged_rows(const Ctx& c, int 
         pf[u] = pack_bf16(pv);
         ps = sum_bf16(pf[u], ps);
       }
-      sn = f32x16{};
 #pragma unroll
       for (int kk = 0; kk < NKK; ++kk) sn = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kfr[kk], qf[kk], sn, 0, 0, 0);
       lsum += ps;
@@ -962,6 +1097,19 @@ template <int HD> __device__ __noinline__ int attn_paged_rows(const Ctx& c, int 
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int d = 0; d < NDB; ++d) oacc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vt[u].turned(d), pf[u], oacc[d], 0, 0, 0);
+      read(Kn, nk, Vn, vk);
+#pragma unroll
+      for (int i = 0; i < NKK; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);             // a matrix instruction,
+        __builtin_amdgcn_sched_group_barrier(0x002, 6 * 8 / NKK, 0);   // vector instructions,
+        __builtin_amdgcn_sched_group_barrier(0x400, 2 * 8 / NKK, 0);   // exponentials
+      }
+#pragma unroll
+      for (int i = 0; i < 2 * NDB; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);             // a read of LDS
+      }
     };
     issue(0);
     if (nkb > 1) issue(1);
@@ -970,14 +1118,15 @@ template <int HD> __device__ __noinline__ int attn_paged_rows(const Ctx& c, int 
     f32x16 sa = {}, sn;
 #pragma unroll
     for (int kk = 0; kk < NKK; ++kk) sa = __builtin_amdgcn_mfma_f32_32x32x16_bf16(FL::frag_kc(lds, 0, kk), qf[kk], sa, 0, 0, 0);
+    read(lds, 32, lds + FA_KB * HD, 0);
     for (int blk = 0; blk < nkb; ++blk) {
       const LDS uint16_t* Ks = lds + (blk % PG_NS) * ST;
       const LDS uint16_t* Kn = lds + ((blk + 1) % PG_NS) * ST;
-      step(s0 + blk * FA_KB, Ks + FA_KB * HD, 0, Ks, 32, sa, sn);
       wait_vm_c<0>();                                                  // block blk + 1 has landed
       __syncthreads();                                                 // ... everyone's, and every wave is past block blk - 1
       if (blk + 2 < nkb) issue(blk + 2);
-      step(s0 + blk * FA_KB + 32, Ks + FA_KB * HD, 32, Kn, 0, sn, sa);
+      step(s0 + blk * FA_KB, sa, sn, Kn, 0, Ks + FA_KB * HD, 32);
+      step(s0 + blk * FA_KB + 32, sn, sa, Kn, 32, Kn + FA_KB * HD, 0);
     }
   }
   lsum += __shfl_xor(lsum, 32, 64);
@@ -988,25 +1137,28 @@ template <int HD> __device__ __noinline__ int attn_paged_rows(const Ctx& c, int 
     for (int r = 0; r < 16; ++r) nf += oacc[d][r] * 0.f;
   if (__syncthreads_or(bad ? 1 : 0)) { if (tid() == 0) c.fail(KVM_ERR_OP_RANGE, t.b, p.k0); return PG_FAILED; }
   if (__syncthreads_or(qok && nf != 0.f ? 1 : 0)) return PG_AGAIN;
-  if (qok) {                                                           // registers r = 4 q .. 4 q + 3 of all products: 4 NDB dims in a row
-    const float inv = p.live == 1 ? 1.f / lsum : 1.f;
-    GLOBAL uint16_t* o = D.o.h() + paged_out(D, t, row);
-    GLOBAL float* y = paged_partial(D, p, p.k, row);
+  // through LDS, whole rows go out
+  LDS float* ol = (LDS float*)(c.smem + PG_WORK);                      // [128][HD + 4]
+  static_assert(PG_WORK + 128 * (HD + 4) * 4 <= KVM_LDS_BYTES, "LDS");
+  const float inv = p.live == 1 ? 1.f / lsum : 1.f;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int d0 = NDB * (8 * q + 4 * g);
-      float x[4 * NDB];
+  for (int r = 0; r < 16; ++r) {                                       // register r of the products: NDB dims in a row
+    LDS float* y = ol + row * (HD + 4) + NDB * (8 * (r >> 2) + 4 * g + (r & 3));
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-#pragma unroll
-        for (int d = 0; d < NDB; ++d) x[NDB * r + d] = oacc[d][4 * q + r] * inv;
-#pragma unroll
-      for (int i = 0; i < 4 * NDB; i += 4) {
-        if (p.live == 1) stwt_bf4(o + d0 + i, x[i], x[i + 1], x[i + 2], x[i + 3]);
-        else stwt_f4(y + d0 + i, f32x4n{x[i], x[i + 1], x[i + 2], x[i + 3]});
-      }
+    for (int d = 0; d < NDB; ++d) y[d] = oacc[d][r] * inv;
+  }
+  if (p.live > 1 && qok && g == 0) { GLOBAL float* y = paged_partial(D, p, p.k, row) + HD; stwt32(y, m); stwt32(y + 1, lsum); }
+  __syncthreads();
+  for (int e = tid(); e < R * (HD / 8); e += KVM_THREADS) {
+    const int r = e / (HD / 8), d = 8 * (e % (HD / 8));
+    const f32x4n a = *(const LDS f32x4n*)(ol + r * (HD + 4) + d), b = *(const LDS f32x4n*)(ol + r * (HD + 4) + d + 4);
+    if (p.live == 1) {
+      GLOBAL uint16_t* o = D.o.h() + paged_out(D, t, r) + d;
+      stwt_bf4(o, a.x, a.y, a.z, a.w); stwt_bf4(o + 4, b.x, b.y, b.z, b.w);
+    } else {
+      GLOBAL float* y = paged_partial(D, p, p.k, r) + d;
+      stwt_f4(y, a); stwt_f4(y + 4, b);
     }
-    if (p.live > 1 && g == 0) { stwt32(y + HD, m); stwt32(y + HD + 1, lsum); }
   }
   return PG_DONE;
 }
@@ -1026,7 +1178,7 @@ __device__ __noinline__ void op_attn_paged(const Ctx& c) {
   LDS long long* pre = (LDS long long*)c.smem;                         // [PG_SEQS + 2]
   LDS int* scu = (LDS int*)(pre + PG_SEQS + 2);                        // [PG_SEQS + 4]
   LDS int* len = scu + PG_SEQS + 4;                                    // [PG_SEQS]
-  LDS int* flag = len + PG_SEQS;                                       // [4], then four sums of 8 bytes
+  LDS int* flag = len + PG_SEQS;                                       // [4], then 12 words of 8 bytes: the waves' sums, longest tiles and numbers of tiles
   LDS long long* tot = (LDS long long*)(flag + 4);
   if (!paged_call_ok(c, D.cu, D.lens, D.B, min(D.q.rows, D.o.rows), (long long)D.table.cols << D.lp, scu)) return;
   WorkPaged W;
@@ -1035,18 +1187,26 @@ __device__ __noinline__ void op_attn_paged(const Ctx& c) {
   W.rows = fast == 2 ? D.tile : min(D.tile, max(32, D.G));             // (the other forms take 32 rows at a time)
   {
     constexpr int PER = PG_SEQS / KVM_THREADS;
-    long long cost[PER], sum = 0;
+    long long cost[PER], sum = 0, most = 0, tiles = 0;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int b = tid() * PER + i;
       cost[i] = 0;
       if (b < D.B) {
-        const int L = D.lens.i()[b];
+        const int L = D.lens.i()[b], n = scu[b + 1] - scu[b];
         len[b] = L;
-        cost[i] = W.head_cost(scu[b + 1] - scu[b], L) * D.Hkv;
-        sum += cost[i];
+        if (n > 0) {
+          const int TT = W.tokens(n);
+          cost[i] = W.head_cost(n, L) * D.Hkv;
+          sum += cost[i];
+          most = max(most, PG_TILE + (long long)L + n);
+          tiles += (long long)((n + TT - 1) / TT) * D.Hkv;
+        }
       }
     }
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) { most = max(most, (long long)__shfl_xor(most, d, 64)); tiles += __shfl_xor(tiles, d, 64); }
+    if (lane() == 0) { tot[4 + wave()] = most; tot[8 + wave()] = tiles; }
     long long upto = sum;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) { const long long y = __shfl_up(upto, d, 64); if (lane() >= d) upto += y; }
@@ -1063,8 +1223,12 @@ __device__ __noinline__ void op_attn_paged(const Ctx& c) {
   }
   W.total = pre[D.B];
   W.share = max((W.total + D.S - 1) / D.S, (long long)PG_SHARE);
-  long long x = W.cut(D.s);
-  const long long end = W.cut(D.s + 1);
+  W.whole = tot[8] + tot[9] + tot[10] + tot[11] <= D.S && max(max(tot[4], tot[5]), max(tot[6], tot[7])) <= W.share + PG_CUT;
+  // Neighbouring shares read the same keys: eight runs of shares, one for the tasks s, s + 8, .. (where tasks go to workers in order, those of one
+  // XCD and its L2).
+  const int mine = D.S % 8 == 0 ? (D.s & 7) * (D.S >> 3) + (D.s >> 3) : D.s;
+  long long x = W.cut(mine);
+  const long long end = W.cut(mine + 1);
   while (x < end) {
     const TilePaged t = W.find(x);
     const long long stop = min(end, t.start + t.cost);
