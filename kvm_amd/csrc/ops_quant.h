@@ -11,38 +11,88 @@ namespace kvm {
 typedef int i32x16_t __attribute__((ext_vector_type(16)));
 
 // ---------------------------------------------------------------------------------------------- rows in 8 bits
-// v of a row (x, RMS-normalised x, silu(x) * x2) in vectors of 8: thread t has vectors t, t + 256, ..
-struct RowsSrc {
-  View x, x2, g; int K, pro; float eps;
-  // How x (and x2) can be read: 1, 2 vectors of f32 and of bf16, 0 element by element. A form of its own for each: a branch on the type between
-  // two loads makes each wait for the one before (a prompt's rows 4,001 x 4,096 59 us a call in place of NEWQ).
-  __device__ int form() const {
-    return rows8_ok(x) && (pro != 2 || (rows8_ok(x2) && x2.dtype == x.dtype)) && (pro != 1 || vec_base(g)) ? x.dtype == 2 ? 2 : 1 : 0;
-  }
-  template <int FORM> __device__ __forceinline__ void load(const View& X, long long row, int j, float (&v)[8]) const {
-    const int n = K - 8 * j;                                           // values from here on
-    const long long o = row * X.cols + 8 * j;
-    if (FORM) {
-      Raw8 w;
-      w.load(View{X.p, 0, 0, FORM == 2 ? 2 : 0, 0}, o); w.get(FORM == 2, v);
+// v of a row (x, RMS-normalised x, silu(x) * x2) in vectors of 8: thread t has vectors t, t + 256, .. How x (and x2) are read, FORM: 1 f32, 2 bf16
+// rows that start at whole words, 3 other bf16 rows, all by 16-byte loads through a descriptor that ends with the row's K values (any alignment of a
+// word, zeros behind the end: only bf16 values that share a word with the last one are masked); 0 element by element, where x and x2 are of two types. A form of its own for each: a branch on the type between two loads makes each
+// wait for the one before.
+template <int FORM> struct RawRow {
+  u32x4_t a, b; uint32_t c;
+  __device__ __forceinline__ void load(const View& X, long long row, int j, int K) {   // vector j of the row
+    const long long e0 = row * X.cols;
+    if constexpr (FORM == 0) {
+      const int n = K - 8 * j;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = e < n ? v[e] : 0.f;
+      for (int e = 0; e < 4; ++e) {
+        a[e] = e < n ? __float_as_uint(X.ld(e0 + 8 * j + e)) : 0u;
+        b[e] = e + 4 < n ? __float_as_uint(X.ld(e0 + 8 * j + 4 + e)) : 0u;
+      }
+    } else if constexpr (FORM == 1) {
+      const __amdgpu_buffer_rsrc_t rs = buf_rsrc((const void*)(X.f() + e0), 4ll * K);
+      a = __builtin_amdgcn_raw_buffer_load_b128(rs, 32 * j, 0, 0);
+      b = __builtin_amdgcn_raw_buffer_load_b128(rs, 32 * j + 16, 0, 0);
     } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = e < n ? X.ld(o + e) : 0.f;
+      const uintptr_t p = (uintptr_t)(X.h() + e0);
+      const __amdgpu_buffer_rsrc_t rs = buf_rsrc((const void*)(p & ~(uintptr_t)3), (2ll * K + (p & 2) + 3) & ~3ll);   // (a last half word with its whole word)
+      a = __builtin_amdgcn_raw_buffer_load_b128(rs, 16 * j, 0, 0);
+      if constexpr (FORM == 3) c = __builtin_amdgcn_raw_buffer_load_b32(rs, 16 * j + 16, 0, 0);
     }
   }
+  __device__ __forceinline__ void get(const View& X, long long row, int j, int K, float (&v)[8]) const {
+    if constexpr (FORM <= 1) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) { v[e] = __uint_as_float(a[e]); v[4 + e] = __uint_as_float(b[e]); }
+    } else {
+      uint32_t w[4] = {a.x, a.y, a.z, a.w};
+      if constexpr (FORM == 3) {
+        const uint32_t odd = (uint32_t)((uintptr_t)(X.h() + row * X.cols) & 2) * 8;        // bits that the row starts into its word
+        w[0] = __builtin_amdgcn_alignbit(a.y, a.x, odd); w[1] = __builtin_amdgcn_alignbit(a.z, a.y, odd);
+        w[2] = __builtin_amdgcn_alignbit(a.w, a.z, odd); w[3] = __builtin_amdgcn_alignbit(c, a.w, odd);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(e & 1 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
+    }
+    if (FORM >= 2 && (FORM == 3 || (K & 1)))
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = 8 * j + e < K ? v[e] : 0.f;
+  }
+};
+struct RowsSrc {
+  View x, x2, g; int K, pro; float eps;
+  __device__ int form() const {
+    if (pro == 2 && x2.dtype != x.dtype) return 0;
+    if (x.dtype != 2) return 1;
+    return ((x.cols | (pro == 2 ? x2.cols : 0)) & 1) == 0 && (((uintptr_t)x.p | (pro == 2 ? (uintptr_t)x2.p : 0)) & 3) == 0 ? 2 : 3;
+  }
+};
+// NV vectors of RB rows on their way, with what stands in front of them.
+template <int FORM, int NV, int RB> struct RowsRaw {
+  RawRow<FORM> x[RB][NV], y[RB][NV];
+  RawRow<1> g[NV];
+  __device__ __forceinline__ void load(const RowsSrc& S, long long r0, int nr, int j0) {
+#pragma unroll
+    for (int i = 0; i < RB; ++i)
+#pragma unroll
+      for (int u = 0; u < NV; ++u) x[i][u].load(S.x, r0 + min(i, nr - 1), j0 + u * KVM_THREADS, S.K);
+    if (S.pro == 1)
+#pragma unroll
+      for (int u = 0; u < NV; ++u) g[u].load(S.g, 0, j0 + u * KVM_THREADS, S.K);
+    if (S.pro == 2)
+#pragma unroll
+      for (int i = 0; i < RB; ++i)
+#pragma unroll
+        for (int u = 0; u < NV; ++u) y[i][u].load(S.x2, r0 + min(i, nr - 1), j0 + u * KVM_THREADS, S.K);
+  }
   // x * rstd * gamma, or silu(x) * x2: rounded after each product
-  template <int FORM> __device__ __forceinline__ void shape(float (&v)[8], long long row, int j, float rstd) const {
-    float y[8];
-    if (pro == 1) {
-      load<FORM ? 1 : 0>(g, 0, j, y);
+  __device__ __forceinline__ void shape(const RowsSrc& S, long long row, int i, int u, int j, float rstd, float (&v)[8]) const {
+    float w[8];
+    if (S.pro == 1) {
+      g[u].get(S.g, 0, j, S.K, w);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) { const float t = v[e] * rstd; v[e] = t * y[e]; }
-    } else if (pro == 2) {
-      load<FORM>(x2, row, j, y);
+      for (int e = 0; e < 8; ++e) { const float t = v[e] * rstd; v[e] = t * w[e]; }
+    } else if (S.pro == 2) {
+      y[i][u].get(S.x2, row, j, S.K, w);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = silu_f(v[e]) * y[e];
+      for (int e = 0; e < 8; ++e) v[e] = silu_f(v[e]) * w[e];
     }
   }
 };
@@ -51,10 +101,27 @@ __device__ __forceinline__ uint32_t q8_big(const float (&v)[8], uint32_t big) { 
   for (int e = 0; e < 8; ++e) big = max(big, __float_as_uint(v[e]) & 0x7fffffffu);
   return big;
 }
+// Sum of doubles over a wave in registers (as lanes_all and rows_all move floats): through LDS four rows' sums took a third of a round.
+template <int CTRL> __device__ __forceinline__ double dpp_d(double v) {
+  const unsigned long long u = __builtin_bit_cast(unsigned long long, v);
+  const unsigned lo = __builtin_amdgcn_update_dpp(0, (int)(unsigned)u, CTRL, 0xf, 0xf, true), hi = __builtin_amdgcn_update_dpp(0, (int)(unsigned)(u >> 32), CTRL, 0xf, 0xf, true);
+  return __builtin_bit_cast(double, ((unsigned long long)hi << 32) | lo);
+}
+__device__ __forceinline__ double wave_all_d(double v) {
+  v += dpp_d<0xB1>(v); v += dpp_d<0x4E>(v); v += dpp_d<0x141>(v); v += dpp_d<0x140>(v);
+  auto both = [](double x, bool far) {
+    const unsigned long long u = __builtin_bit_cast(unsigned long long, x);
+    const unsigned lo = (unsigned)u, hi = (unsigned)(u >> 32);
+    auto a = far ? __builtin_amdgcn_permlane32_swap(lo, lo, false, false) : __builtin_amdgcn_permlane16_swap(lo, lo, false, false);
+    auto b = far ? __builtin_amdgcn_permlane32_swap(hi, hi, false, false) : __builtin_amdgcn_permlane16_swap(hi, hi, false, false);
+    return __builtin_bit_cast(double, ((unsigned long long)b[0] << 32) | a[0]) + __builtin_bit_cast(double, ((unsigned long long)b[1] << 32) | a[1]);
+  };
+  return both(both(v, false), true);
+}
 // One sum or maximum per row over the workgroup, the waves' in order; red: 4 * RB of LDS.
 template <int RB> __device__ __forceinline__ void q8_rows_sum(double (&s)[RB], LDS double* red) {
 #pragma unroll
-  for (int i = 0; i < RB; ++i) s[i] = wave_sum_d(s[i]);
+  for (int i = 0; i < RB; ++i) s[i] = wave_all_d(s[i]);
   __syncthreads();
   if (lane() == 0)
 #pragma unroll
@@ -76,38 +143,43 @@ template <int RB> __device__ __forceinline__ void q8_rows_max(uint32_t (&b)[RB],
   for (int i = 0; i < RB; ++i) b[i] = max(max(red[4 * i], red[4 * i + 1]), max(red[4 * i + 2], red[4 * i + 3]));
 }
 constexpr int Q8_RED = 12;     // doubles of LDS per row in flight
-// nr <= RB rows from r0 on, K <= 2048 NV, held in registers: one read of x, all its loads in flight together, one reduction for the norm
-// and one for the scale whatever RB is. put(i, j, w0, w1): vector j of row r0 + i as bytes; scaled(i, s). Sums of squares in double, so
-// that rstd is the f32 nearest to the exact one whatever the order.
-template <int FORM, int NV, int RB, class Put, class Scaled>
-__device__ __forceinline__ void q8_rows(const RowsSrc& S, long long r0, int nr, LDS double* red, Put put, Scaled scaled) {
+// nr <= RB rows from r0 on, K <= 2048 NV, from `raw` (requested before), held in registers: one reduction for the norm and one for the scale whatever RB
+// is; `next` is called once the rows are out of raw, to request others under the reductions. put(i, j, w0, w1): vector j of row r0 + i as bytes;
+// scaled(i, s). Sums of squares in double, so that rstd is the f32 nearest to the exact one.
+template <int FORM, int NV, int RB, class Put, class Scaled, class Next>
+__device__ __forceinline__ void q8_rows(const RowsSrc& S, RowsRaw<FORM, NV, RB>& raw, long long r0, int nr, LDS double* red, Put put, Scaled scaled, Next next) {
   const int nvec = (S.K + 7) >> 3;
   float v[RB][NV][8];
+  double ss[RB] = {};
 #pragma unroll
   for (int i = 0; i < RB; ++i)
 #pragma unroll
-    for (int u = 0; u < NV; ++u) S.load<FORM>(S.x, r0 + min(i, nr - 1), min(tid() + u * KVM_THREADS, nvec - 1), v[i][u]);
-  double ss[RB] = {};
-  if (S.pro == 1) {
+    for (int u = 0; u < NV; ++u) {
+      raw.x[i][u].get(S.x, r0 + min(i, nr - 1), tid() + u * KVM_THREADS, S.K, v[i][u]);
+      if (S.pro == 1 && i < nr)
 #pragma unroll
-    for (int i = 0; i < RB; ++i)
-#pragma unroll
-      for (int u = 0; u < NV; ++u)
-        if (tid() + u * KVM_THREADS < nvec)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) ss[i] += (double)v[i][u][e] * (double)v[i][u][e];
-    q8_rows_sum<RB>(ss, red);
-  }
+        for (int e = 0; e < 8; ++e) ss[i] += (double)v[i][u][e] * (double)v[i][u][e];
+    }
+  if (S.pro == 1) q8_rows_sum<RB>(ss, red);
   uint32_t big[RB] = {};
+  float mine = 0.f;                                                    // lane i brings the reciprocal root of row i (division and root are 100 instructions)
+  if (S.pro == 1) {
+    double x = ss[0];
+#pragma unroll
+    for (int i = 1; i < RB; ++i) x = lane() == i ? ss[i] : x;
+    mine = (float)(1.0 / sqrt(x / S.K + (double)S.eps));
+  }
 #pragma unroll
   for (int i = 0; i < RB; ++i) {
-    const float rstd = (float)(1.0 / sqrt(ss[i] / S.K + (double)S.eps));
+    if (i >= nr) break;
+    const float rstd = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(mine), i));
 #pragma unroll
     for (int u = 0; u < NV; ++u) {
-      S.shape<FORM>(v[i][u], r0 + min(i, nr - 1), min(tid() + u * KVM_THREADS, nvec - 1), rstd);
+      raw.shape(S, r0 + i, i, u, tid() + u * KVM_THREADS, rstd, v[i][u]);
       big[i] = q8_big(v[i][u], big[i]);
     }
   }
+  next();
   q8_rows_max<RB>(big, red);
 #pragma unroll
   for (int i = 0; i < RB; ++i) {
@@ -127,10 +199,16 @@ template <int FORM, class Put, class Scaled>
 __device__ __forceinline__ void q8_row_long(const RowsSrc& S, long long r, LDS double* red, Put put, Scaled scaled) {
   const int nvec = (S.K + 7) >> 3;
   double ss[1] = {};
+  RowsRaw<FORM, 1, 1> raw;
   float v[8];
+  auto get = [&](int j, float rstd, bool shaped) {
+    raw.load(S, r, 1, j);
+    raw.x[0][0].get(S.x, r, j, S.K, v);
+    if (shaped) raw.shape(S, r, 0, 0, j, rstd, v);
+  };
   if (S.pro == 1) {
     for (int j = tid(); j < nvec; j += KVM_THREADS) {
-      S.load<FORM>(S.x, r, j, v);
+      get(j, 0.f, false);
 #pragma unroll
       for (int e = 0; e < 8; ++e) ss[0] += (double)v[e] * (double)v[e];
     }
@@ -138,27 +216,30 @@ __device__ __forceinline__ void q8_row_long(const RowsSrc& S, long long r, LDS d
   }
   const float rstd = (float)(1.0 / sqrt(ss[0] / S.K + (double)S.eps));
   uint32_t big[1] = {};
-  for (int j = tid(); j < nvec; j += KVM_THREADS) { S.load<FORM>(S.x, r, j, v); S.shape<FORM>(v, r, j, rstd); big[0] = q8_big(v, big[0]); }
+  for (int j = tid(); j < nvec; j += KVM_THREADS) { get(j, rstd, true); big[0] = q8_big(v, big[0]); }
   q8_rows_max<1>(big, red);
   const float s = q8_scale(__uint_as_float(big[0])), inv = s > 0.f ? 1.f / s : 0.f;
   if (tid() == 0) scaled(0, s);
   for (int j = tid(); j < nvec; j += KVM_THREADS) {
     uint32_t w0, w1;
-    S.load<FORM>(S.x, r, j, v); S.shape<FORM>(v, r, j, rstd);
+    get(j, rstd, true);
     q8_pack(v, s, inv, w0, w1);
     put(0, j, w0, w1);
   }
 }
 
 // Op 315. Bound: bytes (K * (2 to 8) read, K written a row). Four rows of up to 4,096 values at once, one of up to 16,384, so that the two
-// reductions' waits are shared.
+// reductions' waits are shared; the next rows are requested before this round's maximum. 4,001 rows of 4,096 bf16 values with the norm:
+// 41 us a call (49 MB, 1.2 TB/s with the launch), bound by the instructions of rounding and norm; 49 with masks on every value and sums of doubles through LDS.
 template <int FORM, int NV> __device__ __noinline__ void rows_q8_t(const Ctx& c) {
-  constexpr int RB = NV == 2 ? 4 : 1;
+  constexpr int RB = NV && NV <= 2 ? 4 : 1;
   const RowsSrc S{uview(c, 0), uview(c, 1), uview(c, 2), rfl(c.i(7)), rfl(c.i(8)), c.f(9)};
   const View q = uview(c, 3), qs = uview(c, 4);
   const int r0 = rfl(c.i(5)), r1 = rfl(c.i(6)), words = min(q.cols, ((S.K + 15) >> 4) << 2), nvec = (S.K + 7) >> 3;
   const bool pair = (q.cols & 1) == 0 && ((uintptr_t)q.p & 7) == 0;
   LDS double* red = (LDS double*)c.smem;
+  RowsRaw<FORM, NV ? NV : 1, RB> raw;
+  if (NV > 0 && r0 < r1) raw.load(S, r0, min(RB, r1 - r0), tid());
   for (int r = r0; r < r1; r += RB) {
     auto word = [&](GLOBAL int* p, int k, uint32_t w) { if (k < words) stwt32i(p + k, (int)w); };
     auto put = [&](int i, int j, uint32_t w0, uint32_t w1) {
@@ -168,16 +249,20 @@ template <int FORM, int NV> __device__ __noinline__ void rows_q8_t(const Ctx& c)
       if (j == nvec - 1 && (nvec & 1)) { word(p, 2 * nvec, 0); word(p, 2 * nvec + 1, 0); }   // up to the multiple of 16 bytes
     };
     auto scaled = [&](int i, float s) { stwt32(qs.f() + (r + i), s); };
-    if constexpr (NV > 0) q8_rows<FORM, NV, RB>(S, r, min(RB, r1 - r), red, put, scaled);
+    auto next = [&]() { if (r + RB < r1) raw.load(S, r + RB, min(RB, r1 - r - RB), tid()); };
+    if constexpr (NV > 0) q8_rows<FORM, NV, RB>(S, raw, r, min(RB, r1 - r), red, put, scaled, next);
     else q8_row_long<FORM>(S, r, red, put, scaled);
   }
 }
 __device__ __noinline__ void op_rows_q8(const Ctx& c) {
   const RowsSrc S{c.buf(0), c.buf(1), c.buf(2), c.i(7), c.i(8), c.f(9)};
   const int form = rfl(S.form());
-  if (form == 2) { if (S.K <= 4096) rows_q8_t<2, 2>(c); else if (S.K <= 16384) rows_q8_t<2, 8>(c); else rows_q8_t<2, 0>(c); }
-  else if (form == 1) { if (S.K <= 4096) rows_q8_t<1, 2>(c); else if (S.K <= 16384) rows_q8_t<1, 8>(c); else rows_q8_t<1, 0>(c); }
-  else if (S.K <= 4096) rows_q8_t<0, 2>(c); else rows_q8_t<0, 0>(c);
+  if (S.K <= 2048 && form) { if (form == 1) rows_q8_t<1, 1>(c); else if (form == 2) rows_q8_t<2, 1>(c); else rows_q8_t<3, 1>(c); }
+  else if (S.K <= 4096) { if (form == 1) rows_q8_t<1, 2>(c); else if (form == 2) rows_q8_t<2, 2>(c); else if (form == 3) rows_q8_t<3, 2>(c); else rows_q8_t<0, 0>(c); }
+  else if (S.K <= 16384 && form) { if (form == 1) rows_q8_t<1, 8>(c); else if (form == 2) rows_q8_t<2, 8>(c); else rows_q8_t<3, 8>(c); }
+  else if (form == 1) rows_q8_t<1, 0>(c);
+  else if (form >= 2) rows_q8_t<3, 0>(c);
+  else rows_q8_t<0, 0>(c);
 }
 
 // ---------------------------------------------------------------------------------------------- product tiles
@@ -422,13 +507,16 @@ template <int FORM, int NV> __device__ __noinline__ void gemv_q8_stage(const Ctx
   const int pitch = rfl(pitch_), lo = rfl(lo_), n = rfl(n_);
   const GemvQ8 G(c);
   const RowsSrc S{G.x, G.x2, G.g, G.K, G.pro, c.f(14)};
+  RowsRaw<FORM, NV ? NV : 1, 1> raw;
+  if (NV > 0) raw.load(S, 0, 1, tid());
   for (int m = 0; m < G.M; ++m) {
+    auto next = [&]() { if (m + 1 < G.M) raw.load(S, m + 1, 1, tid()); };
     auto put = [&](int, int j, uint32_t w0, uint32_t w1) {
       const int o = 8 * j - lo;
       if (o >= 0 && o < n) { *(LDS uint32_t*)(vs_ + gq_at(m, pitch, o)) = w0; *(LDS uint32_t*)(vs_ + gq_at(m, pitch, o + 4)) = w1; }
     };
     auto scaled = [&](int, float s) { scale[m] = s; };
-    if constexpr (NV > 0) q8_rows<FORM, NV, 1>(S, m, 1, red, put, scaled);
+    if constexpr (NV > 0) q8_rows<FORM, NV, 1>(S, raw, m, 1, red, put, scaled, next);
     else q8_row_long<FORM>(S, m, red, put, scaled);
     for (int o = max(0, ((G.K + 7) & ~7) - lo) + 4 * tid(); o < n; o += 4 * KVM_THREADS) *(LDS int*)(vs_ + gq_at(m, pitch, o)) = 0;
   }
@@ -467,16 +555,13 @@ __device__ __forceinline__ void gemv_q8_rows(const Ctx& c, const GemvQ8& G, LDS 
   }
   const RowsSrc S{G.x, G.x2, G.g, G.K, G.pro, 0.f};
   const int form = rfl(S.form());
-  if (form == 2) {
-    if (G.K <= 4096) gemv_q8_stage<2, 2>(c, vs, pitch, lo, n, scale, red);
-    else if (G.K <= 16384) gemv_q8_stage<2, 8>(c, vs, pitch, lo, n, scale, red);
-    else gemv_q8_stage<2, 0>(c, vs, pitch, lo, n, scale, red);
-  } else if (form == 1) {
-    if (G.K <= 4096) gemv_q8_stage<1, 2>(c, vs, pitch, lo, n, scale, red);
-    else if (G.K <= 16384) gemv_q8_stage<1, 8>(c, vs, pitch, lo, n, scale, red);
-    else gemv_q8_stage<1, 0>(c, vs, pitch, lo, n, scale, red);
-  } else if (G.K <= 4096) gemv_q8_stage<0, 2>(c, vs, pitch, lo, n, scale, red);
-  else gemv_q8_stage<0, 0>(c, vs, pitch, lo, n, scale, red);
+#define KVM_STAGE(F, N) gemv_q8_stage<F, N>(c, vs, pitch, lo, n, scale, red)
+  if (G.K <= 4096) { if (form == 1) KVM_STAGE(1, 2); else if (form == 2) KVM_STAGE(2, 2); else if (form == 3) KVM_STAGE(3, 2); else KVM_STAGE(0, 0); }
+  else if (G.K <= 16384 && form) { if (form == 1) KVM_STAGE(1, 8); else if (form == 2) KVM_STAGE(2, 8); else KVM_STAGE(3, 8); }
+  else if (form == 1) KVM_STAGE(1, 0);
+  else if (form >= 2) KVM_STAGE(3, 0);
+  else KVM_STAGE(0, 0);
+#undef KVM_STAGE
 }
 // LDS of one call with a ring of R steps a wave: [ring][rows: M x 2 KC bytes][scales][reductions][sums: 4 x blocks x M x 16], blocks the 16-output
 // blocks of the task, at most GV_GRP. KC (pairs of bytes): the largest part of K in whole steps of all waves that fits.

@@ -33,7 +33,7 @@ __device__ __forceinline__ int q8_of(float x, float s, float inv) {
   return x < 0.f ? -q : q;
 }
 // Eight values of a block of scale s as two words of bytes, the lowest first. x / s is rounded by adding 1.5 * 2^23, exactly so where
-// x * inv is not within 2^-12 of the middle between two whole numbers (it is off by 127 * 2^-22 at most), by q8_of in the others.
+// x * inv is not within 2^-14 of the middle between two whole numbers (it is off by 127 * 2^-22 at most), by q8_of in the others.
 // A NaN scale (or 0) comes with inv = 0.
 __device__ __forceinline__ void q8_pack(const float (&x)[8], float s, float inv, uint32_t& w0, uint32_t& w1) {
   constexpr float MAGIC = 12582912.f;
@@ -45,7 +45,7 @@ __device__ __forceinline__ void q8_pack(const float (&x)[8], float s, float inv,
     far = fmaxf(far, fabsf(fmaf(x[e], inv, -(z - MAGIC))));
     y[e] = __float_as_uint(z);
   }
-  if (far > 0.5f - 0x1p-12f)
+  if (far > 0.5f - 0x1p-14f)
 #pragma unroll
     for (int e = 0; e < 8; ++e) y[e] = (uint32_t)q8_of(x[e], s, inv);
   w0 = __builtin_amdgcn_perm(__builtin_amdgcn_perm(y[3], y[2], 0x0c0c0400u), __builtin_amdgcn_perm(y[1], y[0], 0x0c0c0400u), 0x05040100u);

@@ -22,7 +22,8 @@ def words(q, width):
 
 # (rows, K, pro, dtype, columns of x): one value, ragged and whole rows, every form of the kernel (4,096 and 16,384 values a row, longer, unaligned)
 ROWS = [(1, 1, 0, 'f32', 1), (5, 7, 1, 'bf16', 8), (3, 60, 2, 'bf16', 64), (9, 1001, 0, 'f32', 1001), (6, 1001, 1, 'bf16', 1008), (7, 4096, 1, 'bf16', 4096),
-        (3, 4099, 1, 'f32', 4100), (2, 12288, 2, 'bf16', 12288), (3, 16384, 1, 'f32', 16384), (2, 16390, 1, 'bf16', 16392), (2, 20001, 2, 'f32', 20001)]
+        (3, 4099, 1, 'f32', 4100), (2, 12288, 2, 'bf16', 12288), (3, 16384, 1, 'f32', 16384), (2, 16390, 1, 'bf16', 16392), (2, 20001, 2, 'f32', 20001),
+        (21, 1001, 1, 'bf16', 1001), (5, 777, 2, 'bf16', 777), (3, 5003, 1, 'bf16', 5003), (2, 16401, 2, 'bf16', 16401), (9, 1002, 0, 'bf16', 1002), (4, 12288, 2, 'f32', 12288)]
 
 
 def rows_case(case, seed=0):
