@@ -14,6 +14,13 @@ With `cache='q8'` the KV cache is held in 8 bits: the step appends its keys (nor
 kv_append_q8 and attends with attn_decode_q8 (the layers share its workspace). With a repetition, frequency or presence
 penalty the logits go through logits_adjust before the argmax: every sequence's tokens stand in `hist` (the prompt's `ctx`
 first, as the caller writes them there), its penalties in `par`, and the step adds the token it was given.
+
+With `cache='paged'` a step takes prompts and single tokens together: `rows` new tokens of any of the `batch` sequences, the weights and
+the rows in front of every product in 8 bits (rows_q8 -> matmul_q8 or gemv_q8), the cache in pages (qkv_append_paged, attn_paged).
+The caller writes, between launches, `tok` (the new tokens, sequence after sequence), `cu` (where each sequence's start), `last` (the
+row of each sequence's last one), `lens` (tokens in the cache before the step) and `table` (each sequence's pages) and reads the next token
+of every sequence that had one from `next`. With rows = 0 the step is a decode step: a token of every sequence, its successor goes to
+`tok` and `lens` grows by itself. The weights are the caller's (serving.quantise_rows), zeros until written.
 """
 from __future__ import annotations
 
@@ -47,8 +54,11 @@ class Qwen3Config:
     #                            projection, in place of the gate / up GEMVs and the silu_mul phase (batch 8: 7.19 vs 7.27
     #                            ms). Batch 1 keeps the gate / up GEMVs (inlined in the static kernel; op 311 runs through
     #                            the dispatcher there: 5.03 vs 4.87 ms).
-    cache: str = 'bf16'        # the KV cache: 'bf16', or 'q8' (8 bits, a scale for every block of kv_block tokens)
+    cache: str = 'bf16'        # the KV cache: 'bf16', 'q8' (8 bits, a scale for every block of kv_block tokens) or 'paged' (and 8-bit weights)
     kv_block: int = 64         # cache='q8': tokens of a block
+    page: int = 64             # cache='paged': tokens of a page
+    pages: int = 0             # cache='paged': pages of each layer's cache; 0 = room for ctx + max_new tokens of every sequence
+    rows: int = 0              # cache='paged': new tokens of a step, of any sequence; 0 = one of each (a decode step that continues by itself)
     repetition: float = 1.0    # penalties on tokens of the prompt and of the answer (1, 0, 0: none; rows of `par` may differ later)
     frequency: float = 0.0
     presence: float = 0.0
@@ -68,18 +78,87 @@ def weight_elems(c: Qwen3Config) -> int:
     return c.layers * per_layer + c.vocab * D
 
 
+def _build_paged(c: Qwen3Config, adjust: bool) -> Workload:
+    """The step over paged caches with 8-bit weights."""
+    b = Builder(c.seed)
+    B, D, H, Hkv, hd, F, V, P = c.batch, c.hidden, c.heads, c.kv_heads, c.head_dim, c.ffn, c.vocab, c.tasks_per_phase
+    R, decode = c.rows or c.batch, not c.rows
+    if adjust:
+        raise ValueError("cache='paged' has no penalties: a step's tokens may be a prompt's")
+    if c.rows < 0 or c.pages < 0:
+        raise ValueError(f'rows and pages must not be negative: {c.rows}, {c.pages}')
+    width = -(-(c.ctx + max(c.max_new, R)) // c.page)                   # pages of a sequence
+    pages = c.pages or B * width
+    if pages < width:
+        raise ValueError(f'{pages} pages do not hold one sequence of {width}')
+    start = [R * i // B for i in range(B + 1)]                          # until the caller writes its own: the rows shared out evenly
+    b.values('tok', [(7919 * (i + 1)) % V for i in range(R)], R, 1, 'i32')
+    b.values('lens', [c.ctx] * B, B, 1, 'i32')
+    b.values('cu', start, B + 1, 1, 'i32')
+    b.values('last', [max(0, x - 1) for x in start[1:]], B, 1, 'i32')
+    b.values('table', [i % pages for i in range(B * width)], B, width, 'i32')
+    b.fill('next', B, 1, 'i32')
+    b.normal('wte', V, D, 'f32')
+    b.fill('x', R, D), b.fill('xl', B, D), b.fill('logits', B, V)
+    for n, cols in (('q', H * hd), ('k', Hkv * hd), ('v', Hkv * hd), ('att', H * hd), ('g', F), ('u', F)):
+        b.fill(n, R, cols, 'bf16')
+    space = {K: serving.rows_q8_buffers(b, f'rows{K}', R, K) for K in sorted({D, H * hd, F})} if R > 1 else {}     # one row: inside the products
+    weight = lambda n, N, K: serving.weight_q8_buffers(b, n, N, K)      # noqa: E731
+    layers = []
+    for l in range(c.layers):
+        b.fill(f'ln1.{l}', D, value=1.0), b.fill(f'ln2.{l}', D, value=1.0)
+        b.fill(f'qn.{l}', hd, value=1.0), b.fill(f'kn.{l}', hd, value=1.0)
+        w = {n: weight(f'w{n}.{l}', N, K) for n, N, K in (('q', H * hd, D), ('k', Hkv * hd, D), ('v', Hkv * hd, D), ('o', D, H * hd), ('g', F, D), ('u', F, D), ('d', D, F))}
+        layers.append((w, serving.paged_buffers(b, f'cache{l}.', pages, Hkv, hd, c.page)))
+    b.fill('lnf', D, value=1.0)
+    head = weight('whead', V, D)
+
+    def linear(x, outs, after, res=None, **pro):
+        """The products of x with `outs`, {buffer: weights}, from the same rows in 8 bits, the tasks of a phase shared by their size."""
+        K, total = next(iter(outs.values())).K, sum(w.rows for w in outs.values())
+        if R > 1:
+            after = b.join(serving.rows_q8(b, x, space[K], R, after=after, eps=c.eps, tasks=P, **pro), P)
+            x, pro = space[K], {}
+        return [t for o, w in outs.items() for t in serving.linear_q8(b, x, w, o, R, after=after, res=res, eps=c.eps if pro else 0.0,
+                                                                      tasks=max(1, round(P * w.rows / total)), **pro)]
+
+    prev = [b.task('embedding_fwd', ids='tok', wte='wte', wpe=None, out='x', r0=r0, r1=r1, T=1, d=D) for r0, r1 in split(R, P)]
+    for l, (w, cache) in enumerate(layers):
+        at = linear('x', {n: w[n] for n in 'qkv'}, b.join(prev, P), gamma=f'ln1.{l}')
+        at = serving.qkv_append_paged(b, cache, 'k', 'v', 'table', 'lens', 'cu', q='q', heads=H, qgamma=f'qn.{l}', kgamma=f'kn.{l}', theta=c.theta, eps=c.eps,
+                                      after=b.join(at, P), tasks=P)
+        attended = serving.attn_paged(b, cache, 'q', 'att', 'table', 'lens', 'cu', H, n_max=1 if decode else 0, after=b.join(at, P), tasks=P,
+                                      **({'part': 'att.part', 'cnt': 'att.cnt'} if l else {}))
+        at = linear('att', {'x': w['o']}, b.join(attended, P), res='x')
+        at = linear('x', {n: w[n] for n in 'gu'}, b.join(at, P), gamma=f'ln2.{l}')
+        prev = linear('g', {'x': w['d']}, b.join(at, P), res='x', x2='u')
+    at = [b.task('gather_rows', after=b.join(prev, P), src='x', idx='last', dst='xl', r0=r0, r1=r1, d=D) for r0, r1 in split(B, P)]
+    at = serving.linear_q8(b, 'xl', head, 'logits', B, after=b.join(at, P), gamma='lnf', eps=c.eps, tasks=c.head_tasks or P)
+    at = b.join(at, B)
+    for s in range(B):
+        b.task('argmax', after=at, logits='logits', out='tok' if decode else 'next', r0=s, r1=s + 1, V=V)
+    if decode:
+        b.task('counter_inc', after=attended, x='lens', i0=0, i1=B, delta=1)
+    info = {'config': asdict(c), 'weight_bytes': weight_elems(c), 'kv_bytes_per_step': c.layers * 2 * B * Hkv * (c.ctx + 1) * hd * 2}
+    return Workload(b.spec('step'), b.init_override, info)
+
+
 def build(c: Qwen3Config) -> Workload:
+    adjust = (c.repetition, c.frequency, c.presence) != (1.0, 0.0, 0.0)
+    if c.cache == 'paged':
+        return _build_paged(c, adjust)
+    if c.rows or c.pages:
+        raise ValueError("rows and pages go with cache='paged'")
     b = Builder(c.seed)
     B, D, H, Hkv, hd, F, V = c.batch, c.hidden, c.heads, c.kv_heads, c.head_dim, c.ffn, c.vocab
     Tmax = c.ctx + c.max_new
     S = c.splits or max(1, 256 // (B * Hkv))   # B * Hkv * S = 256 part tasks: one round of the workers
     rows_mode = B > 1
     if c.cache not in ('bf16', 'q8'):
-        raise ValueError(f"cache must be 'bf16' or 'q8': {c.cache!r}")
+        raise ValueError(f"cache must be 'bf16', 'q8' or 'paged': {c.cache!r}")
     if not c.repetition > 0:
         raise ValueError(f'repetition must be positive: {c.repetition}')
     q8 = c.cache == 'q8'
-    adjust = (c.repetition, c.frequency, c.presence) != (1.0, 0.0, 0.0)
     # ---- buffers
     b.values('tok', [(7919 * (i + 1)) % V for i in range(B)], B, 1, 'i32')
     b.values('lens', [c.ctx] * B, B, 1, 'i32')

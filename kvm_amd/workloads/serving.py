@@ -109,6 +109,20 @@ def rows_q8_buffers(b: Builder, name: str, rows: int, K: int) -> RowsQ8:
 weight_q8_buffers = rows_q8_buffers
 
 
+def quantise_rows(x) -> tuple:
+    """(words, scales) of an array [rows, K], what the operator rows_q8 makes of it: the contents of weight_q8_buffers."""
+    import numpy as np
+    x = np.asarray(x, np.float32)
+    with np.errstate(invalid='ignore', over='ignore'):
+        scale = (np.abs(x).max(1, keepdims=True) * np.float32(1 / 127)).astype(np.float32)
+        scale[scale < np.finfo(np.float32).tiny] = 0
+        fine = np.isfinite(x).all(1, keepdims=True)
+        q = np.where(fine & (scale > 0), np.rint(x.astype(np.float64) / np.where(scale > 0, scale, 1).astype(np.float64)), 0)
+    words = np.zeros((x.shape[0], 16 * -(-x.shape[1] // 16)), np.int8)
+    words[:, :x.shape[1]] = q
+    return words.view(np.int32), np.where(fine, scale, np.float32(np.nan))[:, 0]
+
+
 def _pro(gamma, x2) -> int:
     if gamma and x2:
         raise ValueError('gamma (RMSNorm) and x2 (SwiGLU) exclude each other')
