@@ -155,6 +155,7 @@ __device__ __forceinline__ void q8_rows(const RowsSrc& S, RowsRaw<FORM, NV, RB>&
   for (int i = 0; i < RB; ++i)
 #pragma unroll
     for (int u = 0; u < NV; ++u) {
+      if (NV > 2 && u * 8 * KVM_THREADS >= S.K) break;
       raw.x[i][u].get(S.x, r0 + min(i, nr - 1), tid() + u * KVM_THREADS, S.K, v[i][u]);
       if (S.pro == 1 && i < nr)
 #pragma unroll
@@ -175,6 +176,7 @@ __device__ __forceinline__ void q8_rows(const RowsSrc& S, RowsRaw<FORM, NV, RB>&
     const float rstd = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(mine), i));
 #pragma unroll
     for (int u = 0; u < NV; ++u) {
+      if (NV > 2 && u * 8 * KVM_THREADS >= S.K) break;
       raw.shape(S, r0 + i, i, u, tid() + u * KVM_THREADS, rstd, v[i][u]);
       big[i] = q8_big(v[i][u], big[i]);
     }
@@ -188,6 +190,7 @@ __device__ __forceinline__ void q8_rows(const RowsSrc& S, RowsRaw<FORM, NV, RB>&
     if (tid() == 0) scaled(i, s);
 #pragma unroll
     for (int u = 0; u < NV; ++u) {
+      if (NV > 2 && u * 8 * KVM_THREADS >= S.K) break;
       uint32_t w0, w1;
       q8_pack(v[i][u], s, inv, w0, w1);
       if (tid() + u * KVM_THREADS < nvec) put(i, tid() + u * KVM_THREADS, w0, w1);

@@ -120,7 +120,7 @@ def _build_paged(c: Qwen3Config, adjust: bool) -> Workload:
             after = b.join(serving.rows_q8(b, x, space[K], R, after=after, eps=c.eps, tasks=P, **pro), P)
             x, pro = space[K], {}
         return [t for o, w in outs.items() for t in serving.linear_q8(b, x, w, o, R, after=after, res=res, eps=c.eps if pro else 0.0,
-                                                                      tasks=max(1, round(P * w.rows / total)), **pro)]
+                                                                      tasks=max(1, P * w.rows // total), **pro)]
 
     prev = [b.task('embedding_fwd', ids='tok', wte='wte', wpe=None, out='x', r0=r0, r1=r1, T=1, d=D) for r0, r1 in split(R, P)]
     for l, (w, cache) in enumerate(layers):
