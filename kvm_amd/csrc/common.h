@@ -109,7 +109,7 @@ struct KvmSchedDev {
 };
 
 struct KvmRec;
-// Counts that the tasks of a launch leave at 0 when all of them have run (the arrivals of ops 310 and 313).
+// Counts that the tasks of a launch leave at 0 when all of them have run (the arrivals of ops 310, 313 and 319).
 struct KvmCountRange { int* p; long long n; };
 
 struct KvmDevState {

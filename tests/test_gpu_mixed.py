@@ -206,6 +206,18 @@ def test_attend_long(case, tasks):
     _attend(case, tasks=tasks, times=3, n_max=max(case[6]))
 
 
+@pytest.mark.parametrize('case', [(64, 128, 2, 8, 'bf16', [3000, 100], [3, 1]), (16, 64, 1, 4, 'bf16', [3000, 7], [70, 5]), (16, 64, 2, 4, 'f32', [3000], [9]),
+                                  (64, 100, 1, 3, 'f32', [2500], [4])], ids=str)
+@pytest.mark.parametrize('tasks', [2, 9, 256])
+def test_attend_more_tokens_than_the_hint(case, tasks):
+    """Tiles hold no more rows than the partials have room for: sequences that bring more tokens than n_max are taken in more tiles."""
+    print(f'attend hint {case} {tasks}', flush=True)
+    (lb, _), _, _ = mg.attend_graph(case, np.random.default_rng(2), tasks=tasks, n_max=1)
+    group = case[3] // case[2]
+    assert next(m for m in lb.metadata['buffers'] if m['name'] == 'o.part')['rows'] == 2 * tasks * group
+    _attend(case, tasks=tasks, n_max=1)
+
+
 @pytest.mark.parametrize('case', [mg.ATTENDS[1], mg.ATTENDS[2], mg.ATTENDS[5], mg.ATTENDS[7], mg.ATTENDS[9]], ids=str)
 @pytest.mark.parametrize('bad', [np.nan, np.inf, -np.inf])
 def test_what_a_row_does_not_see(case, bad):
