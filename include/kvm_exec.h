@@ -142,7 +142,7 @@ int kvm_submit_stream(KvmExec* ex, const MvmTaskDesc* tasks, int ntasks, const i
 // Waits for the launch, then fills `res` (reference: close/finish, mvm_exec.cu:1505-1540). Every task's stores are out by then, the
 // kernel itself may still be ending (work on the executor's stream comes behind it). The calling thread polls the launch's report
 // for up to 500 us, after that it waits with the stream. HIP errors that other calls left with the thread are not looked at. After a device
-// error the next launch starts clean, the arrival counts of ops 310 and 313 included.
+// error the next launch starts clean, the arrival counts of ops 310, 313 and 319 included.
 int kvm_finish(KvmExec* ex, KvmResult* res);
 // Runs the whole submitted graph again on the current buffer contents (versions restart from their set values):
 // reset + launch, asynchronous. Used for repeated training steps / decode tokens; kvm_finish collects it.
