@@ -117,24 +117,26 @@ def _build_paged(c: Qwen3Config, adjust: bool) -> Workload:
         """The products of x with `outs`, {buffer: weights}, from the same rows in 8 bits, the tasks of a phase shared by their size."""
         K, total = next(iter(outs.values())).K, sum(w.rows for w in outs.values())
         if R > 1:
-            after = b.join(serving.rows_q8(b, x, space[K], R, after=after, eps=c.eps, tasks=P, **pro), P)
+            after = serving.after_all(b, serving.rows_q8(b, x, space[K], R, after=serving.after_all(b, after, min(R, P)), eps=c.eps, tasks=P, **pro), P)
             x, pro = space[K], {}
+        else:
+            after = serving.after_all(b, after, P)
         return [t for o, w in outs.items() for t in serving.linear_q8(b, x, w, o, R, after=after, res=res, eps=c.eps if pro else 0.0,
                                                                       tasks=max(1, P * w.rows // total), **pro)]
 
     prev = [b.task('embedding_fwd', ids='tok', wte='wte', wpe=None, out='x', r0=r0, r1=r1, T=1, d=D) for r0, r1 in split(R, P)]
     for l, (w, cache) in enumerate(layers):
-        at = linear('x', {n: w[n] for n in 'qkv'}, b.join(prev, P), gamma=f'ln1.{l}')
+        at = linear('x', {n: w[n] for n in 'qkv'}, prev, gamma=f'ln1.{l}')
         at = serving.qkv_append_paged(b, cache, 'k', 'v', 'table', 'lens', 'cu', q='q', heads=H, qgamma=f'qn.{l}', kgamma=f'kn.{l}', theta=c.theta, eps=c.eps,
-                                      after=b.join(at, P), tasks=P)
-        attended = serving.attn_paged(b, cache, 'q', 'att', 'table', 'lens', 'cu', H, n_max=1 if decode else 0, after=b.join(at, P), tasks=P,
+                                      after=serving.after_all(b, at, min(R, P)), tasks=P)
+        attended = serving.attn_paged(b, cache, 'q', 'att', 'table', 'lens', 'cu', H, n_max=1 if decode else 0, after=serving.after_all(b, at, P), tasks=P,
                                       **({'part': 'att.part', 'cnt': 'att.cnt'} if l else {}))
-        at = linear('att', {'x': w['o']}, b.join(attended, P), res='x')
-        at = linear('x', {n: w[n] for n in 'gu'}, b.join(at, P), gamma=f'ln2.{l}')
-        prev = linear('g', {'x': w['d']}, b.join(at, P), res='x', x2='u')
-    at = [b.task('gather_rows', after=b.join(prev, P), src='x', idx='last', dst='xl', r0=r0, r1=r1, d=D) for r0, r1 in split(B, P)]
-    at = serving.linear_q8(b, 'xl', head, 'logits', B, after=b.join(at, P), gamma='lnf', eps=c.eps, tasks=c.head_tasks or P)
-    at = b.join(at, B)
+        at = linear('att', {'x': w['o']}, attended, res='x')
+        at = linear('x', {n: w[n] for n in 'gu'}, at, gamma=f'ln2.{l}')
+        prev = linear('g', {'x': w['d']}, at, res='x', x2='u')
+    at = [b.task('gather_rows', after=serving.after_all(b, prev, min(B, P)), src='x', idx='last', dst='xl', r0=r0, r1=r1, d=D) for r0, r1 in split(B, P)]
+    at = serving.linear_q8(b, 'xl', head, 'logits', B, after=serving.after_all(b, at, c.head_tasks or P), gamma='lnf', eps=c.eps, tasks=c.head_tasks or P)
+    at = serving.after_all(b, at, B)
     for s in range(B):
         b.task('argmax', after=at, logits='logits', out='tok' if decode else 'next', r0=s, r1=s + 1, V=V)
     if decode:

@@ -109,6 +109,14 @@ def rows_q8_buffers(b: Builder, name: str, rows: int, K: int) -> RowsQ8:
 weight_q8_buffers = rows_q8_buffers
 
 
+EDGES = 4096
+
+
+def after_all(b: Builder, preds: list[str], n: int) -> list[str]:
+    """What `n` tasks that need all of `preds` wait for: these, where that is few edges, else one task between (a hop of its own)."""
+    return preds if len(preds) * n <= EDGES else b.join(preds, n)
+
+
 def quantise_rows(x) -> tuple:
     """(words, scales) of an array [rows, K], what the operator rows_q8 makes of it: the contents of weight_q8_buffers."""
     import numpy as np
@@ -159,7 +167,7 @@ def linear_q8(b: Builder, x: str, w: RowsQ8, out: str, M: int, after=(), x2: str
             rows = RowsQ8(out + '.x', out + '.xs', M, K) if b.has(out + '.x') else rows_q8_buffers(b, out + '.x', M, K)
         if rows.K != K or rows.rows < M:
             raise ValueError(f'the workspace holds {rows.rows} rows of {rows.K} bytes: {M} rows of {K} needed')
-        after = b.join(rows_q8(b, x, rows, M, after, x2, gamma, eps, tasks), tasks)
+        after = after_all(b, rows_q8(b, x, rows, M, after, x2, gamma, eps, tasks), tasks)
     kw = dict(w=w.q, sw=w.s, out=out, bias=bias, res=res, K=K)
     if M <= 16:
         if rows is None:
