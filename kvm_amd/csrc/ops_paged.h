@@ -589,7 +589,7 @@ __device__ __noinline__ int attn_paged_general(const Ctx& c, int b_, int h_, int
       for (int i = 0; i < 4; ++i) {
         const int key = kb + 4 * sub + i;
         const bool on = key <= lim && key < p.k1;
-        const float e = on ? exp2f(x[i] - top) : -1.f;
+        const float e = !on ? -1.f : x[i] == -INFINITY ? 0.f : exp2f(x[i] - top);   // (all of a block may be -inf, and later ones not)
         if (on) sum += e;
         ps[row * (KB + 4) + 4 * sub + i] = e;
       }

@@ -245,6 +245,23 @@ def test_what_a_row_does_not_see(case, bad):
     f64.near(got[fine], want[fine], mg.attend_bound(case, mag, sabs, case[4] == 'f32')[fine], case[4])
 
 
+@pytest.mark.parametrize('case', [(64, 100, 1, 3, 'f32', [300], [2]), (16, 64, 1, 4, 'f32', [300], [1]), (64, 128, 1, 4, 'bf16', [300], [3]), (32, 128, 1, 2, 'bf16', [300], [70]),
+                                  (16, 6, 1, 1, 'bf16', [3000], [1])], ids=str)
+@pytest.mark.parametrize('tasks', [1, 32])
+def test_seen_keys_of_score_minus_infinity(case, tasks):
+    """Keys whose score is -inf have no weight where another key's is finite, also where they fill a block."""
+    print(f'attend -inf {case} {tasks}', flush=True)
+    page, hd, hkv, heads, dt, lens, new = case
+    rng = np.random.default_rng(4)
+
+    def kv(kc, vc, table):
+        t = np.arange(200)
+        kc[table[0, t // page], :, t % page, 0] = -np.inf
+        return kc, vc
+    q = lambda rows: mg.bf(np.abs(rng.standard_normal((rows, heads, hd))) + 0.1, dt)   # noqa: E731
+    _attend(case, tasks=tasks, kv=kv, q=q)
+
+
 def test_attend_large_scores():
     """Scores in the thousands: a weight of one, the others nothing."""
     print('attend large scores', flush=True)
