@@ -89,6 +89,31 @@ def test_after_a_stopped_call_on_own_buffers():
     ex.close()
 
 
+@pytest.mark.parametrize('path', [PATH_STATIC, PATH_DYNAMIC])
+@pytest.mark.parametrize('M', [1, 5, 40])
+def test_weights_of_the_same_graph(M, path):
+    """Weights that a task in front brings to 8 bits are not read before it has, launch after launch."""
+    print(f'weights of the same graph {M} path {path}', flush=True)
+    N, K = 500, 1040
+    rng = np.random.default_rng(6)
+    b, data = Builder(0), {}
+    sg.add(b, data, 'x', rng.standard_normal((M, K)).astype(np.float32)), sg.add(b, data, 'raw', np.zeros((N, K), np.float32))
+    w = serving.weight_q8_buffers(b, 'w', N, K)
+    b.fill('out', M, N)
+    serving.linear_q8(b, 'x', w, 'out', M, after=serving.rows_q8(b, 'raw', w, N))
+    lb, init = sg.compiled(b, data)
+    ex = Executor.from_bundle(lb, buffers=init, path=path)
+    x = f64.quantise(data['x'])
+    for _ in range(4):
+        raw = rng.standard_normal((N, K)).astype(np.float32)
+        ex.write('raw', raw)
+        ex.relaunch()
+        ex.finish()
+        want, bound = f64.product(*x, *f64.quantise(raw))
+        f64.near(ex.read('out').reshape(M, N), want, bound, 'f32')
+    ex.close()
+
+
 def _buffers(b):
     lb = bl.load(compiler.compile_spec(b.spec()))
     return lb, {m['name']: torch.zeros((m['rows'], m['cols']), dtype=TORCH[m['dtype']], device='cuda') for m in lb.metadata['buffers']}
