@@ -164,7 +164,7 @@ __device__ void publish(const KvmDevState& S, int slot, int var, int ver) {
   if (!__hip_atomic_compare_exchange_strong(&S.version[var], &expect, ver, __ATOMIC_ACQ_REL, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) {
     int z = 0;
     if (__hip_atomic_compare_exchange_strong(&S.cnt->err_code, &z, (int)KVM_ERR_VERSION_GAP, __ATOMIC_RELAXED, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) {
-      S.cnt->err_slot = slot; S.cnt->err_a = expect; S.cnt->err_b = ver;
+      st_relaxed(&S.cnt->err_slot, slot); st_relaxed(&S.cnt->err_a, expect); st_relaxed(&S.cnt->err_b, ver);   // (write-through: a function of its own)
     }
     return;
   }
