@@ -164,6 +164,7 @@ static void cache_paged(Check& k) {
   k.need(page == 16 || page == 32 || page == 64 || page == 128, "page must be 16, 32, 64 or 128");
   k.need(hd > 0 && hd <= 256 && hd % 2 == 0, "hd must be even, up to 256");
   k.need(B > 0 && B <= 1024 && Hkv > 0, "B must be 1 .. 1024, Hkv positive");
+  k.need(k.I("H") <= 65536 && Hkv <= 65536, "H and Hkv must be at most 65536");   // (rows in flight times heads stay below 2^31)
   const MvmBuf *kc = k.B("kc"), *vc = k.B("vc"), *tb = k.B("table");
   if (!kc || !vc || !tb || !k.err.empty()) return;
   k.need(kc->rows == vc->rows && kc->rows >= (long long)Hkv * page, "kc and vc must have the same rows, a page at least");

@@ -164,6 +164,12 @@ def test_attend_refusals(change, what):
     _refused(lb, 'attn_paged', change, what)
 
 
+@pytest.mark.parametrize('change', [{'H': 65537}, {'Hkv': 65537}], ids=str)
+def test_more_heads_than_row_counts_hold(change):
+    _refused(mg.append_graph(mg.APPENDS[2], np.random.default_rng(0))[0][0], 'qkv_append_paged', change, 'at most 65536')
+    _refused(mg.attend_graph(mg.ATTENDS[1], np.random.default_rng(0))[0][0], 'attn_paged', change, 'at most 65536')
+
+
 def test_builder_refusals():
     b = Builder(0)
     with pytest.raises(ValueError, match='page'):
