@@ -692,18 +692,12 @@ __device__ __forceinline__ int paged_waves(const Ctx& c, const AttnPaged& D, con
 //           16-byte load of a key is its part of the operand, and the rows' order makes the scores' registers the B operand of
 //   P V     the same instruction, A = V transposed: a lane loads HD / 16 dims of 8 keys, whole rows of the page to 16 lanes, and turns them
 //           in registers (one byte permute for two values), dims DPL m + i to row m of product i.
-// Probabilities are bf16; the running maximum moves only when a row's grows by more than 2^8. The waves' states
-// meet in LDS. A call: 48 single tokens behind 5,000 others each (0.98 GB) 255 us, 3.9 TB/s; one behind 32,000 64 us, of which launch, the
-// pieces' entry and the merge are 40.
-// The sum of eight bf16 weights onto s: what the second product weighs with is what the row is divided by, so that the rounding of a large weight
-// cancels.
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-__device__ __forceinline__ float sum_bf16(bf16x8 p, float s) {
-  const bf16x2 one = {(__bf16)1.f, (__bf16)1.f};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) s = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{p[2 * i], p[2 * i + 1]}, one, s, false);
-  return s;
-}
+// A probability goes into the second product as two bf16 operands, its rounding and the rounding of what that leaves (16 bits: rounded once to bf16
+// it put the results 0.0023 from 64 bits where the store's own rounding is 0.0017; here the second half of the products costs 1%, the tiles of more
+// rows 13 to 19%); the running maximum moves only when a row's grows by more than 2^8. The waves' states meet in LDS. A call: 48 single tokens
+// behind 5,000 others each (0.98 GB) 241 us, 4.1 TB/s; one behind 32,000 64 us, of which launch, the pieces' entry and the merge are 40.
+// The sum of eight weights onto s.
+__device__ __forceinline__ float sum8(const float (&p)[8], float s) { return s + (((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]))); }
 template <int HD, int NT> __device__ __noinline__ int attn_paged_keys(const Ctx& c, int b_, int h_, int L_, int row0_, int tok0_, int ntok_, int k0_, int k1_, int k_, int live_, int i0_) {
   constexpr int NK = HD / 32, DPL = HD / 16, RW = 16 * NT;
   const AttnPaged D(c);
@@ -805,10 +799,12 @@ template <int HD, int NT> __device__ __noinline__ int attn_paged_keys(const Ctx&
       float pv[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) pv[i] = __builtin_amdgcn_exp2f(x[i] - base);
-      const bf16x8 pb = pack_bf16(pv);
-      ls[n] = sum_bf16(pb, ls[n]);
+      const Pieces<2> pb = split_bf16<2>(pv);
+      ls[n] = sum8(pv, ls[n]);
 #pragma unroll
-      for (int i = 0; i < DPL; ++i) acc[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vt[i], pb, acc[n][i], 0, 0, 0);
+      for (int k = 1; k >= 0; --k)
+#pragma unroll
+        for (int i = 0; i < DPL; ++i) acc[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vt[i], pb.p[k], acc[n][i], 0, 0, 0);
     }
   };
   if (w < nu) {
@@ -943,9 +939,9 @@ template <int HD, int NT> __device__ __noinline__ int attn_paged_keys_f32(const 
 // 64 keys come from the pages straight into LDS for all of them, three stages, the places of up to PG_IDS pieces of pages in LDS. In transposed
 // space: S^T = K Q^T by v_mfma_f32_32x32x16_bf16 (a lane owns a query row), O^T += V^T P^T with P^T's registers as they are. V lies row by row;
 // a lane reads HD / 32 dims of 8 keys and turns them in registers (a byte permute for two values), dims HD / 32 * m + i to row m of product i:
-// transposing reads of LDS run at a third of the rate. 32 keys at a time, the scores of the next ones under the softmax of these: with 64 the
-// fragments and scores under way pass 256 registers. A block of 64 keys takes 128 rows 1.9 us (565 TFLOP/s over 256 CUs), some 520 instructions
-// a wave of which 32 are products; 1,000 tokens of 32 heads behind 3,750 185 us a call.
+// transposing reads of LDS run at a third of the rate. P^T is two operands, as above. 32 keys at a time, the scores of the next ones under the
+// softmax of these: with 64 the fragments and scores under way pass 256 registers. A block of 64 keys takes 128 rows 2.3 us (470 TFLOP/s over
+// 256 CUs; 1.9 with P^T rounded once), some 630 instructions a wave of which 48 are products; 1,000 tokens of 32 heads behind 3,750 271 us a call.
 constexpr int PG_IDS = 2048, PG_NS = 3;
 __device__ __forceinline__ void dma16_at(unsigned long long src, unsigned dst) {   // 16 bytes a lane from its own address to LDS byte dst (uniform) + 16 * lane
   asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" :: "s"(dst), "v"(src) : "memory", "m0");
@@ -1080,7 +1076,7 @@ template <int HD> __device__ __noinline__ int attn_paged_rows(const Ctx& c, int 
         m = top;
       }
       const float base = m == -INFINITY ? 0.f : m;
-      bf16x8 pf[2];
+      Pieces<2> pf[2];
       float ps = 0.f;
       sn = f32x16{};
       // a product of the next scores, two exponentials and what belongs to them, in turn; then the products of P, their operands and the reads
@@ -1090,8 +1086,8 @@ template <int HD> __device__ __noinline__ int attn_paged_rows(const Ctx& c, int 
         float pv[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) pv[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sa[8 * u + i], D.sl2, -base));
-        pf[u] = pack_bf16(pv);
-        ps = sum_bf16(pf[u], ps);
+        pf[u] = split_bf16<2>(pv);
+        ps = sum8(pv, ps);
       }
 #pragma unroll
       for (int kk = 0; kk < NKK; ++kk) sn = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kfr[kk], qf[kk], sn, 0, 0, 0);
@@ -1099,7 +1095,7 @@ template <int HD> __device__ __noinline__ int attn_paged_rows(const Ctx& c, int 
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int d = 0; d < NDB; ++d) oacc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vt[u].turned(d), pf[u], oacc[d], 0, 0, 0);
+        for (int d = 0; d < NDB; ++d) oacc[d] = mfma_pieces(vt[u].turned(d), pf[u], oacc[d]);
       read(Kn, nk, Vn, vk);
 #pragma unroll
       for (int i = 0; i < NKK; ++i) {
