@@ -309,7 +309,8 @@ __device__ __forceinline__ GLOBAL float* paged_partial(const AttnPaged& D, const
 __device__ __forceinline__ long long paged_out(const AttnPaged& D, const TilePaged& t, int r) {
   return (long long)(t.row0 + r / D.G) * D.o.cols + (long long)(t.h * D.G + r % D.G) * D.hd;
 }
-// The piece that counts itself last merges the tile's rows, in the pieces' order whichever it is; maxima are in units of log2.
+// The piece that counts itself last merges the tile's rows, in the pieces' order whichever it is; maxima are in units of log2. A piece of weight 0
+// counts too: a NaN or an infinity that a row sees there stays one.
 // Few rows: a thread has four dims of a row and a share of the pieces, 16 of them requested at once with their maxima and sums; the shares meet
 // in LDS. Many rows: first the pieces' weights, to LDS, then four dims of four rows a thread at once.
 template <bool PAIRS> __device__ __forceinline__ f32x4n paged_dims(const GLOBAL float* y, int d, int hd) {
@@ -356,7 +357,7 @@ template <bool PAIRS> __device__ __noinline__ void paged_merge_few(const Ctx& c,
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const float w = paged_weight(m[u], top);
-      if (w != 0.f) { a += w * x[u]; z += w * s[u]; }
+      a += w * x[u]; z += w * s[u];                                    // (behind the last piece: that one again, with weight 0)
     }
   }
   LDS float* sh = (LDS float*)(c.smem + PG_WORK);                      // [256][6]
@@ -408,7 +409,7 @@ template <bool PAIRS, bool TABLE, int NI, int U> __device__ __forceinline__ void
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           const float v = TABLE ? W[min(k0 + u, p.live - 1) * R + r[i]] : paged_weight(w[i][u], M[r[i]]);
-          if (k0 + u < p.live && v != 0.f) a[i] += v * x[i][u];
+          if (k0 + u < p.live) a[i] += v * x[i][u];
         }
     }
 #pragma unroll
@@ -446,7 +447,7 @@ template <bool PAIRS> __device__ __noinline__ void paged_merge_many(const Ctx& c
       for (int k = 0; k < live; ++k) {
         const float w = paged_weight(W[k * R + tid()], top);
         W[k * R + tid()] = w;
-        if (w != 0.f) z += w * S[k * R + tid()];
+        z += w * S[k * R + tid()];
       }
       M[tid()] = top; Z[tid()] = z;
     }
