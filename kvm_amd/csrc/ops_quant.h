@@ -5,6 +5,7 @@
 #include "ops_gemm.h"
 #include "ops_decode.h"
 #include "ops_serve.h"
+#include "gemv_q8_geo.h"
 
 namespace kvm {
 
@@ -495,7 +496,7 @@ struct GemvQ8 {
       : x(uview(c, 0)), x2(uview(c, 1)), g(uview(c, 2)), w(uview(c, 3)), sw(uview(c, 4)), out(uview(c, 5)), bias(uview(c, 6)), res(uview(c, 7)), sx(uview(c, 8)),
         n0(rfl(c.i(9))), n1(rfl(c.i(10))), K(rfl(c.i(11))), M(rfl(c.i(12))), pro(rfl(c.i(13))) { Ke = ((K + 511) >> 9) << 8; }
   __device__ View stream() const { return View{w.p, w.rows, 2 * w.cols, 2, 0}; }
-  __device__ bool fast() const { return q8_fast(w, n1 - n0 + 16, 2 * Ke); }
+  __device__ bool fast() const { return q8_fast(w, n1 - n0 + 16, 4 * Ke); }   // (all parts of K are less than twice as long)
   __device__ void put(int m, int n, int sum, float s) const {
     float y = (float)sum * s;
     y *= sw.f()[n];
@@ -569,15 +570,14 @@ __device__ __forceinline__ void gemv_q8_rows(const Ctx& c, const GemvQ8& G, LDS 
 #undef KVM_STAGE
 }
 // LDS of one call with a ring of R steps a wave: [ring][rows: M x 2 KC bytes][scales][reductions][sums: 4 x blocks x M x 16], blocks the 16-output
-// blocks of the task, at most GV_GRP. KC (pairs of bytes): the largest part of K in whole steps of all waves that fits.
-struct GqGeo { int KC, pitch, vs, scale, red, part, grp; };
+// blocks of the task, at most GV_GRP. KC (pairs of bytes): a part of K in whole steps of all waves, K all parts of it together.
+struct GqGeo { int K, KC, pitch, vs, scale, red, part, grp; };
 __device__ __forceinline__ GqGeo gq_geo(int Ke, int M, int R, int n) {
   GqGeo g;
   g.grp = min((n + 15) >> 4, GV_GRP);
-  const int rest = R * KVM_WAVES * GV_STEP + 64 + Q8_RED * 8 + KVM_WAVES * g.grp * M * 16 * 4, steps = Ke >> 8;
-  int parts = 1;
-  while (parts < steps && (steps % parts || rest + M * (2 * Ke / parts) > KVM_LDS_BYTES)) ++parts;
-  g.KC = Ke / parts; g.pitch = 2 * g.KC;
+  const int rest = R * KVM_WAVES * GV_STEP + 64 + Q8_RED * 8 + KVM_WAVES * g.grp * M * 16 * 4;
+  g.KC = gq_part_steps(Ke >> 8, M * 512, KVM_LDS_BYTES - rest) << 8;
+  g.K = (Ke + g.KC - 1) / g.KC * g.KC; g.pitch = 2 * g.KC;
   g.vs = R * KVM_WAVES * GV_STEP;
   g.scale = g.vs + M * g.pitch;
   g.red = g.scale + 64;
@@ -588,7 +588,8 @@ static_assert(4 * KVM_WAVES * GV_STEP + 64 + Q8_RED * 8 + KVM_WAVES * GV_GRP * 1
 static_assert(12 * KVM_WAVES * GV_STEP + 64 + Q8_RED * 8 + KVM_WAVES * GV_GRP * 4 * 16 * 4 + 4 * 512 <= KVM_LDS_BYTES, "LDS");
 template <int R> __device__ __forceinline__ void gemv_q8_prefetch_r(const GemvQ8& G, LDS char* smem) {
   GvStream<> ws;
-  ws.init(G.stream(), G.n0, G.n1, G.Ke, gq_geo(G.Ke, G.M, R, G.n1 - G.n0).KC);
+  const GqGeo geo = gq_geo(G.Ke, G.M, R, G.n1 - G.n0);
+  ws.init(G.stream(), G.n0, G.n1, geo.K, geo.KC);
   LDS char* ring = smem + wave() * R * GV_STEP;
 #pragma unroll
   for (int j = 0; j < R; ++j) ws.template issue<R>(ring);
@@ -601,9 +602,9 @@ __device__ __noinline__ void gemv_q8_prefetch(const Ctx& c) {
 }
 template <int R> __device__ __noinline__ void gemv_q8_stream(const Ctx& c) {
   const GemvQ8 G(c);
-  const int M = G.M, K = G.Ke, PM = 16 * M;                                     // K in pairs of bytes
-  const GqGeo geo = gq_geo(K, M, R, G.n1 - G.n0);
-  const int KC = geo.KC;
+  const int M = G.M, PM = 16 * M;
+  const GqGeo geo = gq_geo(G.Ke, M, R, G.n1 - G.n0);
+  const int K = geo.K, KC = geo.KC;                                             // in pairs of bytes
   LDS char* vs = c.smem + geo.vs;
   LDS float* scale = (LDS float*)(c.smem + geo.scale);
   LDS int* part = (LDS int*)(c.smem + geo.part);
