@@ -143,6 +143,12 @@ def rows_q8(b: Builder, x: str, out: RowsQ8, M: int, after=(), x2: str | None = 
             for r0, r1 in split(M, tasks)]
 
 
+def _workspace(b: Builder, out: str, K: int) -> RowsQ8:
+    """The buffers of an earlier call's workspace, as what they hold: as many rows as both have, of K bytes or of fewer if they are narrower."""
+    (rows, words), (r, c) = _shape(b, out + '.x'), _shape(b, out + '.xs')
+    return RowsQ8(out + '.x', out + '.xs', min(rows, r * c), min(K, 4 * words))
+
+
 def matmul_q8_tile(M: int, N: int, tasks: int = 256) -> tuple[int, int, int]:
     """(tile, rows, columns): the largest tile of which there are about as many as workers. Fewer and larger ones lose (333 x 2,777, K 1,001:
     46 us with 66 tiles of 128 x 128, 40 with 264 of 64 x 64, though those take two rounds)."""
@@ -155,16 +161,19 @@ def matmul_q8_tile(M: int, N: int, tasks: int = 256) -> tuple[int, int, int]:
 def linear_q8(b: Builder, x: str, w: RowsQ8, out: str, M: int, after=(), x2: str | None = None, gamma: str | None = None, bias: str | None = None,
               res: str | None = None, eps: float = 0.0, tasks: int = 256, rows: RowsQ8 | None = None) -> list[str]:
     """out = x' w^T (+ bias) (+ res), the first M rows of x (x' as in rows_q8) and w [N, K] in 8 bits. One row is quantised inside the tasks
-    of the product (gemv_q8), more in a phase of their own, into the workspace `rows` (declared here as out + '.x' when absent; layers that
-    follow each other may share one of the same K). `x` may be rows that are in 8 bits already (RowsQ8)."""
+    of the product (gemv_q8), more in a phase of their own, into the workspace `rows` (declared here as out + '.x' when absent, or that of an
+    earlier call with this `out` if it is large enough; layers that follow each other may share one of the same K). `x` may be rows that are in 8 bits
+    already (RowsQ8)."""
     N, K = w.rows, w.K
     if isinstance(x, RowsQ8):
         if gamma or x2 or x.K != K:
             raise ValueError(f'rows in 8 bits go in as they are, with the K of the weights: K {x.K} and {K}')
+        if x.rows < M:
+            raise ValueError(f'{M} rows of {x.q} wanted, which holds {x.rows} rows')
         rows = x
     elif M > 1:
         if rows is None:
-            rows = RowsQ8(out + '.x', out + '.xs', M, K) if b.has(out + '.x') else rows_q8_buffers(b, out + '.x', M, K)
+            rows = _workspace(b, out, K) if b.has(out + '.x') and b.has(out + '.xs') else rows_q8_buffers(b, out + '.x', M, K)
         if rows.K != K or rows.rows < M:
             raise ValueError(f'the workspace holds {rows.rows} rows of {rows.K} bytes: {M} rows of {K} needed')
         after = after_all(b, rows_q8(b, x, rows, M, after, x2, gamma, eps, tasks), tasks)
