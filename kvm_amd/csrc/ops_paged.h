@@ -242,22 +242,24 @@ struct PiecePaged { int k0, k1, k, live, i0; };
 // The work of a call over its tasks: a tile costs PG_TILE and one per key up to the last that it sees; tiles in order of sequence, kv head
 // and token are cut into equal shares, in all tasks alike from the lengths. A cut within PG_SNAP of a tile's end moves there: a small piece
 // costs more than it balances; where there is a task for every tile and none is longer than a share by PG_CUT, about what the partials and the
-// merge of a cut cost, no tile is cut. Tiles of up to 32 rows are a sequence's new tokens as a whole (the waves share the keys); longer ones have `tile`
-// rows (the waves share the rows).
+// merge of a cut cost, no tile is cut: a tile costs 1 then, a task has one or none, and these are spread over all tasks (shared out by their keys
+// some tasks had two and others none: 1,000 tokens of 32 heads behind 3,750, 256 tiles, 272 us in place of 182). Tiles of up to 32 rows are a
+// sequence's new tokens as a whole (the waves share the keys); longer ones have `tile` rows (the waves share the rows).
 constexpr int PG_TILE = 256, PG_SNAP = 320, PG_SHARE = 512, PG_CUT = 1024;
 struct WorkPaged {
   const LDS long long* pre;    // [B + 1] cost of the sequences before
   const LDS int *cu, *len;
   int B, Hkv, G, rows;
   long long share, total;
-  bool whole;                  // tiles are not cut
+  int S;
+  bool whole;                  // tiles are not cut, the costs are numbers of tiles
   __device__ __forceinline__ int tokens(int n) const { return max(1, min(n, rows / G)); }   // of a tile, whose rows fit in the partials'
   // cost of the first j tiles of TT tokens of one head, none of them the last, ragged one
-  __device__ __forceinline__ static long long upto(long long j, long long L, long long TT) { return j * (PG_TILE + L) + TT * (j * (j + 1) / 2); }
+  __device__ __forceinline__ long long upto(long long j, long long L, long long TT) const { return whole ? j : j * (PG_TILE + L) + TT * (j * (j + 1) / 2); }
   __device__ __forceinline__ long long head_cost(int n, int L) const {
     if (n <= 0) return 0;
     const int TT = tokens(n), nt = (n + TT - 1) / TT;
-    return upto(nt - 1, L, TT) + PG_TILE + L + n;
+    return whole ? nt : upto(nt - 1, L, TT) + PG_TILE + L + n;
   }
   __device__ __forceinline__ TilePaged find(long long x) const {
     int b = 0;
@@ -273,15 +275,15 @@ struct WorkPaged {
     TilePaged t;
     t.b = b; t.h = h; t.L = L; t.row0 = r0 + lo * TT; t.tok0 = lo * TT; t.ntok = min(TT, n - lo * TT);
     t.start = p0 + h * hc + upto(lo, L, TT);
-    t.cost = PG_TILE + (long long)L + t.tok0 + t.ntok;
+    t.cost = whole ? 1 : PG_TILE + (long long)L + t.tok0 + t.ntok;
     return t;
   }
   __device__ __forceinline__ long long cut(int i) const {
+    if (whole) return i == S ? total : (unsigned)i * (unsigned)total / (unsigned)S;   // (i < S and total <= S, at most 65,536)
     const long long x = min(i * share, total);
     if (x == total) return total;
     const TilePaged t = find(x);
     const long long off = x - t.start;
-    if (whole) return off < t.cost - off ? t.start : t.start + t.cost;
     return off < PG_SNAP ? t.start : t.cost - off < PG_SNAP ? t.start + t.cost : x;
   }
   // The piece [x, end) of a tile: its keys, and which of how many pieces it is.
@@ -942,7 +944,7 @@ template <int HD, int NT> __device__ __noinline__ int attn_paged_keys_f32(const 
 // a lane reads HD / 32 dims of 8 keys and turns them in registers (a byte permute for two values), dims HD / 32 * m + i to row m of product i:
 // transposing reads of LDS run at a third of the rate. P^T is two operands, as above. 32 keys at a time, the scores of the next ones under the
 // softmax of these: with 64 the fragments and scores under way pass 256 registers. A block of 64 keys takes 128 rows 2.3 us (470 TFLOP/s over
-// 256 CUs; 1.9 with P^T rounded once), some 630 instructions a wave of which 48 are products; 1,000 tokens of 32 heads behind 3,750 271 us a call.
+// 256 CUs; 1.9 with P^T rounded once), some 630 instructions a wave of which 48 are products; 1,000 tokens of 32 heads behind 3,750 182 us a call.
 constexpr int PG_IDS = 2048, PG_NS = 3;
 __device__ __forceinline__ void dma16_at(unsigned long long src, unsigned dst) {   // 16 bytes a lane from its own address to LDS byte dst (uniform) + 16 * lane
   asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" :: "s"(dst), "v"(src) : "memory", "m0");
@@ -1185,7 +1187,8 @@ __device__ __noinline__ void op_attn_paged(const Ctx& c) {
   W.pre = pre; W.cu = scu; W.len = len; W.B = D.B; W.Hkv = D.Hkv; W.G = D.G;
   const int fast = D.fast();
   W.rows = fast == 2 ? D.tile : min(D.tile, max(32, D.G));             // (the other forms take 32 rows at a time)
-  {
+  W.whole = false; W.S = D.S;
+  for (;;) {                                                           // what the sequences cost and the sums in front of each: in keys, then maybe in tiles
     constexpr int PER = PG_SEQS / KVM_THREADS;
     long long cost[PER], sum = 0, most = 0, tiles = 0;
 #pragma unroll
@@ -1220,10 +1223,13 @@ __device__ __noinline__ void op_attn_paged(const Ctx& c) {
       if (b < D.B) { pre[b] = at; at += cost[i]; if (b == D.B - 1) pre[D.B] = at; }
     }
     __syncthreads();
+    W.total = pre[D.B];
+    if (W.whole) break;
+    W.share = max((W.total + D.S - 1) / D.S, (long long)PG_SHARE);
+    if (rfl(tot[8] + tot[9] + tot[10] + tot[11] > D.S || max(max(tot[4], tot[5]), max(tot[6], tot[7])) > W.share + PG_CUT)) break;
+    W.whole = true;
+    __syncthreads();                                                   // the sums are read
   }
-  W.total = pre[D.B];
-  W.share = max((W.total + D.S - 1) / D.S, (long long)PG_SHARE);
-  W.whole = tot[8] + tot[9] + tot[10] + tot[11] <= D.S && max(max(tot[4], tot[5]), max(tot[6], tot[7])) <= W.share + PG_CUT;
   // Neighbouring shares read the same keys: eight runs of shares, one for the tasks s, s + 8, .. (where tasks go to workers in order, those of one
   // XCD and its L2).
   const int mine = D.S % 8 == 0 ? (D.s & 7) * (D.S >> 3) + (D.s >> 3) : D.s;
