@@ -14,8 +14,8 @@ typedef int i32x16_t __attribute__((ext_vector_type(16)));
 // ---------------------------------------------------------------------------------------------- rows in 8 bits
 // v of a row (x, RMS-normalised x, silu(x) * x2) in vectors of 8: thread t has vectors t, t + 256, .. How x (and x2) are read, FORM: 1 f32, 2 bf16
 // rows that start at whole words, 3 other bf16 rows, all by 16-byte loads through a descriptor that ends with the row's K values (any alignment of a
-// word, zeros behind the end: only bf16 values that share a word with the last one are masked); 0 element by element, where x and x2 are of two types. A form of its own for each: a branch on the type between two loads makes each
-// wait for the one before.
+// word, zeros behind the end: only bf16 values that share a word with the last one are masked); 0 element by element, where x and x2 are of two types.
+// A form of its own for each: a branch on the type between two loads makes each wait for the one before.
 template <int FORM> struct RawRow {
   u32x4_t a, b; uint32_t c;
   __device__ __forceinline__ void load(const View& X, long long row, int j, int K) {   // vector j of the row
@@ -234,7 +234,8 @@ __device__ __forceinline__ void q8_row_long(const RowsSrc& S, long long r, LDS d
 
 // Op 315. Bound: bytes (K * (2 to 8) read, K written a row). Four rows of up to 4,096 values at once, one of up to 16,384, so that the two
 // reductions' waits are shared; the next rows are requested before this round's maximum. 4,001 rows of 4,096 bf16 values with the norm:
-// 41 us a call (49 MB, 1.2 TB/s with the launch), bound by the instructions of rounding and norm; 49 with masks on every value and sums of doubles through LDS.
+// 41 us a call (49 MB, 1.2 TB/s with the launch); 7 us for four rows, about half of it instructions of rounding and norm, the rest waits of one wave a
+// SIMD. 49 with masks on every value and sums of doubles through LDS.
 template <int FORM, int NV> __device__ __noinline__ void rows_q8_t(const Ctx& c) {
   constexpr int RB = NV && NV <= 2 ? 4 : 1;
   const RowsSrc S{uview(c, 0), uview(c, 1), uview(c, 2), rfl(c.i(7)), rfl(c.i(8)), c.f(9)};

@@ -19,8 +19,9 @@ With `cache='paged'` a step takes prompts and single tokens together: `rows` new
 the rows in front of every product in 8 bits (rows_q8 -> matmul_q8 or gemv_q8), the cache in pages (qkv_append_paged, attn_paged).
 The caller writes, between launches, `tok` (the new tokens, sequence after sequence), `cu` (where each sequence's start), `last` (the
 row of each sequence's last one), `lens` (tokens in the cache before the step) and `table` (each sequence's pages) and reads the next token
-of every sequence that had one from `next`. With rows = 0 the step is a decode step: a token of every sequence, its successor goes to
-`tok` and `lens` grows by itself. The weights are the caller's (serving.quantise_rows), zeros until written.
+of every sequence that had one from `next`. Products and rows in 8 bits run over all `rows`, however many a step brings. With rows = 0 the
+step is a decode step: a token of every sequence, its successor goes to `tok` and `lens` grows by itself. The weights are the caller's
+(serving.quantise_rows), zeros until written.
 """
 from __future__ import annotations
 
