@@ -139,7 +139,7 @@ __device__ __noinline__ void op_qkv_append_paged(const Ctx& c) {
 // Head sizes 64 and 128, rows in whole vectors, one type for the new rows and one for where they go. Bound: bytes for prompts, a few dependent
 // loads (row numbers, length, page, row) and the launch for single tokens. A (row, head) is HD / 8 lanes of 8 values; a row's angles are
 // computed once for all its heads; four items' loads are requested together. A call (launch ~13 us): 96 tokens of 48 heads of 128 24 us, prompts of
-// 1,900 rows of 24 heads of 64 in f32 36 us (24 MB).
+// 1,900 rows of 24 heads of 64 in f32 40 us (24 MB).
 template <int HD, bool FROM16> __device__ __noinline__ void append_paged_t(const Ctx& c) {
   constexpr int LPR = HD / 8, RPP = KVM_THREADS / LPR, NR = 4;
   const AppendPaged A(c);
@@ -243,7 +243,7 @@ struct PiecePaged { int k0, k1, k, live, i0; };
 // and token are cut into equal shares, in all tasks alike from the lengths. A cut within PG_SNAP of a tile's end moves there: a small piece
 // costs more than it balances; where there is a task for every tile and none is longer than a share by PG_CUT, about what the partials and the
 // merge of a cut cost, no tile is cut: a tile costs 1 then, a task has one or none, and these are spread over all tasks (shared out by their keys
-// some tasks had two and others none: 1,000 tokens of 32 heads behind 3,750, 256 tiles, 272 us in place of 182). Tiles of up to 32 rows are a
+// some tasks had two and others none: 1,000 tokens of 32 heads behind 3,750, 256 tiles, 272 us in place of 175). Tiles of up to 32 rows are a
 // sequence's new tokens as a whole (the waves share the keys); longer ones have `tile` rows (the waves share the rows).
 constexpr int PG_TILE = 256, PG_SNAP = 320, PG_SHARE = 512, PG_CUT = 1024;
 struct WorkPaged {
@@ -835,7 +835,7 @@ template <int HD, int NT> __device__ __noinline__ int attn_paged_keys(const Ctx&
 
 // The same tiles in f32 storage, v_mfma_f32_16x16x4_f32 (exact products): units of 16 keys; a lane's 16-byte load of a key is four dims of it, of
 // which product i takes the i-th from all lanes (k = l / 16), and the scores' registers r are, row by row, P's operand for the keys 4 k + r,
-// whose values the lane has loaded. A call: 100 rows of 16 heads of 64 behind ~1,000 tokens each 56 us, its tasks' chain of dependent loads.
+// whose values the lane has loaded. A call: 100 rows of 16 heads of 64 behind ~1,000 tokens each 53 us, its tasks' chain of dependent loads.
 template <int HD, int NT> __device__ __noinline__ int attn_paged_keys_f32(const Ctx& c, int b_, int h_, int L_, int row0_, int tok0_, int ntok_, int k0_, int k1_, int k_, int live_, int i0_) {
   constexpr int NK = HD / 16, DPL = HD / 16, NV = DPL / 4;
   const AttnPaged D(c);
@@ -944,7 +944,7 @@ template <int HD, int NT> __device__ __noinline__ int attn_paged_keys_f32(const 
 // a lane reads HD / 32 dims of 8 keys and turns them in registers (a byte permute for two values), dims HD / 32 * m + i to row m of product i:
 // transposing reads of LDS run at a third of the rate. P^T is two operands, as above. 32 keys at a time, the scores of the next ones under the
 // softmax of these: with 64 the fragments and scores under way pass 256 registers. A block of 64 keys takes 128 rows 2.3 us (470 TFLOP/s over
-// 256 CUs; 1.9 with P^T rounded once), some 630 instructions a wave of which 48 are products; 1,000 tokens of 32 heads behind 3,750 182 us a call.
+// 256 CUs; 1.9 with P^T rounded once), some 630 instructions a wave of which 48 are products; 1,000 tokens of 32 heads behind 3,750 175 us a call.
 constexpr int PG_IDS = 2048, PG_NS = 3;
 __device__ __forceinline__ void dma16_at(unsigned long long src, unsigned dst) {   // 16 bytes a lane from its own address to LDS byte dst (uniform) + 16 * lane
   asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" :: "s"(dst), "v"(src) : "memory", "m0");

@@ -234,8 +234,8 @@ __device__ __forceinline__ void q8_row_long(const RowsSrc& S, long long r, LDS d
 
 // Op 315. Bound: bytes (K * (2 to 8) read, K written a row). Four rows of up to 4,096 values at once, one of up to 16,384, so that the two
 // reductions' waits are shared; the next rows are requested before this round's maximum. 4,001 rows of 4,096 bf16 values with the norm:
-// 41 us a call (49 MB, 1.2 TB/s with the launch); 7 us for four rows, about half of it instructions of rounding and norm, the rest waits of one wave a
-// SIMD. 49 with masks on every value and sums of doubles through LDS.
+// 43 us a call (49 MB, 1.1 TB/s with the launch); 7 us for four rows, about half of it instructions of rounding and norm, the rest waits of one wave a
+// SIMD. Masks on every value and sums of doubles through LDS made it 49 where this took 41.
 template <int FORM, int NV> __device__ __noinline__ void rows_q8_t(const Ctx& c) {
   constexpr int RB = NV && NV <= 2 ? 4 : 1;
   const RowsSrc S{uview(c, 0), uview(c, 1), uview(c, 2), rfl(c.i(7)), rfl(c.i(8)), c.f(9)};
@@ -489,8 +489,8 @@ __device__ __noinline__ void op_matmul_q8(const Ctx& c) {
 // ---------------------------------------------------------------------------------------------- rows of weights, streamed
 // Op 317. Bound: the weights' bytes (N * K), as the bf16 stream of ops 134 and 301, whose ring and cursor it uses (a row of bytes is a row of
 // half as many bf16 values); K is rounded up to whole steps of all waves, the bytes behind K are 0 in the staged rows. A step of a wave is two
-// v_mfma_i32_16x16x64_i8. A call: 12,288 x 4,096 for one row with the norm 35 us, of which the weights' 50 MB take ~15, launch ~13 and the row's
-// norm and rounding inside every task ~6; 4,096 x 12,288 for 8 rows behind rows_q8 47.
+// v_mfma_i32_16x16x64_i8. A call: 12,288 x 4,096 for one row with the norm 38 us, of which the weights' 50 MB take ~15, launch ~13 and the row's
+// norm and rounding inside every task ~6; 4,096 x 12,288 for 8 rows behind rows_q8 50.
 struct GemvQ8 {
   View x, x2, g, w, sw, out, bias, res, sx; int n0, n1, K, M, pro, Ke;
   __device__ explicit GemvQ8(const Ctx& c)
